@@ -265,7 +265,7 @@ def _own_append(s):
 def _own_attend(s):
     from spectra_amd import kernels as K
     if "workspace" not in s:  # kept for all layers and steps, as a serving loop does
-        s["workspace"] = K.paged_attend_workspace(s["heads"], s["kv_heads"], s["head_dim"], s["q"].device)
+        s["workspace"] = K.paged_attend_workspace(s["head_dim"], s["q"].device)
     return K.paged_attend(s["q"], s["kv_lens"], s["q_start"], s["table"], s["k"], s["v"], cap=s["cap"], window=s["window"],
                           slopes=s["slopes"], prefix=s["prefix"], workspace=s["workspace"])
 
