@@ -28,6 +28,8 @@
  *                           <- spectra/engine.py:1690-1697 sample_token (temperature 0)
  *   spectra_kv4_quantize, spectra_kv4_dequantize, spectra_attend_decode_q4
  *                           <- spectra/engine.py:614-700 the 4-bit KV cache
+ *   spectra_paged_rope_append, spectra_paged_attend
+ *                           <- no counterpart: the caches above for a batch of sequences
  */
 #ifndef SPECTRA_HIP_H_
 #define SPECTRA_HIP_H_
@@ -368,6 +370,70 @@ int spectra_greedy_next(const void* logits, int64_t n, int64_t* token, int64_t* 
  * instead of a scan of the logits (engine.py:1690-1697, with the argmax in the lm_head). */
 int spectra_greedy_finish(void* argmax_key, int64_t* token, int64_t* history, int64_t hist_len, int64_t* pos,
                           spectra_stream_t stream);
+
+/* ---- the paged KV cache: many sequences -----------------------------------------------------
+ * The caches above hold one sequence; these serve a batch of them (no counterpart in the
+ * reference, whose caches are per model: engine.py:614-700, :1387-1415).  A pool of pages, each
+ * [kv_heads, page_size, head_dim] and contiguous, `page_stride` elements (codes: bytes) apart:
+ * fp16, bf16, or the 4-bit codes of spectra_kv4_quantize with their fp16 scales and uint8 zero
+ * points [kv_heads, page_size, head_dim / 32] a page.  Position p of sequence b is row
+ * p % page_size of page block_table[b, p / page_size] (int32 [batch, table_width], rows
+ * table_stride apart).  head_dim 64 or 128; page_size a power of two >= 16; every page 16-byte
+ * aligned.  A call's tokens are those of the sequences one after another: q_start int32
+ * [batch + 1] (q_start[0] = 0, never decreasing), and kv_lens int32 [batch] counts each
+ * sequence's positions with its tokens of this call, which are its last ones.  Tokens behind
+ * q_start[batch] (a padded batch) are left alone.  All three are read on the device: a captured
+ * step follows them.  A page id outside [0, num_pages) or a position past the table is never
+ * read or written: appending skips it, and attention gives NaN to every row that sees it.
+ */
+typedef enum { SPECTRA_KV_F16 = 0, SPECTRA_KV_BF16 = 1, SPECTRA_KV_4BIT = 2 } spectra_kv_kind_t;
+
+typedef struct spectra_paged_kv {
+  int32_t kind;              /* spectra_kv_kind_t; activations: bf16 for BF16 pages, fp16 otherwise */
+  int32_t kv_heads, head_dim, page_size;
+  int64_t num_pages;
+  void* k; void* v; int64_t page_stride;
+  void* k_scales; void* v_scales; int64_t scale_stride; /* 4BIT: fp16, elements from page to page */
+  void* k_zeros; void* v_zeros; int64_t zero_stride;    /* 4BIT: uint8 */
+  int32_t batch, table_width;
+  const int32_t* block_table; int64_t table_stride;
+  const int32_t* kv_lens;
+  const int32_t* q_start;
+} spectra_paged_kv_t;
+
+/* spectra_rope_append for a paged cache, bit-identical in what it rotates and stores: rotates the
+ * q and k heads of `tokens` fused-QKV rows (row stride ldqkv: heads q heads, kv_heads k heads,
+ * kv_heads v heads) at their positions (cos_t, sin_t fp32 [rope_rows, head_dim / 2]; NULL = no
+ * rotation), appends k and v, 4-bit pages through the quantizer of spectra_kv4_quantize, and
+ * writes q_rot [tokens, heads, head_dim].  A token without a position in [0, rope_rows) appends
+ * nothing and gets NaN queries.  Two tokens never write the same row unless two sequences name
+ * the same page for positions they append: such rows then hold either's values, or a mix. */
+int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
+                              const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads, void* q_rot,
+                              spectra_stream_t stream);
+
+/* Attention of a ragged batch over its pages (one token a sequence, a few drafted ones, or a
+ * prompt's): token t of sequence b at position i, query head h (KV head h / (heads / kv_heads)):
+ *   out[t, h] = sum_j p_j v_j,   p = softmax over the visible j of
+ *               f(scale q[t, h] . k_j) - slopes[h] |i - j|,   f(x) = cap tanh(x / cap), or x
+ *                                                             when cap is 0
+ * j is visible when j < kv_lens[b], j <= i or j < prefix[b], and i - j < window or window is 0.
+ * fp32 scores, softmax and sums; weights rounded to the activations' 16 bits for the product
+ * with v; 4-bit values stand for fp16((q - z) * s).  A row that sees no key, or only scores of
+ * -inf, is zero; what a row does not see (rows of a page past the length, later tokens) does not
+ * reach it, whatever it holds, infinities and NaN included.  q [tokens, heads, head_dim], token
+ * stride ldq (a multiple of 8, heads contiguous), out contiguous, both 16-byte aligned; slopes
+ * fp32 [heads] and prefix int32 [batch] may be NULL.
+ * workspace: spectra_paged_attend_workspace(head_dim) bytes, 16-byte aligned: arrival counters
+ * (SPECTRA_PAGED_COUNTER_BYTES at its start), then partial sums of sequences whose keys are
+ * split.  ZERO the counters before its first use; every complete call leaves them at zero, so a
+ * workspace serves later calls of any shape with that head_dim; calls sharing one must not
+ * overlap. */
+#define SPECTRA_PAGED_COUNTER_BYTES 16384
+size_t spectra_paged_attend_workspace(int32_t head_dim);
+int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q, int64_t ldq, int64_t tokens, int32_t heads,
+                         float scale, float cap, int32_t window, const float* slopes, const int32_t* prefix,
+                         void* workspace, size_t workspace_bytes, void* out, spectra_stream_t stream);
 
 /* Measurement only (no counterpart in the reference): the fixed cost of one launch and
  * the time of a plain HBM stream, the floor and ceiling a one-launch GEMV is held against.

@@ -49,6 +49,22 @@ class GemvFusion(ctypes.Structure):
                 ("residual", c_void_p), ("residual_stride", c_int64), ("argmax_key", c_void_p)]
 
 
+KV_F16, KV_BF16, KV_4BIT = 0, 1, 2  # spectra_kv_kind_t
+PAGED_COUNTER_BYTES = 16384  # SPECTRA_PAGED_COUNTER_BYTES
+
+
+class PagedKv(ctypes.Structure):
+    """Mirror of ``spectra_paged_kv_t``."""
+    _fields_ = [("kind", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32),
+                ("num_pages", c_int64),
+                ("k", c_void_p), ("v", c_void_p), ("page_stride", c_int64),
+                ("k_scales", c_void_p), ("v_scales", c_void_p), ("scale_stride", c_int64),
+                ("k_zeros", c_void_p), ("v_zeros", c_void_p), ("zero_stride", c_int64),
+                ("batch", c_int32), ("table_width", c_int32),
+                ("block_table", c_void_p), ("table_stride", c_int64),
+                ("kv_lens", c_void_p), ("q_start", c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/spectra_hip.h declares
 SIGNATURES = {
     "spectra_version": (c_char_p, []),
@@ -97,6 +113,12 @@ SIGNATURES = {
     "spectra_kv4_dequantize": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
     "spectra_attend_decode_q4": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
                                            c_int32] + [c_void_p] * 8 + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "spectra_paged_rope_append": (c_int32, [ctypes.POINTER(PagedKv), c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                            c_int64, c_int32, c_void_p, c_void_p]),
+    "spectra_paged_attend_workspace": (c_size_t, [c_int32]),
+    "spectra_paged_attend": (c_int32, [ctypes.POINTER(PagedKv), c_void_p, c_int64, c_int64, c_int32, ctypes.c_float,
+                                       ctypes.c_float, c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+                                       c_void_p]),
     "spectra_measure_empty": (c_int32, [c_int32, c_int32, c_void_p]),
     "spectra_measure_read": (c_int32, [c_void_p, c_size_t, c_int32, c_int32, c_void_p, c_void_p]),
 }

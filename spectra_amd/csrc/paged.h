@@ -1,0 +1,184 @@
+// The paged KV cache: what its kernels share.
+//
+// A pool of pages, each [kv_heads][page][head_dim] (one KV head's rows of a page are one contiguous
+// run), in fp16, bf16, or 4 bits (codes, fp16 scales and zero points of groups of 32 dims, the
+// layout of the contiguous 4-bit cache with a page in the place of max_seq).  Sequence b's
+// position p is row p % page of page table[b][p / page].  Its last n = q_start[b + 1] -
+// q_start[b] positions of kv_lens[b] are the tokens q_start[b] .. of the call.
+//
+// Tables and lengths live on the device and are read by every kernel, so a captured step follows
+// them without the host; the kernels take them as they come: ids outside the pool and positions
+// outside the table are never turned into addresses.
+#pragma once
+
+#include "common.h"
+
+namespace spectra {
+
+constexpr int kPagedPieces = 128;  // most pieces of a tile's keys
+
+struct PagedKv {
+  uint8_t *k, *v;       // 16-bit rows, or 4-bit codes
+  uint16_t *ks, *vs;    // 4-bit: scales
+  uint8_t *kz, *vz;     // 4-bit: zero points
+  int64_t page_bytes;   // from one page to the next: of k and v,
+  int64_t scale_step;   // of the scales (elements),
+  int64_t zero_step;    // of the zero points
+  const int *table, *lens, *q_start;
+  int64_t table_stride;
+  int num_pages, kv_heads, page_shift, batch, table_width, tokens;
+};
+
+// Validates the descriptor for a call of `tokens` tokens and `heads` query heads, and fills the
+// device form (api side of every paged entry).
+int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, PagedKv* out);
+
+// A sequence's part of the call: its first token, how many, and its keys after them.  Starts
+// are clamped to the call's tokens, lengths to what the table can hold plus one (a position past
+// it is a fault of the caller's that its rows report as NaN).
+struct PagedSeq {
+  int q0, n, len;
+};
+__device__ __forceinline__ PagedSeq paged_seq(int s0, int s1, int len, int tokens) {
+  s0 = min(max(s0, 0), tokens);
+  s1 = min(max(s1, s0), tokens);
+  return {s0, s1 - s0, max(len, 0)};
+}
+
+__device__ __forceinline__ int sread(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A scalar load: p the same in every lane, its memory written by no kernel of this library.
+__device__ __forceinline__ int sload(const int* p) {
+  return *(const __attribute__((address_space(4))) int*)p;
+}
+
+// The sequence of token t, found by the whole wave: 64 starts a step, so up to 64 sequences cost
+// one load.  batch when t lies behind the last sequence.
+__device__ __forceinline__ int paged_find(const int* q_start, int batch, int t, int lane) {
+  int lo = 0, span = batch;
+  while (span > 0) {
+    const int step = (span + 63) >> 6, at = lo + (lane + 1) * step;
+    const int v = at <= lo + span ? q_start[at] : 0x7fffffff;
+    lo += step * __builtin_popcountll(__ballot(at <= lo + span && v <= t));
+    if (step == 1) break;
+    span = min(step, batch - lo);
+  }
+  return sread(lo);
+}
+
+// ---- attention: scores, and the shares of the work ----------------------------------------------
+
+// What turns a product q . k into a score in log2 units: x = mul (q . k), or with a cap
+// cap2 tanh(mul (q . k)) computed as cap2 (1 - 2 / (1 + 2^(t2 (q . k)))) (t2 = 2 log2(e) mul), less
+// slope2 |i - j| where slopes are given.  MOD false: neither.
+struct PagedScore {
+  float mul;           // scale log2(e) without a cap; with one t2
+  float cap2;          // 0: no cap
+  const float* slopes; // [heads] or NULL
+  const int* prefix;   // [batch] or NULL
+  int window;          // 0: none
+};
+template <bool MOD>
+__device__ __forceinline__ float paged_score(float x, const PagedScore& sc, float slope2, float dist) {
+  if constexpr (!MOD) {
+    return x * sc.mul;
+  } else {
+    float y = x * sc.mul;
+    if (sc.cap2 > 0.0f) y = sc.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y)));
+    return __builtin_fmaf(-slope2, __builtin_fabsf(dist), y);
+  }
+}
+
+// Keys [lo, hi) that the query at position i sees, of a sequence of len keys.
+struct PagedRange {
+  int lo, hi;
+};
+__device__ __forceinline__ PagedRange paged_range(int i, int len, int prefix, int window) {
+  const int hi = min(max(i + 1, prefix), len);
+  return {window > 0 ? max(i - window + 1, 0) : 0, hi};
+}
+
+// A unit of work: one piece of the keys of one tile of `rows` query rows (token-major, the g heads
+// of a KV head beside each other) of one KV head of one sequence.
+struct PagedUnit {
+  PagedSeq seq;
+  int b, kvh, tile, piece, pieces, slot, prefix;
+};
+
+// Inclusive sum over the lanes up to this one, on the VALU (row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// The u-th unit, worked out by every wave from the lengths themselves, so that ragged batches are
+// shared out evenly with no plan on the host: the tiles' key steps (of `ks` keys) are counted,
+// and tiles of more steps than target units would get each (and than min_steps) are cut into pieces.  At most
+// tiles + target units; pieces' partial results take slots, at most 2 target of them (a cut tile
+// has fewer than twice its steps over the steps of a piece).  Lengths that did not fit in
+// max_slots would leave a tile in one piece.  false: u is past the last unit.
+__device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, int ks, int min_steps, int target,
+                                           int max_slots,
+                                           const PagedScore& sc, int u, int lane, PagedUnit& un) {
+  const int capacity = kv.table_width << kv.page_shift;
+  PagedSeq sq;
+  int tiles, steps;
+  auto take = [&](int c0) __attribute__((always_inline)) {
+    const int b = min(c0 + lane, kv.batch - 1);
+    sq = paged_seq(kv.q_start[b], kv.q_start[b + 1], kv.lens[b], kv.tokens);
+    tiles = c0 + lane < kv.batch ? (sq.n * g + rows - 1) / rows : 0;
+    int span = min(sq.len, capacity);
+    if (sc.window > 0 && sc.prefix == nullptr) span = min((int64_t)span, (int64_t)sc.window + rows / g + 16);
+    steps = max((span + ks - 1) / ks, 1);
+  };
+  float work = 0.0f;
+  for (int c0 = 0; c0 < kv.batch; c0 += 64) {
+    take(c0);
+    work += (float)tiles * (float)steps;
+  }
+  work = wave_sum(work) * (float)kv.kv_heads;  // (the same in every lane and wave)
+  const int piece_steps = (int)fminf(fmaxf(ceilf(work / (float)target), (float)min_steps), 1e9f);
+  int base = 0, slot0 = 0;
+  for (int c0 = 0; c0 < kv.batch; c0 += 64) {
+    if (kv.batch > 64) take(c0);
+    const int pieces = min((steps + piece_steps - 1) / piece_steps, kPagedPieces);
+    const int units = kv.kv_heads * tiles * pieces;
+    const int end = base + wave_scan(units), slots = pieces > 1 ? units : 0, send = slot0 + wave_scan(slots);
+    const uint64_t past = __ballot(end > u);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
+      un.b = c0 + at;
+      un.seq = {of(sq.q0), of(sq.n), of(sq.len)};
+      un.pieces = of(pieces);
+      const int nt = of(tiles), first = of(send - slots);
+      int r = u - of(end - units);
+      un.kvh = r % kv.kv_heads;
+      r /= kv.kv_heads;
+      un.piece = r % un.pieces;
+      un.tile = nt - 1 - r / un.pieces;  // (causal tiles: the longest first)
+      if (u < of(end - units) || un.tile < 0) return false;  // (starts that never were a batch: sums that wrapped)
+      const int slot = first + (un.kvh * nt + un.tile) * un.pieces;
+      if (un.pieces > 1 && (slot < 0 || slot > max_slots - un.pieces)) {
+        if (un.piece > 0) return false;
+        un.pieces = 1;
+      }
+      un.slot = slot + un.piece;
+      un.prefix = sc.prefix != nullptr ? max(sload(sc.prefix + un.b), 0) : 0;
+      // (the same in every lane, told to the compiler: addresses made of them stay scalar)
+      un = {{sread(un.seq.q0), sread(un.seq.n), sread(un.seq.len)}, sread(un.b), sread(un.kvh), sread(un.tile),
+            sread(un.piece), sread(un.pieces), sread(un.slot), sread(un.prefix)};
+      return true;
+    }
+    base = __builtin_amdgcn_readlane(end, 63);
+    slot0 = __builtin_amdgcn_readlane(send, 63);
+  }
+  return false;
+}
+
+}  // namespace spectra

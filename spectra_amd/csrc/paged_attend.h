@@ -1,0 +1,202 @@
+// What the paged attention kernels share: operand types, the joining of a tile's pieces, and the
+// row-by-row path.
+#pragma once
+
+#include "kv4.h"
+#include "paged.h"
+
+namespace spectra {
+
+enum { kKvF16 = SPECTRA_KV_F16, kKvBf16 = SPECTRA_KV_BF16, kKv4 = SPECTRA_KV_4BIT };
+
+typedef _Float16 ph2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 pb2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 pb8_t __attribute__((ext_vector_type(8)));
+typedef float pf2_t __attribute__((ext_vector_type(2)));
+typedef float pf4_t __attribute__((ext_vector_type(4)));
+typedef float pf16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t pu4_t __attribute__((ext_vector_type(4)));
+
+// D = A B + C of 16 x 16 x 32: lane l holds row (A) or column (B) l % 16, contraction slots
+// 8 (l / 16) .. + 7; of D column l % 16, rows 4 (l / 16) .. + 3.
+template <bool BF>
+__device__ __forceinline__ pf4_t mfma16(pu4_t a, pu4_t b, pf4_t c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pb8_t, a), __builtin_bit_cast(pb8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
+}
+
+// The same of 32 x 32 x 16: row or column l % 32, slots 8 (l / 32) .. + 7; of D column l % 32, element r
+// is row 8 (r / 4) + 4 (l / 32) + r % 4.
+template <bool BF>
+__device__ __forceinline__ pf16_t mfma32(pu4_t a, pu4_t b, pf16_t c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pb8_t, a), __builtin_bit_cast(pb8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
+}
+
+// Two weights rounded to 16 bits (to nearest even), x in the low half.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (BF) {
+    const pf2_t v = {x, y};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pb2_t));
+  } else {
+    const pf2_t v = {x, y};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, ph2_t));
+  }
+}
+
+// Four pairs of 4-bit codes (nibbles n and n + 4 of w, n = 0 .. 3) as fp16((q - z) * s): 1024 + q is
+// the fp16 with q in its last bits, and 1024 + q - (1024 + z) is exact.  nz: the pair -(1024 + z),
+// s: the pair of scales.
+__device__ __forceinline__ pu4_t kv4_pairs(uint32_t w, ph2_t nz, ph2_t s) {
+  pu4_t r;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const uint32_t c = ((w >> (4 * n)) & 0x000f000fu) | 0x64006400u;
+    r[n] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(ph2_t, c) + nz) * s);
+  }
+  return r;
+}
+
+// One element of the pages (the row-by-row path's reads).
+template <int HD, int KIND>
+__device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int page, int64_t row, int d) {
+  const uint8_t* p = (value ? kv.v : kv.k) + page * kv.page_bytes;
+  if constexpr (KIND == kKv4) {
+    const uint32_t c = (p[row * (HD / 2) + d / 2] >> (4 * (d & 1))) & 15u;
+    const float s = h2f((value ? kv.vs : kv.ks)[page * kv.scale_step + row * (HD / 32) + d / 32]);
+    const float z = (float)(value ? kv.vz : kv.kz)[page * kv.zero_step + row * (HD / 32) + d / 32];
+    return h2f(f2h(((float)c - z) * s));
+  } else {
+    const uint16_t h = ((const uint16_t*)p)[row * HD + d];
+    return KIND == kKvBf16 ? bf2f(h) : h2f(h);
+  }
+}
+
+// One row by itself, every key that it does not see left out: the path of rows that came out
+// infinite or NaN beside rows that see other keys (a weight of zero times an infinity is NaN in the
+// matrix product).  A wave a row: lane = key for the scores, lane = HD / 64 dims for the sums.
+template <int HD, int KIND, bool MOD>
+__device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& sc, const PagedUnit& un, int g,
+                                       const uint16_t* q, int64_t ldq, int heads, int row, uint16_t* out) {
+  constexpr bool BF = KIND == kKvBf16;
+  constexpr int DL = HD / 64;
+  const int lane = threadIdx.x & 63;
+  const int tok = row / g, head = un.kvh * g + row % g, i = un.seq.len - un.seq.n + tok;
+  const uint16_t* qr = q + (int64_t)(un.seq.q0 + tok) * ldq + head * HD;
+  const PagedRange rg = paged_range(i, un.seq.len, un.prefix, sc.window);
+  const int capacity = kv.table_width << kv.page_shift, mask = (1 << kv.page_shift) - 1;
+  const float slope2 = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
+  float m = -INFINITY, l = 0.0f, acc[DL] = {};
+  for (int j0 = rg.lo; j0 < min(rg.hi, capacity); j0 += 64) {
+    const int j = j0 + lane;
+    const bool see = j < min(rg.hi, capacity);
+    const int page = see ? kv.table[un.b * kv.table_stride + (j >> kv.page_shift)] : 0;
+    const bool bad = (uint32_t)page >= (uint32_t)kv.num_pages;
+    const int64_t r = ((int64_t)un.kvh << kv.page_shift) + (j & mask);
+    float x = -INFINITY;
+    if (see) {
+      x = 0.0f;
+      for (int d = 0; d < HD; ++d) x += (BF ? bf2f(qr[d]) : h2f(qr[d])) * paged_elem<HD, KIND>(kv, false, bad ? 0 : page, r, d);
+      x = bad ? NAN : paged_score<MOD>(x, sc, slope2, (float)(i - j));
+    }
+    const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.0f : mn;
+    const float corr = __builtin_amdgcn_exp2f(m - mu), e = see ? __builtin_amdgcn_exp2f(x - mu) : 0.0f;
+    m = mn;
+    l = l * corr + wave_sum(e);
+#pragma unroll
+    for (int d = 0; d < DL; ++d) acc[d] *= corr;
+    for (int n = 0; n < 64 && j0 + n < min(rg.hi, capacity); ++n) {
+      const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), n));
+      const int pg = __builtin_amdgcn_readlane(bad ? 0 : page, n);
+      const int64_t rn = ((int64_t)un.kvh << kv.page_shift) + ((j0 + n) & mask);
+#pragma unroll
+      for (int d = 0; d < DL; ++d) acc[d] += p * paged_elem<HD, KIND>(kv, true, pg, rn, DL * lane + d);
+    }
+  }
+  if (rg.hi > capacity) l = NAN;
+#pragma unroll
+  for (int d = 0; d < DL; ++d) {
+    const float v = l == 0.0f ? 0.0f : acc[d] / l;
+    out[((int64_t)(un.seq.q0 + tok) * heads + head) * HD + DL * lane + d] = BF ? f2bf(v) : f2h(v);
+  }
+}
+
+// Arrival of a piece at its tile's counter, its partial sums complete (every thread has waited for
+// its stores); true in every thread of the last of `pieces`, which leaves the counter at zero.
+__device__ __forceinline__ bool paged_arrive(uint32_t* counter, int pieces, int* flag) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = n == (uint32_t)(pieces - 1);
+    if (n == (uint32_t)(pieces - 1)) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// A row's pieces joined (in their order, whatever order they arrived in): dims d .. d + 3 of the sum
+// of weight times value, and the sum of weights.  A piece's record: [rows][HD + 2], the row's sums,
+// their maximum and the sum of weights; an empty piece has maximum -inf and sum 0 (a NaN sum
+// beside it is a NaN score's).
+template <int HD, int ROWS>
+__device__ __forceinline__ float paged_join(const float* base, int pieces, int row, int d, float (&v)[4]) {
+  float mm = -INFINITY, den = 0.0f;
+  v[0] = v[1] = v[2] = v[3] = 0.0f;
+  for (int p0 = 0; p0 < pieces; p0 += 8) {
+    float pm[8], pl[8], x[8][4];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float* p = base + ((int64_t)min(p0 + u, pieces - 1) * ROWS + row) * (HD + 2);
+      pm[u] = load_dev(p + HD);
+      pl[u] = load_dev(p + HD + 1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[u][e] = load_dev(p + d + e);
+    }
+    float mn = mm;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) mn = fmaxf(mn, pm[u]);
+    const float corr = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mm - mn);
+    den *= corr;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= corr;
+    mm = mn;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (p0 + u >= pieces) continue;
+      const float f = pm[u] == -INFINITY ? (pl[u] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(pm[u] - mm);
+      den += f * pl[u];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += f * x[u][e];
+    }
+  }
+  return den;
+}
+
+// The host side of a launch, shared by the kernels' translation units.
+struct PagedLaunch {
+  PagedKv kv;
+  PagedScore sc;
+  const uint16_t* q;
+  int64_t ldq;
+  uint16_t* out;
+  int heads, g, kind, hd, units;  // units: the grid
+  uint32_t* counters;
+  float* slots;
+  hipStream_t stream;
+  bool mod;
+};
+// Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows.
+constexpr int kFewTarget = 1024, kFewSlots = 2 * kFewTarget, kFewKeys = 128;
+int launch_paged_few(const PagedLaunch& a, int rows);
+// Many rows a sequence (prompts): tiles of 128 rows.
+constexpr int kManyRows = 128, kManyKeys = 64, kManyMinSteps = 8, kManyTarget = 256, kManySlots = 2 * kManyTarget;
+int launch_paged_many(const PagedLaunch& a);
+
+}  // namespace spectra

@@ -1,0 +1,399 @@
+// Attention over a paged KV cache for few rows a sequence: one token, or a few drafted ones, times
+// the query heads of a KV head, in tiles of 16 or 32 rows.
+//
+// Bound by reading the cache once.  So nothing of it goes through LDS: a wave takes 32 keys at a
+// time straight into the registers that the matrix instructions read, the next 32 in flight
+// behind them.  Scores are computed transposed, S^T = K Q^T (16 x 16 x 32): a lane's 16 bytes of a key
+// row are the A operand as they lie in memory, and the lane ends with the scores of the keys
+// 4 (l / 16) + 0 .. 3 of each 16 for row l % 16 of the tile.  Those are the B operand of O^T = V^T P^T when the
+// contraction takes the keys in that order, so the weights never move; V is loaded by the same
+// order (a lane: HD / 16 dims of its 8 keys) and turned by byte permutes.  4-bit pages are
+// expanded in the registers (codes of a key's row as they lie; Q is put in the codes' order once).
+//
+// A unit of work (paged_unit) is a piece of the keys of a tile; its 4 waves take 32-key tiles in
+// turn and meet in LDS at the end, pieces in the workspace, where the last to arrive joins them.
+#include "paged_attend.h"
+
+namespace spectra {
+
+constexpr int kFewThreads = 256;
+
+// 32 keys of K and V as they lie: tile t, register r.
+template <int HD, int KIND>
+struct FewTile {
+  pu4_t k[2][HD / 32];
+  uint32_t v[2][4][HD / 32];
+};
+template <int HD>
+struct FewTile<HD, kKv4> {
+  uint32_t k[2][HD / 32], v[2][4], ks[2], vs[2][4], kz[2], vz[2][4];  // (scales and zero points: low bits)
+};
+
+template <int HD, int KIND, int NT, bool MOD>
+__global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
+    paged_few_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
+                     uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
+  constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
+  constexpr int ROWS = 16 * NT, KS = HD / 32, DPL = HD / 16, RS = HD + 4;
+  constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;  // bytes of a row of a page
+  __shared__ __align__(16) float red[4 * 16 * RS];
+  __shared__ float wm[4][ROWS], wl[4][ROWS];
+  __shared__ int flag;
+  __shared__ uint32_t redo;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), c = lane & 15, q4 = lane >> 4;
+  PagedUnit un;
+  if (!paged_unit(kv, g, ROWS, kFewKeys, 1, kFewTarget, kFewSlots, sc, blockIdx.x, lane, un)) return;
+  const PagedSeq sq = un.seq;
+  const int r0 = un.tile * ROWS, nrows = min(ROWS, sq.n * g - r0);
+  const int tok0 = sread(r0 / g), tok1 = sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;  // the tile's tokens, position of token 0
+  const int capacity = kv.table_width << kv.page_shift, pmask = (1 << kv.page_shift) - 1;
+  // keys that some row of the tile sees, and those that every row does
+  const PagedRange ra = paged_range(i0 + tok0, sq.len, un.prefix, sc.window);
+  const PagedRange rb = paged_range(i0 + tok1, sq.len, un.prefix, sc.window);
+  const int klo = ra.lo, khi = min(rb.hi, capacity), alo = rb.lo, ahi = ra.hi;
+  const int kbeg = klo & ~31;
+  const int steps = khi > kbeg ? (khi - kbeg + kFewKeys - 1) / kFewKeys : 0;
+  const int sbeg = sread((int)((int64_t)steps * un.piece / un.pieces));
+  const int send = sread((int)((int64_t)steps * (un.piece + 1) / un.pieces));
+
+  // the lane's rows (column c of each 16): their queries, B operands
+  PagedRange rg[NT];
+  float slope2[NT], fpos[NT];
+  pu4_t qf[NT][KS];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + 16 * nt + c;
+    const bool ok = 16 * nt + c < nrows;
+    const int tok = ok ? r / g : tok0, head = un.kvh * g + (ok ? r - tok * g : 0);
+    rg[nt] = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
+    slope2[nt] = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
+    fpos[nt] = (float)(i0 + tok);
+    const uint16_t* qr = q + (int64_t)(sq.q0 + tok) * ldq + head * HD;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      pu4_t x = {0, 0, 0, 0};
+      if (ok) x = *(const pu4_t*)(qr + (Q4 ? (HD / 4) * q4 + 8 * s : 32 * s + 8 * q4));
+      if (Q4)  // pairs in the order of the expanded codes: dims n, n + 4
+        x = (pu4_t){__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+                    __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
+      qf[nt][s] = x;
+    }
+  }
+
+  // ---- loads: page ids a tile ahead of its rows, rows a tile ahead of their use
+  const int* tab = kv.table + un.b * kv.table_stride;
+  auto page_of = [&](int key) __attribute__((always_inline)) {
+    return sread(sload(tab + min(key >> kv.page_shift, kv.table_width - 1)));
+  };
+  typedef FewTile<HD, KIND> Tile;
+  const uint32_t koff = (uint32_t)(Q4 ? c * ROWB + q4 * (HD / 8) : c * ROWB + 16 * q4);
+  const uint32_t voff = (uint32_t)(4 * q4 * ROWB + c * (ROWB / 16));
+  auto load = [&](Tile& t, int key0, int p0, int p1) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int id = h ? p1 : p0;
+      const int64_t pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
+      const int row = (un.kvh << kv.page_shift) + ((key0 + 16 * h) & pmask);
+      const uint8_t* kb = kv.k + pg * kv.page_bytes + (int64_t)row * ROWB;
+      const uint8_t* vb = kv.v + pg * kv.page_bytes + (int64_t)row * ROWB;
+      if constexpr (Q4) {
+        const int64_t so = pg * kv.scale_step + (int64_t)row * (HD / 32), zo = pg * kv.zero_step + (int64_t)row * (HD / 32);
+        if constexpr (HD == 128) {
+          const uint4 x = load_at<uint4>(kb, koff);
+          t.k[h][0] = x.x;
+          t.k[h][1] = x.y;
+          t.k[h][2] = x.z;
+          t.k[h][3] = x.w;
+        } else {
+          const uint2 x = load_at<uint2>(kb, koff);
+          t.k[h][0] = x.x;
+          t.k[h][1] = x.y;
+        }
+        const uint32_t kg = c * (HD / 32) + (HD == 128 ? q4 : q4 >> 1);
+        t.ks[h] = load_at<uint16_t>(kv.ks + so, 2 * kg);
+        t.kz[h] = load_at<uint8_t>(kv.kz + zo, kg);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (HD == 128) t.v[h][i] = load_at<uint32_t>(vb, voff + i * ROWB);
+          else t.v[h][i] = load_at<uint16_t>(vb, voff + i * ROWB);
+          const uint32_t vg = (4 * q4 + i) * (HD / 32) + (c * DPL) / 32;
+          t.vs[h][i] = load_at<uint16_t>(kv.vs + so, 2 * vg);
+          t.vz[h][i] = load_at<uint8_t>(kv.vz + zo, vg);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) t.k[h][s] = __builtin_bit_cast(pu4_t, load_at<uint4>(kb, koff + 64 * s));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (HD == 128) {
+            const uint4 x = load_at<uint4>(vb, voff + i * ROWB);
+            t.v[h][i][0] = x.x;
+            t.v[h][i][1] = x.y;
+            t.v[h][i][2] = x.z;
+            t.v[h][i][3] = x.w;
+          } else {
+            const uint2 x = load_at<uint2>(vb, voff + i * ROWB);
+            t.v[h][i][0] = x.x;
+            t.v[h][i][1] = x.y;
+          }
+        }
+      }
+    }
+  };
+
+  float m[NT], l[NT];
+  pf4_t o[NT][DPL];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt] = -INFINITY;
+    l[nt] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) o[nt][j] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  auto compute = [&](const Tile& t, int key0, int p0, int p1) __attribute__((always_inline)) {
+    const bool edge = key0 < klo || key0 + 32 > khi;  // keys that no row sees: their values must not reach the product
+    pf4_t s[NT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (Q4) {
+        const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0xe400u | t.kz[h]));  // -(1024 + z)
+        const _Float16 sf = __builtin_bit_cast(_Float16, (uint16_t)t.ks[h]);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+          const pu4_t a = kv4_pairs(t.k[h][st], (ph2_t){z, z}, (ph2_t){sf, sf});
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s[nt][h] = mfma16<BF>(a, qf[nt][st], s[nt][h]);
+        }
+      } else {
+#pragma unroll
+        for (int st = 0; st < KS; ++st)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s[nt][h] = mfma16<BF>(t.k[h][st], qf[nt][st], s[nt][h]);
+      }
+    }
+    const bool bad0 = (uint32_t)p0 >= (uint32_t)kv.num_pages, bad1 = (uint32_t)p1 >= (uint32_t)kv.num_pages;
+    const bool part = key0 < alo || key0 + 32 > ahi || bad0 || bad1;
+    pu4_t pf[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[8];
+      float mn = m[nt];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // key key0 + 16 (e / 4) + 4 q4 + e % 4
+        x[e] = paged_score<MOD>(s[nt][e >> 2][e & 3], sc, slope2[nt],
+                                MOD ? fpos[nt] - (float)(key0 + 4 * q4) - (float)(16 * (e >> 2) + (e & 3)) : 0.0f);
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = key0 + 16 * (e >> 2) + 4 * q4 + (e & 3);
+          if ((e >> 2) ? bad1 : bad0) x[e] = NAN;
+          if (key < rg[nt].lo || key >= min(rg[nt].hi, capacity)) x[e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mn = fmaxf(mn, x[e]);
+      mn = fmaxf(mn, lane_xor<16>(mn, lane));
+      mn = fmaxf(mn, lane_xor<32>(mn, lane));
+      const float mu = mn == -INFINITY ? 0.0f : mn;
+      if (__ballot(mn > m[nt]) != 0) {
+        const float corr = __builtin_amdgcn_exp2f(m[nt] - mu);
+        l[nt] *= corr;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[nt][j][i] *= corr;
+        m[nt] = mn;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(x[e] - mu);
+        l[nt] += x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pf[nt][e] = pack2<BF>(x[2 * e], x[2 * e + 1]);
+    }
+    // O^T += V^T P^T, dims DPL (l % 16) + j at step j: the 8 keys' values of a dim, in pairs of keys
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    if (edge) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int key = key0 + 16 * (p >> 1) + 4 * q4 + 2 * (p & 1);
+        keep[p] = (key >= klo && key < khi ? 0xffffu : 0u) | (key + 1 >= klo && key + 1 < khi ? 0xffff0000u : 0u);
+      }
+    }
+    if constexpr (Q4) {
+      constexpr int HALF = HD / 64;  // codes of 4 dims each
+      pu4_t a[4 * HALF];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int h = p >> 1, i = 2 * (p & 1);
+        const uint32_t z2 = t.vz[h][i] | (t.vz[h][i + 1] << 16) | 0xe400e400u;
+        const uint32_t s2 = (t.vs[h][i] | (t.vs[h][i + 1] << 16)) & keep[p];
+#pragma unroll
+        for (int u = 0; u < HALF; ++u) {
+          const uint32_t w = __builtin_amdgcn_perm(t.v[h][i + 1], t.v[h][i], u ? 0x07060302u : 0x05040100u);
+          const pu4_t x = kv4_pairs(w, __builtin_bit_cast(ph2_t, z2), __builtin_bit_cast(ph2_t, s2));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) a[4 * u + n][p] = x[n];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < DPL; ++j)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[nt][j] = mfma16<BF>(a[j], pf[nt], o[nt][j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) {
+        pu4_t a;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          a[p] = __builtin_amdgcn_perm(t.v[p >> 1][2 * (p & 1) + 1][j >> 1], t.v[p >> 1][2 * (p & 1)][j >> 1],
+                                       (j & 1) ? 0x07060302u : 0x05040100u);
+          if (edge) a[p] &= keep[p];
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[nt][j] = mfma16<BF>(a, pf[nt], o[nt][j]);
+      }
+    }
+  };
+
+  const int kend = min(khi, kbeg + send * kFewKeys);
+  int key = kbeg + sbeg * kFewKeys + 32 * wave;
+  if (key < kend) {
+    Tile ta, tb;
+    int a0 = page_of(key), a1 = page_of(key + 16), b0 = 0, b1 = 0;
+    load(ta, key, a0, a1);
+    b0 = page_of(key + kFewKeys);
+    b1 = page_of(key + kFewKeys + 16);
+    while (true) {
+      if (key + kFewKeys < kend) load(tb, key + kFewKeys, b0, b1);
+      int n0 = page_of(key + 2 * kFewKeys), n1 = page_of(key + 2 * kFewKeys + 16);
+      compute(ta, key, a0, a1);
+      key += kFewKeys;
+      if (key >= kend) break;
+      if (key + kFewKeys < kend) load(ta, key + kFewKeys, n0, n1);
+      a0 = n0;
+      a1 = n1;
+      n0 = page_of(key + 2 * kFewKeys);
+      n1 = page_of(key + 2 * kFewKeys + 16);
+      compute(tb, key, b0, b1);
+      b0 = n0;
+      b1 = n1;
+      key += kFewKeys;
+      if (key >= kend) break;
+    }
+  }
+
+  // ---- the waves meet: sums of a 16-row half at a time, in LDS
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    l[nt] += lane_xor<16>(l[nt], lane);
+    l[nt] += lane_xor<32>(l[nt], lane);
+    if (q4 == 0) {
+      wm[wave][16 * nt + c] = m[nt];
+      wl[wave][16 * nt + c] = l[nt];
+    }
+  }
+  if (tid == 0) redo = 0;
+  const bool mixed = tok1 > tok0;  // rows that see different keys
+  float* part = slots + (int64_t)un.slot * ROWS * (HD + 2);
+  auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
+    const int r = r0 + row, tok = r / g, head = un.kvh * g + (r - tok * g);
+    const bool past = paged_range(i0 + tok, sq.len, un.prefix, sc.window).hi > capacity;
+    float y[4];
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = past ? NAN : den == 0.0f ? 0.0f : v[e] / den;
+      odd |= !(__builtin_fabsf(y[e]) < INFINITY);
+    }
+    if (mixed && odd) atomicOr(&redo, 1u << row);
+    const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
+    *(uint2*)(out + ((int64_t)(sq.q0 + tok) * heads + head) * HD + d) = w;
+  };
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if (16 * nt >= nrows) break;
+    if (nt > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < DPL; j += 4)
+        *(float4*)(red + (wave * 16 + c) * RS + DPL * (4 * q4 + i) + j) =
+            make_float4(o[nt][j][i], o[nt][j + 1][i], o[nt][j + 2][i], o[nt][j + 3][i]);
+    __syncthreads();
+    for (int it = tid; it < 16 * HD / 4; it += kFewThreads) {
+      const int r = it / (HD / 4), row = 16 * nt + r, d = 4 * (it % (HD / 4));
+      if (row >= nrows) break;
+      float mm = -INFINITY, den = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, wm[w][row]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        // (a wave without keys for the row: weight 0, also where the others' maximum is NaN's -inf)
+        const float f = wm[w][row] == -INFINITY ? (wl[w][row] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(wm[w][row] - mm);
+        const float4 x = *(const float4*)(red + (w * 16 + r) * RS + d);
+        den += f * wl[w][row];
+        v[0] += f * x.x;
+        v[1] += f * x.y;
+        v[2] += f * x.z;
+        v[3] += f * x.w;
+      }
+      if (un.pieces == 1) {
+        write(row, d, v, den);
+      } else {
+        float* p = part + (int64_t)row * (HD + 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) store_dev(p + d + e, v[e]);
+        if (d == 0) {
+          store_dev(p + HD, mm);
+          store_dev(p + HD + 1, den);
+        }
+      }
+    }
+  }
+  if (un.pieces > 1) {
+    const int first = un.slot - un.piece;
+    if (!paged_arrive(counters + first, un.pieces, &flag)) return;
+    // the last to arrive joins the pieces, in their order
+    const float* base = slots + (int64_t)first * ROWS * (HD + 2);
+    for (int it = tid; it < nrows * (HD / 4); it += kFewThreads) {
+      const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
+      float v[4];
+      const float den = paged_join<HD, ROWS>(base, un.pieces, row, d, v);
+      write(row, d, v, den);
+    }
+  }
+  if (!mixed) return;
+  __syncthreads();  // (writes of the rows to be done over are complete)
+  for (uint32_t r = redo & ~0u; r != 0; r &= r - 1) {
+    const int row = __builtin_ctz(r);
+    if ((row & 3) == wave) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + row, out);
+  }
+}
+
+template <int HD, int KIND, int NT, bool MOD>
+static int launch_few(const PagedLaunch& a) {
+  paged_few_kernel<HD, KIND, NT, MOD><<<dim3((unsigned)a.units), dim3(kFewThreads), 0, a.stream>>>(
+      a.kv, a.sc, a.q, a.ldq, a.g, a.heads, a.counters, a.slots, a.out);
+  SPECTRA_HIP_CHECK(hipGetLastError());
+  return SPECTRA_OK;
+}
+template <int HD, int KIND>
+static int launch_few_of(const PagedLaunch& a, int rows) {
+  if (rows == 16) return a.mod ? launch_few<HD, KIND, 1, true>(a) : launch_few<HD, KIND, 1, false>(a);
+  return a.mod ? launch_few<HD, KIND, 2, true>(a) : launch_few<HD, KIND, 2, false>(a);
+}
+int launch_paged_few(const PagedLaunch& a, int rows) {
+  if (a.hd == 64)
+    return a.kind == kKv4      ? launch_few_of<64, kKv4>(a, rows)
+           : a.kind == kKvBf16 ? launch_few_of<64, kKvBf16>(a, rows)
+                               : launch_few_of<64, kKvF16>(a, rows);
+  return a.kind == kKv4      ? launch_few_of<128, kKv4>(a, rows)
+         : a.kind == kKvBf16 ? launch_few_of<128, kKvBf16>(a, rows)
+                             : launch_few_of<128, kKvF16>(a, rows);
+}
+
+}  // namespace spectra

@@ -18,6 +18,7 @@ computes on the host and there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 from collections import OrderedDict
 from typing import List, Optional, Tuple
@@ -30,7 +31,8 @@ __all__ = ["fused_w4a16_gemv_hdsq", "batched_w4a16_gemm", "w4a16_linear", "w4_de
            "QWeightOperands", "GEMV_MAX_M", "w4_embedding", "rmsnorm", "rope_append", "attend_decode",
            "attend_workspace_bytes", "attend_prefill", "silu_mul", "greedy_next", "argmax_slots", "greedy_finish",
            "w4a16_gemv_fused", "kv4_quantize",
-           "kv4_dequantize", "attend_decode_q4", "validate_outliers"]
+           "kv4_dequantize", "attend_decode_q4", "paged_rope_append", "paged_attend", "paged_attend_workspace",
+           "validate_outliers"]
 
 GEMV_MAX_M = 4  # rows served by the GEMV family; larger batches go to the MFMA GEMM
 # rows from which the GEMM entry runs the prefill library path (W_eff dequantized in the
@@ -728,4 +730,153 @@ def attend_decode_q4(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
     L.check("spectra_attend_decode_q4", lib.spectra_attend_decode_q4(
         qkv.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), heads, kv, hd, lmax, w, *ptrs,
         workspace.data_ptr(), workspace.numel() * workspace.element_size(), out.data_ptr(), _stream(qkv.device)))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# the paged KV cache: a batch of sequences
+# ---------------------------------------------------------------------------
+def _paged_kv(x: torch.Tensor, heads: int, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
+              k_pages, v_pages) -> L.PagedKv:
+    """The checked descriptor of a paged cache and its batch, for activations like ``x``."""
+    dev = x.device
+    quantized = not isinstance(k_pages, torch.Tensor)
+    ks, vs = (tuple(k_pages), tuple(v_pages)) if quantized else ((k_pages,), (v_pages,))
+    if not x.is_cuda or x.dtype not in ((torch.float16,) if quantized else (torch.float16, torch.bfloat16)):
+        raise ValueError("activations must be fp16 (bf16 on bf16 pages) on the GPU")
+    if len(ks) != len(vs) or (quantized and len(ks) != 3) or ks[0].dim() != 4:
+        raise ValueError("k_pages and v_pages must be [pages, kv_heads, page, d], or (codes, scales, zeros) of that")
+    pages, kv, page, d = ks[0].shape
+    d = 2 * d if quantized else d
+    shapes = [(torch.uint8, d // 2), (torch.float16, d // 32), (torch.uint8, d // 32)] if quantized else [(x.dtype, d)]
+    for kt, vt, (dtype, last) in zip(ks, vs, shapes):
+        for t in (kt, vt):
+            if t.dtype != dtype or t.shape != (pages, kv, page, last) or t.device != dev:
+                raise ValueError(f"pages of head size {d} must be {dtype} [{pages}, {kv}, {page}, {last}] on {dev}, got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+            if t.stride()[1:] != (page * last, last, 1) or t.stride(0) != kt.stride(0):
+                raise ValueError("a page must be contiguous, and k and v equally far from page to page")
+    if pages == 0:
+        raise ValueError("the pool has no pages")
+    if heads <= 0 or heads % kv:
+        raise ValueError(f"heads ({heads}) must be a multiple of the pages' {kv} KV heads")
+    for t, name, n in ((kv_lens, "kv_lens", 1), (q_start, "q_start", 1), (block_table, "block_table", 2)):
+        if t.dtype != torch.int32 or t.device != dev or t.dim() != n or t.stride(-1) != 1:
+            raise ValueError(f"{name} must be int32 with {n} dimension(s) on {dev}, its rows contiguous")
+    batch = kv_lens.numel()
+    if q_start.numel() != batch + 1 or block_table.shape[0] != batch:
+        raise ValueError(f"{batch} sequences need a q_start of {batch + 1} and a block_table of {batch} rows")
+    p = L.PagedKv()
+    p.kind = L.KV_4BIT if quantized else L.KV_BF16 if x.dtype == torch.bfloat16 else L.KV_F16
+    p.kv_heads, p.head_dim, p.page_size, p.num_pages = kv, d, page, pages
+    p.k, p.v, p.page_stride = ks[0].data_ptr(), vs[0].data_ptr(), ks[0].stride(0)
+    if quantized:
+        p.k_scales, p.v_scales, p.scale_stride = ks[1].data_ptr(), vs[1].data_ptr(), ks[1].stride(0)
+        p.k_zeros, p.v_zeros, p.zero_stride = ks[2].data_ptr(), vs[2].data_ptr(), ks[2].stride(0)
+    p.batch, p.table_width = batch, block_table.shape[1]
+    p.block_table, p.table_stride = block_table.data_ptr(), block_table.stride(0)
+    p.kv_lens, p.q_start = kv_lens.data_ptr(), q_start.data_ptr()
+    return p
+
+
+def paged_rope_append(qkv: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
+                      cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], heads: int, k_pages, v_pages,
+                      q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rope_append`` for a batch of sequences on a paged cache: rotates the q / k heads of the
+    fused-QKV rows ``qkv`` [T, (heads + 2 kv) * d], appends k and v to the sequences' pages and
+    returns the rotated q [T, heads, d].
+
+    ``k_pages`` / ``v_pages`` [pages, kv, page, d] of qkv's type (fp16 or bf16), or 4-bit (codes
+    uint8 [pages, kv, page, d/2], scales fp16 and zeros uint8 [pages, kv, page, d/32]) for fp16
+    qkv; pages may lie apart (a view of a larger pool), a page is contiguous; d 64 or 128, page
+    a power of two >= 16.  Position p of sequence b is row p % page of page
+    ``block_table[b, p // page]``.  Sequence b's tokens are rows q_start[b] .. q_start[b + 1] - 1,
+    the last of its ``kv_lens[b]`` positions (so lengths count the call's tokens); all int32 on
+    the device.  ``cos`` / ``sin`` fp32 [rows, d/2], or None for no rotation.  A token past the
+    rope table, the block table or on a page id outside the pool appends nothing (past the rope
+    table its queries are NaN); rows behind q_start[-1] are left alone."""
+    if qkv.dim() != 2:
+        raise ValueError("qkv must be [T, (heads + 2 kv) * d]")
+    p = _paged_kv(qkv, heads, kv_lens, q_start, block_table, k_pages, v_pages)
+    T, d = qkv.shape[0], p.head_dim
+    if qkv.shape[1] != (heads + 2 * p.kv_heads) * d:
+        raise ValueError(f"qkv rows must hold (heads + 2 kv) * d = {(heads + 2 * p.kv_heads) * d} values")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin must both be given or both be None")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or
+                              t.shape[1] != d // 2 or t.shape != cos.shape or t.device != qkv.device):
+            raise ValueError(f"{name} must be contiguous fp32 [rows, d/2] on {qkv.device}")
+    qkv, ld = _rows(qkv, "qkv", 16)
+    if q_out is None:
+        q_out = torch.empty((T, heads, d), device=qkv.device, dtype=qkv.dtype)
+    elif q_out.dtype != qkv.dtype or q_out.shape != (T, heads, d) or not q_out.is_contiguous() or q_out.device != qkv.device:
+        raise ValueError(f"q_out must be contiguous {qkv.dtype} [{T}, {heads}, {d}] on {qkv.device}")
+    if T == 0:
+        return q_out
+    lib = L.load()
+    with torch.cuda.device(qkv.device):
+        L.check("spectra_paged_rope_append", lib.spectra_paged_rope_append(
+            ctypes.byref(p), qkv.data_ptr(), ld, T, cos.data_ptr() if cos is not None else None,
+            sin.data_ptr() if sin is not None else None, cos.shape[0] if cos is not None else 0, heads, q_out.data_ptr(),
+            _stream(qkv.device)))
+    return q_out
+
+
+def paged_attend_workspace(head_dim: int, device: Optional[torch.device] = None) -> torch.Tensor:
+    """A workspace for ``paged_attend`` calls of one head size (any batch and shape), ready for
+    use: one may serve every layer and step of a stream, but calls that overlap (two streams, two
+    captured graphs replayed at once) need one each."""
+    need = int(L.load().spectra_paged_attend_workspace(head_dim))
+    if need == 0:
+        raise ValueError(f"paged attention serves head sizes 64 and 128, got {head_dim}")
+    ws = torch.empty(need, device=device or torch.device("cuda"), dtype=torch.uint8)
+    ws[:L.PAGED_COUNTER_BYTES].zero_()  # the arrival counters, which every call leaves at zero
+    return ws
+
+
+def paged_attend(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor, k_pages,
+                 v_pages, *, scale: Optional[float] = None, cap: float = 0.0, window: int = 0,
+                 slopes: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None,
+                 workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a ragged batch over a paged cache (as ``paged_rope_append`` fills it): one
+    token a sequence, a few drafted ones, or whole prompts.  ``q`` [T, heads, d] (rows may be a
+    view of wider ones); returns [T, heads, d].
+
+    The token at position i of sequence b sees the keys j < kv_lens[b] with j <= i, or
+    j < prefix[b] (int32 [batch]), and with ``window`` > 0 only those with i - j < window.  A
+    score is scale q.k (1/sqrt(d) by default), capped as cap * tanh(. / cap) when ``cap`` > 0,
+    less slopes[h] |i - j| (fp32 [heads]).  fp32 scores and softmax; the weights are rounded to q's
+    type for the product with v; 4-bit values stand for fp16((q - z) * s).  A row that sees no key
+    is zero; one that would need a page outside the pool or past the table is NaN; rows behind
+    q_start[-1] are left alone.  ``workspace``: ``paged_attend_workspace(d)``; by default a fresh
+    one, which costs a small kernel."""
+    if q.dim() != 3:
+        raise ValueError("q must be [T, heads, d]")
+    T, heads, d = q.shape
+    p = _paged_kv(q, heads, kv_lens, q_start, block_table, k_pages, v_pages)
+    if d != p.head_dim:
+        raise ValueError(f"q has head size {d}, the pages {p.head_dim}")
+    if q.stride(2) != 1 or q.stride(1) != d or q.data_ptr() % 16 or (T > 1 and (q.stride(0) % 8 or q.stride(0) < heads * d)):
+        q = q.clone(memory_format=torch.contiguous_format)
+    for t, name, dtype, n in ((slopes, "slopes", torch.float32, heads), (prefix, "prefix", torch.int32, p.batch)):
+        if t is not None and (t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or t.device != q.device):
+            raise ValueError(f"{name} must be contiguous {dtype} [{n}] on {q.device}")
+    if workspace is None:
+        workspace = paged_attend_workspace(d, q.device)
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {q.device}")
+    if out is None:
+        out = torch.empty((T, heads, d), device=q.device, dtype=q.dtype)
+    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
+        raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)} on {q.device}")
+    if T == 0:
+        return out
+    lib = L.load()
+    with torch.cuda.device(q.device):
+        L.check("spectra_paged_attend", lib.spectra_paged_attend(
+            ctypes.byref(p), q.data_ptr(), q.stride(0) if T > 1 else heads * d, T, heads,
+            1.0 / math.sqrt(d) if scale is None else float(scale), float(cap), int(window),
+            slopes.data_ptr() if slopes is not None else None, prefix.data_ptr() if prefix is not None else None,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), out.data_ptr(), _stream(q.device)))
     return out

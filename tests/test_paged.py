@@ -1,0 +1,697 @@
+"""The paged KV cache: appending with the rotation on the way, and attention over the pages, against plain
+computations in 64 bits.
+
+Tolerances of attention, elementwise, from the roundings that the operator has: u = eps / 2 of the activations' type
+for the output and for every weight (relative to the sum A of weight times |value|; half the smallest subnormal for
+weights below fp16's range); and the scores' error delta, which scales every weight by exp(delta) and thus moves
+numerator and denominator by at most 2 delta A: fp32 products and sums of d terms (d 2^-24 of the sum of |q k|), a cap
+(a few 2^-23 of it, from exp2 and the reciprocal) and the bias (2^-22 of it)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from spectra_amd import _lib as L
+
+KINDS = ["fp16", "bf16", "4bit"]
+_DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "4bit": torch.float16}
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _values(cache, kind):
+    """What 4-bit rows stand for, in 64 bits."""
+    if kind != "4bit":
+        return cache.double()
+    codes, scales, zeros = cache
+    q = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).double()
+    z, s = (t.double().repeat_interleave(32, -1) for t in (zeros, scales))
+    return ((q - z) * s).half().double()
+
+
+class Batch:
+    """A batch on scattered pages: ``n`` tokens of the call and ``lens`` keys per sequence.  Rows of the pool that no
+    sequence fills hold NaN; table entries that none needs, ids outside the pool."""
+
+    def __init__(self, kind, n, lens, heads, kv, d, page, seed=0, pad=0, pages_apart=False):
+        g = _gen(seed)
+        self.kind, self.n, self.lens, self.heads, self.kv, self.d, self.page = kind, n, lens, heads, kv, d, page
+        dt = _DT[kind]
+        need = [-(-m // page) for m in lens]
+        pages = sum(need) + 1
+        order = torch.randperm(pages, generator=g, device="cuda").int()
+        self.table = torch.full((len(n), max(need + [1]) + 1), 1 << 30, dtype=torch.int32, device="cuda")
+        self.table[:, ::2] = -7
+        self.valid = torch.zeros(pages, page, dtype=torch.bool, device="cuda")
+        at = 0
+        for b, (m, w) in enumerate(zip(lens, need)):
+            self.table[b, :w] = order[at: at + w]
+            at += w
+            for p in range(w):
+                self.valid[self.table[b, p].long(), : min(page, m - p * page)] = True
+        step = 2 if pages_apart else 1  # pages apart: every second page of a larger pool
+
+        def pool(last, dtype):
+            return torch.zeros(pages * step, kv, page, last, dtype=dtype, device="cuda")[::step]
+
+        def rand(*shape):
+            return torch.randn(*shape, generator=g, device="cuda").to(dt)
+
+        if kind == "4bit":
+            from spectra_amd import kernels as K
+            self.k, self.v = [], []
+            for out in (self.k, self.v):
+                for t in K.kv4_quantize(rand(pages * kv, page, d)):
+                    x = pool(t.shape[-1], t.dtype)
+                    x.copy_(t.view(pages, kv, page, -1))
+                    out.append(x)
+                out[1].masked_fill_(~self.valid[:, None, :, None], float("nan"))
+            self.k, self.v = tuple(self.k), tuple(self.v)
+        else:
+            self.k, self.v = pool(d, dt), pool(d, dt)
+            for x in (self.k, self.v):
+                x.copy_(rand(pages, kv, page, d).masked_fill(~self.valid[:, None, :, None], float("nan")))
+        starts = [0]
+        for m in n:
+            starts.append(starts[-1] + m)
+        self.q_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        self.kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        self.tokens = starts[-1] + pad
+        self.q = rand(self.tokens, heads, d)
+        self.rand = rand
+
+    def rows(self, b):
+        """Keys and values of sequence b [kv, len, d], 64 bits."""
+        ids = self.table[b, : -(-self.lens[b] // self.page)].long()
+        return [_values(tuple(t[ids] for t in c) if self.kind == "4bit" else c[ids], self.kind).transpose(0, 1)
+                .reshape(self.kv, -1, self.d)[:, : self.lens[b]] for c in (self.k, self.v)]
+
+    def reference(self, scale=None, cap=0.0, window=0, slopes=None, prefix=None):
+        """Output and elementwise tolerance, by sequence and head."""
+        scale = 1.0 / math.sqrt(self.d) if scale is None else scale
+        u = torch.finfo(_DT[self.kind]).eps / 2
+        sub = 2.0 ** -25 if self.kind != "bf16" else 0.0
+        out = torch.zeros(self.tokens, self.heads, self.d, dtype=torch.float64, device="cuda")
+        tol = torch.zeros_like(out)
+        at = 0
+        for b, (n, m) in enumerate(zip(self.n, self.lens)):
+            if n == 0:
+                continue
+            k, v = self.rows(b)
+            i = torch.arange(m - n, m, device="cuda")[:, None]
+            j = torch.arange(m, device="cuda")[None]
+            see = (j <= i) | (j < (int(prefix[b]) if prefix is not None else 0))
+            if window:
+                see &= i - j < window
+            for h in range(self.heads):
+                kh, vh = k[h * self.kv // self.heads], v[h * self.kv // self.heads]
+                qh = self.q[at: at + n, h].double()
+                x = qh @ kh.T * scale
+                delta = self.d * 2.0 ** -24 * (qh.abs() @ kh.abs().T * scale).amax(-1, keepdim=True) if m else 0.0
+                if cap:
+                    x = cap * torch.tanh(x / cap)
+                    delta = delta + cap * 2.0 ** -20
+                if slopes is not None:
+                    bias = float(slopes[h]) * (i - j).abs()
+                    x = x - bias
+                    delta = delta + 2.0 ** -22 * bias.amax() if m else delta
+                x = x.masked_fill(~see, -math.inf)
+                top = x.amax(-1, keepdim=True) if m else torch.zeros(n, 1, device="cuda", dtype=torch.float64)
+                e = torch.exp(x - torch.where(top == -math.inf, 0.0, top))
+                e = torch.where(see, e, 0.0)
+                total = e.sum(-1, keepdim=True)
+                vis = torch.where(see, 1.0, 0.0).double()
+                clean = vh.masked_fill(~torch.isfinite(vh), 0.0)
+                o = (e @ clean) / torch.where(total == 0, 1.0, total)
+                lost = ~torch.isfinite(vh)  # a value that is not finite reaches the rows that see it, no others
+                o = o.masked_fill((vis @ lost.double()) > 0, math.nan)
+                a = (e @ clean.abs()) / torch.where(total == 0, 1.0, total)
+                out[at: at + n, h] = o
+                tol[at: at + n, h] = u * o.abs() + (u + 2 * delta + 2.0 ** -20) * a + \
+                    sub * (1 + (vis @ clean.abs()) / torch.where(total == 0, 1.0, total))
+            at += n
+        return out, tol
+
+    def attend(self, **kw):
+        from spectra_amd import kernels as K
+        return K.paged_attend(self.q, self.kv_lens, self.q_start, self.table, self.k, self.v, **kw)
+
+    def check(self, **kw):
+        """Runs on an output that already holds something, compares, and returns the output."""
+        out = torch.full_like(self.q, 7.0)
+        got = self.attend(out=out, **kw)
+        assert got is out
+        kw.pop("workspace", None)
+        want, tol = self.reference(**kw)
+        used = sum(self.n)
+        assert torch.all(out[used:] == 7.0), "rows behind the last sequence were written"
+        x, y = out[:used].double(), want[:used]
+        assert torch.equal(torch.isnan(x), torch.isnan(y))
+        off = ((x - y).abs() - tol[:used]).nan_to_num(-1.0).max()
+        assert off <= 0, f"{float(off):.3g} outside the tolerance"
+        return out
+
+
+# -- attention: forms, sizes, masks --------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,d", [(24, 8, 128), (4, 4, 64), (14, 2, 64), (16, 1, 128), (5, 1, 128)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_single_tokens(hip, kind, heads, kv, d, page):
+    lens = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 300, 517, 0]
+    n = [1] * 15 + [0]
+    Batch(kind, n, lens, heads, kv, d, page, seed=heads + page, pad=3).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,d", [(8, 4, 64), (24, 8, 128), (32, 1, 64)])
+def test_drafted_tokens(hip, kind, heads, kv, d):
+    n = [5, 1, 4, 2, 0, 7, 3]
+    lens = [5, 40, 131, 700, 12, 263, 64]
+    Batch(kind, n, lens, heads, kv, d, 32, seed=3, pad=1).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,d,page", [(6, 2, 128, 16), (4, 4, 64, 128), (7, 1, 64, 32)])
+@pytest.mark.parametrize("n,lens", [([1, 90, 257, 0, 33], [70, 90, 300, 0, 512]), ([129], [129]), ([64, 200], [1000, 200])])
+def test_prompts(hip, kind, heads, kv, d, page, n, lens):
+    Batch(kind, n, lens, heads, kv, d, page, seed=len(n), pad=2).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [[1, 1, 1], [3, 2, 4], [150, 40, 77]])
+@pytest.mark.parametrize("mods", [dict(cap=2.0), dict(slopes=True), dict(window=50), dict(prefix=True),
+                                  dict(window=1), dict(cap=30.0, slopes=True, window=200, prefix=True), dict(scale=0.4)])
+def test_scores_and_masks(hip, kind, n, mods):
+    b = Batch(kind, n, [200, 333, 150], 6, 2, 64, 16, seed=5)
+    mods = dict(mods)
+    if "slopes" in mods:
+        mods["slopes"] = torch.exp2(-torch.arange(1, 7, device="cuda").float())
+    if "prefix" in mods:
+        mods["prefix"] = torch.tensor([64, 0, 1000], dtype=torch.int32, device="cuda")
+    b.check(**mods)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "4bit"])
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_long_caches_split(hip, kind, n):
+    """Few tiles of long caches: every tile's keys in many pieces, joined in order."""
+    b = Batch(kind, [n, n], [9001, 4000], 4, 2, 128, 64, seed=9)
+    from spectra_amd import kernels as K
+    ws = K.paged_attend_workspace(128)
+    first = b.check(workspace=ws)
+    for _ in range(3):
+        assert torch.equal(b.attend(workspace=ws), first), "the same call gave other bits"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [65, 200])
+def test_many_sequences(hip, batch):
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 300, (batch,), generator=g).tolist()
+    n = [min(m, 1) for m in lens]
+    Batch("fp16", n, lens, 3, 1, 64, 16, seed=batch, pad=5).check()
+    n = [min(m, int(x)) for m, x in zip(lens, torch.randint(0, 60, (batch,), generator=g))]
+    Batch("bf16", n, lens, 3, 1, 64, 16, seed=batch).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_without_keys(hip, kind):
+    """More tokens than keys (positions below zero), and scores that are all -inf: zeros."""
+    b = Batch(kind, [4, 2, 150], [2, 0, 100], 4, 2, 64, 16, seed=1)
+    out = torch.full_like(b.q, 7.0)
+    b.attend(out=out)
+    assert torch.all(out[:2] == 0) and torch.all(out[4:6] == 0) and torch.all(out[6:56] == 0)
+    assert torch.all(torch.isfinite(out)) and torch.all(out[2:4].abs().amax(-1) > 0)
+    if kind == "fp16":
+        b = Batch(kind, [1, 1], [20, 20], 4, 2, 64, 32, seed=1)
+        b.k[:] = 60000.0
+        b.q[0] = -60000.0  # every product is -inf in the scores' type times nothing: -2.3e11 each, finite and equal
+        v = b.rows(0)[1].mean(1)
+        got = b.attend()[0].double().view(2, 2, 64)
+        assert torch.allclose(got, v[:, None].expand(2, 2, 64), atol=2e-3)
+        b.k[:] = float("inf")
+        b.q[0] = -1.0  # scores of -inf weigh nothing
+        assert torch.all(b.attend()[0] == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("n,lens", [([1, 1], [40, 70]), ([4, 3], [40, 70]), ([40, 130], [40, 300])])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_what_a_row_does_not_see_stays_out(hip, kind, n, lens, what):
+    """Values of the last token, and of keys before a window, that are not finite reach only the rows that see them."""
+    b = Batch(kind, n, lens, 4, 2, 64, 16, seed=4)
+    for s, m in enumerate(lens):
+        page = b.table[s].long()
+        b.v[page[(m - 1) // 16], :, (m - 1) % 16] = what
+        b.v[page[0], :, 3] = what
+        b.k[page[0], :, 4] = what
+    for kw in (dict(window=30), dict(window=20, cap=5.0)):
+        out = b.attend(**kw)
+        keep = (b.k.clone(), b.v.clone())
+        for s in range(len(n)):  # keys before every window of the call's tokens: cleaned, they change nothing
+            if lens[s] - n[s] - 30 > 5:
+                page = b.table[s].long()
+                b.v[page[0], :, 3] = 0.0
+                b.k[page[0], :, 4] = 0.0
+        assert torch.equal(torch.isnan(out), torch.isnan(b.attend(**kw)))
+        assert torch.equal(out.nan_to_num(5.0), b.attend(**kw).nan_to_num(5.0))
+        b.k, b.v = keep
+    out = b.attend(window=20)
+    at = 0
+    for s, (m, t) in enumerate(zip(lens, n)):
+        pos = torch.arange(m - t, m, device="cuda")
+        sees = (pos == m - 1) | (pos < 3 + 20) & (pos >= 3) | (pos < 4 + 20) & (pos >= 4)
+        fine = torch.isfinite(out[at: at + t]).all(-1).all(-1)
+        assert torch.all(fine[~sees]), "a row that sees only finite keys is not finite"
+        assert not torch.any(fine[(pos == m - 1)])
+        at += t
+    # the rows that see only finite keys are those of the same batch without the others
+    clean = Batch(kind, n, lens, 4, 2, 64, 16, seed=4)
+    want, tol = clean.reference(window=20)
+    at = 0
+    for s, (m, t) in enumerate(zip(lens, n)):
+        pos = torch.arange(m - t, m, device="cuda")
+        far = (pos != m - 1) & (pos >= 4 + 20)
+        x = (out[at: at + t].double() - want[at: at + t]).abs() <= tol[at: at + t]
+        assert torch.all(x[far])
+        at += t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 3, 100])
+def test_pages_outside_the_pool(hip, kind, n):
+    """A page id outside the pool, or a position past the table: NaN for the rows that see it, nobody else."""
+    b = Batch(kind, [n, n], [200, 200], 4, 2, 64, 16, seed=6)
+    fine = b.attend()
+    for bad in (-1, 1 << 30, b.valid.shape[0]):
+        keep = b.table[0, 11].clone()
+        b.table[0, 11] = bad  # positions 176 .. 191
+        out = b.attend()
+        sees = torch.arange(200 - n, 200, device="cuda") >= 176
+        assert torch.all(torch.isnan(out[:n][sees])) and torch.equal(out[:n][~sees], fine[:n][~sees])
+        assert torch.equal(out[n:], fine[n:])
+        assert torch.equal(b.attend(window=8)[n - 1], Batch(kind, [n, n], [200, 200], 4, 2, 64, 16, seed=6)
+                           .attend(window=8)[n - 1])  # the last token's window is past it
+        b.table[0, 11] = keep
+    lens = b.kv_lens.clone()
+    b.kv_lens[0] = 1 << 20  # far past the table
+    out = b.attend()
+    assert torch.all(torch.isnan(out[:n])) and torch.equal(out[n:], fine[n:])
+    b.kv_lens.copy_(lens)
+    assert torch.equal(b.attend(), fine)
+
+
+# -- appending ------------------------------------------------------------------------------------
+def _tables(rows, d):
+    inv = 1.0 / (500000.0 ** (torch.arange(0, d, 2, dtype=torch.float32, device="cuda") / d))
+    ang = torch.arange(rows, dtype=torch.float32, device="cuda")[:, None] * inv
+    return ang.cos(), ang.sin()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,d,page", [(24, 8, 128, 16), (4, 4, 64, 64), (5, 1, 64, 32)])
+@pytest.mark.parametrize("n,lens", [([1], [1]), ([1, 1, 0, 1], [17, 300, 5, 64]), ([70, 3, 0, 129], [70, 40, 9, 400])])
+@pytest.mark.parametrize("turn", [True, False])
+def test_append(hip, kind, heads, kv, d, page, n, lens, turn):
+    from spectra_amd import kernels as K
+    b = Batch(kind, n, lens, heads, kv, d, page, seed=2, pad=2, pages_apart=True)
+    wide = b.rand(b.tokens, (heads + 2 * kv) * d + 16)
+    qkv = wide[:, 8:-8]  # rows inside wider ones
+    cos, sin = _tables(max(lens), d)
+    before = [t.clone() for c in (b.k, b.v) for t in (c if kind == "4bit" else (c,))]
+    q_out = torch.full((b.tokens, heads, d), 7.0, dtype=qkv.dtype, device="cuda")
+    q = K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, cos if turn else None, sin if turn else None, heads,
+                            b.k, b.v, q_out=q_out)
+    assert q is q_out and torch.all(q[sum(n):] == 7.0)
+    after = [t for c in (b.k, b.v) for t in (c if kind == "4bit" else (c,))]
+    # every row of the pool: the appended ones by the contiguous cache's kernels or in 64 bits, the rest as it was
+    at = 0
+    want = [t.clone() for t in before]
+    u = torch.finfo(_DT[kind]).eps / 2
+    for s, (t, m) in enumerate(zip(n, lens)):
+        if t == 0:
+            continue
+        pos = torch.arange(m - t, m, device="cuda")
+        x = qkv[at: at + t].double().view(t, heads + 2 * kv, d)
+        c, sn = (y[pos].double()[:, None] for y in (cos, sin))
+        lo, hi = x[:, :heads + kv].chunk(2, -1)
+        rot = torch.cat([lo * c - hi * sn, hi * c + lo * sn], -1) if turn else x[:, :heads + kv]
+        size = torch.cat([(lo * c).abs() + (hi * sn).abs(), (hi * c).abs() + (lo * sn).abs()], -1)
+        # one rounding to 16 bits of a sum that fp32 holds to 3 roundings of its parts
+        tol = u * rot.abs() + (1 + u) * 3 * 2.0 ** -24 * size + (2.0 ** -25 if kind != "bf16" else 0.0)
+        assert torch.all((q[at: at + t].double() - rot[:, :heads]).abs() <= tol[:, :heads])
+        ids, r = b.table[s][pos // page].long(), pos % page
+        if kind == "bf16":
+            got = after[0][ids, :, r].double()
+            assert torch.all((got - rot[:, heads:]).abs() <= tol[:, heads:])
+            want[0][ids, :, r] = after[0][ids, :, r]
+            want[1][ids, :, r] = x[:, heads + kv:].to(torch.bfloat16)
+        else:  # bit for bit what the contiguous cache gets
+            ones, zeros = torch.ones(m, d // 2, device="cuda"), torch.zeros(m, d // 2, device="cuda")
+            kc, vc = (torch.zeros(kv, m, d, dtype=torch.float16, device="cuda") for _ in range(2))
+            qr = K.rope_append(qkv[at: at + t].contiguous(), pos, cos[:m].contiguous() if turn else ones,
+                               sin[:m].contiguous() if turn else zeros, heads, kv, kc, vc)
+            assert torch.equal(qr, q[at: at + t])
+            new = [kc[:, m - t:], vc[:, m - t:]]
+            if kind == "4bit":
+                new = [y for c4 in new for y in K.kv4_quantize(c4.contiguous())]
+            for w, y in zip(want, new):
+                w[ids, :, r] = y.transpose(0, 1)
+        at += t
+    for w, a in zip(want, after):
+        assert torch.equal(w.view(torch.uint8) if w.is_floating_point() else w, a.contiguous().view(torch.uint8)
+                           if a.is_floating_point() else a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_append_outside(hip, kind):
+    """Tokens without a row to write: page ids outside the pool, positions past the block table, past the rope table
+    (NaN queries) or below zero.  Nothing is written for them; the others go on."""
+    from spectra_amd import kernels as K
+    heads, kv, d = 4, 2, 64
+    b = Batch(kind, [3, 4, 2, 2, 5], [20, 40, 64, 30, 3], heads, kv, d, 16, seed=8)
+    qkv = b.rand(b.tokens, (heads + 2 * kv) * d)
+    cos, sin = _tables(48, d)
+    b.table[0, 1] = -5                     # positions 16 .. 19: sequence 0's tokens are 17 .. 19
+    b.table[1, 2] = b.valid.shape[0]       # positions 32 .. 47: sequence 1's tokens are 36 .. 39
+    parts = lambda: [t for c in (b.k, b.v) for t in (c if kind == "4bit" else (c,))]  # noqa: E731
+    before = [t.clone() for t in parts()]
+    b.kv_lens[2] = 64                      # positions 62, 63: past the rope table of 48
+    q = K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, cos, sin, heads, b.k, b.v)
+    assert torch.all(torch.isfinite(q[:7])) and torch.all(torch.isnan(q[7:9])) and torch.all(torch.isnan(q[11:13]))
+    assert torch.all(torch.isfinite(q[9:11])) and torch.all(torch.isfinite(q[13:]))
+    changed = torch.zeros_like(b.valid)
+    for x, y in zip(before, parts()):
+        same = x.view(torch.uint8) == y.contiguous().view(torch.uint8)
+        changed |= ~same.all(-1).all(1)
+    want = torch.zeros_like(b.valid)
+    want[b.table[3, 1].long(), 28 - 16: 30 - 16] = True
+    want[b.table[4, 0].long(), 0:3] = True
+    assert torch.equal(changed, want)
+    b.kv_lens[3] = 1 << 20                 # past the block table, no rotation: no row either
+    before = [t.clone() for t in parts()]
+    K.paged_rope_append(qkv[9:11], b.kv_lens[3:4], torch.tensor([0, 2], dtype=torch.int32, device="cuda"), b.table[3:4],
+                        None, None, heads, b.k, b.v)
+    for x, y in zip(before, parts()):
+        assert torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
+# -- together, as a serving loop uses them --------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_generation_together(hip, kind):
+    """Prompts in two chunks, then captured single-token steps whose lengths advance on the device: every step against
+    attention in 64 bits over all that was appended, and against the same step run eagerly."""
+    from spectra_amd import kernels as K
+    heads, kv, d, page, steps = 6, 2, 64, 16, 5
+    n0 = [50, 3, 131]
+    batch, most = len(n0), 160
+    b = Batch(kind, n0, [most] * batch, heads, kv, d, page, seed=11)
+    cos, sin = _tables(most, d)
+    ws = K.paged_attend_workspace(d)
+    hist = [[] for _ in n0]  # per sequence: (k rotated, v) rows as stored, 64 bits
+
+    def note(qkv, n, lens):
+        at = 0
+        for s, (t, m) in enumerate(zip(n, lens)):
+            ids, pos = b.table[s], torch.arange(m - t, m, device="cuda")
+            rows = [_values(tuple(y[ids[pos // page].long(), :, pos % page] for y in c) if kind == "4bit"
+                            else c[ids[pos // page].long(), :, pos % page], kind) for c in (b.k, b.v)]
+            hist[s].append(rows)
+            x = qkv[at: at + t].double().view(t, -1, d)[:, heads + kv:]
+            # v as stored: itself, or within half a step of its group (a scale of range / 15, and fp16's roundings)
+            step = (x.unflatten(-1, (-1, 32)).amax(-1) - x.unflatten(-1, (-1, 32)).amin(-1)) / 15
+            bound = (0.51 * step.repeat_interleave(32, -1) + 2.0 ** -9) if kind == "4bit" else 0.0
+            assert torch.all((rows[1] - x).abs() <= bound + (0.5 * step.repeat_interleave(32, -1) if kind == "4bit" else 0))
+            at += t
+
+    def want(q, n):
+        outs, at = [], 0
+        for s, t in enumerate(n):
+            k, v = (torch.cat([r[i] for r in hist[s]]) for i in (0, 1))  # [len, kv, d]
+            m = k.shape[0]
+            see = torch.arange(m, device="cuda")[None] <= torch.arange(m - t, m, device="cuda")[:, None]
+            g = heads // kv
+            x = torch.einsum("thd,mhd->htm", q[at: at + t].double(), k.repeat_interleave(g, 1)) / math.sqrt(d)
+            p = torch.softmax(x.masked_fill(~see, -math.inf), -1)
+            outs.append(torch.einsum("htm,mhd->thd", p, v.repeat_interleave(g, 1)))
+            at += t
+        return torch.cat(outs)
+
+    u = torch.finfo(_DT[kind]).eps / 2
+
+    def step(qkv, lens, starts):
+        q = K.paged_rope_append(qkv, lens, starts, b.table, cos, sin, heads, b.k, b.v)
+        return q, K.paged_attend(q, lens, starts, b.table, b.k, b.v, workspace=ws)
+
+    def close(got, q, n):
+        y = want(q, n)
+        # values of deviation 1: an output's own rounding, and the weights' against a sum of weight times |value| <= 6
+        assert torch.all((got.double() - y).abs() <= u * y.abs() + (u + 2.0 ** -12) * 6)
+
+    lens = [0] * batch
+    for chunk in ([20, 1, 100], [30, 2, 31]):
+        lens = [m + t for m, t in zip(lens, chunk)]
+        starts = torch.tensor([0] + torch.tensor(chunk).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+        qkv = b.rand(sum(chunk), (heads + 2 * kv) * d)
+        q, o = step(qkv, torch.tensor(lens, dtype=torch.int32, device="cuda"), starts)
+        note(qkv, chunk, lens)
+        close(o, q, chunk)
+    ones = torch.arange(batch + 1, dtype=torch.int32, device="cuda")
+    dev_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qkv = b.rand(batch, (heads + 2 * kv) * d)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(qkv, dev_lens + 1, ones)  # warm-up; the capture's first replay writes the same rows again
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dev_lens += 1
+        q, o = step(qkv, dev_lens, ones)
+    for i in range(steps):
+        qkv.copy_(b.rand(batch, (heads + 2 * kv) * d))
+        graph.replay()
+        torch.cuda.synchronize()
+        lens = [m + 1 for m in lens]
+        assert dev_lens.tolist() == lens
+        note(qkv, [1] * batch, lens)
+        close(o, q, [1] * batch)
+        eq, eo = step(qkv, dev_lens, ones)  # eager, between the replays
+        assert torch.equal(eq, q) and torch.equal(eo, o)
+
+
+@pytest.mark.gpu
+def test_against_the_contiguous_kernels(hip):
+    """One sequence: within the two kernels' roundings of attend_decode and attend_prefill on a contiguous cache."""
+    from spectra_amd import kernels as K
+    heads, kv, d, m = 24, 8, 128, 777
+    b = Batch("fp16", [m], [m], heads, kv, d, 64, seed=12)
+    k, v = (x.half().contiguous() for x in b.rows(0))
+    old = K.attend_prefill(b.q, torch.arange(m, device="cuda"), m, k, v)
+    _, tol = b.reference()
+    assert torch.all((b.attend().double() - old.double()).abs() <= 2 * tol)
+    one = Batch("fp16", [1], [m], heads, kv, d, 64, seed=12)
+    kk, vv = (x.half().contiguous() for x in one.rows(0))
+    qkv = torch.cat([one.q.reshape(-1), kk[:, -1].reshape(-1), vv[:, -1].reshape(-1)])
+    old = K.attend_decode(qkv, torch.tensor([m - 1], device="cuda"), None, None, heads, kv, kk, vv)
+    _, tol = one.reference()
+    assert torch.all((one.attend()[0].double() - old.double()).abs() <= 2 * tol[0])
+
+
+@pytest.mark.gpu
+def test_strided_queries_and_streams(hip):
+    """Queries inside wider rows, and calls on another stream than the current default, with a workspace each."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [1, 1, 1, 1], [100, 3000, 64, 7], 8, 2, 64, 32, seed=13)
+    want = b.attend()
+    wide = torch.randn(4, 12, 64, device="cuda").half()
+    wide[:, 2:10] = b.q
+    b.q = wide[:, 2:10]
+    assert torch.equal(b.attend(), want)
+    odd = torch.zeros(4 * 8 * 64 + 4, dtype=torch.float16, device="cuda")[4:].view(4, 8, 64)
+    odd.copy_(wide[:, 2:10])
+    b.q = odd  # 8-byte aligned: copied
+    assert torch.equal(b.attend(), want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [K.paged_attend_workspace(64) for _ in streams]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for s, ws in zip(streams, spaces):
+            with torch.cuda.stream(s):
+                outs.append(b.attend(workspace=ws))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
+def test_empty_calls(hip):
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [0, 0], [5, 9], 4, 2, 64, 16, seed=14)
+    assert b.attend().shape == (0, 4, 64)
+    q = K.paged_rope_append(torch.empty(0, 8 * 64, dtype=torch.float16, device="cuda"), b.kv_lens, b.q_start, b.table,
+                            None, None, 4, b.k, b.v)
+    assert q.shape == (0, 4, 64)
+    b = Batch("fp16", [0, 0], [5, 9], 4, 2, 64, 16, seed=14, pad=3)  # tokens, none of a sequence
+    out = torch.full_like(b.q, 7.0)
+    assert torch.all(b.attend(out=out) == 7.0)
+
+
+@pytest.mark.gpu
+def test_refusals(hip):
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [2, 1], [40, 20], 4, 2, 64, 16, seed=15)
+    good = dict(q=b.q, kv_lens=b.kv_lens, q_start=b.q_start, block_table=b.table, k_pages=b.k, v_pages=b.v)
+
+    def bad(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            K.paged_attend(**{**good, **kw})
+
+    bad("fp16", q=b.q.float())
+    bad("pages of head size", q=b.q.bfloat16())
+    bad("q has head size", q=b.q[..., :32].contiguous())
+    bad("multiple", q=b.q[:, :3])
+    bad("kv_lens", kv_lens=b.kv_lens.long())
+    bad("q_start", q_start=b.q_start.float())
+    bad("block_table", block_table=b.table.t())
+    bad("sequences need", q_start=b.q_start[:2])
+    bad("pages of head size", v_pages=b.v[:-1])
+    bad("contiguous", k_pages=b.k.transpose(1, 2).contiguous().transpose(1, 2))
+    bad("k_pages and v_pages", k_pages=(b.k, b.k), v_pages=(b.v, b.v))
+    bad("power of two", k_pages=b.k[:, :, :8].contiguous(), v_pages=b.v[:, :, :8].contiguous())
+    bad("slopes", slopes=torch.ones(3, device="cuda"))
+    bad("prefix", prefix=torch.ones(2, device="cuda"))
+    bad("cap", cap=-1.0)
+    bad("cap", cap=float("nan"))
+    bad("scale", scale=0.0)
+    bad("window", window=-1)
+    bad("out", out=torch.empty(2, 4, 64, dtype=torch.float16, device="cuda"))
+    with pytest.raises(L.SpectraError) as e:
+        K.paged_attend(**good, workspace=torch.zeros(1024, dtype=torch.uint8, device="cuda"))
+    assert e.value.status == L.ERR_WORKSPACE
+    with pytest.raises(ValueError, match="head sizes"):
+        K.paged_attend_workspace(96)
+    with pytest.raises(L.SpectraError) as e:
+        c = Batch("fp16", [1], [4], 2, 2, 32, 16, seed=15)
+        K.paged_attend(c.q, c.kv_lens, c.q_start, c.table, c.k, c.v, workspace=K.paged_attend_workspace(64))
+    assert e.value.status == L.ERR_UNSUPPORTED
+    rows = torch.zeros(3, 8 * 64, dtype=torch.float16, device="cuda")
+    args = [rows, b.kv_lens, b.q_start, b.table, None, None, 4, b.k, b.v]
+
+    def bad_append(match, at, value):
+        with pytest.raises(ValueError, match=match):
+            K.paged_rope_append(*[value if i == at else x for i, x in enumerate(args)])
+
+    bad_append("rows must hold", 0, rows[:, :-8])
+    bad_append("fp16", 0, rows.float())
+    bad_append("both", 4, torch.ones(40, 32, device="cuda"))
+    bad_append("multiple", 6, 3)
+    with pytest.raises(ValueError, match="cos"):
+        K.paged_rope_append(*args[:4], torch.ones(40, 16, device="cuda"), torch.ones(40, 16, device="cuda"), *args[6:])
+
+
+# -- the C entries' refusals, without a GPU -------------------------------------------------------
+def _desc(**kw):
+    p = L.PagedKv()
+    p.kind, p.kv_heads, p.head_dim, p.page_size, p.num_pages = L.KV_F16, 2, 64, 16, 10
+    p.k, p.v, p.page_stride = 0x10000, 0x20000, 2 * 16 * 64
+    p.batch, p.table_width, p.table_stride = 3, 4, 4
+    p.block_table, p.kv_lens, p.q_start = 0x30000, 0x31000, 0x32000
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+_BAD = [(dict(kind=3), "kind"), (dict(kv_heads=0), "kv_heads"), (dict(kv_heads=3), "multiple"), (dict(head_dim=96), "64 or 128"),
+        (dict(page_size=8), "power of two"), (dict(page_size=48), "power of two"), (dict(num_pages=0), "num_pages"),
+        (dict(batch=0), "batch"), (dict(table_width=0), "table"), (dict(table_stride=3), "stride"), (dict(k=None), "NULL"),
+        (dict(kv_lens=None), "NULL"), (dict(page_stride=100), "page stride"), (dict(k=0x10008), "16-byte"),
+        (dict(page_stride=2 * 16 * 64 + 4), "16-byte"), (dict(kind=L.KV_4BIT), "scales"),
+        (dict(table_width=1 << 28, table_stride=1 << 28), "positions")]
+
+
+@pytest.mark.parametrize("bad,msg", _BAD)
+def test_descriptor_refusals(bad, msg):
+    lib = L.load()
+    p = _desc(**bad)
+    st = lib.spectra_paged_rope_append(ctypes.byref(p), 0x40000, 8 * 64, 5, None, None, 0, 4, 0x50000, None)
+    assert st in (L.ERR_INVALID, L.ERR_UNSUPPORTED) and msg in lib.spectra_last_error().decode()
+    st = lib.spectra_paged_attend(ctypes.byref(p), 0x40000, 4 * 64, 5, 4, 0.125, 0.0, 0, None, None, 0x60000, 1 << 40,
+                                  0x50000, None)
+    assert st in (L.ERR_INVALID, L.ERR_UNSUPPORTED) and msg in lib.spectra_last_error().decode()
+
+
+@pytest.mark.parametrize("change,status,msg", [
+    (dict(q=None), L.ERR_INVALID, "NULL"), (dict(q=0x40008), L.ERR_INVALID, "16-byte"), (dict(ldq=100), L.ERR_INVALID, "stride"),
+    (dict(ldq=4 * 64 + 4), L.ERR_INVALID, "stride"), (dict(tokens=0), L.ERR_INVALID, "tokens"),
+    (dict(tokens=1 << 31), L.ERR_INVALID, "tokens"), (dict(scale=float("nan")), L.ERR_INVALID, "scale"),
+    (dict(cap=float("inf")), L.ERR_INVALID, "cap"), (dict(window=-3), L.ERR_INVALID, "window"),
+    (dict(ws=None), L.ERR_WORKSPACE, "workspace"), (dict(size=1 << 20), L.ERR_WORKSPACE, "workspace"),
+    (dict(ws=0x60008), L.ERR_INVALID, "workspace")])
+def test_attend_refusals(change, status, msg):
+    lib = L.load()
+    a = dict(q=0x40000, ldq=4 * 64, tokens=5, scale=0.125, cap=0.0, window=0, ws=0x60000, size=1 << 40)
+    a.update(change)
+    p = _desc()
+    st = lib.spectra_paged_attend(ctypes.byref(p), a["q"], a["ldq"], a["tokens"], 4, a["scale"], a["cap"], a["window"],
+                                  None, None, a["ws"], a["size"], 0x50000, None)
+    assert st == status and msg in lib.spectra_last_error().decode()
+
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(qkv=None), "NULL"), (dict(ld=8 * 64 - 8), "stride"), (dict(ld=8 * 64 + 4), "16-byte"), (dict(cos=0x70000), "both"),
+    (dict(cos=0x70000, sin=0x80000, rows=0), "rope_rows"), (dict(cos=0x70004, sin=0x80000, rows=9), "16-byte"),
+    (dict(tokens=0), "tokens")])
+def test_append_refusals(change, msg):
+    lib = L.load()
+    a = dict(qkv=0x40000, ld=8 * 64, tokens=5, cos=None, sin=None, rows=0)
+    a.update(change)
+    p = _desc()
+    st = lib.spectra_paged_rope_append(ctypes.byref(p), a["qkv"], a["ld"], a["tokens"], a["cos"], a["sin"], a["rows"], 4,
+                                       0x50000, None)
+    assert st == L.ERR_INVALID and msg in lib.spectra_last_error().decode()
+
+
+def test_descriptor_layout_matches_c(tmp_path):
+    import os
+    import subprocess
+    fields = [f[0] for f in L.PagedKv._fields_]
+    src = '#include <stdio.h>\n#include <stddef.h>\n#include "spectra_hip.h"\nint main(void){\n'
+    src += 'printf("%zu %d\\n", sizeof(spectra_paged_kv_t), SPECTRA_PAGED_COUNTER_BYTES);\n'
+    for f in fields:
+        src += f'printf("%zu\\n", offsetof(spectra_paged_kv_t, {f}));\n'
+    c, exe = tmp_path / "layout.c", tmp_path / "layout"
+    c.write_text(src + "return 0;}\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(c), "-o", str(exe)], check=True)
+    v = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert v[:2] == [ctypes.sizeof(L.PagedKv), L.PAGED_COUNTER_BYTES]
+    for f, off in zip(fields, v[2:]):
+        assert getattr(L.PagedKv, f).offset == off, f
+
+
+def test_wrapper_refuses_host_tensors():
+    from spectra_amd import kernels as K
+    q = torch.zeros(1, 4, 64, dtype=torch.float16)
+    one = torch.ones(1, dtype=torch.int32)
+    pages = torch.zeros(2, 2, 16, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        K.paged_attend(q, one, torch.tensor([0, 1], dtype=torch.int32), one[:, None], pages, pages)
+    with pytest.raises(ValueError, match="GPU"):
+        K.paged_rope_append(torch.zeros(1, 8 * 64, dtype=torch.float16), one, torch.tensor([0, 1], dtype=torch.int32),
+                            one[:, None], None, None, 4, pages, pages)
