@@ -18,7 +18,7 @@ INCLUDE = os.path.join(ROOT, "include")
 OBJDIR = os.path.join(PKG, "_obj")
 LIB = os.path.join(PKG, "libspectra_hip.so")
 TORCH_OPS_LIB = os.path.join(PKG, "_spectra_torch.so")
-TORCH_OPS_SOURCE = "torch_ops.cpp"
+TORCH_OPS_SOURCES = ["torch_ops.cpp", "torch_paged.cpp"]
 SOURCES = ["api.hip", "quant.hip", "dequant.hip", "gemv.hip", "gemv_f16.hip", "gemv_bf16.hip", "gemv_stream_f16.hip", "gemv_stream_bf16.hip", "gemv_rows_plain.hip", "gemv_rows_pro.hip", "gemv_rows_lm.hip", "gemv_rows_multi_f16.hip", "gemv_rows_multi_bf16.hip", "gemm.hip", "mid.hip", "prefill.hip", "skinny.hip", "outliers.hip", "decode.hip", "attend_prefill.hip", "paged_append.hip", "paged_few.hip", "paged_many.hip", "measure.hip"]
 ARCH = "gfx950"
 
@@ -50,7 +50,7 @@ def _compile(src: str) -> str:
 
 
 def build_torch_ops(verbose: bool = True) -> str:
-    """The operator registration (csrc/torch_ops.cpp): host C++ only, compiled with the host
+    """The operator registrations (csrc/torch_ops.cpp, csrc/torch_paged.cpp): host C++ only, compiled with the host
     compiler against the installed torch's headers and linked to libspectra_hip.so, which it
     finds next to itself (rpath $ORIGIN)."""
     import torch
@@ -63,7 +63,7 @@ def build_torch_ops(verbose: bool = True) -> str:
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{tdir}/include", f"-I{tdir}/include/torch/csrc/api/include", f"-I{INCLUDE}", "-I/opt/rocm/include",
-           os.path.join(CSRC, TORCH_OPS_SOURCE),
+           *(os.path.join(CSRC, f) for f in TORCH_OPS_SOURCES),
            f"-L{tdir}/lib", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", f"-L{PKG}", "-lspectra_hip",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tdir}/lib", "-o", tmp]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -18,7 +18,7 @@ computes on the host and there is no fallback path.
 from __future__ import annotations
 
 import ctypes
-import math
+import re
 import weakref
 from collections import OrderedDict
 from typing import List, Optional, Tuple
@@ -736,47 +736,26 @@ def attend_decode_q4(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
 # ---------------------------------------------------------------------------
 # the paged KV cache: a batch of sequences
 # ---------------------------------------------------------------------------
-def _paged_kv(x: torch.Tensor, heads: int, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
-              k_pages, v_pages) -> L.PagedKv:
-    """The checked descriptor of a paged cache and its batch, for activations like ``x``."""
-    dev = x.device
-    quantized = not isinstance(k_pages, torch.Tensor)
-    ks, vs = (tuple(k_pages), tuple(v_pages)) if quantized else ((k_pages,), (v_pages,))
-    if not x.is_cuda or x.dtype not in ((torch.float16,) if quantized else (torch.float16, torch.bfloat16)):
-        raise ValueError("activations must be fp16 (bf16 on bf16 pages) on the GPU")
-    if len(ks) != len(vs) or (quantized and len(ks) != 3) or ks[0].dim() != 4:
-        raise ValueError("k_pages and v_pages must be [pages, kv_heads, page, d], or (codes, scales, zeros) of that")
-    pages, kv, page, d = ks[0].shape
-    d = 2 * d if quantized else d
-    shapes = [(torch.uint8, d // 2), (torch.float16, d // 32), (torch.uint8, d // 32)] if quantized else [(x.dtype, d)]
-    for kt, vt, (dtype, last) in zip(ks, vs, shapes):
-        for t in (kt, vt):
-            if t.dtype != dtype or t.shape != (pages, kv, page, last) or t.device != dev:
-                raise ValueError(f"pages of head size {d} must be {dtype} [{pages}, {kv}, {page}, {last}] on {dev}, got "
-                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
-            if t.stride()[1:] != (page * last, last, 1) or t.stride(0) != kt.stride(0):
-                raise ValueError("a page must be contiguous, and k and v equally far from page to page")
-    if pages == 0:
-        raise ValueError("the pool has no pages")
-    if heads <= 0 or heads % kv:
-        raise ValueError(f"heads ({heads}) must be a multiple of the pages' {kv} KV heads")
-    for t, name, n in ((kv_lens, "kv_lens", 1), (q_start, "q_start", 1), (block_table, "block_table", 2)):
-        if t.dtype != torch.int32 or t.device != dev or t.dim() != n or t.stride(-1) != 1:
-            raise ValueError(f"{name} must be int32 with {n} dimension(s) on {dev}, its rows contiguous")
-    batch = kv_lens.numel()
-    if q_start.numel() != batch + 1 or block_table.shape[0] != batch:
-        raise ValueError(f"{batch} sequences need a q_start of {batch + 1} and a block_table of {batch} rows")
-    p = L.PagedKv()
-    p.kind = L.KV_4BIT if quantized else L.KV_BF16 if x.dtype == torch.bfloat16 else L.KV_F16
-    p.kv_heads, p.head_dim, p.page_size, p.num_pages = kv, d, page, pages
-    p.k, p.v, p.page_stride = ks[0].data_ptr(), vs[0].data_ptr(), ks[0].stride(0)
-    if quantized:
-        p.k_scales, p.v_scales, p.scale_stride = ks[1].data_ptr(), vs[1].data_ptr(), ks[1].stride(0)
-        p.k_zeros, p.v_zeros, p.zero_stride = ks[2].data_ptr(), vs[2].data_ptr(), ks[2].stride(0)
-    p.batch, p.table_width = batch, block_table.shape[1]
-    p.block_table, p.table_stride = block_table.data_ptr(), block_table.stride(0)
-    p.kv_lens, p.q_start = kv_lens.data_ptr(), q_start.data_ptr()
-    return p
+_PAGED_OPS = {}
+
+
+def _paged_op(name: str, *args):
+    """One registered operator over the C entry (csrc/torch_paged.cpp): its checks raise ValueError,
+    the library's other failures SpectraError."""
+    op = _PAGED_OPS.get(name)
+    if op is None:
+        op = _PAGED_OPS[name] = getattr(L.load_torch_ops(), name).default
+    try:
+        return op(*args)
+    except RuntimeError as e:
+        status = re.search(r"(spectra_\w+) failed \((-\d+)\): (.*)", str(e))
+        if status is None:
+            raise
+        raise L.SpectraError(status[1], int(status[2]), status[3]) from None
+
+
+def _pages(p) -> List[torch.Tensor]:
+    return [p] if isinstance(p, torch.Tensor) else list(p)
 
 
 def paged_rope_append(qkv: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
@@ -795,31 +774,12 @@ def paged_rope_append(qkv: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.T
     the device.  ``cos`` / ``sin`` fp32 [rows, d/2], or None for no rotation.  A token past the
     rope table, the block table or on a page id outside the pool appends nothing (past the rope
     table its queries are NaN); rows behind q_start[-1] are left alone."""
-    if qkv.dim() != 2:
-        raise ValueError("qkv must be [T, (heads + 2 kv) * d]")
-    p = _paged_kv(qkv, heads, kv_lens, q_start, block_table, k_pages, v_pages)
-    T, d = qkv.shape[0], p.head_dim
-    if qkv.shape[1] != (heads + 2 * p.kv_heads) * d:
-        raise ValueError(f"qkv rows must hold (heads + 2 kv) * d = {(heads + 2 * p.kv_heads) * d} values")
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin must both be given or both be None")
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or
-                              t.shape[1] != d // 2 or t.shape != cos.shape or t.device != qkv.device):
-            raise ValueError(f"{name} must be contiguous fp32 [rows, d/2] on {qkv.device}")
-    qkv, ld = _rows(qkv, "qkv", 16)
+    if not qkv.is_cuda:
+        raise ValueError("qkv must be on the GPU")
+    args = (qkv, kv_lens, q_start, block_table, cos, sin, heads, _pages(k_pages), _pages(v_pages))
     if q_out is None:
-        q_out = torch.empty((T, heads, d), device=qkv.device, dtype=qkv.dtype)
-    elif q_out.dtype != qkv.dtype or q_out.shape != (T, heads, d) or not q_out.is_contiguous() or q_out.device != qkv.device:
-        raise ValueError(f"q_out must be contiguous {qkv.dtype} [{T}, {heads}, {d}] on {qkv.device}")
-    if T == 0:
-        return q_out
-    lib = L.load()
-    with torch.cuda.device(qkv.device):
-        L.check("spectra_paged_rope_append", lib.spectra_paged_rope_append(
-            ctypes.byref(p), qkv.data_ptr(), ld, T, cos.data_ptr() if cos is not None else None,
-            sin.data_ptr() if sin is not None else None, cos.shape[0] if cos is not None else 0, heads, q_out.data_ptr(),
-            _stream(qkv.device)))
+        return _paged_op("paged_rope_append", *args)
+    _paged_op("paged_rope_append_out", *args, q_out)
     return q_out
 
 
@@ -851,32 +811,13 @@ def paged_attend(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
     is zero; one that would need a page outside the pool or past the table is NaN; rows behind
     q_start[-1] are left alone.  ``workspace``: ``paged_attend_workspace(d)``; by default a fresh
     one, which costs a small kernel."""
-    if q.dim() != 3:
-        raise ValueError("q must be [T, heads, d]")
-    T, heads, d = q.shape
-    p = _paged_kv(q, heads, kv_lens, q_start, block_table, k_pages, v_pages)
-    if d != p.head_dim:
-        raise ValueError(f"q has head size {d}, the pages {p.head_dim}")
-    if q.stride(2) != 1 or q.stride(1) != d or q.data_ptr() % 16 or (T > 1 and (q.stride(0) % 8 or q.stride(0) < heads * d)):
-        q = q.clone(memory_format=torch.contiguous_format)
-    for t, name, dtype, n in ((slopes, "slopes", torch.float32, heads), (prefix, "prefix", torch.int32, p.batch)):
-        if t is not None and (t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or t.device != q.device):
-            raise ValueError(f"{name} must be contiguous {dtype} [{n}] on {q.device}")
-    if workspace is None:
-        workspace = paged_attend_workspace(d, q.device)
-    elif workspace.device != q.device or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous on {q.device}")
+    if not q.is_cuda:
+        raise ValueError("q must be on the GPU")
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    args = (q, kv_lens, q_start, block_table, _pages(k_pages), _pages(v_pages), scale, cap, window, slopes, prefix,
+            workspace)
     if out is None:
-        out = torch.empty((T, heads, d), device=q.device, dtype=q.dtype)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
-        raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)} on {q.device}")
-    if T == 0:
-        return out
-    lib = L.load()
-    with torch.cuda.device(q.device):
-        L.check("spectra_paged_attend", lib.spectra_paged_attend(
-            ctypes.byref(p), q.data_ptr(), q.stride(0) if T > 1 else heads * d, T, heads,
-            1.0 / math.sqrt(d) if scale is None else float(scale), float(cap), int(window),
-            slopes.data_ptr() if slopes is not None else None, prefix.data_ptr() if prefix is not None else None,
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), out.data_ptr(), _stream(q.device)))
+        return _paged_op("paged_attend", *args)
+    _paged_op("paged_attend_out", *args, out)
     return out
