@@ -141,39 +141,64 @@ __device__ __forceinline__ bool paged_arrive(uint32_t* counter, int pieces, int*
   return *flag != 0;
 }
 
+// The running maximum lags: sums are rescaled only where a score passes the maximum they refer to by
+// kPagedSlack (so hardly ever after the first steps), and weights are 2^(score - maximum +
+// kPagedRaise), at most 2^15: inside fp16's range, with its subnormals 2^-21 below the largest.
+constexpr float kPagedSlack = 8.0f, kPagedRaise = 7.0f;
+
+// The factor that brings sums of maximum m and total l to the maximum mm.  Without keys (-inf and
+// 0): 0; a total of NaN (NaN scores do not show in a maximum): 1.
+__device__ __forceinline__ float paged_weight(float m, float l, float mm) {
+  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - mm);
+}
+
+// A piece's record in the workspace: [rows][HD] sums of weight times value, [rows] (maximum, total).
+template <int HD>
+__host__ __device__ constexpr int paged_slot(int rows) {
+  return rows * (HD + 2);
+}
+__device__ __forceinline__ void store_dev2(float* p, float x, float y) {
+  __hip_atomic_store((uint64_t*)p, (uint64_t)__builtin_bit_cast(uint32_t, x) | (uint64_t)__builtin_bit_cast(uint32_t, y) << 32,
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_dev2(const float* p) {
+  const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
+}
+
 // A row's pieces joined (in their order, whatever order they arrived in): dims d .. d + 3 of the sum
-// of weight times value, and the sum of weights.  A piece's record: [rows][HD + 2], the row's sums,
-// their maximum and the sum of weights; an empty piece has maximum -inf and sum 0 (a NaN sum
-// beside it is a NaN score's).
+// of weight times value, and the total.
 template <int HD, int ROWS>
 __device__ __forceinline__ float paged_join(const float* base, int pieces, int row, int d, float (&v)[4]) {
+  constexpr int U = 4;  // pieces in flight
   float mm = -INFINITY, den = 0.0f;
   v[0] = v[1] = v[2] = v[3] = 0.0f;
-  for (int p0 = 0; p0 < pieces; p0 += 8) {
-    float pm[8], pl[8], x[8][4];
+  for (int p0 = 0; p0 < pieces; p0 += U) {
+    float2 ml[U], x[U][2];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float* p = base + ((int64_t)min(p0 + u, pieces - 1) * ROWS + row) * (HD + 2);
-      pm[u] = load_dev(p + HD);
-      pl[u] = load_dev(p + HD + 1);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[u][e] = load_dev(p + d + e);
+    for (int u = 0; u < U; ++u) {
+      const float* p = base + (int64_t)min(p0 + u, pieces - 1) * paged_slot<HD>(ROWS);
+      ml[u] = load_dev2(p + ROWS * HD + 2 * row);
+      x[u][0] = load_dev2(p + row * HD + d);
+      x[u][1] = load_dev2(p + row * HD + d + 2);
     }
     float mn = mm;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) mn = fmaxf(mn, pm[u]);
-    const float corr = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mm - mn);
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+    const float corr = paged_weight(mm, den, mn);
     den *= corr;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= corr;
     mm = mn;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (p0 + u >= pieces) continue;
-      const float f = pm[u] == -INFINITY ? (pl[u] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(pm[u] - mm);
-      den += f * pl[u];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += f * x[u][e];
+      const float f = paged_weight(ml[u].x, ml[u].y, mm);
+      den += f * ml[u].y;
+      v[0] += f * x[u][0].x;
+      v[1] += f * x[u][0].y;
+      v[2] += f * x[u][1].x;
+      v[3] += f * x[u][1].y;
     }
   }
   return den;
@@ -195,8 +220,8 @@ struct PagedLaunch {
 // Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows.
 constexpr int kFewTarget = 1024, kFewSlots = 2 * kFewTarget, kFewKeys = 128;
 int launch_paged_few(const PagedLaunch& a, int rows);
-// Many rows a sequence (prompts): tiles of 128 rows.
-constexpr int kManyRows = 128, kManyKeys = 64, kManyMinSteps = 8, kManyTarget = 256, kManySlots = 2 * kManyTarget;
-int launch_paged_many(const PagedLaunch& a);
+// Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.
+constexpr int kManyBig = 384, kManyKeys = 64, kManyMinSteps = 8, kManyTarget = 256, kManySlots = 2 * kManyTarget;
+int launch_paged_many(const PagedLaunch& a, int rows);
 
 }  // namespace spectra

@@ -196,9 +196,8 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       for (int e = 0; e < 8; ++e) mn = fmaxf(mn, x[e]);
       mn = fmaxf(mn, lane_xor<16>(mn, lane));
       mn = fmaxf(mn, lane_xor<32>(mn, lane));
-      const float mu = mn == -INFINITY ? 0.0f : mn;
-      if (__ballot(mn > m[nt]) != 0) {
-        const float corr = __builtin_amdgcn_exp2f(m[nt] - mu);
+      if (__ballot(mn > m[nt] + kPagedSlack) != 0) {
+        const float corr = __builtin_amdgcn_exp2f(m[nt] - (mn == -INFINITY ? 0.0f : mn));
         l[nt] *= corr;
 #pragma unroll
         for (int j = 0; j < DPL; ++j)
@@ -206,6 +205,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
           for (int i = 0; i < 4; ++i) o[nt][j][i] *= corr;
         m[nt] = mn;
       }
+      const float mu = m[nt] == -INFINITY ? 0.0f : m[nt] - kPagedRaise;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[e] = __builtin_amdgcn_exp2f(x[e] - mu);
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   }
   if (tid == 0) redo = 0;
   const bool mixed = tok1 > tok0;  // rows that see different keys
-  float* part = slots + (int64_t)un.slot * ROWS * (HD + 2);
+  float* part = slots + (int64_t)un.slot * paged_slot<HD>(ROWS);
   auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
     const int r = r0 + row, tok = r / g, head = un.kvh * g + (r - tok * g);
     const bool past = paged_range(i0 + tok, sq.len, un.prefix, sc.window).hi > capacity;
@@ -332,8 +332,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       for (int w = 0; w < 4; ++w) mm = fmaxf(mm, wm[w][row]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        // (a wave without keys for the row: weight 0, also where the others' maximum is NaN's -inf)
-        const float f = wm[w][row] == -INFINITY ? (wl[w][row] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(wm[w][row] - mm);
+        const float f = paged_weight(wm[w][row], wl[w][row], mm);
         const float4 x = *(const float4*)(red + (w * 16 + r) * RS + d);
         den += f * wl[w][row];
         v[0] += f * x.x;
@@ -344,13 +343,9 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       if (un.pieces == 1) {
         write(row, d, v, den);
       } else {
-        float* p = part + (int64_t)row * (HD + 2);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) store_dev(p + d + e, v[e]);
-        if (d == 0) {
-          store_dev(p + HD, mm);
-          store_dev(p + HD + 1, den);
-        }
+        store_dev2(part + row * HD + d, v[0], v[1]);
+        store_dev2(part + row * HD + d + 2, v[2], v[3]);
+        if (d == 0) store_dev2(part + ROWS * HD + 2 * row, mm, den);
       }
     }
   }
@@ -358,7 +353,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
     const int first = un.slot - un.piece;
     if (!paged_arrive(counters + first, un.pieces, &flag)) return;
     // the last to arrive joins the pieces, in their order
-    const float* base = slots + (int64_t)first * ROWS * (HD + 2);
+    const float* base = slots + (int64_t)first * paged_slot<HD>(ROWS);
     for (int it = tid; it < nrows * (HD / 4); it += kFewThreads) {
       const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
       float v[4];

@@ -24,22 +24,24 @@ constexpr int many_lds() {
   return 2 * (kManyKeys * HD * 2 + HD * kManyVRow);
 }
 
-template <int HD, int KIND, bool MOD>
+template <int HD, int KIND, bool MOD, int QH>
 __global__ void __launch_bounds__(kManyThreads, 2)
     paged_many_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                       uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
   constexpr int CH = HD / 8, KS = HD / 16, DT = HD / 32;  // 8-dim chunks, 16-dim steps, 32-dim tiles
   constexpr int KL = kManyKeys * CH / kManyThreads;       // K chunks a thread copies
+  constexpr int ROWS = 32 * QH, TL = QH / 2;              // 32-key tiles of a step that a wave takes
   constexpr int ROWB = Q4 ? HD / 2 : 2 * HD, KBYTES = kManyKeys * HD * 2;
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int flag;
-  __shared__ uint32_t redo[4];
+  __shared__ uint32_t redo[QH];
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), gh = lane >> 5, ln = lane & 31;
+  const int qh = wave % QH, kh = wave / QH;  // the wave's 32 rows, and its share of a step's keys
   PagedUnit un;
-  if (!paged_unit(kv, g, kManyRows, kManyKeys, kManyMinSteps, kManyTarget, kManySlots, sc, blockIdx.x, lane, un)) return;
+  if (!paged_unit(kv, g, ROWS, kManyKeys, kManyMinSteps, kManyTarget, kManySlots, sc, blockIdx.x, lane, un)) return;
   const PagedSeq sq = un.seq;
-  const int r0 = un.tile * kManyRows, nrows = min(kManyRows, sq.n * g - r0);
+  const int r0 = un.tile * ROWS, nrows = min(ROWS, sq.n * g - r0);
   const int tok0 = sread(r0 / g), tok1 = sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;
   const int capacity = kv.table_width << kv.page_shift, pmask = (1 << kv.page_shift) - 1;
   // keys that some row of the tile sees
@@ -50,12 +52,12 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   const int sbeg = sread((int)((int64_t)steps * un.piece / un.pieces));
   const int send = sread((int)((int64_t)steps * (un.piece + 1) / un.pieces));
   // this wave's rows: keys that some see, and those that all do; the lane's row
-  const int wr0 = min(32 * wave, nrows - 1), wr1 = min(32 * wave + 31, nrows - 1);
+  const int wr0 = min(32 * qh, nrows - 1), wr1 = min(32 * qh + 31, nrows - 1);
   const PagedRange wa = paged_range(i0 + (r0 + wr0) / g, sq.len, un.prefix, sc.window);
   const PagedRange wb = paged_range(i0 + (r0 + wr1) / g, sq.len, un.prefix, sc.window);
   const int wlo = wa.lo, whi = min(wb.hi, capacity), alo = wb.lo, ahi = min(wa.hi, capacity);
-  const bool live = 32 * wave < nrows, ok = 32 * wave + ln < nrows;
-  const int rr = r0 + min(32 * wave + ln, nrows - 1), tok = rr / g, head = un.kvh * g + (rr - tok * g);
+  const bool live = 32 * qh < nrows, ok = 32 * qh + ln < nrows;
+  const int rr = r0 + min(32 * qh + ln, nrows - 1), tok = rr / g, head = un.kvh * g + (rr - tok * g);
   const PagedRange rg = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
   const float slope2 = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
   const float fpos = (float)(i0 + tok - 4 * gh);
@@ -71,62 +73,56 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     }
   }
 
-  // ---- staging: a step is 4 blocks of 16 keys, each in one page.  K chunk i of a thread: block
-  // i (HD 128) or 2 i + wave / 2, key tid / CH % 16 of it.  V: a wave's block, 4 keys x 8 dims a lane.
+  // ---- staging: a step is 4 blocks of 16 keys, each in one page; a wave copies one block, so it
+  // needs one page id a step.  K: 16-byte chunk kc of the rows krow + i (64 / CH); V: 4 keys x 8 dims.
   const int* tab = kv.table + un.b * kv.table_stride;
-  struct Ids {
-    int p[4];
+  auto page_of = [&](int k0) __attribute__((always_inline)) {
+    return sread(sload(tab + min((k0 + 16 * wave) >> kv.page_shift, kv.table_width - 1)));
   };
-  auto ids_of = [&](int k0) __attribute__((always_inline)) {
-    Ids r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.p[i] = sread(sload(tab + min((k0 + 16 * i) >> kv.page_shift, kv.table_width - 1)));
-    return r;
-  };
-  const int kc = tid % CH, krow = (tid / CH) & 15, vq = lane & 3, vo = (lane >> 2) % CH;
-  const bool vlane = lane < 4 * CH;  // (head_dim 64: half the lanes have no piece, and load another's)
+  const int kc = lane % CH, krow = lane / CH, vq = lane & 3, vo = (lane >> 2) % CH;
+  const bool vlane = lane < 4 * CH;  // (head_dim 64: half the lanes have no piece of V, and load another's)
   struct Stage {
     pu4_t k[Q4 ? 1 : KL], v[Q4 ? 1 : 4];
     uint32_t kw[KL], ks[KL], kz[KL], vw[4], vs[4], vz[4];  // 4-bit: codes, scales, zero points
+    bool bad;
   } st;
-  auto load = [&](int k0, const Ids& id) __attribute__((always_inline)) {
+  auto load = [&](int k0, int id) __attribute__((always_inline)) {
+    st.bad = (uint32_t)id >= (uint32_t)kv.num_pages;
+    const int64_t pg = st.bad ? 0 : id;
+    const int row = (un.kvh << kv.page_shift) + ((k0 + 16 * wave) & pmask);
+    const int64_t at = pg * kv.page_bytes + row * ROWB;
+    const uint8_t *kb = kv.k + at, *vb = kv.v + at;
+    const int64_t so = Q4 ? pg * kv.scale_step + row * (HD / 32) : 0, zo = Q4 ? pg * kv.zero_step + row * (HD / 32) : 0;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
-      const int blk = CH == 16 ? i : 2 * i + (wave >> 1);
-      const int id1 = CH == 16 ? id.p[i] : (wave >> 1) ? id.p[(2 * i + 1) & 3] : id.p[(2 * i) & 3];
-      const int64_t pg = (uint32_t)id1 < (uint32_t)kv.num_pages ? id1 : 0;
-      const int64_t row = ((int64_t)un.kvh << kv.page_shift) + ((k0 + 16 * blk) & pmask);
-      const uint8_t* kb = kv.k + pg * kv.page_bytes + row * ROWB;
+      const int r = krow + i * (64 / CH);
       if constexpr (Q4) {
-        st.kw[i] = load_at<uint32_t>(kb, krow * ROWB + 4 * kc);
-        st.ks[i] = load_at<uint16_t>(kv.ks + pg * kv.scale_step + row * (HD / 32), 2 * (krow * (HD / 32) + kc / 4));
-        st.kz[i] = load_at<uint8_t>(kv.kz + pg * kv.zero_step + row * (HD / 32), krow * (HD / 32) + kc / 4);
+        st.kw[i] = load_at<uint32_t>(kb, r * ROWB + 4 * kc);
+        st.ks[i] = load_at<uint16_t>(kv.ks + so, 2 * (r * (HD / 32) + kc / 4));
+        st.kz[i] = load_at<uint8_t>(kv.kz + zo, r * (HD / 32) + kc / 4);
       } else {
-        st.k[i] = __builtin_bit_cast(pu4_t, load_at<uint4>(kb, krow * ROWB + 16 * kc));
+        st.k[i] = __builtin_bit_cast(pu4_t, load_at<uint4>(kb, r * ROWB + 16 * kc));
       }
     }
-    const int id1 = wave == 0 ? id.p[0] : wave == 1 ? id.p[1] : wave == 2 ? id.p[2] : id.p[3];
-    const int64_t pg = (uint32_t)id1 < (uint32_t)kv.num_pages ? id1 : 0;
-    const int64_t row = ((int64_t)un.kvh << kv.page_shift) + ((k0 + 16 * wave) & pmask);
-    const uint8_t* vb = kv.v + pg * kv.page_bytes + row * ROWB;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int vr = 4 * vq + j;
+      const int r = 4 * vq + j;
       if constexpr (Q4) {
-        st.vw[j] = load_at<uint32_t>(vb, vr * ROWB + 4 * vo);
-        st.vs[j] = load_at<uint16_t>(kv.vs + pg * kv.scale_step + row * (HD / 32), 2 * (vr * (HD / 32) + vo / 4));
-        st.vz[j] = load_at<uint8_t>(kv.vz + pg * kv.zero_step + row * (HD / 32), vr * (HD / 32) + vo / 4);
+        st.vw[j] = load_at<uint32_t>(vb, r * ROWB + 4 * vo);
+        st.vs[j] = load_at<uint16_t>(kv.vs + so, 2 * (r * (HD / 32) + vo / 4));
+        st.vz[j] = load_at<uint8_t>(kv.vz + zo, r * (HD / 32) + vo / 4);
       } else {
-        st.v[j] = __builtin_bit_cast(pu4_t, load_at<uint4>(vb, vr * ROWB + 16 * vo));
+        st.v[j] = __builtin_bit_cast(pu4_t, load_at<uint4>(vb, r * ROWB + 16 * vo));
       }
     }
   };
+  constexpr uint32_t nan2 = BF ? 0x7fc07fc0u : 0x7e007e00u;
   auto store = [&](int k0, uint8_t* buf) __attribute__((always_inline)) {
     uint8_t* ks = buf;
     uint8_t* vs = buf + KBYTES;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
-      const int key = 16 * (CH == 16 ? i : 2 * i + (wave >> 1)) + krow;
+      const int key = 16 * wave + krow + i * (64 / CH);
       pu4_t x;
       if constexpr (Q4) {
         const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0xe400u | st.kz[i]));
@@ -135,24 +131,17 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       } else {
         x = st.k[i];
       }
+      if (st.bad) x = (pu4_t){nan2, nan2, nan2, nan2};  // no such page: scores of NaN
       *(pu4_t*)(ks + key * (HD * 2) + 16 * (kc ^ (key & (CH - 1)))) = x;
     }
     if (vlane) {
       const int kq = 16 * wave + 4 * vq;
-      uint32_t keep[2] = {~0u, ~0u};
-      if (k0 < klo || k0 + kManyKeys > khi) {  // keys that no row sees: their values must not reach the product
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int key = k0 + kq + 2 * p;
-          keep[p] = (key >= klo && key < khi ? 0xffffu : 0u) | (key + 1 >= klo && key + 1 < khi ? 0xffff0000u : 0u);
-        }
-      }
       uint32_t w[2][8];  // pair of keys, dim
       if constexpr (Q4) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const uint32_t z2 = st.vz[2 * p] | (st.vz[2 * p + 1] << 16) | 0xe400e400u;
-          const uint32_t s2 = (st.vs[2 * p] | (st.vs[2 * p + 1] << 16)) & keep[p];
+          const uint32_t s2 = st.vs[2 * p] | (st.vs[2 * p + 1] << 16);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const pu4_t x = kv4_pairs(__builtin_amdgcn_perm(st.vw[2 * p + 1], st.vw[2 * p], u ? 0x07060302u : 0x05040100u),
@@ -166,7 +155,16 @@ __global__ void __launch_bounds__(kManyThreads, 2)
         for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            w[p][e] = __builtin_amdgcn_perm(st.v[2 * p + 1][e >> 1], st.v[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u) & keep[p];
+            w[p][e] = __builtin_amdgcn_perm(st.v[2 * p + 1][e >> 1], st.v[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+      }
+      if (k0 < klo || k0 + kManyKeys > khi) {  // keys that no row sees: their values must not reach the product
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int key = k0 + kq + 2 * p;
+          const uint32_t keep = (key >= klo && key < khi ? 0xffffu : 0u) | (key + 1 >= klo && key + 1 < khi ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[p][e] &= keep;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) *(uint2*)(vs + (8 * vo + e) * kManyVRow + 2 * kq) = make_uint2(w[0][e], w[1][e]);
@@ -179,53 +177,49 @@ __global__ void __launch_bounds__(kManyThreads, 2)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  auto compute = [&](int k0, const uint8_t* buf, const Ids& id) __attribute__((always_inline)) {
-    if (!live || k0 >= whi || k0 + kManyKeys <= wlo) return;
+  auto compute = [&](int k0, const uint8_t* buf) __attribute__((always_inline)) {
+    const int kw = k0 + 32 * TL * kh;  // this wave's keys
+    if (!live || kw >= whi || kw + 32 * TL <= wlo) return;
     const uint8_t* ks = buf;
     const uint8_t* vs = buf + KBYTES;
-    pf16_t s[2];
+    pf16_t s[TL];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TL; ++t) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
-      const int key = 32 * t + ln;
+      const int key = 32 * (TL * kh + t) + ln;
 #pragma unroll
       for (int st = 0; st < KS; ++st)
         s[t] = mfma32<BF>(*(const pu4_t*)(ks + key * (HD * 2) + 16 * ((2 * st + gh) ^ (key & (CH - 1)))), qf[st], s[t]);
     }
-    // score r of tile t: key k0 + 32 t + 8 (r / 4) + 4 gh + r % 4
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (uint32_t)id.p[i] >= (uint32_t)kv.num_pages ? 1u << i : 0u;
+    // score r of tile t: key kw + 32 t + 8 (r / 4) + 4 gh + r % 4
     if constexpr (MOD) {
-      const float base = fpos - (float)k0;
+      const float base = fpos - (float)kw;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TL; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[t][r] = paged_score<true>(s[t][r], sc, slope2, base - (float)(32 * t + 8 * (r >> 2) + (r & 3)));
     }
-    if (k0 < alo || k0 + kManyKeys > ahi || bad != 0) {
+    if (kw < alo || kw + 32 * TL > ahi) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TL; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * t + 8 * (r >> 2) + 4 * gh + (r & 3);
-          if ((bad >> (2 * t + (r >> 3))) & 1) s[t][r] = NAN;
+          const int key = kw + 32 * t + 8 * (r >> 2) + 4 * gh + (r & 3);
           if (key < rg.lo || key >= min(rg.hi, capacity)) s[t][r] = -INFINITY;
         }
     }
     const float mul = MOD ? 1.0f : sc.mul;
     float mn = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < TL; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mn = fmaxf(mn, s[t][r]);
     mn = fmaxf(mn, lane_xor<32>(mn, lane)) * mul;
-    mn = fmaxf(m, mn);
-    const float mu = mn == -INFINITY ? 0.0f : mn;
-    if (__ballot(mn > m) != 0) {
-      const float corr = __builtin_amdgcn_exp2f(m - mu);
+    if (__ballot(mn > m + kPagedSlack) != 0) {
+      mn = fmaxf(m, mn);
+      const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
       l *= corr;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -233,9 +227,10 @@ __global__ void __launch_bounds__(kManyThreads, 2)
         for (int r = 0; r < 16; ++r) o[d][r] *= corr;
       m = mn;
     }
-    pu4_t pf[2][2];
+    const float mu = m == -INFINITY ? 0.0f : m - kPagedRaise;
+    pu4_t pf[TL][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < TL; ++t)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], mul, -mu));
@@ -246,9 +241,9 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     // O^T += V^T P^T: step (t, u) contracts keys 32 t + 16 u + {4 gh + 0 .. 3, 8 + 4 gh + 0 .. 3}
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const uint8_t* vrow = vs + (32 * d + ln) * kManyVRow + 8 * gh;
+      const uint8_t* vrow = vs + (32 * d + ln) * kManyVRow + 64 * TL * kh + 8 * gh;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TL; ++t)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const uint2 a = *(const uint2*)(vrow + 2 * (32 * t + 16 * u)), b = *(const uint2*)(vrow + 2 * (32 * t + 16 * u + 8));
@@ -258,34 +253,73 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   };
 
   if (sbeg < send) {
+    constexpr int BUF = many_lds<HD>() / 2;
     int k0 = kbeg + sbeg * kManyKeys;
     const int kend = kbeg + send * kManyKeys;
-    Ids id = ids_of(k0), next = ids_of(k0 + kManyKeys);
-    load(k0, id);
+    load(k0, page_of(k0));
+    int next = page_of(k0 + kManyKeys);
     store(k0, lds);
     __syncthreads();
-    for (int b = 0;; b ^= 1) {
-      const bool more = k0 + kManyKeys < kend;
+    while (true) {  // (two steps a turn: the buffers' addresses are constants)
+      bool more = k0 + kManyKeys < kend;
       if (more) load(k0 + kManyKeys, next);
-      const Ids after = ids_of(k0 + 2 * kManyKeys);
-      compute(k0, lds + b * (many_lds<HD>() / 2), id);
+      next = page_of(k0 + 2 * kManyKeys);
+      compute(k0, lds);
       if (!more) break;
       k0 += kManyKeys;
-      store(k0, lds + (b ^ 1) * (many_lds<HD>() / 2));
+      store(k0, lds + BUF);
       __syncthreads();
-      id = next;
-      next = after;
+      more = k0 + kManyKeys < kend;
+      if (more) load(k0 + kManyKeys, next);
+      next = page_of(k0 + 2 * kManyKeys);
+      compute(k0, lds + BUF);
+      if (!more) break;
+      k0 += kManyKeys;
+      store(k0, lds);
+      __syncthreads();
     }
   }
 
   l += lane_xor<32>(l, lane);
+  if constexpr (QH == 2) {  // the key halves meet
+    float4* red = (float4*)lds;  // [query half][4 DT][lane]
+    float2* ml = (float2*)(lds + 2 * 16 * DT * 64 * 4);
+    static_assert(2 * 16 * DT * 64 * 4 + 2 * 64 * 8 <= many_lds<HD>(), "a half's sums fit the buffers");
+    __syncthreads();
+    if (kh == 1) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          red[(qh * 4 * DT + 4 * d + r) * 64 + lane] = make_float4(o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
+      ml[qh * 64 + lane] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (kh == 0) {
+      const float2 x = ml[qh * 64 + lane];
+      const float mm = fmaxf(m, x.x);
+      const float c0 = paged_weight(m, l, mm), c1 = paged_weight(x.x, x.y, mm);
+      l = l * c0 + x.y * c1;
+      m = mm;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float4 y = red[(qh * 4 * DT + 4 * d + r) * 64 + lane];
+          o[d][4 * r] = o[d][4 * r] * c0 + y.x * c1;
+          o[d][4 * r + 1] = o[d][4 * r + 1] * c0 + y.y * c1;
+          o[d][4 * r + 2] = o[d][4 * r + 2] * c0 + y.z * c1;
+          o[d][4 * r + 3] = o[d][4 * r + 3] * c0 + y.w * c1;
+        }
+    }
+  }
   const bool mixed = tok1 > tok0;  // rows that see different keys
   uint32_t again = 0;              // this wave's rows to be done over
   if (un.pieces == 1) {
     const bool past = rg.hi > capacity;
     const float inv = past ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
     bool odd = false;
-    if (ok) {
+    if (ok && kh == 0) {
       uint16_t* orow = out + ((int64_t)(sq.q0 + tok) * heads + head) * HD;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -304,24 +338,25 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     again = (uint32_t)(b | (b >> 32));
   } else {
     const int first = un.slot - un.piece;
-    if (tid < 4) redo[tid] = 0;
-    if (ok) {
-      float* p = slots + ((int64_t)un.slot * kManyRows + 32 * wave + ln) * (HD + 2);
+    if (tid < QH) redo[tid] = 0;
+    if (ok && kh == 0) {
+      float* p = slots + (int64_t)un.slot * paged_slot<HD>(ROWS);
+      float* row = p + (32 * qh + ln) * HD;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) store_dev(p + 32 * d + 8 * (r >> 2) + 4 * gh + (r & 3), o[d][r]);
-      if (gh == 0) {
-        store_dev(p + HD, m);
-        store_dev(p + HD + 1, l);
-      }
+        for (int r = 0; r < 4; ++r) {
+          store_dev2(row + 32 * d + 8 * r + 4 * gh, o[d][4 * r], o[d][4 * r + 1]);
+          store_dev2(row + 32 * d + 8 * r + 4 * gh + 2, o[d][4 * r + 2], o[d][4 * r + 3]);
+        }
+      if (gh == 0) store_dev2(p + ROWS * HD + 2 * (32 * qh + ln), m, l);
     }
     if (!paged_arrive(counters + first, un.pieces, &flag)) return;
-    const float* base = slots + (int64_t)first * kManyRows * (HD + 2);
+    const float* base = slots + (int64_t)first * paged_slot<HD>(ROWS);
     for (int it = tid; it < nrows * (HD / 4); it += kManyThreads) {
       const int row = it / (HD / 4), d = 4 * (it % (HD / 4)), r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g);
       float v[4], y[4];
-      const float den = paged_join<HD, kManyRows>(base, un.pieces, row, d, v);
+      const float den = paged_join<HD, ROWS>(base, un.pieces, row, d, v);
       const bool past = paged_range(i0 + t, sq.len, un.prefix, sc.window).hi > capacity;
       bool odd = false;
 #pragma unroll
@@ -333,29 +368,36 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       *(uint2*)(out + ((int64_t)(sq.q0 + t) * heads + h) * HD + d) = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
     }
     __syncthreads();
-    again = redo[wave];
+    again = kh == 0 ? redo[qh] : 0;
   }
   if (!mixed) return;
   for (uint32_t r = sread(again); r != 0; r &= r - 1)
-    paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + 32 * wave + __builtin_ctz(r), out);
+    paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + 32 * qh + __builtin_ctz(r), out);
 }
 
-template <int HD, int KIND, bool MOD>
+template <int HD, int KIND, bool MOD, int QH>
 static int launch_many(const PagedLaunch& a) {
-  const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD>;
+  const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD, QH>;
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
-  paged_many_kernel<HD, KIND, MOD><<<dim3((unsigned)a.units), dim3(kManyThreads), many_lds<HD>(), a.stream>>>(
+  paged_many_kernel<HD, KIND, MOD, QH><<<dim3((unsigned)a.units), dim3(kManyThreads), many_lds<HD>(), a.stream>>>(
       a.kv, a.sc, a.q, a.ldq, a.g, a.heads, a.counters, a.slots, a.out);
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
 }
-template <int HD>
-static int launch_many_of(const PagedLaunch& a) {
-  if (a.kind == kKv4) return a.mod ? launch_many<HD, kKv4, true>(a) : launch_many<HD, kKv4, false>(a);
-  if (a.kind == kKvBf16) return a.mod ? launch_many<HD, kKvBf16, true>(a) : launch_many<HD, kKvBf16, false>(a);
-  return a.mod ? launch_many<HD, kKvF16, true>(a) : launch_many<HD, kKvF16, false>(a);
+template <int HD, int KIND>
+static int launch_many_of(const PagedLaunch& a, int rows) {
+  if (rows == 64) return a.mod ? launch_many<HD, KIND, true, 2>(a) : launch_many<HD, KIND, false, 2>(a);
+  return a.mod ? launch_many<HD, KIND, true, 4>(a) : launch_many<HD, KIND, false, 4>(a);
 }
-int launch_paged_many(const PagedLaunch& a) { return a.hd == 64 ? launch_many_of<64>(a) : launch_many_of<128>(a); }
+int launch_paged_many(const PagedLaunch& a, int rows) {
+  if (a.hd == 64)
+    return a.kind == kKv4      ? launch_many_of<64, kKv4>(a, rows)
+           : a.kind == kKvBf16 ? launch_many_of<64, kKvBf16>(a, rows)
+                               : launch_many_of<64, kKvF16>(a, rows);
+  return a.kind == kKv4      ? launch_many_of<128, kKv4>(a, rows)
+         : a.kind == kKvBf16 ? launch_many_of<128, kKvBf16>(a, rows)
+                             : launch_many_of<128, kKvF16>(a, rows);
+}
 
 }  // namespace spectra
 
@@ -363,7 +405,7 @@ using namespace spectra;
 
 namespace {
 size_t slot_floats(int hd) {
-  const size_t few = (size_t)kFewSlots * 32, many = (size_t)kManySlots * kManyRows;
+  const size_t few = (size_t)kFewSlots * 32, many = (size_t)kManySlots * 128;
   return (few > many ? few : many) * (hd + 2);
 }
 }  // namespace
@@ -410,15 +452,17 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   a.counters = (uint32_t*)workspace;
   a.slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
   a.stream = (hipStream_t)stream;
-  // rows a sequence has on average pick the tile: 16, 32 or 128 rows
+  // Rows a sequence has on average pick the tile: 16 or 32 rows of the few, 64 or 128 of the many
+  // (64, whose key steps two waves share, while 128 would leave compute units idle).
   const int64_t all = tokens * a.g, seqs = tokens < kv->batch ? tokens : kv->batch;
-  const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kManyRows;
-  const int keys = rows == kManyRows ? kManyKeys : kFewKeys, target = rows == kManyRows ? kManyTarget : kFewTarget;
+  const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv->kv_heads * all <= 128 * kManyBig ? 64 : 128;
+  const bool many = rows >= 64;
+  const int keys = many ? kManyKeys : kFewKeys, target = many ? kManyTarget : kFewTarget;
   // at most this many tiles, and units (a tile has no more pieces than its table has key steps)
   const int64_t tiles = kv->kv_heads * (all / rows + seqs);
   const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;
   const int64_t units = std::min(tiles + target + 16, tiles * cuts);
   SPECTRA_REQUIRE(units < (1LL << 31), "tokens out of range");
   a.units = (int)units;
-  return rows == kManyRows ? launch_paged_many(a) : launch_paged_few(a, rows);
+  return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
 }
