@@ -17,11 +17,32 @@
 namespace spectra {
 
 constexpr int kManyThreads = 256;
-constexpr int kManyVRow = 2 * kManyKeys + 8;  // bytes of a transposed V row (padded: conflict-free 8-byte reads)
 
+// The buffers of keys, then of values: two each, a row of 16-byte chunks a key.  Chunk c of key r lies
+// at c ^ (r & 7) in K's rows (eight rows' equal chunks, which lanes read at once, on different
+// banks) and at c ^ v_turn(r) in V's (four rows' 64 bytes, read transposed, on different banks).
 template <int HD>
 constexpr int many_lds() {
-  return 2 * (kManyKeys * HD * 2 + HD * kManyVRow);
+  return 4 * kManyKeys * HD * 2;
+}
+template <int HD>
+__device__ __forceinline__ int v_turn(int r) {
+  return HD == 128 ? (r & 3) << 2 : (r & 2) << 1;
+}
+
+// 64 lanes' 16 bytes at base + off (a lane's own) to LDS at `to` + 16 lane, with no register between.
+// Nothing waits for it but an s_waitcnt vmcnt.
+__device__ __forceinline__ void copy_lds(const uint8_t* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+
+typedef __attribute__((address_space(3))) uint8_t* lds_t;
+typedef short ps4_t __attribute__((ext_vector_type(4)));
+
+// Four keys' values of one dim: of each 16 lanes, lanes 4 k .. 4 k + 3 name 4 dims each of key k, and
+// lane i gets dim i of the four.
+__device__ __forceinline__ uint2 read_turned(const uint8_t* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4_t*)(lds_t)p));
 }
 
 template <int HD, int KIND, bool MOD, int QH>
@@ -32,7 +53,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   constexpr int CH = HD / 8, KS = HD / 16, DT = HD / 32;  // 8-dim chunks, 16-dim steps, 32-dim tiles
   constexpr int KL = kManyKeys * CH / kManyThreads;       // K chunks a thread copies
   constexpr int ROWS = 32 * QH, TL = QH / 2;              // 32-key tiles of a step that a wave takes
-  constexpr int ROWB = Q4 ? HD / 2 : 2 * HD, KBYTES = kManyKeys * HD * 2;
+  constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int flag;
   __shared__ uint32_t redo[QH];
@@ -51,12 +72,12 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   const int steps = khi > kbeg ? (khi - kbeg + kManyKeys - 1) / kManyKeys : 0;
   const int sbeg = sread((int)((int64_t)steps * un.piece / un.pieces));
   const int send = sread((int)((int64_t)steps * (un.piece + 1) / un.pieces));
-  // this wave's rows: keys that some see, and those that all do; the lane's row
+  // keys that all of this wave's rows see; the lane's row
   const int wr0 = min(32 * qh, nrows - 1), wr1 = min(32 * qh + 31, nrows - 1);
   const PagedRange wa = paged_range(i0 + (r0 + wr0) / g, sq.len, un.prefix, sc.window);
   const PagedRange wb = paged_range(i0 + (r0 + wr1) / g, sq.len, un.prefix, sc.window);
-  const int wlo = wa.lo, whi = min(wb.hi, capacity), alo = wb.lo, ahi = min(wa.hi, capacity);
-  const bool live = 32 * qh < nrows, ok = 32 * qh + ln < nrows;
+  const int alo = wb.lo, ahi = min(wa.hi, capacity);
+  const bool ok = 32 * qh + ln < nrows;
   const int rr = r0 + min(32 * qh + ln, nrows - 1), tok = rr / g, head = un.kvh * g + (rr - tok * g);
   const PagedRange rg = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
   const float slope2 = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
@@ -74,100 +95,63 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   }
 
   // ---- staging: a step is 4 blocks of 16 keys, each in one page; a wave copies one block, so it
-  // needs one page id a step.  K: 16-byte chunk kc of the rows krow + i (64 / CH); V: 4 keys x 8 dims.
+  // needs one page id a step.  16-bit rows go to LDS directly; 4-bit ones through registers, where
+  // they are expanded (K's in the order of its codes, as Q is; V's put back in order).
   const int* tab = kv.table + un.b * kv.table_stride;
   auto page_of = [&](int k0) __attribute__((always_inline)) {
     return sread(sload(tab + min((k0 + 16 * wave) >> kv.page_shift, kv.table_width - 1)));
   };
-  const int kc = lane % CH, krow = lane / CH, vq = lane & 3, vo = (lane >> 2) % CH;
-  const bool vlane = lane < 4 * CH;  // (head_dim 64: half the lanes have no piece of V, and load another's)
-  struct Stage {
-    pu4_t k[Q4 ? 1 : KL], v[Q4 ? 1 : 4];
-    uint32_t kw[KL], ks[KL], kz[KL], vw[4], vs[4], vz[4];  // 4-bit: codes, scales, zero points
-    bool bad;
-  } st;
-  auto load = [&](int k0, int id) __attribute__((always_inline)) {
-    st.bad = (uint32_t)id >= (uint32_t)kv.num_pages;
-    const int64_t pg = st.bad ? 0 : id;
+  constexpr int KB = kManyKeys * HD * 2, RPI = 64 / CH;  // bytes of a buffer, rows of 64 lanes' chunks
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t)lds;
+  const int kc = lane % CH, krow = lane / CH;
+  constexpr uint32_t nan2 = BF ? 0x7fc07fc0u : 0x7e007e00u;
+  struct Codes {
+    uint32_t w[KL], s[KL], z[KL];
+  } kcodes, vcodes;
+  auto fetch = [&](bool value, int k0, int id, int buf, Codes& cd) __attribute__((always_inline)) {
+    const int64_t pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
     const int row = (un.kvh << kv.page_shift) + ((k0 + 16 * wave) & pmask);
-    const int64_t at = pg * kv.page_bytes + row * ROWB;
-    const uint8_t *kb = kv.k + at, *vb = kv.v + at;
-    const int64_t so = Q4 ? pg * kv.scale_step + row * (HD / 32) : 0, zo = Q4 ? pg * kv.zero_step + row * (HD / 32) : 0;
+    const uint8_t* base = (value ? kv.v : kv.k) + pg * kv.page_bytes + row * ROWB;
+    if constexpr (Q4) {
+      const uint16_t* sb = (value ? kv.vs : kv.ks) + pg * kv.scale_step + row * (HD / 32);
+      const uint8_t* zb = (value ? kv.vz : kv.kz) + pg * kv.zero_step + row * (HD / 32);
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      const int r = krow + i * (64 / CH);
-      if constexpr (Q4) {
-        st.kw[i] = load_at<uint32_t>(kb, r * ROWB + 4 * kc);
-        st.ks[i] = load_at<uint16_t>(kv.ks + so, 2 * (r * (HD / 32) + kc / 4));
-        st.kz[i] = load_at<uint8_t>(kv.kz + zo, r * (HD / 32) + kc / 4);
-      } else {
-        st.k[i] = __builtin_bit_cast(pu4_t, load_at<uint4>(kb, r * ROWB + 16 * kc));
+      for (int i = 0; i < KL; ++i) {
+        const int r = krow + i * RPI;
+        cd.w[i] = load_at<uint32_t>(base, r * ROWB + 4 * kc);
+        cd.s[i] = load_at<uint16_t>(sb, 2 * (r * (HD / 32) + kc / 4));
+        cd.z[i] = load_at<uint8_t>(zb, r * (HD / 32) + kc / 4);
       }
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = 4 * vq + j;
-      if constexpr (Q4) {
-        st.vw[j] = load_at<uint32_t>(vb, r * ROWB + 4 * vo);
-        st.vs[j] = load_at<uint16_t>(kv.vs + so, 2 * (r * (HD / 32) + vo / 4));
-        st.vz[j] = load_at<uint8_t>(kv.vz + zo, r * (HD / 32) + vo / 4);
-      } else {
-        st.v[j] = __builtin_bit_cast(pu4_t, load_at<uint4>(vb, r * ROWB + 16 * vo));
+      for (int i = 0; i < KL; ++i) {
+        const int r = krow + i * RPI;
+        copy_lds(base, r * ROWB + 16 * (kc ^ (value ? v_turn<HD>(r) : r & 7)),
+                 lds0 + (value ? 2 * KB : 0) + buf * KB + (16 * wave + i * RPI) * HD * 2);
       }
     }
   };
-  constexpr uint32_t nan2 = BF ? 0x7fc07fc0u : 0x7e007e00u;
-  auto store = [&](int k0, uint8_t* buf) __attribute__((always_inline)) {
-    uint8_t* ks = buf;
-    uint8_t* vs = buf + KBYTES;
+  // What was fetched is in place, with NaN for keys of a page that is not there, and zeros for values
+  // of keys that no row sees (they must not reach the product).
+  auto land = [&](bool value, int k0, int id, int buf, const Codes& cd) __attribute__((always_inline)) {
+    uint8_t* to = lds + (value ? 2 * KB : 0) + buf * KB;
+    const bool edge = value && (k0 < klo || k0 + kManyKeys > khi), bad = !value && (uint32_t)id >= (uint32_t)kv.num_pages;
+    if (!Q4 && !edge && !bad) return;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
-      const int key = 16 * wave + krow + i * (64 / CH);
-      pu4_t x;
+      const int r = krow + i * RPI, key = 16 * wave + r;
+      const bool out = edge && (k0 + key < klo || k0 + key >= khi);
+      pu4_t x = {0, 0, 0, 0};
       if constexpr (Q4) {
-        const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0xe400u | st.kz[i]));
-        const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)st.ks[i]);
-        x = kv4_pairs(st.kw[i], (ph2_t){z, z}, (ph2_t){s, s});
-      } else {
-        x = st.k[i];
+        const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0xe400u | cd.z[i]));
+        const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)(out ? 0 : cd.s[i]));
+        x = kv4_pairs(cd.w[i], (ph2_t){z, z}, (ph2_t){s, s});
+        if (value)
+          x = (pu4_t){__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
+                      __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
       }
-      if (st.bad) x = (pu4_t){nan2, nan2, nan2, nan2};  // no such page: scores of NaN
-      *(pu4_t*)(ks + key * (HD * 2) + 16 * (kc ^ (key & (CH - 1)))) = x;
-    }
-    if (vlane) {
-      const int kq = 16 * wave + 4 * vq;
-      uint32_t w[2][8];  // pair of keys, dim
-      if constexpr (Q4) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const uint32_t z2 = st.vz[2 * p] | (st.vz[2 * p + 1] << 16) | 0xe400e400u;
-          const uint32_t s2 = st.vs[2 * p] | (st.vs[2 * p + 1] << 16);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const pu4_t x = kv4_pairs(__builtin_amdgcn_perm(st.vw[2 * p + 1], st.vw[2 * p], u ? 0x07060302u : 0x05040100u),
-                                      __builtin_bit_cast(ph2_t, z2), __builtin_bit_cast(ph2_t, s2));
-#pragma unroll
-            for (int n = 0; n < 4; ++n) w[p][4 * u + n] = x[n];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            w[p][e] = __builtin_amdgcn_perm(st.v[2 * p + 1][e >> 1], st.v[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
-      }
-      if (k0 < klo || k0 + kManyKeys > khi) {  // keys that no row sees: their values must not reach the product
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int key = k0 + kq + 2 * p;
-          const uint32_t keep = (key >= klo && key < khi ? 0xffffu : 0u) | (key + 1 >= klo && key + 1 < khi ? 0xffff0000u : 0u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[p][e] &= keep;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) *(uint2*)(vs + (8 * vo + e) * kManyVRow + 2 * kq) = make_uint2(w[0][e], w[1][e]);
+      if (bad) x = (pu4_t){nan2, nan2, nan2, nan2};
+      if (Q4 || bad || out) *(pu4_t*)(to + key * HD * 2 + 16 * (kc ^ (value ? v_turn<HD>(key) : key & 7))) = x;
     }
   };
 
@@ -177,22 +161,35 @@ __global__ void __launch_bounds__(kManyThreads, 2)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  auto compute = [&](int k0, const uint8_t* buf) __attribute__((always_inline)) {
+  // a wave's scores of a step: element r of tile t is key kw + 32 t + 8 (r / 4) + 4 gh + r % 4
+  constexpr int NK = TL * KS, NV = 2 * TL * DT, RING = 4;  // matrix instructions of Q K^T and P V; operands in flight
+  const int kbase = (32 * TL * kh + ln) * HD * 2;
+  auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
+    const int t = i / KS, st = i % KS;
+    return *(const pu4_t*)(lds + buf * KB + kbase + 64 * t * HD + 16 * ((2 * (st & 3) + gh) ^ (ln & 7)) + 128 * (st >> 2));
+  };
+  const int vi = lane & 15, vbase = (32 * TL * kh + 4 * gh + (vi >> 2)) * HD * 2 + 8 * (vi & 1);
+  const int vchunk = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
+  auto read_v = [&](int buf, int i) __attribute__((always_inline)) {  // 16 keys i / DT, 32 dims i % DT
+    const uint8_t* p = lds + 2 * KB + buf * KB + vbase + 16 * ((4 * (i % DT) + vchunk) ^ v_turn<HD>(vi >> 2)) + 32 * (i / DT) * HD;
+    const uint2 x = read_turned(p), y = read_turned(p + 16 * HD);
+    return (pu4_t){x.x, x.y, y.x, y.y};
+  };
+  constexpr pf16_t zero = {};
+  auto product = [&](pf16_t (&s)[TL], int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) s[i / KS] = mfma32<BF>(read_k(buf, i), qf[i % KS], i % KS == 0 ? zero : s[i / KS]);
+  };
+  // One step: softmax of its scores s, their product with its values, and the next step's scores
+  // into sn (past the last: of whatever its buffer holds, used by nothing).  The order is written out (the compiler would wait for every operand
+  // where it is used): operands are read RING instructions ahead, and the exponentials stand
+  // between the matrix instructions of Q K^T, which run beneath them.
+  auto step = [&](int k0, pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf) __attribute__((always_inline)) {
     const int kw = k0 + 32 * TL * kh;  // this wave's keys
-    if (!live || kw >= whi || kw + 32 * TL <= wlo) return;
-    const uint8_t* ks = buf;
-    const uint8_t* vs = buf + KBYTES;
-    pf16_t s[TL];
+    pu4_t ring[RING];
 #pragma unroll
-    for (int t = 0; t < TL; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
-      const int key = 32 * (TL * kh + t) + ln;
-#pragma unroll
-      for (int st = 0; st < KS; ++st)
-        s[t] = mfma32<BF>(*(const pu4_t*)(ks + key * (HD * 2) + 16 * ((2 * st + gh) ^ (key & (CH - 1)))), qf[st], s[t]);
-    }
-    // score r of tile t: key kw + 32 t + 8 (r / 4) + 4 gh + r % 4
+    for (int i = 0; i < RING; ++i) ring[i] = read_k(buf ^ 1, i);
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (MOD) {
       const float base = fpos - (float)kw;
 #pragma unroll
@@ -229,54 +226,68 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     }
     const float mu = m == -INFINITY ? 0.0f : m - kPagedRaise;
     pu4_t pf[TL][2];
+    auto weights = [&](int i) __attribute__((always_inline)) {  // the i-th pair
+      const int t = i >> 3, r = 2 * (i & 7);
+      const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], mul, -mu));
+      const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], mul, -mu));
+      l += e0 + e1;
+      pf[t][r >> 3][(r & 7) >> 1] = pack2<BF>(e0, e1);
+    };
 #pragma unroll
-    for (int t = 0; t < TL; ++t)
+    for (int i = 0; i < NK; ++i) {
+      sn[i / KS] = mfma32<BF>(ring[i % RING], qf[i % KS], i % KS == 0 ? zero : sn[i / KS]);
+      ring[i % RING] = i + RING < NK ? read_k(buf ^ 1, i + RING) : read_v(buf, i + RING - NK);
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], mul, -mu));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], mul, -mu));
-        l += e0 + e1;
-        pf[t][r >> 3][(r & 7) >> 1] = pack2<BF>(e0, e1);
-      }
-    // O^T += V^T P^T: step (t, u) contracts keys 32 t + 16 u + {4 gh + 0 .. 3, 8 + 4 gh + 0 .. 3}
+      for (int j = i * 8 * TL / NK; j < (i + 1) * 8 * TL / NK; ++j) weights(j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // O^T += V^T P^T, 16 keys and 32 dims at a time; keys 16 u + {4 gh + 0 .. 3, 8 + 4 gh + 0 .. 3}
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const uint8_t* vrow = vs + (32 * d + ln) * kManyVRow + 64 * TL * kh + 8 * gh;
-#pragma unroll
-      for (int t = 0; t < TL; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint2 a = *(const uint2*)(vrow + 2 * (32 * t + 16 * u)), b = *(const uint2*)(vrow + 2 * (32 * t + 16 * u + 8));
-          o[d] = mfma32<BF>((pu4_t){a.x, a.y, b.x, b.y}, pf[t][u], o[d]);
-        }
+    for (int i = 0; i < NV; ++i) {
+      const int u = i / DT;
+      o[i % DT] = mfma32<BF>(ring[i % RING], pf[u >> 1][u & 1], o[i % DT]);
+      if (i + RING < NV) ring[i % RING] = read_v(buf, i + RING);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
   if (sbeg < send) {
-    constexpr int BUF = many_lds<HD>() / 2;
+    // At step s the buffers hold K of s + 1 and V of s; K of s + 2 and V of s + 1 are on their way.
     int k0 = kbeg + sbeg * kManyKeys;
     const int kend = kbeg + send * kManyKeys;
-    load(k0, page_of(k0));
-    int next = page_of(k0 + kManyKeys);
-    store(k0, lds);
+    pf16_t s0[TL], s1[TL];
+    int id0 = page_of(k0), id1 = page_of(k0 + kManyKeys), id2 = page_of(k0 + 2 * kManyKeys);
+    auto wait = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+    fetch(false, k0, id0, 0, kcodes);
+    fetch(true, k0, id0, 0, vcodes);
+    wait();
+    land(false, k0, id0, 0, kcodes);
+    land(true, k0, id0, 0, vcodes);
+    fetch(false, k0 + kManyKeys, id1, 1, kcodes);
+    wait();
+    land(false, k0 + kManyKeys, id1, 1, kcodes);
     __syncthreads();
-    while (true) {  // (two steps a turn: the buffers' addresses are constants)
-      bool more = k0 + kManyKeys < kend;
-      if (more) load(k0 + kManyKeys, next);
-      next = page_of(k0 + 2 * kManyKeys);
-      compute(k0, lds);
-      if (!more) break;
-      k0 += kManyKeys;
-      store(k0, lds + BUF);
+    product(s0, 0);
+    __syncthreads();  // (K of the first step is read: its buffer is free)
+    auto turn = [&](pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf) __attribute__((always_inline)) {
+      const bool more = k0 + kManyKeys < kend;
+      if (more) {
+        fetch(false, k0 + 2 * kManyKeys, id2, buf, kcodes);
+        fetch(true, k0 + kManyKeys, id1, buf ^ 1, vcodes);
+      }
+      const int id3 = page_of(k0 + 3 * kManyKeys);
+      step(k0, s, sn, buf);
+      if (!more) return false;
+      wait();
+      land(false, k0 + 2 * kManyKeys, id2, buf, kcodes);
+      land(true, k0 + kManyKeys, id1, buf ^ 1, vcodes);
       __syncthreads();
-      more = k0 + kManyKeys < kend;
-      if (more) load(k0 + kManyKeys, next);
-      next = page_of(k0 + 2 * kManyKeys);
-      compute(k0, lds + BUF);
-      if (!more) break;
+      id1 = id2;
+      id2 = id3;
       k0 += kManyKeys;
-      store(k0, lds);
-      __syncthreads();
+      return true;
+    };
+    while (turn(s0, s1, 0) && turn(s1, s0, 1)) {
     }
   }
 
