@@ -68,25 +68,52 @@ __device__ __forceinline__ int paged_find(const int* q_start, int batch, int t, 
 
 // ---- attention: scores, and the shares of the work ----------------------------------------------
 
-// What turns a product q . k into a score in log2 units: x = mul (q . k), or with a cap
-// cap2 tanh(mul (q . k)) computed as cap2 (1 - 2 / (1 + 2^(t2 (q . k)))) (t2 = 2 log2(e) mul), less
-// slope2 |i - j| where slopes are given.  MOD false: neither.
+// What turns products x = q . k into scores in log2 units, up to a constant of the row (softmax
+// knows none): mul x, or with a cap
+//   cap2 tanh(t x / 2) = cap2 (1 - 2 / (1 + 2^(t2 x)))  ->  2 cap2 (-1 / (1 + 2^(t2 x)))
+// (t2 = 2 log2(e) scale / cap, cap2 = cap log2(e)); less slope2 |i - j|, which for keys up to the row's
+// position is slope2 (j - i).
 struct PagedScore {
-  float mul;           // scale log2(e) without a cap; with one t2
+  float mul;           // scale log2(e); with a cap t2
   float cap2;          // 0: no cap
   const float* slopes; // [heads] or NULL
   const int* prefix;   // [batch] or NULL
   int window;          // 0: none
 };
-template <bool MOD>
-__device__ __forceinline__ float paged_score(float x, const PagedScore& sc, float slope2, float dist) {
-  if constexpr (!MOD) {
-    return x * sc.mul;
-  } else {
-    float y = x * sc.mul;
-    if (sc.cap2 > 0.0f) y = sc.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y)));
-    return __builtin_fmaf(-slope2, __builtin_fabsf(dist), y);
+
+// Applies cap and bias to T tiles of N products; far: the row's position less the first key's, at(n):
+// the n-th product's key after it (tiles 32 or 16 N / 4 keys apart).  The scores are the result's
+// factor times what is left in s.
+template <int T, int N, typename V, typename F>
+__device__ __forceinline__ float paged_scores(V (&s)[T], const PagedScore& sc, float slope2, float far, F at) {
+  float mul = sc.mul;
+  if (sc.cap2 > 0.0f) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        s[t][n] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[t][n] * mul));
+    mul = 2.0f * sc.cap2;
   }
+  if (sc.slopes != nullptr) {
+    constexpr int STEP = N == 16 ? 32 : 16;
+    if (sc.prefix == nullptr) {
+      const float first = -slope2 * far;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          s[t][n] = __builtin_fmaf(s[t][n], mul, __builtin_fmaf(slope2, (float)(STEP * t + at(n)), first));
+    } else {  // (keys after the row's position too)
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          s[t][n] = __builtin_fmaf(s[t][n], mul, -slope2 * __builtin_fabsf(far - (float)(STEP * t + at(n))));
+    }
+    mul = 1.0f;
+  }
+  return mul;
 }
 
 // Keys [lo, hi) that the query at position i sees, of a sequence of len keys.

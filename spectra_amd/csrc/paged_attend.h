@@ -50,6 +50,15 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
   }
 }
 
+// sum + both of a pair of weights as rounded, in fp32 (one instruction).
+template <bool BF>
+__device__ __forceinline__ float add2(uint32_t w, float sum) {
+  if constexpr (BF)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pb2_t, w), __builtin_bit_cast(pb2_t, 0x3f803f80u), sum, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(ph2_t, w), __builtin_bit_cast(ph2_t, 0x3c003c00u), sum, false);
+}
+
 // Four pairs of 4-bit codes (nibbles n and n + 4 of w, n = 0 .. 3) as fp16((q - z) * s): 1024 + q is
 // the fp16 with q in its last bits, and 1024 + q - (1024 + z) is exact.  nz: the pair -(1024 + z),
 // s: the pair of scales.
@@ -103,7 +112,10 @@ __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& s
     if (see) {
       x = 0.0f;
       for (int d = 0; d < HD; ++d) x += (BF ? bf2f(qr[d]) : h2f(qr[d])) * paged_elem<HD, KIND>(kv, false, bad ? 0 : page, r, d);
-      x = bad ? NAN : paged_score<MOD>(x, sc, slope2, (float)(i - j));
+      pf4_t one[1] = {{x, x, x, x}};
+      float mul = sc.mul;
+      if constexpr (MOD) mul = paged_scores<1, 4>(one, sc, slope2, (float)(i - j), [](int) { return 0; });
+      x = bad ? NAN : one[0][0] * mul;
     }
     const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.0f : mn;
     const float corr = __builtin_amdgcn_exp2f(m - mu), e = see ? __builtin_amdgcn_exp2f(x - mu) : 0.0f;

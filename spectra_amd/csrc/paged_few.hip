@@ -178,18 +178,19 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
     pu4_t pf[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float x[8];
-      float mn = m[nt];
+      // scores of the keys key0 + 16 (e / 4) + 4 q4 + e % 4
+      float x[8], mn = m[nt], mul = sc.mul;
+      if constexpr (MOD)
+        mul = paged_scores<2, 4>(s[nt], sc, slope2[nt], fpos[nt] - (float)(key0 + 4 * q4), [](int n) { return n; });
 #pragma unroll
-      for (int e = 0; e < 8; ++e)  // key key0 + 16 (e / 4) + 4 q4 + e % 4
-        x[e] = paged_score<MOD>(s[nt][e >> 2][e & 3], sc, slope2[nt],
-                                MOD ? fpos[nt] - (float)(key0 + 4 * q4) - (float)(16 * (e >> 2) + (e & 3)) : 0.0f);
+      for (int e = 0; e < 8; ++e) x[e] = s[nt][e >> 2][e & 3] * mul;
       if (part) {
+        const int from = rg[nt].lo - key0 - 4 * q4, to = min(rg[nt].hi, capacity) - key0 - 4 * q4;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int key = key0 + 16 * (e >> 2) + 4 * q4 + (e & 3);
+          const int at = 16 * (e >> 2) + (e & 3);
           if ((e >> 2) ? bad1 : bad0) x[e] = NAN;
-          if (key < rg[nt].lo || key >= min(rg[nt].hi, capacity)) x[e] = -INFINITY;
+          if (at < from || at >= to) x[e] = -INFINITY;
         }
       }
 #pragma unroll

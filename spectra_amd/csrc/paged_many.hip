@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   // a wave's scores of a step: element r of tile t is key kw + 32 t + 8 (r / 4) + 4 gh + r % 4
-  constexpr int NK = TL * KS, NV = 2 * TL * DT, RING = 4;  // matrix instructions of Q K^T and P V; operands in flight
+  constexpr int NK = TL * KS, NV = 2 * TL * DT;  // matrix instructions of Q K^T and of P V, and operands in flight
+  constexpr int RING = 4, RINGV = 8;
   const int kbase = (32 * TL * kh + ln) * HD * 2;
   auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
     const int t = i / KS, st = i % KS;
@@ -186,28 +187,22 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   // between the matrix instructions of Q K^T, which run beneath them.
   auto step = [&](int k0, pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf) __attribute__((always_inline)) {
     const int kw = k0 + 32 * TL * kh;  // this wave's keys
-    pu4_t ring[RING];
+    pu4_t ring[RINGV];
 #pragma unroll
     for (int i = 0; i < RING; ++i) ring[i] = read_k(buf ^ 1, i);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (MOD) {
-      const float base = fpos - (float)kw;
-#pragma unroll
-      for (int t = 0; t < TL; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] = paged_score<true>(s[t][r], sc, slope2, base - (float)(32 * t + 8 * (r >> 2) + (r & 3)));
-    }
+    float mul = sc.mul;
+    if constexpr (MOD) mul = paged_scores<TL, 16>(s, sc, slope2, fpos - (float)kw, [](int r) { return 8 * (r >> 2) + (r & 3); });
     if (kw < alo || kw + 32 * TL > ahi) {
+      const int from = rg.lo - kw - 4 * gh, to = min(rg.hi, capacity) - kw - 4 * gh;
 #pragma unroll
       for (int t = 0; t < TL; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = kw + 32 * t + 8 * (r >> 2) + 4 * gh + (r & 3);
-          if (key < rg.lo || key >= min(rg.hi, capacity)) s[t][r] = -INFINITY;
+          const int at = 32 * t + 8 * (r >> 2) + (r & 3);
+          if (at < from || at >= to) s[t][r] = -INFINITY;
         }
     }
-    const float mul = MOD ? 1.0f : sc.mul;
     float mn = -INFINITY;
 #pragma unroll
     for (int t = 0; t < TL; ++t)
@@ -230,23 +225,26 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       const int t = i >> 3, r = 2 * (i & 7);
       const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], mul, -mu));
       const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], mul, -mu));
-      l += e0 + e1;
-      pf[t][r >> 3][(r & 7) >> 1] = pack2<BF>(e0, e1);
+      const uint32_t w = pack2<BF>(e0, e1);
+      l = add2<BF>(w, l);
+      pf[t][r >> 3][(r & 7) >> 1] = w;
     };
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       sn[i / KS] = mfma32<BF>(ring[i % RING], qf[i % KS], i % KS == 0 ? zero : sn[i / KS]);
-      ring[i % RING] = i + RING < NK ? read_k(buf ^ 1, i + RING) : read_v(buf, i + RING - NK);
+      ring[i % RING] = i + RING < NK ? read_k(buf ^ 1, i + RING) : read_v(buf, i + RING - NK);  // (NK is a multiple of RING)
 #pragma unroll
       for (int j = i * 8 * TL / NK; j < (i + 1) * 8 * TL / NK; ++j) weights(j);
       __builtin_amdgcn_sched_barrier(0);
     }
     // O^T += V^T P^T, 16 keys and 32 dims at a time; keys 16 u + {4 gh + 0 .. 3, 8 + 4 gh + 0 .. 3}
 #pragma unroll
+    for (int i = RING; i < RINGV; ++i) ring[i] = read_v(buf, i);
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = i / DT;
-      o[i % DT] = mfma32<BF>(ring[i % RING], pf[u >> 1][u & 1], o[i % DT]);
-      if (i + RING < NV) ring[i % RING] = read_v(buf, i + RING);
+      o[i % DT] = mfma32<BF>(ring[i % RINGV], pf[u >> 1][u & 1], o[i % DT]);
+      if (i + RINGV < NV) ring[i % RINGV] = read_v(buf, i + RINGV);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
