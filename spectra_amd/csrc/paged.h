@@ -18,16 +18,17 @@ namespace spectra {
 constexpr int kPagedPieces = 128;  // most pieces of a tile's keys
 
 struct PagedKv {
-  uint8_t *k, *v;       // 16-bit rows, or 4-bit codes
-  uint16_t *ks, *vs;    // 4-bit: scales
-  uint8_t *kz, *vz;     // 4-bit: zero points
-  int64_t page_bytes;   // from one page to the next: of k and v,
-  int64_t scale_step;   // of the scales (elements),
-  int64_t zero_step;    // of the zero points
+  uint8_t *k, *v;    // 16-bit rows, or 4-bit codes
+  uint8_t *ks, *vs;  // 4-bit: scales (fp16)
+  uint8_t *kz, *vz;  // 4-bit: zero points
+  uint32_t page_step, scale_step, zero_step;  // from one page to the next, in 16 bytes
   const int *table, *lens, *q_start;
   int64_t table_stride;
   int num_pages, kv_heads, page_shift, batch, table_width, tokens;
 };
+
+// Bytes from the pool's start to a page.
+__device__ __forceinline__ uint64_t paged_at(int page, uint32_t step) { return ((uint64_t)(uint32_t)page * step) << 4; }
 
 // Validates the descriptor for a call of `tokens` tokens and `heads` query heads, and fills the
 // device form (api side of every paged entry).

@@ -98,16 +98,16 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int d = i + p * h2;
-          *(uint32_t*)(kv.k + page * kv.page_bytes + hr * (hd / 2) + d / 2) = pk[p];
+          *(uint32_t*)(kv.k + paged_at(page, kv.page_step) + hr * (hd / 2) + d / 2) = pk[p];
           if ((d & 31) == 0) {
-            kv.ks[page * kv.scale_step + hr * (hd / 32) + d / 32] = sb[p];
-            kv.kz[page * kv.zero_step + hr * (hd / 32) + d / 32] = zb[p];
+            *(uint16_t*)(kv.ks + paged_at(page, kv.scale_step) + 2 * (hr * (hd / 32) + d / 32)) = sb[p];
+            kv.kz[paged_at(page, kv.zero_step) + hr * (hd / 32) + d / 32] = zb[p];
           }
         }
       }
     } else if (hh >= heads && keep) {
       const int64_t hr = ((int64_t)(hh - heads) << kv.page_shift) + r;
-      uint16_t* dst = (uint16_t*)(kv.k + page * kv.page_bytes) + hr * hd + i;
+      uint16_t* dst = (uint16_t*)(kv.k + paged_at(page, kv.page_step)) + hr * hd + i;
       *(uint4*)dst = lo;
       *(uint4*)(dst + h2) = hi;
     }
@@ -119,14 +119,14 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
       uint8_t zb;
       kv4_quant_chunk(a, pk, sb, zb);
       if (keep) {
-        *(uint32_t*)(kv.v + page * kv.page_bytes + hr * (hd / 2) + i / 2) = pk;
+        *(uint32_t*)(kv.v + paged_at(page, kv.page_step) + hr * (hd / 2) + i / 2) = pk;
         if ((i & 31) == 0) {
-          kv.vs[page * kv.scale_step + hr * (hd / 32) + i / 32] = sb;
-          kv.vz[page * kv.zero_step + hr * (hd / 32) + i / 32] = zb;
+          *(uint16_t*)(kv.vs + paged_at(page, kv.scale_step) + 2 * (hr * (hd / 32) + i / 32)) = sb;
+          kv.vz[paged_at(page, kv.zero_step) + hr * (hd / 32) + i / 32] = zb;
         }
       }
     } else if (keep) {
-      *(uint4*)((uint16_t*)(kv.v + page * kv.page_bytes) + hr * hd + i) = a;
+      *(uint4*)((uint16_t*)(kv.v + paged_at(page, kv.page_step)) + hr * hd + i) = a;
     }
   }
 }
@@ -165,12 +165,17 @@ int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, Page
   }
   SPECTRA_REQUIRE(at % 16 == 0 && (kv->num_pages == 1 || step % 16 == 0),
                   "pages must start at 16-byte aligned addresses");
+  const int64_t far = kv->page_stride * (q4 ? 1 : 2);
+  SPECTRA_REQUIRE(kv->num_pages == 1 || (far >> 4 < (1LL << 32) && kv->scale_stride >> 3 < (1LL << 32) && kv->zero_stride >> 4 < (1LL << 32)),
+                  "page stride too large");
+  const bool one = kv->num_pages == 1;
   int shift = 0;
   while ((1 << shift) < kv->page_size) ++shift;
-  *out = PagedKv{(uint8_t*)kv->k, (uint8_t*)kv->v, (uint16_t*)kv->k_scales, (uint16_t*)kv->v_scales,
-                 (uint8_t*)kv->k_zeros, (uint8_t*)kv->v_zeros, kv->page_stride * (q4 ? 1 : 2), kv->scale_stride,
-                 kv->zero_stride, kv->block_table, kv->kv_lens, kv->q_start, kv->table_stride, (int)kv->num_pages,
-                 kv->kv_heads, shift, kv->batch, kv->table_width, (int)tokens};
+  *out = PagedKv{(uint8_t*)kv->k, (uint8_t*)kv->v, (uint8_t*)kv->k_scales, (uint8_t*)kv->v_scales,
+                 (uint8_t*)kv->k_zeros, (uint8_t*)kv->v_zeros, one ? 0 : (uint32_t)(far >> 4),
+                 one ? 0 : (uint32_t)(kv->scale_stride >> 3), one ? 0 : (uint32_t)(kv->zero_stride >> 4),
+                 kv->block_table, kv->kv_lens, kv->q_start, kv->table_stride, (int)kv->num_pages, kv->kv_heads, shift,
+                 kv->batch, kv->table_width, (int)tokens};
   return SPECTRA_OK;
 }
 

@@ -59,27 +59,48 @@ __device__ __forceinline__ float add2(uint32_t w, float sum) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(ph2_t, w), __builtin_bit_cast(ph2_t, 0x3c003c00u), sum, false);
 }
 
-// Four pairs of 4-bit codes (nibbles n and n + 4 of w, n = 0 .. 3) as fp16((q - z) * s): 1024 + q is
-// the fp16 with q in its last bits, and 1024 + q - (1024 + z) is exact.  nz: the pair -(1024 + z),
-// s: the pair of scales.
-__device__ __forceinline__ pu4_t kv4_pairs(uint32_t w, ph2_t nz, ph2_t s) {
-  pu4_t r;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const uint32_t c = ((w >> (4 * n)) & 0x000f000fu) | 0x64006400u;
-    r[n] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(ph2_t, c) + nz) * s);
-  }
-  return r;
+// Four pairs of 4-bit codes (nibbles n and n + 4 of w, n = 0 .. 3) as fp16((q - z) * s).  q in the last
+// bits of the fp16 1024 is 1024 + q, and in bits 4 .. 7 of 64 it is 64 + q, so a pair takes one
+// instruction (three for each shift, mask and merge: 19 a word instead of 13); the differences
+// from 1024 + z and 64 + z are exact.
+struct Kv4Zero {
+  ph2_t n1024, n64;  // -(1024 + z), -(64 + z) of a pair
+};
+__device__ __forceinline__ Kv4Zero kv4_zero(uint32_t z) {  // z: two zero points, 16 bits each
+  const ph2_t n = __builtin_bit_cast(ph2_t, z | 0xe400e400u);
+  return {n, n + (ph2_t){(_Float16)960.0f, (_Float16)960.0f}};
+}
+__device__ __forceinline__ pu4_t kv4_pairs(uint32_t w, const Kv4Zero& z, ph2_t s) {
+  auto pair = [](uint32_t x, uint32_t mask, uint32_t one) __attribute__((always_inline)) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(one));
+    return __builtin_bit_cast(ph2_t, r);
+  };
+  const uint32_t w8 = w >> 8;
+  return (pu4_t){__builtin_bit_cast(uint32_t, (pair(w, 0x000f000fu, 0x64006400u) + z.n1024) * s),
+                 __builtin_bit_cast(uint32_t, (pair(w, 0x00f000f0u, 0x54005400u) + z.n64) * s),
+                 __builtin_bit_cast(uint32_t, (pair(w8, 0x000f000fu, 0x64006400u) + z.n1024) * s),
+                 __builtin_bit_cast(uint32_t, (pair(w8, 0x00f000f0u, 0x54005400u) + z.n64) * s)};
+}
+
+// Loads at a wave's base plus a lane's offset plus a constant: one address register.
+template <typename T>
+__device__ __forceinline__ T load_from(const void* base, uint32_t lane_off, int imm) {
+  typedef const __attribute__((address_space(1))) uint8_t* gbyte_t;
+  const gbyte_t p = (gbyte_t)base + (uint64_t)lane_off + imm;
+  if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, *(const __attribute__((address_space(1))) pu4_t*)p);
+  else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, *(const __attribute__((address_space(1))) uint64_t*)p);
+  else return *(const __attribute__((address_space(1))) T*)p;
 }
 
 // One element of the pages (the row-by-row path's reads).
 template <int HD, int KIND>
 __device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int page, int64_t row, int d) {
-  const uint8_t* p = (value ? kv.v : kv.k) + page * kv.page_bytes;
+  const uint8_t* p = (value ? kv.v : kv.k) + paged_at(page, kv.page_step);
   if constexpr (KIND == kKv4) {
     const uint32_t c = (p[row * (HD / 2) + d / 2] >> (4 * (d & 1))) & 15u;
-    const float s = h2f((value ? kv.vs : kv.ks)[page * kv.scale_step + row * (HD / 32) + d / 32]);
-    const float z = (float)(value ? kv.vz : kv.kz)[page * kv.zero_step + row * (HD / 32) + d / 32];
+    const float s = h2f(*(const uint16_t*)((value ? kv.vs : kv.ks) + paged_at(page, kv.scale_step) + 2 * (row * (HD / 32) + d / 32)));
+    const float z = (float)(value ? kv.vz : kv.kz)[paged_at(page, kv.zero_step) + row * (HD / 32) + d / 32];
     return h2f(f2h(((float)c - z) * s));
   } else {
     const uint16_t h = ((const uint16_t*)p)[row * HD + d];

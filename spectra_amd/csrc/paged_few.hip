@@ -88,51 +88,50 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   typedef FewTile<HD, KIND> Tile;
   const uint32_t koff = (uint32_t)(Q4 ? c * ROWB + q4 * (HD / 8) : c * ROWB + 16 * q4);
   const uint32_t voff = (uint32_t)(4 * q4 * ROWB + c * (ROWB / 16));
+  const uint32_t kgroup = c * (HD / 32) + (HD == 128 ? q4 : q4 >> 1), vgroup = 4 * q4 * (HD / 32) + (c * DPL) / 32;
   auto load = [&](Tile& t, int key0, int p0, int p1) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int id = h ? p1 : p0;
-      const int64_t pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
+      const int pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
       const int row = (un.kvh << kv.page_shift) + ((key0 + 16 * h) & pmask);
-      const uint8_t* kb = kv.k + pg * kv.page_bytes + (int64_t)row * ROWB;
-      const uint8_t* vb = kv.v + pg * kv.page_bytes + (int64_t)row * ROWB;
+      const uint64_t at = paged_at(pg, kv.page_step) + row * ROWB;
+      const uint8_t *kb = kv.k + at, *vb = kv.v + at;
       if constexpr (Q4) {
-        const int64_t so = pg * kv.scale_step + (int64_t)row * (HD / 32), zo = pg * kv.zero_step + (int64_t)row * (HD / 32);
+        const uint64_t so = paged_at(pg, kv.scale_step) + row * (HD / 16), zo = paged_at(pg, kv.zero_step) + row * (HD / 32);
         if constexpr (HD == 128) {
-          const uint4 x = load_at<uint4>(kb, koff);
+          const uint4 x = load_from<uint4>(kb, koff, 0);
           t.k[h][0] = x.x;
           t.k[h][1] = x.y;
           t.k[h][2] = x.z;
           t.k[h][3] = x.w;
         } else {
-          const uint2 x = load_at<uint2>(kb, koff);
+          const uint2 x = load_from<uint2>(kb, koff, 0);
           t.k[h][0] = x.x;
           t.k[h][1] = x.y;
         }
-        const uint32_t kg = c * (HD / 32) + (HD == 128 ? q4 : q4 >> 1);
-        t.ks[h] = load_at<uint16_t>(kv.ks + so, 2 * kg);
-        t.kz[h] = load_at<uint8_t>(kv.kz + zo, kg);
+        t.ks[h] = load_from<uint16_t>(kv.ks + so, 2 * kgroup, 0);
+        t.kz[h] = load_from<uint8_t>(kv.kz + zo, kgroup, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (HD == 128) t.v[h][i] = load_at<uint32_t>(vb, voff + i * ROWB);
-          else t.v[h][i] = load_at<uint16_t>(vb, voff + i * ROWB);
-          const uint32_t vg = (4 * q4 + i) * (HD / 32) + (c * DPL) / 32;
-          t.vs[h][i] = load_at<uint16_t>(kv.vs + so, 2 * vg);
-          t.vz[h][i] = load_at<uint8_t>(kv.vz + zo, vg);
+          if constexpr (HD == 128) t.v[h][i] = load_from<uint32_t>(vb, voff, i * ROWB);
+          else t.v[h][i] = load_from<uint16_t>(vb, voff, i * ROWB);
+          t.vs[h][i] = load_from<uint16_t>(kv.vs + so, 2 * vgroup, i * (HD / 16));
+          t.vz[h][i] = load_from<uint8_t>(kv.vz + zo, vgroup, i * (HD / 32));
         }
       } else {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) t.k[h][s] = __builtin_bit_cast(pu4_t, load_at<uint4>(kb, koff + 64 * s));
+        for (int s = 0; s < KS; ++s) t.k[h][s] = __builtin_bit_cast(pu4_t, load_from<uint4>(kb, koff, 64 * s));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (HD == 128) {
-            const uint4 x = load_at<uint4>(vb, voff + i * ROWB);
+            const uint4 x = load_from<uint4>(vb, voff, i * ROWB);
             t.v[h][i][0] = x.x;
             t.v[h][i][1] = x.y;
             t.v[h][i][2] = x.z;
             t.v[h][i][3] = x.w;
           } else {
-            const uint2 x = load_at<uint2>(vb, voff + i * ROWB);
+            const uint2 x = load_from<uint2>(vb, voff, i * ROWB);
             t.v[h][i][0] = x.x;
             t.v[h][i][1] = x.y;
           }
@@ -158,11 +157,11 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[nt][h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (Q4) {
-        const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0xe400u | t.kz[h]));  // -(1024 + z)
-        const _Float16 sf = __builtin_bit_cast(_Float16, (uint16_t)t.ks[h]);
+        const Kv4Zero z = kv4_zero(t.kz[h] | t.kz[h] << 16);
+        const ph2_t sf = __builtin_bit_cast(ph2_t, t.ks[h] | t.ks[h] << 16);
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
-          const pu4_t a = kv4_pairs(t.k[h][st], (ph2_t){z, z}, (ph2_t){sf, sf});
+          const pu4_t a = kv4_pairs(t.k[h][st], z, sf);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) s[nt][h] = mfma16<BF>(a, qf[nt][st], s[nt][h]);
         }
@@ -230,12 +229,12 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         const int h = p >> 1, i = 2 * (p & 1);
-        const uint32_t z2 = t.vz[h][i] | (t.vz[h][i + 1] << 16) | 0xe400e400u;
+        const Kv4Zero z2 = kv4_zero(t.vz[h][i] | t.vz[h][i + 1] << 16);
         const uint32_t s2 = (t.vs[h][i] | (t.vs[h][i + 1] << 16)) & keep[p];
 #pragma unroll
         for (int u = 0; u < HALF; ++u) {
           const uint32_t w = __builtin_amdgcn_perm(t.v[h][i + 1], t.v[h][i], u ? 0x07060302u : 0x05040100u);
-          const pu4_t x = kv4_pairs(w, __builtin_bit_cast(ph2_t, z2), __builtin_bit_cast(ph2_t, s2));
+          const pu4_t x = kv4_pairs(w, z2, __builtin_bit_cast(ph2_t, s2));
 #pragma unroll
           for (int n = 0; n < 4; ++n) a[4 * u + n][p] = x[n];
         }

@@ -109,18 +109,17 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     uint32_t w[KL], s[KL], z[KL];
   } kcodes, vcodes;
   auto fetch = [&](bool value, int k0, int id, int buf, Codes& cd) __attribute__((always_inline)) {
-    const int64_t pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
+    const int pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
     const int row = (un.kvh << kv.page_shift) + ((k0 + 16 * wave) & pmask);
-    const uint8_t* base = (value ? kv.v : kv.k) + pg * kv.page_bytes + row * ROWB;
+    const uint8_t* base = (value ? kv.v : kv.k) + paged_at(pg, kv.page_step) + row * ROWB;
     if constexpr (Q4) {
-      const uint16_t* sb = (value ? kv.vs : kv.ks) + pg * kv.scale_step + row * (HD / 32);
-      const uint8_t* zb = (value ? kv.vz : kv.kz) + pg * kv.zero_step + row * (HD / 32);
+      const uint8_t* sb = (value ? kv.vs : kv.ks) + paged_at(pg, kv.scale_step) + row * (HD / 16);
+      const uint8_t* zb = (value ? kv.vz : kv.kz) + paged_at(pg, kv.zero_step) + row * (HD / 32);
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
-        const int r = krow + i * RPI;
-        cd.w[i] = load_at<uint32_t>(base, r * ROWB + 4 * kc);
-        cd.s[i] = load_at<uint16_t>(sb, 2 * (r * (HD / 32) + kc / 4));
-        cd.z[i] = load_at<uint8_t>(zb, r * (HD / 32) + kc / 4);
+        cd.w[i] = load_from<uint32_t>(base, krow * ROWB + 4 * kc, i * RPI * ROWB);
+        cd.s[i] = load_from<uint16_t>(sb, 2 * (krow * (HD / 32) + kc / 4), i * RPI * (HD / 16));
+        cd.z[i] = load_from<uint8_t>(zb, krow * (HD / 32) + kc / 4, i * RPI * (HD / 32));
       }
     } else {
 #pragma unroll
@@ -143,9 +142,8 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       const bool out = edge && (k0 + key < klo || k0 + key >= khi);
       pu4_t x = {0, 0, 0, 0};
       if constexpr (Q4) {
-        const _Float16 z = __builtin_bit_cast(_Float16, (uint16_t)(0xe400u | cd.z[i]));
-        const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)(out ? 0 : cd.s[i]));
-        x = kv4_pairs(cd.w[i], (ph2_t){z, z}, (ph2_t){s, s});
+        const uint32_t s = out ? 0 : cd.s[i];
+        x = kv4_pairs(cd.w[i], kv4_zero(cd.z[i] | cd.z[i] << 16), __builtin_bit_cast(ph2_t, s | s << 16));
         if (value)
           x = (pu4_t){__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
                       __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
