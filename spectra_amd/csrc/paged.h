@@ -144,6 +144,113 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// Key steps that a tile of about `tokens` tokens may have.
+__device__ __forceinline__ int paged_steps(const PagedKv& kv, const PagedScore& sc, int len, int tokens, int ks) {
+  int span = min(len, kv.table_width << kv.page_shift);
+  if (sc.window > 0 && sc.prefix == nullptr) span = (int)min((int64_t)span, (int64_t)sc.window + tokens + 16);
+  return (span + ks - 1) / ks;
+}
+
+// A batch's tiles and their key steps in one line, the steps of a tile beside each other, and one of
+// equal shares of it: what a workgroup works through, whole tiles and at most two parts of one (a
+// tile's steps by the table's lengths, an upper bound: a part is a fraction of what the rows of the
+// tile see).  Worked out by every wave from the lengths themselves, so ragged batches are shared
+// out evenly with no plan on the host.
+struct PagedLine {
+  int total, each, more;  // the line's length; shares hold `each` steps, the first `more` of them one more
+  int begin, end;         // this share
+
+  __device__ __forceinline__ int start(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int owner(int x) const {  // the share that holds step x
+    const int big = more * (each + 1);
+    return (int)(x < big ? (uint32_t)x / (uint32_t)(each + 1) : more + (uint32_t)(x - big) / (uint32_t)each);
+  }
+};
+struct PagedPart {
+  PagedSeq seq;
+  int b, kvh, tile, prefix;
+  int t0, steps;  // the tile's place in the line, its steps
+  int from, to;   // this part of them
+};
+class PagedWalk {
+ public:
+  PagedLine line;
+
+  __device__ __forceinline__ PagedWalk(const PagedKv& kv, int g, int rows, int ks, const PagedScore& sc, int w, int groups, int lane)
+      : kv_(kv), sc_(sc), g_(g), rows_(rows), ks_(ks), lane_(lane), grain_(0), c0_(0), base_(0) {
+    float sum = 0.0f;
+    for (int c0 = 0; c0 < kv.batch; c0 += 64) {
+      take(c0);
+      sum += (float)tiles_ * (float)steps_;
+    }
+    sum = wave_sum(sum) * (float)kv.kv_heads;  // (the same in every lane and wave)
+    while (sum > 536870912.0f) {  // past 32 bits: steps of 2, 4, .. steps
+      sum *= 0.5f;
+      ++grain_;
+    }
+    int total = 0;
+    if (kv.batch <= 64) {
+      if (grain_ > 0) take(0);
+      scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
+      total = __builtin_amdgcn_readlane(scan_, 63);
+    } else {
+      for (int c0 = 0; c0 < kv.batch; c0 += 64) {
+        take(c0);
+        total += __builtin_amdgcn_readlane(wave_scan(kv.kv_heads * tiles_ * steps_), 63);
+      }
+      take(0);
+      scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
+    }
+    line.total = max(total, 0);
+    line.each = (int)((uint32_t)line.total / (uint32_t)groups);
+    line.more = line.total - line.each * groups;
+    line.begin = sread(line.start(w));
+    line.end = sread(line.start(w + 1));
+  }
+
+  // The part of the share that begins at x; x never goes back.  false: there is none.
+  __device__ __forceinline__ bool part(int x, PagedPart& p) {
+    uint64_t past;
+    while ((past = __ballot(base_ + scan_ > x)) == 0) {
+      base_ += __builtin_amdgcn_readlane(scan_, 63);
+      c0_ += 64;
+      if (c0_ >= kv_.batch) return false;
+      take(c0_);
+      scan_ = wave_scan(kv_.kv_heads * tiles_ * steps_);
+    }
+    const int at = __builtin_ctzll(past);
+    auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
+    const int steps = of(steps_), nt = of(tiles_), r = x - (base_ + of(scan_ - kv_.kv_heads * tiles_ * steps_));
+    if (r < 0 || steps <= 0 || nt <= 0) return false;  // (starts that never were a batch: sums that wrapped)
+    const int t = r / steps, from = r - t * steps;
+    if ((int64_t)x - from + steps > line.total) return false;
+    // (the same in every lane, told to the compiler: addresses made of them stay scalar)
+    p.seq = {sread(of(seq_.q0)), sread(of(seq_.n)), sread(of(seq_.len))};
+    p.b = sread(c0_ + at);
+    p.kvh = sread(t / nt);
+    p.tile = sread(t % nt);
+    p.steps = sread(steps);
+    p.from = sread(from);
+    p.t0 = sread(x - from);
+    p.to = sread(min(steps, from + line.end - x));
+    p.prefix = sc_.prefix != nullptr ? max(sread(sload(sc_.prefix + p.b)), 0) : 0;
+    return p.kvh < kv_.kv_heads;
+  }
+
+ private:
+  __device__ __forceinline__ void take(int c0) {
+    const int b = min(c0 + lane_, kv_.batch - 1);
+    seq_ = paged_seq(kv_.q_start[b], kv_.q_start[b + 1], kv_.lens[b], kv_.tokens);
+    tiles_ = c0 + lane_ < kv_.batch ? (seq_.n * g_ + rows_ - 1) / rows_ : 0;
+    steps_ = paged_steps(kv_, sc_, seq_.len, rows_ / g_, ks_);
+    steps_ = max((steps_ + (1 << grain_) - 1) >> grain_, 1);
+  }
+  const PagedKv& kv_;
+  const PagedScore& sc_;
+  int g_, rows_, ks_, lane_, grain_, c0_, base_, scan_, tiles_, steps_;
+  PagedSeq seq_;
+};
+
 // The u-th unit, worked out by every wave from the lengths themselves, so that ragged batches are
 // shared out evenly with no plan on the host: the tiles' key steps (of `ks` keys) are counted,
 // and tiles of more steps than target units would get each (and than min_steps) are cut into pieces.  At most
@@ -153,16 +260,13 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, int ks, int min_steps, int target,
                                            int max_slots,
                                            const PagedScore& sc, int u, int lane, PagedUnit& un) {
-  const int capacity = kv.table_width << kv.page_shift;
   PagedSeq sq;
   int tiles, steps;
   auto take = [&](int c0) __attribute__((always_inline)) {
     const int b = min(c0 + lane, kv.batch - 1);
     sq = paged_seq(kv.q_start[b], kv.q_start[b + 1], kv.lens[b], kv.tokens);
     tiles = c0 + lane < kv.batch ? (sq.n * g + rows - 1) / rows : 0;
-    int span = min(sq.len, capacity);
-    if (sc.window > 0 && sc.prefix == nullptr) span = min((int64_t)span, (int64_t)sc.window + rows / g + 16);
-    steps = max((span + ks - 1) / ks, 1);
+    steps = max(paged_steps(kv, sc, sq.len, rows / g, ks), 1);
   };
   float work = 0.0f;
   for (int c0 = 0; c0 < kv.batch; c0 += 64) {

@@ -111,8 +111,8 @@ __device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int p
 // One row by itself, every key that it does not see left out: the path of rows that came out
 // infinite or NaN beside rows that see other keys (a weight of zero times an infinity is NaN in the
 // matrix product).  A wave a row: lane = key for the scores, lane = HD / 64 dims for the sums.
-template <int HD, int KIND, bool MOD>
-__device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& sc, const PagedUnit& un, int g,
+template <int HD, int KIND, bool MOD, typename U>
+__device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& sc, const U& un, int g,
                                        const uint16_t* q, int64_t ldq, int heads, int row, uint16_t* out) {
   constexpr bool BF = KIND == kKvBf16;
   constexpr int DL = HD / 64;
@@ -199,10 +199,10 @@ __device__ __forceinline__ float2 load_dev2(const float* p) {
   return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
 }
 
-// A row's pieces joined (in their order, whatever order they arrived in): dims d .. d + 3 of the sum
+// A row's pieces (slot_of(p) the p-th's record) joined in their order, whatever order they arrived in: dims d .. d + 3 of the sum
 // of weight times value, and the total.
-template <int HD, int ROWS>
-__device__ __forceinline__ float paged_join(const float* base, int pieces, int row, int d, float (&v)[4]) {
+template <int HD, int ROWS, typename F>
+__device__ __forceinline__ float paged_join(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
   constexpr int U = 4;  // pieces in flight
   float mm = -INFINITY, den = 0.0f;
   v[0] = v[1] = v[2] = v[3] = 0.0f;
@@ -210,7 +210,7 @@ __device__ __forceinline__ float paged_join(const float* base, int pieces, int r
     float2 ml[U], x[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float* p = base + (int64_t)min(p0 + u, pieces - 1) * paged_slot<HD>(ROWS);
+      const float* p = slots + (int64_t)slot_of(min(p0 + u, pieces - 1)) * paged_slot<HD>(ROWS);
       ml[u] = load_dev2(p + ROWS * HD + 2 * row);
       x[u][0] = load_dev2(p + row * HD + d);
       x[u][1] = load_dev2(p + row * HD + d + 2);
@@ -250,8 +250,10 @@ struct PagedLaunch {
   hipStream_t stream;
   bool mod;
 };
-// Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows.
-constexpr int kFewTarget = 1024, kFewSlots = 2 * kFewTarget, kFewKeys = 128;
+// Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows, as many
+// workgroups as are resident at once, and two partial tiles each at most.
+constexpr int kFewKeys = 128, kFewGroups = 512;
+constexpr int few_groups(int rows) { return rows == 16 ? kFewGroups : kFewGroups / 2; }
 int launch_paged_few(const PagedLaunch& a, int rows);
 // Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.
 constexpr int kManyBig = 384, kManyKeys = 64, kManyMinSteps = 8, kManyTarget = 256, kManySlots = 2 * kManyTarget;

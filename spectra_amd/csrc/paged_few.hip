@@ -10,8 +10,9 @@
 // order (a lane: HD / 16 dims of its 8 keys) and turned by byte permutes.  4-bit pages are
 // expanded in the registers (codes of a key's row as they lie; Q is put in the codes' order once).
 //
-// A unit of work (paged_unit) is a piece of the keys of a tile; its 4 waves take 32-key tiles in
-// turn and meet in LDS at the end, pieces in the workspace, where the last to arrive joins them.
+// As many workgroups as are resident at once share the batch's key steps evenly (PagedWalk); a
+// part's 4 waves take 32 keys in turn and meet in LDS at its end, and the parts of a tile that
+// several workgroups hold meet in the workspace, where the last to arrive joins them.
 #include "paged_attend.h"
 
 namespace spectra {
@@ -39,10 +40,14 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   __shared__ __align__(16) float red[4 * 16 * RS];
   __shared__ float wm[4][ROWS], wl[4][ROWS];
   __shared__ int flag;
-  __shared__ uint32_t redo;
+  __shared__ uint32_t redo[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), c = lane & 15, q4 = lane >> 4;
-  PagedUnit un;
-  if (!paged_unit(kv, g, ROWS, kFewKeys, 1, kFewTarget, kFewSlots, sc, blockIdx.x, lane, un)) return;
+  PagedWalk walk(kv, g, ROWS, kFewKeys, sc, blockIdx.x, gridDim.x, lane);
+  PagedPart un;
+  if (tid == 0) redo[0] = 0;
+  int turn = 1;
+  for (int x = walk.line.begin; x < walk.line.end && walk.part(x, un); x = un.t0 + un.to) {
+  turn ^= 1;
   const PagedSeq sq = un.seq;
   const int r0 = un.tile * ROWS, nrows = min(ROWS, sq.n * g - r0);
   const int tok0 = sread(r0 / g), tok1 = sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;  // the tile's tokens, position of token 0
@@ -53,8 +58,12 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   const int klo = ra.lo, khi = min(rb.hi, capacity), alo = rb.lo, ahi = ra.hi;
   const int kbeg = klo & ~31;
   const int steps = khi > kbeg ? (khi - kbeg + kFewKeys - 1) / kFewKeys : 0;
-  const int sbeg = sread((int)((int64_t)steps * un.piece / un.pieces));
-  const int send = sread((int)((int64_t)steps * (un.piece + 1) / un.pieces));
+  const bool whole = un.from == 0 && un.to == un.steps;
+  int sbeg = un.from, send = un.to;
+  if (steps != un.steps) {  // (fewer than the line counted: a window, or the causal end)
+    sbeg = sread((int)((uint64_t)(uint32_t)steps * (uint32_t)un.from / (uint32_t)un.steps));
+    send = sread((int)((uint64_t)(uint32_t)steps * (uint32_t)un.to / (uint32_t)un.steps));
+  }
 
   // the lane's rows (column c of each 16): their queries, B operands
   PagedRange rg[NT];
@@ -296,9 +305,10 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       wl[wave][16 * nt + c] = l[nt];
     }
   }
-  if (tid == 0) redo = 0;
   const bool mixed = tok1 > tok0;  // rows that see different keys
-  float* part = slots + (int64_t)un.slot * paged_slot<HD>(ROWS);
+  // this share's parts of tiles that others hold the rest of: one may come first, one last
+  const int slot = 2 * (int)blockIdx.x + (x != walk.line.begin);
+  float* part = slots + (int64_t)slot * paged_slot<HD>(ROWS);
   auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
     const int r = r0 + row, tok = r / g, head = un.kvh * g + (r - tok * g);
     const bool past = paged_range(i0 + tok, sq.len, un.prefix, sc.window).hi > capacity;
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       y[e] = past ? NAN : den == 0.0f ? 0.0f : v[e] / den;
       odd |= !(__builtin_fabsf(y[e]) < INFINITY);
     }
-    if (mixed && odd) atomicOr(&redo, 1u << row);
+    if (mixed && odd) atomicOr(&redo[turn], 1u << row);
     const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
     *(uint2*)(out + ((int64_t)(sq.q0 + tok) * heads + head) * HD + d) = w;
   };
@@ -324,6 +334,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
         *(float4*)(red + (wave * 16 + c) * RS + DPL * (4 * q4 + i) + j) =
             make_float4(o[nt][j][i], o[nt][j + 1][i], o[nt][j + 2][i], o[nt][j + 3][i]);
     __syncthreads();
+    if (nt == 0 && tid == 0) redo[turn ^ 1] = 0;  // (every wave is past the last part's)
     for (int it = tid; it < 16 * HD / 4; it += kFewThreads) {
       const int r = it / (HD / 4), row = 16 * nt + r, d = 4 * (it % (HD / 4));
       if (row >= nrows) break;
@@ -340,7 +351,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
         v[2] += f * x.z;
         v[3] += f * x.w;
       }
-      if (un.pieces == 1) {
+      if (whole) {
         write(row, d, v, den);
       } else {
         store_dev2(part + row * HD + d, v[0], v[1]);
@@ -349,23 +360,26 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       }
     }
   }
-  if (un.pieces > 1) {
-    const int first = un.slot - un.piece;
-    if (!paged_arrive(counters + first, un.pieces, &flag)) return;
-    // the last to arrive joins the pieces, in their order
-    const float* base = slots + (int64_t)first * paged_slot<HD>(ROWS);
-    for (int it = tid; it < nrows * (HD / 4); it += kFewThreads) {
-      const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
-      float v[4];
-      const float den = paged_join<HD, ROWS>(base, un.pieces, row, d, v);
-      write(row, d, v, den);
+  if (!whole) {
+    const PagedLine& ln = walk.line;
+    const int w0 = ln.owner(un.t0), pieces = ln.owner(un.t0 + un.steps - 1) - w0 + 1;
+    const int first = 2 * w0 + (ln.start(w0) != un.t0);
+    auto slot_of = [&](int p) __attribute__((always_inline)) { return p == 0 ? first : 2 * (w0 + p); };
+    if (paged_arrive(counters + first, pieces, &flag)) {  // the last to arrive joins them
+      for (int it = tid; it < nrows * (HD / 4); it += kFewThreads) {
+        const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
+        float v[4];
+        const float den = paged_join<HD, ROWS>(slots, slot_of, pieces, row, d, v);
+        write(row, d, v, den);
+      }
     }
   }
-  if (!mixed) return;
-  __syncthreads();  // (writes of the rows to be done over are complete)
-  for (uint32_t r = redo & ~0u; r != 0; r &= r - 1) {
-    const int row = __builtin_ctz(r);
-    if ((row & 3) == wave) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + row, out);
+  __syncthreads();  // (rows to be done over are known, and LDS is free for the next part)
+  if (mixed)
+    for (uint32_t r = redo[turn]; r != 0; r &= r - 1) {
+      const int row = __builtin_ctz(r);
+      if ((row & 3) == wave) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + row, out);
+    }
   }
 }
 

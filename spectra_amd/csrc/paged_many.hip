@@ -359,11 +359,10 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       if (gh == 0) store_dev2(p + ROWS * HD + 2 * (32 * qh + ln), m, l);
     }
     if (!paged_arrive(counters + first, un.pieces, &flag)) return;
-    const float* base = slots + (int64_t)first * paged_slot<HD>(ROWS);
     for (int it = tid; it < nrows * (HD / 4); it += kManyThreads) {
       const int row = it / (HD / 4), d = 4 * (it % (HD / 4)), r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g);
       float v[4], y[4];
-      const float den = paged_join<HD, ROWS>(base, un.pieces, row, d, v);
+      const float den = paged_join<HD, ROWS>(slots, [&](int p) { return first + p; }, un.pieces, row, d, v);
       const bool past = paged_range(i0 + t, sq.len, un.prefix, sc.window).hi > capacity;
       bool odd = false;
 #pragma unroll
@@ -412,7 +411,7 @@ using namespace spectra;
 
 namespace {
 size_t slot_floats(int hd) {
-  const size_t few = (size_t)kFewSlots * 32, many = (size_t)kManySlots * 128;
+  const size_t few = (size_t)2 * kFewGroups * 16, many = (size_t)kManySlots * 128;
   return (few > many ? few : many) * (hd + 2);
 }
 }  // namespace
@@ -426,7 +425,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
                                     int32_t heads, float scale, float cap, int32_t window, const float* slopes,
                                     const int32_t* prefix, void* workspace, size_t workspace_bytes, void* out,
                                     spectra_stream_t stream) {
-  static_assert(4 * kFewSlots <= SPECTRA_PAGED_COUNTER_BYTES && 4 * kManySlots <= SPECTRA_PAGED_COUNTER_BYTES,
+  static_assert(8 * kFewGroups <= SPECTRA_PAGED_COUNTER_BYTES && 4 * kManySlots <= SPECTRA_PAGED_COUNTER_BYTES,
                 "a counter for every slot");
   PagedLaunch a;
   if (int st = paged_args(kv, tokens, heads, &a.kv); st != SPECTRA_OK) return st;
@@ -464,12 +463,12 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   const int64_t all = tokens * a.g, seqs = tokens < kv->batch ? tokens : kv->batch;
   const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv->kv_heads * all <= 128 * kManyBig ? 64 : 128;
   const bool many = rows >= 64;
-  const int keys = many ? kManyKeys : kFewKeys, target = many ? kManyTarget : kFewTarget;
-  // at most this many tiles, and units (a tile has no more pieces than its table has key steps)
+  const int keys = many ? kManyKeys : kFewKeys;
+  // at most this many tiles, each of at most as many key steps as its table has
   const int64_t tiles = kv->kv_heads * (all / rows + seqs);
   const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;
-  const int64_t units = std::min(tiles + target + 16, tiles * cuts);
-  SPECTRA_REQUIRE(units < (1LL << 31), "tokens out of range");
+  SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
+  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(rows), tiles * cuts);
   a.units = (int)units;
   return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
 }
