@@ -93,6 +93,19 @@ __device__ __forceinline__ T load_from(const void* base, uint32_t lane_off, int 
   else return *(const __attribute__((address_space(1))) T*)p;
 }
 
+// 64 lanes' 16 bytes at base + off (a lane's own), or 16 or 4 bytes at a lane's address, to LDS at
+// `to` + 16 (4) lane, with no register between.  Nothing waits for them but an s_waitcnt vmcnt.
+__device__ __forceinline__ void copy_lds(const uint8_t* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_lds16(const uint8_t* p, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_lds4(const uint8_t* p, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(p) : "memory", "m0");
+}
+typedef __attribute__((address_space(3))) uint8_t* lds_t;
+
 // One element of the pages (the row-by-row path's reads).
 template <int HD, int KIND>
 __device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int page, int64_t row, int d) {
@@ -252,8 +265,10 @@ struct PagedLaunch {
 };
 // Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows, as many
 // workgroups as are resident at once, and two partial tiles each at most.
-constexpr int kFewKeys = 128, kFewGroups = 512;
-constexpr int few_groups(int rows) { return rows == 16 ? kFewGroups : kFewGroups / 2; }
+constexpr int kFewKeys = 128;
+constexpr int few_resident(int kind, int rows) { return rows == 32 ? 1 : kind == kKv4 ? 3 : 2; }  // workgroups a compute unit
+constexpr int few_groups(int kind, int rows) { return 256 * few_resident(kind, rows); }
+constexpr int kFewSlotRows = 2 * few_groups(kKv4, 16) * 16;  // the most: two records of 16 rows each
 int launch_paged_few(const PagedLaunch& a, int rows);
 // Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.
 constexpr int kManyBig = 384, kManyKeys = 64, kManyMinSteps = 8, kManyTarget = 256, kManySlots = 2 * kManyTarget;

@@ -19,25 +19,36 @@ namespace spectra {
 
 constexpr int kFewThreads = 256;
 
-// 32 keys of K and V as they lie: tile t, register r.
-template <int HD, int KIND>
+// 32 keys of 16-bit K and V as they lie: tile t, register r.
+template <int HD>
 struct FewTile {
   pu4_t k[2][HD / 32];
   uint32_t v[2][4][HD / 32];
+  bool bad[2];  // a page that is not there
 };
+// 32 keys of 4-bit K and V in LDS, a wave's own: codes, scales and zero points of both.
 template <int HD>
-struct FewTile<HD, kKv4> {
-  uint32_t k[2][HD / 32], v[2][4], ks[2], vs[2][4], kz[2], vz[2][4];  // (scales and zero points: low bits)
+struct FewCodes {
+  static constexpr int kCodes = 16 * HD, kScales = 2 * HD, kZeros = HD;  // bytes of 32 keys
+  static constexpr int kV = kCodes, kS = 2 * kCodes, kZ = kS + 2 * kScales, kBytes = kZ + 2 * kZeros;
+  static constexpr int kCopies = HD == 128 ? 7 : 4;  // instructions that bring them
+  static constexpr int kDepth = 2;                   // tiles in LDS
 };
+template <int HD, int KIND>
+constexpr int few_lds() {
+  const int red = 4 * 16 * (HD + 4) * 4, ring = KIND == kKv4 ? 4 * FewCodes<HD>::kDepth * FewCodes<HD>::kBytes : 0;
+  return red > ring ? red : ring;
+}
 
 template <int HD, int KIND, int NT, bool MOD>
-__global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kFewThreads, few_resident(KIND, 16 * NT))
     paged_few_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                      uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
   constexpr int ROWS = 16 * NT, KS = HD / 32, DPL = HD / 16, RS = HD + 4;
   constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;  // bytes of a row of a page
-  __shared__ __align__(16) float red[4 * 16 * RS];
+  __shared__ __align__(16) uint8_t pool[few_lds<HD, KIND>()];  // 4-bit keys on their way; at the end the waves' sums
+  float* red = (float*)pool;
   __shared__ float wm[4][ROWS], wl[4][ROWS];
   __shared__ int flag;
   __shared__ uint32_t redo[2];
@@ -94,59 +105,63 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   auto page_of = [&](int key) __attribute__((always_inline)) {
     return sread(sload(tab + min(key >> kv.page_shift, kv.table_width - 1)));
   };
-  typedef FewTile<HD, KIND> Tile;
-  const uint32_t koff = (uint32_t)(Q4 ? c * ROWB + q4 * (HD / 8) : c * ROWB + 16 * q4);
-  const uint32_t voff = (uint32_t)(4 * q4 * ROWB + c * (ROWB / 16));
-  const uint32_t kgroup = c * (HD / 32) + (HD == 128 ? q4 : q4 >> 1), vgroup = 4 * q4 * (HD / 32) + (c * DPL) / 32;
+  typedef FewTile<HD> Tile;
+  const uint32_t koff = (uint32_t)(c * ROWB + 16 * q4), voff = (uint32_t)(4 * q4 * ROWB + c * (ROWB / 16));
   auto load = [&](Tile& t, int key0, int p0, int p1) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int id = h ? p1 : p0;
-      const int pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
+      t.bad[h] = (uint32_t)id >= (uint32_t)kv.num_pages;
       const int row = (un.kvh << kv.page_shift) + ((key0 + 16 * h) & pmask);
-      const uint64_t at = paged_at(pg, kv.page_step) + row * ROWB;
+      const uint64_t at = paged_at(t.bad[h] ? 0 : id, kv.page_step) + row * ROWB;
       const uint8_t *kb = kv.k + at, *vb = kv.v + at;
-      if constexpr (Q4) {
-        const uint64_t so = paged_at(pg, kv.scale_step) + row * (HD / 16), zo = paged_at(pg, kv.zero_step) + row * (HD / 32);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) t.k[h][s] = __builtin_bit_cast(pu4_t, load_from<uint4>(kb, koff, 64 * s));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         if constexpr (HD == 128) {
-          const uint4 x = load_from<uint4>(kb, koff, 0);
-          t.k[h][0] = x.x;
-          t.k[h][1] = x.y;
-          t.k[h][2] = x.z;
-          t.k[h][3] = x.w;
+          const uint4 x = load_from<uint4>(vb, voff, i * ROWB);
+          t.v[h][i][0] = x.x;
+          t.v[h][i][1] = x.y;
+          t.v[h][i][2] = x.z;
+          t.v[h][i][3] = x.w;
         } else {
-          const uint2 x = load_from<uint2>(kb, koff, 0);
-          t.k[h][0] = x.x;
-          t.k[h][1] = x.y;
-        }
-        t.ks[h] = load_from<uint16_t>(kv.ks + so, 2 * kgroup, 0);
-        t.kz[h] = load_from<uint8_t>(kv.kz + zo, kgroup, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (HD == 128) t.v[h][i] = load_from<uint32_t>(vb, voff, i * ROWB);
-          else t.v[h][i] = load_from<uint16_t>(vb, voff, i * ROWB);
-          t.vs[h][i] = load_from<uint16_t>(kv.vs + so, 2 * vgroup, i * (HD / 16));
-          t.vz[h][i] = load_from<uint8_t>(kv.vz + zo, vgroup, i * (HD / 32));
-        }
-      } else {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) t.k[h][s] = __builtin_bit_cast(pu4_t, load_from<uint4>(kb, koff, 64 * s));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (HD == 128) {
-            const uint4 x = load_from<uint4>(vb, voff, i * ROWB);
-            t.v[h][i][0] = x.x;
-            t.v[h][i][1] = x.y;
-            t.v[h][i][2] = x.z;
-            t.v[h][i][3] = x.w;
-          } else {
-            const uint2 x = load_from<uint2>(vb, voff, i * ROWB);
-            t.v[h][i][0] = x.x;
-            t.v[h][i][1] = x.y;
-          }
+          const uint2 x = load_from<uint2>(vb, voff, i * ROWB);
+          t.v[h][i][0] = x.x;
+          t.v[h][i][1] = x.y;
         }
       }
     }
+  };
+  // 4 bits: to LDS at `to`, whose last reads are complete; bit h: the page of half h is not there
+  typedef FewCodes<HD> C;
+  auto fetch = [&](uint32_t to, int key0, int p0, int p1) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const bool b0 = (uint32_t)p0 >= (uint32_t)kv.num_pages, b1 = (uint32_t)p1 >= (uint32_t)kv.num_pages;
+    p0 = b0 ? 0 : p0;
+    p1 = b1 ? 0 : p1;
+    const int row0 = (un.kvh << kv.page_shift) + (key0 & pmask), row1 = (un.kvh << kv.page_shift) + ((key0 + 16) & pmask);
+    const uint64_t a0 = paged_at(p0, kv.page_step) + row0 * ROWB, a1 = paged_at(p1, kv.page_step) + row1 * ROWB;
+    const uint64_t s0 = paged_at(p0, kv.scale_step) + row0 * (HD / 16), s1 = paged_at(p1, kv.scale_step) + row1 * (HD / 16);
+    const uint64_t z0 = paged_at(p0, kv.zero_step) + row0 * (HD / 32), z1 = paged_at(p1, kv.zero_step) + row1 * (HD / 32);
+    if constexpr (HD == 128) {
+      const uint32_t off = 16 * lane;
+      copy_lds(kv.k + a0, off, to);
+      copy_lds(kv.k + a1, off, to + 1024);
+      copy_lds(kv.v + a0, off, to + C::kV);
+      copy_lds(kv.v + a1, off, to + C::kV + 1024);
+      const uint64_t s = (lane < 32 ? s0 : s1) + 4 * (lane & 31);
+      copy_lds4(kv.ks + s, to + C::kS);
+      copy_lds4(kv.vs + s, to + C::kS + C::kScales);
+      copy_lds4((lane < 32 ? kv.kz : kv.vz) + ((lane & 16) == 0 ? z0 : z1) + 4 * (lane & 15), to + C::kZ);
+    } else {
+      const uint64_t a = (lane < 32 ? a0 : a1) + 16 * (lane & 31);
+      copy_lds16(kv.k + a, to);
+      copy_lds16(kv.v + a, to + C::kV);
+      copy_lds4((lane < 32 ? kv.ks : kv.vs) + ((lane & 16) == 0 ? s0 : s1) + 4 * (lane & 15), to + C::kS);
+      if (lane < 32) copy_lds4((lane < 16 ? kv.kz : kv.vz) + ((lane & 8) == 0 ? z0 : z1) + 4 * (lane & 7), to + C::kZ);
+    }
+    return (b0 ? 1 : 0) | (b1 ? 2 : 0);
   };
 
   float m[NT], l[NT];
@@ -158,7 +173,8 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[nt][j] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
   }
-  auto compute = [&](const Tile& t, int key0, int p0, int p1) __attribute__((always_inline)) {
+  // t: the tile's registers, or its place in LDS
+  auto compute = [&](const auto& t, int key0, bool bad0, bool bad1) __attribute__((always_inline)) {
     const bool edge = key0 < klo || key0 + 32 > khi;  // keys that no row sees: their values must not reach the product
     pf4_t s[NT][2];
 #pragma unroll
@@ -166,11 +182,23 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[nt][h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (Q4) {
-        const Kv4Zero z = kv4_zero(t.kz[h] | t.kz[h] << 16);
-        const ph2_t sf = __builtin_bit_cast(ph2_t, t.ks[h] | t.ks[h] << 16);
+        const int key = 16 * h + c, kg = HD == 128 ? q4 : q4 >> 1;  // group of the lane's dims
+        const uint32_t zb = t[C::kZ + key * (HD / 32) + kg], sb = *(const uint16_t*)(t + C::kS + 2 * (key * (HD / 32) + kg));
+        const Kv4Zero z = kv4_zero(zb | zb << 16);
+        const ph2_t sf = __builtin_bit_cast(ph2_t, sb | sb << 16);
+        uint32_t w[KS];
+        if constexpr (HD == 128) {
+          const pu4_t x = *(const pu4_t*)(t + key * ROWB + 16 * q4);
+#pragma unroll
+          for (int st = 0; st < KS; ++st) w[st] = x[st];
+        } else {
+          const uint2 x = *(const uint2*)(t + key * ROWB + 8 * q4);
+          w[0] = x.x;
+          w[1] = x.y;
+        }
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
-          const pu4_t a = kv4_pairs(t.k[h][st], z, sf);
+          const pu4_t a = kv4_pairs(w[st], z, sf);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) s[nt][h] = mfma16<BF>(a, qf[nt][st], s[nt][h]);
         }
@@ -181,7 +209,6 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
           for (int nt = 0; nt < NT; ++nt) s[nt][h] = mfma16<BF>(t.k[h][st], qf[nt][st], s[nt][h]);
       }
     }
-    const bool bad0 = (uint32_t)p0 >= (uint32_t)kv.num_pages, bad1 = (uint32_t)p1 >= (uint32_t)kv.num_pages;
     const bool part = key0 < alo || key0 + 32 > ahi || bad0 || bad1;
     pu4_t pf[NT];
 #pragma unroll
@@ -234,24 +261,40 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
     }
     if constexpr (Q4) {
       constexpr int HALF = HD / 64;  // codes of 4 dims each
-      pu4_t a[4 * HALF];
+      const int vg = c * DPL / 32;   // group of the lane's dims
+      Kv4Zero z2[4];
+      ph2_t s2[4];
+      uint32_t v0[4], v1[4];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const int h = p >> 1, i = 2 * (p & 1);
-        const Kv4Zero z2 = kv4_zero(t.vz[h][i] | t.vz[h][i + 1] << 16);
-        const uint32_t s2 = (t.vs[h][i] | (t.vs[h][i + 1] << 16)) & keep[p];
-#pragma unroll
-        for (int u = 0; u < HALF; ++u) {
-          const uint32_t w = __builtin_amdgcn_perm(t.v[h][i + 1], t.v[h][i], u ? 0x07060302u : 0x05040100u);
-          const pu4_t x = kv4_pairs(w, z2, __builtin_bit_cast(ph2_t, s2));
-#pragma unroll
-          for (int n = 0; n < 4; ++n) a[4 * u + n][p] = x[n];
+        const int key = 16 * (p >> 1) + 4 * q4 + 2 * (p & 1);  // and the next
+        const uint8_t* zp = t + C::kZ + C::kZeros + key * (HD / 32) + vg;
+        z2[p] = kv4_zero((uint32_t)zp[0] | (uint32_t)zp[HD / 32] << 16);
+        const uint8_t* sp = t + C::kS + C::kScales + 2 * (key * (HD / 32) + vg);
+        s2[p] = __builtin_bit_cast(ph2_t, ((uint32_t)*(const uint16_t*)sp | (uint32_t)*(const uint16_t*)(sp + HD / 16) << 16) & keep[p]);
+        const uint8_t* vp = t + C::kV + key * ROWB + c * (ROWB / 16);
+        if constexpr (HD == 128) {
+          v0[p] = *(const uint32_t*)vp;
+          v1[p] = *(const uint32_t*)(vp + ROWB);
+        } else {
+          v0[p] = *(const uint16_t*)vp;
+          v1[p] = *(const uint16_t*)(vp + ROWB);
         }
       }
 #pragma unroll
-      for (int j = 0; j < DPL; ++j)
+      for (int u = 0; u < HALF; ++u) {
+        pu4_t a[4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) o[nt][j] = mfma16<BF>(a[j], pf[nt], o[nt][j]);
+        for (int p = 0; p < 4; ++p) {
+          const pu4_t x = kv4_pairs(__builtin_amdgcn_perm(v1[p], v0[p], u ? 0x07060302u : 0x05040100u), z2[p], s2[p]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) a[n][p] = x[n];
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[nt][4 * u + n] = mfma16<BF>(a[n], pf[nt], o[nt][4 * u + n]);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < DPL; ++j) {
@@ -270,7 +313,39 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 
   const int kend = min(khi, kbeg + send * kFewKeys);
   int key = kbeg + sbeg * kFewKeys + 32 * wave;
-  if (key < kend) {
+  if constexpr (Q4) {
+    // page ids a tile ahead of the copies, copies kDepth - 1 tiles ahead of their use
+    constexpr int D = C::kDepth;
+    uint8_t* mine = pool + wave * D * C::kBytes;
+    const uint32_t at0 = (uint32_t)(uintptr_t)(lds_t)mine;
+    int p0 = page_of(key), p1 = page_of(key + 16), put = 0, ahead = key;
+    uint32_t bad = 0;  // two bits a tile on its way, the next one's last
+    int n = 0;         // tiles on their way
+    auto send_one = [&]() __attribute__((always_inline)) {
+      bad |= (uint32_t)fetch(at0 + put * C::kBytes, ahead, p0, p1) << (2 * n);
+      ++n;
+      put = put == D - 1 ? 0 : put + 1;
+      ahead += kFewKeys;
+      p0 = page_of(ahead);
+      p1 = page_of(ahead + 16);
+    };
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i)
+      if (ahead < kend) send_one();
+    for (int get = 0; key < kend; key += kFewKeys) {
+      if (ahead < kend) {
+        send_one();
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * C::kCopies) : "memory");  // all but the later tiles'
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      compute(mine + get * C::kBytes, key, (bad & 1) != 0, (bad & 2) != 0);
+      bad >>= 2;
+      --n;
+      get = get == D - 1 ? 0 : get + 1;
+    }
+    __syncthreads();  // (the waves' sums go where the codes were)
+  } else if (key < kend) {
     Tile ta, tb;
     int a0 = page_of(key), a1 = page_of(key + 16), b0 = 0, b1 = 0;
     load(ta, key, a0, a1);
@@ -279,7 +354,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
     while (true) {
       if (key + kFewKeys < kend) load(tb, key + kFewKeys, b0, b1);
       int n0 = page_of(key + 2 * kFewKeys), n1 = page_of(key + 2 * kFewKeys + 16);
-      compute(ta, key, a0, a1);
+      compute(ta, key, ta.bad[0], ta.bad[1]);
       key += kFewKeys;
       if (key >= kend) break;
       if (key + kFewKeys < kend) load(ta, key + kFewKeys, n0, n1);
@@ -287,7 +362,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       a1 = n1;
       n0 = page_of(key + 2 * kFewKeys);
       n1 = page_of(key + 2 * kFewKeys + 16);
-      compute(tb, key, b0, b1);
+      compute(tb, key, tb.bad[0], tb.bad[1]);
       b0 = n0;
       b1 = n1;
       key += kFewKeys;

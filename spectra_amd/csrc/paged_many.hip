@@ -30,13 +30,6 @@ __device__ __forceinline__ int v_turn(int r) {
   return HD == 128 ? (r & 3) << 2 : (r & 2) << 1;
 }
 
-// 64 lanes' 16 bytes at base + off (a lane's own) to LDS at `to` + 16 lane, with no register between.
-// Nothing waits for it but an s_waitcnt vmcnt.
-__device__ __forceinline__ void copy_lds(const uint8_t* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
-}
-
-typedef __attribute__((address_space(3))) uint8_t* lds_t;
 typedef short ps4_t __attribute__((ext_vector_type(4)));
 
 // Four keys' values of one dim: of each 16 lanes, lanes 4 k .. 4 k + 3 name 4 dims each of key k, and
@@ -411,7 +404,7 @@ using namespace spectra;
 
 namespace {
 size_t slot_floats(int hd) {
-  const size_t few = (size_t)2 * kFewGroups * 16, many = (size_t)kManySlots * 128;
+  const size_t few = kFewSlotRows, many = (size_t)kManySlots * 128;
   return (few > many ? few : many) * (hd + 2);
 }
 }  // namespace
@@ -425,7 +418,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
                                     int32_t heads, float scale, float cap, int32_t window, const float* slopes,
                                     const int32_t* prefix, void* workspace, size_t workspace_bytes, void* out,
                                     spectra_stream_t stream) {
-  static_assert(8 * kFewGroups <= SPECTRA_PAGED_COUNTER_BYTES && 4 * kManySlots <= SPECTRA_PAGED_COUNTER_BYTES,
+  static_assert(8 * few_groups(kKv4, 16) <= SPECTRA_PAGED_COUNTER_BYTES && 4 * kManySlots <= SPECTRA_PAGED_COUNTER_BYTES,
                 "a counter for every slot");
   PagedLaunch a;
   if (int st = paged_args(kv, tokens, heads, &a.kv); st != SPECTRA_OK) return st;
@@ -468,7 +461,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   const int64_t tiles = kv->kv_heads * (all / rows + seqs);
   const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;
   SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
-  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(rows), tiles * cuts);
+  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(kv->kind, rows), tiles * cuts);
   a.units = (int)units;
   return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
 }
