@@ -177,7 +177,7 @@ class PagedWalk {
   PagedLine line;
 
   __device__ __forceinline__ PagedWalk(const PagedKv& kv, int g, int rows, int ks, const PagedScore& sc, int w, int groups, int lane)
-      : kv_(kv), sc_(sc), g_(g), rows_(rows), ks_(ks), lane_(lane), grain_(0), c0_(0), base_(0) {
+      : kv_(kv), sc_(sc), g_(g), rows_(rows), ks_(ks), lane_(lane), grain_(0), pad_(0), c0_(0), base_(0) {
     float sum = 0.0f;
     for (int c0 = 0; c0 < kv.batch; c0 += 64) {
       take(c0);
@@ -188,24 +188,26 @@ class PagedWalk {
       sum *= 0.5f;
       ++grain_;
     }
-    int total = 0;
-    if (kv.batch <= 64) {
-      if (grain_ > 0) take(0);
-      scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
-      total = __builtin_amdgcn_readlane(scan_, 63);
+    if (grain_ > 0) take(0);
+    int total = count();
+    line.each = (int)((uint32_t)max(total, 0) / (uint32_t)groups);
+    line.more = max(total, 0) - line.each * groups;
+    // where the tiles can be cut into as many equal pieces of their own, no share has parts of two
+    pad_ = line.each + (line.more > 0);
+    const int padded = pad_ > 0 ? count() : 0;
+    if (pad_ > 0 && padded >= 0 && padded <= groups * (int64_t)pad_) {
+      total = padded;
+      line.each = pad_;
+      line.more = 0;
     } else {
-      for (int c0 = 0; c0 < kv.batch; c0 += 64) {
-        take(c0);
-        total += __builtin_amdgcn_readlane(wave_scan(kv.kv_heads * tiles_ * steps_), 63);
-      }
-      take(0);
-      scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
+      pad_ = 0;
+      if (kv.batch <= 64) take(0);
     }
+    if (kv.batch > 64) take(0);
+    scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
     line.total = max(total, 0);
-    line.each = (int)((uint32_t)line.total / (uint32_t)groups);
-    line.more = line.total - line.each * groups;
-    line.begin = sread(line.start(w));
-    line.end = sread(line.start(w + 1));
+    line.begin = sread(min(line.start(w), line.total));
+    line.end = sread(min(line.start(w + 1), line.total));
   }
 
   // The part of the share that begins at x; x never goes back.  false: there is none.
@@ -238,16 +240,26 @@ class PagedWalk {
   }
 
  private:
+  // The line's length, with tiles of whole pad_ steps where there is one.
+  __device__ __forceinline__ int count() {
+    int total = 0;
+    for (int c0 = 0; c0 < kv_.batch; c0 += 64) {
+      if (kv_.batch > 64 || pad_ > 0) take(c0);
+      total += __builtin_amdgcn_readlane(wave_scan(kv_.kv_heads * tiles_ * steps_), 63);
+    }
+    return total;
+  }
   __device__ __forceinline__ void take(int c0) {
     const int b = min(c0 + lane_, kv_.batch - 1);
     seq_ = paged_seq(kv_.q_start[b], kv_.q_start[b + 1], kv_.lens[b], kv_.tokens);
     tiles_ = c0 + lane_ < kv_.batch ? (seq_.n * g_ + rows_ - 1) / rows_ : 0;
     steps_ = paged_steps(kv_, sc_, seq_.len, rows_ / g_, ks_);
     steps_ = max((steps_ + (1 << grain_) - 1) >> grain_, 1);
+    if (pad_ > 0) steps_ = (int)((uint32_t)(steps_ + pad_ - 1) / (uint32_t)pad_) * pad_;
   }
   const PagedKv& kv_;
   const PagedScore& sc_;
-  int g_, rows_, ks_, lane_, grain_, c0_, base_, scan_, tiles_, steps_;
+  int g_, rows_, ks_, lane_, grain_, pad_, c0_, base_, scan_, tiles_, steps_;
   PagedSeq seq_;
 };
 

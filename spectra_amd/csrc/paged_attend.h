@@ -214,12 +214,11 @@ __device__ __forceinline__ float2 load_dev2(const float* p) {
 
 // A row's pieces (slot_of(p) the p-th's record) joined in their order, whatever order they arrived in: dims d .. d + 3 of the sum
 // of weight times value, and the total.
-template <int HD, int ROWS, typename F>
-__device__ __forceinline__ float paged_join(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
-  constexpr int U = 4;  // pieces in flight
+template <int HD, int ROWS, int U, typename F>
+__device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
   float mm = -INFINITY, den = 0.0f;
   v[0] = v[1] = v[2] = v[3] = 0.0f;
-  for (int p0 = 0; p0 < pieces; p0 += U) {
+  for (int p0 = 0; p0 < pieces; p0 += U) {  // U in flight
     float2 ml[U], x[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -249,6 +248,11 @@ __device__ __forceinline__ float paged_join(const float* slots, F slot_of, int p
   }
   return den;
 }
+template <int HD, int ROWS, typename F>
+__device__ __forceinline__ float paged_join(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
+  return pieces <= 4 ? paged_join_by<HD, ROWS, 4>(slots, slot_of, pieces, row, d, v)
+                     : paged_join_by<HD, ROWS, 16>(slots, slot_of, pieces, row, d, v);
+}
 
 // The host side of a launch, shared by the kernels' translation units.
 struct PagedLaunch {
@@ -266,12 +270,18 @@ struct PagedLaunch {
 // Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows, as many
 // workgroups as are resident at once, and two partial tiles each at most.
 constexpr int kFewKeys = 128;
-constexpr int few_resident(int kind, int rows) { return rows == 32 ? 1 : kind == kKv4 ? 3 : 2; }  // workgroups a compute unit
-constexpr int few_groups(int kind, int rows) { return 256 * few_resident(kind, rows); }
-constexpr int kFewSlotRows = 2 * few_groups(kKv4, 16) * 16;  // the most: two records of 16 rows each
+// workgroups a compute unit (by their registers)
+constexpr int few_resident(int kind, int hd, int rows) {
+  return rows == 32 ? (hd == 128 ? 1 : 2) : kind == kKv4 ? 3 : 2;
+}
+constexpr int few_groups(int kind, int hd, int rows) { return 256 * few_resident(kind, hd, rows); }
+constexpr int kFewSlotRows = 2 * 512 * 32;  // the most: two records each, of 512 workgroups of 32 rows
+static_assert(2 * few_groups(kKv4, 128, 16) * 16 <= kFewSlotRows && 2 * few_groups(kKv4, 64, 32) * 32 <= kFewSlotRows, "");
 int launch_paged_few(const PagedLaunch& a, int rows);
 // Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.
-constexpr int kManyBig = 384, kManyKeys = 64, kManyMinSteps = 8, kManyTarget = 256, kManySlots = 2 * kManyTarget;
+constexpr int many_waves(int rows) { return 4; }
+constexpr int many_keys(int waves) { return 16 * waves; }  // of a step
+constexpr int kManyBig = 512, kManyMinKeys = 512, kManyTarget = 256, kManySlots = 2 * kManyTarget;
 int launch_paged_many(const PagedLaunch& a, int rows);
 
 }  // namespace spectra

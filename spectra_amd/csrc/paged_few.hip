@@ -41,7 +41,7 @@ constexpr int few_lds() {
 }
 
 template <int HD, int KIND, int NT, bool MOD>
-__global__ void __launch_bounds__(kFewThreads, few_resident(KIND, 16 * NT))
+__global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
     paged_few_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                      uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;

@@ -16,14 +16,17 @@
 
 namespace spectra {
 
-constexpr int kManyThreads = 256;
 
 // The buffers of keys, then of values: two each, a row of 16-byte chunks a key.  Chunk c of key r lies
-// at c ^ (r & 7) in K's rows (eight rows' equal chunks, which lanes read at once, on different
-// banks) and at c ^ v_turn(r) in V's (four rows' 64 bytes, read transposed, on different banks).
-template <int HD>
+// at c ^ k_turn(r) in K's rows (16 rows' equal chunks, which lanes read at once, on different banks)
+// and at c ^ v_turn(r) in V's (four rows' 64 bytes, read transposed, on different banks).
+template <int HD, int W>
 constexpr int many_lds() {
-  return 4 * kManyKeys * HD * 2;
+  return 4 * many_keys(W) * HD * 2;
+}
+template <int HD>
+__device__ __forceinline__ int k_turn(int r) {
+  return HD == 128 ? r & 15 : (r >> 1) & 7;
 }
 template <int HD>
 __device__ __forceinline__ int v_turn(int r) {
@@ -38,14 +41,16 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4_t*)(lds_t)p));
 }
 
-template <int HD, int KIND, bool MOD, int QH>
-__global__ void __launch_bounds__(kManyThreads, 2)
+template <int HD, int KIND, bool MOD, int QH, int W>
+__global__ void __launch_bounds__(64 * W, 2)
     paged_many_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                       uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
   constexpr int CH = HD / 8, KS = HD / 16, DT = HD / 32;  // 8-dim chunks, 16-dim steps, 32-dim tiles
-  constexpr int KL = kManyKeys * CH / kManyThreads;       // K chunks a thread copies
-  constexpr int ROWS = 32 * QH, TL = QH / 2;              // 32-key tiles of a step that a wave takes
+  constexpr int KEYS = many_keys(W), THREADS = 64 * W;    // keys of a step
+  constexpr int KL = KEYS * CH / THREADS;                 // K chunks a thread copies
+  constexpr int KH = W / QH;                              // waves that share a step's keys
+  constexpr int ROWS = 32 * QH, TL = KEYS / (32 * KH);    // 32-key tiles of a step that a wave takes
   constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int flag;
@@ -53,7 +58,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), gh = lane >> 5, ln = lane & 31;
   const int qh = wave % QH, kh = wave / QH;  // the wave's 32 rows, and its share of a step's keys
   PagedUnit un;
-  if (!paged_unit(kv, g, ROWS, kManyKeys, kManyMinSteps, kManyTarget, kManySlots, sc, blockIdx.x, lane, un)) return;
+  if (!paged_unit(kv, g, ROWS, KEYS, kManyMinKeys / KEYS, kManyTarget, kManySlots, sc, blockIdx.x, lane, un)) return;
   const PagedSeq sq = un.seq;
   const int r0 = un.tile * ROWS, nrows = min(ROWS, sq.n * g - r0);
   const int tok0 = sread(r0 / g), tok1 = sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;
@@ -61,8 +66,8 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   // keys that some row of the tile sees
   const PagedRange ra = paged_range(i0 + tok0, sq.len, un.prefix, sc.window);
   const PagedRange rb = paged_range(i0 + tok1, sq.len, un.prefix, sc.window);
-  const int klo = ra.lo, khi = min(rb.hi, capacity), kbeg = klo & ~(kManyKeys - 1);
-  const int steps = khi > kbeg ? (khi - kbeg + kManyKeys - 1) / kManyKeys : 0;
+  const int klo = ra.lo, khi = min(rb.hi, capacity), kbeg = klo & ~(KEYS - 1);
+  const int steps = khi > kbeg ? (khi - kbeg + KEYS - 1) / KEYS : 0;
   const int sbeg = sread((int)((int64_t)steps * un.piece / un.pieces));
   const int send = sread((int)((int64_t)steps * (un.piece + 1) / un.pieces));
   // keys that all of this wave's rows see; the lane's row
@@ -87,14 +92,14 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     }
   }
 
-  // ---- staging: a step is 4 blocks of 16 keys, each in one page; a wave copies one block, so it
-  // needs one page id a step.  16-bit rows go to LDS directly; 4-bit ones through registers, where
+  // ---- staging: a step is a block of 16 keys a wave, in one page: a wave copies its block and needs one
+  // page id a step.  16-bit rows go to LDS directly; 4-bit ones through registers, where
   // they are expanded (K's in the order of its codes, as Q is; V's put back in order).
   const int* tab = kv.table + un.b * kv.table_stride;
   auto page_of = [&](int k0) __attribute__((always_inline)) {
     return sread(sload(tab + min((k0 + 16 * wave) >> kv.page_shift, kv.table_width - 1)));
   };
-  constexpr int KB = kManyKeys * HD * 2, RPI = 64 / CH;  // bytes of a buffer, rows of 64 lanes' chunks
+  constexpr int KB = KEYS * HD * 2, RPI = 64 / CH;  // bytes of a buffer, rows of 64 lanes' chunks
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t)lds;
   const int kc = lane % CH, krow = lane / CH;
   constexpr uint32_t nan2 = BF ? 0x7fc07fc0u : 0x7e007e00u;
@@ -118,7 +123,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
         const int r = krow + i * RPI;
-        copy_lds(base, r * ROWB + 16 * (kc ^ (value ? v_turn<HD>(r) : r & 7)),
+        copy_lds(base, r * ROWB + 16 * (kc ^ (value ? v_turn<HD>(r) : k_turn<HD>(r))),
                  lds0 + (value ? 2 * KB : 0) + buf * KB + (16 * wave + i * RPI) * HD * 2);
       }
     }
@@ -127,7 +132,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   // of keys that no row sees (they must not reach the product).
   auto land = [&](bool value, int k0, int id, int buf, const Codes& cd) __attribute__((always_inline)) {
     uint8_t* to = lds + (value ? 2 * KB : 0) + buf * KB;
-    const bool edge = value && (k0 < klo || k0 + kManyKeys > khi), bad = !value && (uint32_t)id >= (uint32_t)kv.num_pages;
+    const bool edge = value && (k0 < klo || k0 + KEYS > khi), bad = !value && (uint32_t)id >= (uint32_t)kv.num_pages;
     if (!Q4 && !edge && !bad) return;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
                       __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
       }
       if (bad) x = (pu4_t){nan2, nan2, nan2, nan2};
-      if (Q4 || bad || out) *(pu4_t*)(to + key * HD * 2 + 16 * (kc ^ (value ? v_turn<HD>(key) : key & 7))) = x;
+      if (Q4 || bad || out) *(pu4_t*)(to + key * HD * 2 + 16 * (kc ^ (value ? v_turn<HD>(key) : k_turn<HD>(key)))) = x;
     }
   };
 
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   const int kbase = (32 * TL * kh + ln) * HD * 2;
   auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
     const int t = i / KS, st = i % KS;
-    return *(const pu4_t*)(lds + buf * KB + kbase + 64 * t * HD + 16 * ((2 * (st & 3) + gh) ^ (ln & 7)) + 128 * (st >> 2));
+    return *(const pu4_t*)(lds + buf * KB + kbase + 64 * t * HD + 16 * ((2 * st + gh) ^ k_turn<HD>(ln)));
   };
   const int vi = lane & 15, vbase = (32 * TL * kh + 4 * gh + (vi >> 2)) * HD * 2 + 8 * (vi & 1);
   const int vchunk = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
@@ -242,38 +247,38 @@ __global__ void __launch_bounds__(kManyThreads, 2)
 
   if (sbeg < send) {
     // At step s the buffers hold K of s + 1 and V of s; K of s + 2 and V of s + 1 are on their way.
-    int k0 = kbeg + sbeg * kManyKeys;
-    const int kend = kbeg + send * kManyKeys;
+    int k0 = kbeg + sbeg * KEYS;
+    const int kend = kbeg + send * KEYS;
     pf16_t s0[TL], s1[TL];
-    int id0 = page_of(k0), id1 = page_of(k0 + kManyKeys), id2 = page_of(k0 + 2 * kManyKeys);
+    int id0 = page_of(k0), id1 = page_of(k0 + KEYS), id2 = page_of(k0 + 2 * KEYS);
     auto wait = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
     fetch(false, k0, id0, 0, kcodes);
     fetch(true, k0, id0, 0, vcodes);
     wait();
     land(false, k0, id0, 0, kcodes);
     land(true, k0, id0, 0, vcodes);
-    fetch(false, k0 + kManyKeys, id1, 1, kcodes);
+    fetch(false, k0 + KEYS, id1, 1, kcodes);
     wait();
-    land(false, k0 + kManyKeys, id1, 1, kcodes);
+    land(false, k0 + KEYS, id1, 1, kcodes);
     __syncthreads();
     product(s0, 0);
     __syncthreads();  // (K of the first step is read: its buffer is free)
     auto turn = [&](pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf) __attribute__((always_inline)) {
-      const bool more = k0 + kManyKeys < kend;
+      const bool more = k0 + KEYS < kend;
       if (more) {
-        fetch(false, k0 + 2 * kManyKeys, id2, buf, kcodes);
-        fetch(true, k0 + kManyKeys, id1, buf ^ 1, vcodes);
+        fetch(false, k0 + 2 * KEYS, id2, buf, kcodes);
+        fetch(true, k0 + KEYS, id1, buf ^ 1, vcodes);
       }
-      const int id3 = page_of(k0 + 3 * kManyKeys);
+      const int id3 = page_of(k0 + 3 * KEYS);
       step(k0, s, sn, buf);
       if (!more) return false;
       wait();
-      land(false, k0 + 2 * kManyKeys, id2, buf, kcodes);
-      land(true, k0 + kManyKeys, id1, buf ^ 1, vcodes);
+      land(false, k0 + 2 * KEYS, id2, buf, kcodes);
+      land(true, k0 + KEYS, id1, buf ^ 1, vcodes);
       __syncthreads();
       id1 = id2;
       id2 = id3;
-      k0 += kManyKeys;
+      k0 += KEYS;
       return true;
     };
     while (turn(s0, s1, 0) && turn(s1, s0, 1)) {
@@ -281,36 +286,51 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   }
 
   l += lane_xor<32>(l, lane);
-  if constexpr (QH == 2) {  // the key halves meet
-    float4* red = (float4*)lds;  // [query half][4 DT][lane]
-    float2* ml = (float2*)(lds + 2 * 16 * DT * 64 * 4);
-    static_assert(2 * 16 * DT * 64 * 4 + 2 * 64 * 8 <= many_lds<HD>(), "a half's sums fit the buffers");
+  if constexpr (KH > 1) {  // the waves that shared the keys meet
+    float4* red = (float4*)lds;  // [wave past the first QH][4 DT][lane]
+    float2* ml = (float2*)(lds + (W - QH) * 16 * DT * 64 * 4);
+    static_assert((W - QH) * (16 * DT * 64 * 4 + 64 * 8) <= many_lds<HD, W>(), "their sums fit the buffers");
     __syncthreads();
-    if (kh == 1) {
+    if (kh > 0) {
+      const int at = wave - QH;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          red[(qh * 4 * DT + 4 * d + r) * 64 + lane] = make_float4(o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
-      ml[qh * 64 + lane] = make_float2(m, l);
+          red[(at * 4 * DT + 4 * d + r) * 64 + lane] = make_float4(o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
+      ml[at * 64 + lane] = make_float2(m, l);
     }
     __syncthreads();
     if (kh == 0) {
-      const float2 x = ml[qh * 64 + lane];
-      const float mm = fmaxf(m, x.x);
-      const float c0 = paged_weight(m, l, mm), c1 = paged_weight(x.x, x.y, mm);
-      l = l * c0 + x.y * c1;
+      float2 x[KH - 1];
+      float mm = m;
+#pragma unroll
+      for (int k = 0; k < KH - 1; ++k) {
+        x[k] = ml[(k * QH + qh) * 64 + lane];
+        mm = fmaxf(mm, x[k].x);
+      }
+      const float c0 = paged_weight(m, l, mm);
+      l *= c0;
       m = mm;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float4 y = red[(qh * 4 * DT + 4 * d + r) * 64 + lane];
-          o[d][4 * r] = o[d][4 * r] * c0 + y.x * c1;
-          o[d][4 * r + 1] = o[d][4 * r + 1] * c0 + y.y * c1;
-          o[d][4 * r + 2] = o[d][4 * r + 2] * c0 + y.z * c1;
-          o[d][4 * r + 3] = o[d][4 * r + 3] * c0 + y.w * c1;
-        }
+        for (int r = 0; r < 16; ++r) o[d][r] *= c0;
+#pragma unroll
+      for (int k = 0; k < KH - 1; ++k) {
+        const float c = paged_weight(x[k].x, x[k].y, mm);
+        l += c * x[k].y;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float4 y = red[((k * QH + qh) * 4 * DT + 4 * d + r) * 64 + lane];
+            o[d][4 * r] += c * y.x;
+            o[d][4 * r + 1] += c * y.y;
+            o[d][4 * r + 2] += c * y.z;
+            o[d][4 * r + 3] += c * y.w;
+          }
+      }
     }
   }
   const bool mixed = tok1 > tok0;  // rows that see different keys
@@ -352,10 +372,10 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       if (gh == 0) store_dev2(p + ROWS * HD + 2 * (32 * qh + ln), m, l);
     }
     if (!paged_arrive(counters + first, un.pieces, &flag)) return;
-    for (int it = tid; it < nrows * (HD / 4); it += kManyThreads) {
+    for (int it = tid; it < nrows * (HD / 4); it += THREADS) {
       const int row = it / (HD / 4), d = 4 * (it % (HD / 4)), r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g);
       float v[4], y[4];
-      const float den = paged_join<HD, ROWS>(slots, [&](int p) { return first + p; }, un.pieces, row, d, v);
+      const float den = paged_join_by<HD, ROWS, 4>(slots, [&](int p) { return first + p; }, un.pieces, row, d, v);
       const bool past = paged_range(i0 + t, sq.len, un.prefix, sc.window).hi > capacity;
       bool odd = false;
 #pragma unroll
@@ -374,19 +394,19 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + 32 * qh + __builtin_ctz(r), out);
 }
 
-template <int HD, int KIND, bool MOD, int QH>
+template <int HD, int KIND, bool MOD, int QH, int W>
 static int launch_many(const PagedLaunch& a) {
-  const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD, QH>;
+  const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD, QH, W>;
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
-  paged_many_kernel<HD, KIND, MOD, QH><<<dim3((unsigned)a.units), dim3(kManyThreads), many_lds<HD>(), a.stream>>>(
+  paged_many_kernel<HD, KIND, MOD, QH, W><<<dim3((unsigned)a.units), dim3(64 * W), many_lds<HD, W>(), a.stream>>>(
       a.kv, a.sc, a.q, a.ldq, a.g, a.heads, a.counters, a.slots, a.out);
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
 }
 template <int HD, int KIND>
 static int launch_many_of(const PagedLaunch& a, int rows) {
-  if (rows == 64) return a.mod ? launch_many<HD, KIND, true, 2>(a) : launch_many<HD, KIND, false, 2>(a);
-  return a.mod ? launch_many<HD, KIND, true, 4>(a) : launch_many<HD, KIND, false, 4>(a);
+  if (rows == 64) return a.mod ? launch_many<HD, KIND, true, 2, many_waves(64)>(a) : launch_many<HD, KIND, false, 2, many_waves(64)>(a);
+  return a.mod ? launch_many<HD, KIND, true, 4, many_waves(128)>(a) : launch_many<HD, KIND, false, 4, many_waves(128)>(a);
 }
 int launch_paged_many(const PagedLaunch& a, int rows) {
   if (a.hd == 64)
@@ -418,7 +438,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
                                     int32_t heads, float scale, float cap, int32_t window, const float* slopes,
                                     const int32_t* prefix, void* workspace, size_t workspace_bytes, void* out,
                                     spectra_stream_t stream) {
-  static_assert(8 * few_groups(kKv4, 16) <= SPECTRA_PAGED_COUNTER_BYTES && 4 * kManySlots <= SPECTRA_PAGED_COUNTER_BYTES,
+  static_assert(8 * few_groups(kKv4, 128, 16) <= SPECTRA_PAGED_COUNTER_BYTES && 4 * kManySlots <= SPECTRA_PAGED_COUNTER_BYTES,
                 "a counter for every slot");
   PagedLaunch a;
   if (int st = paged_args(kv, tokens, heads, &a.kv); st != SPECTRA_OK) return st;
@@ -456,12 +476,12 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   const int64_t all = tokens * a.g, seqs = tokens < kv->batch ? tokens : kv->batch;
   const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv->kv_heads * all <= 128 * kManyBig ? 64 : 128;
   const bool many = rows >= 64;
-  const int keys = many ? kManyKeys : kFewKeys;
+  const int keys = many ? many_keys(many_waves(rows)) : kFewKeys;
   // at most this many tiles, each of at most as many key steps as its table has
   const int64_t tiles = kv->kv_heads * (all / rows + seqs);
   const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;
   SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
-  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(kv->kind, rows), tiles * cuts);
+  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(kv->kind, kv->head_dim, rows), tiles * cuts);
   a.units = (int)units;
   return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
 }
