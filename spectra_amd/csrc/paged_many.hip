@@ -106,11 +106,22 @@ __global__ void __launch_bounds__(64 * W, 2)
   struct Codes {
     uint32_t w[KL], s[KL], z[KL];
   } kcodes, vcodes;
-  auto fetch = [&](bool value, int k0, int id, int buf, Codes& cd) __attribute__((always_inline)) {
-    const int pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0;
+  // where a wave's block of step k0 begins in K (and V, their pages lying alike)
+  auto place = [&](int k0, int id) __attribute__((always_inline)) {
     const int row = (un.kvh << kv.page_shift) + ((k0 + 16 * wave) & pmask);
-    const uint8_t* base = (value ? kv.v : kv.k) + paged_at(pg, kv.page_step) + row * ROWB;
+    return paged_at((uint32_t)id < (uint32_t)kv.num_pages ? id : 0, kv.page_step) + row * ROWB;
+  };
+  auto copy = [&](bool value, uint64_t at, int buf, int i) __attribute__((always_inline)) {
+    const int r = krow + i * RPI;
+    const uint8_t* base = (value ? kv.v : kv.k) + at;
+    const uint32_t off = r * ROWB + 16 * (kc ^ (value ? v_turn<HD>(r) : k_turn<HD>(r)));
+    const uint32_t to = lds0 + (value ? 2 * KB : 0) + buf * KB + (16 * wave + i * RPI) * HD * 2;
+    copy_lds(base, off, to);
+  };
+  auto fetch = [&](bool value, int k0, int id, int buf, Codes& cd) __attribute__((always_inline)) {
     if constexpr (Q4) {
+      const int pg = (uint32_t)id < (uint32_t)kv.num_pages ? id : 0, row = (un.kvh << kv.page_shift) + ((k0 + 16 * wave) & pmask);
+      const uint8_t* base = (value ? kv.v : kv.k) + paged_at(pg, kv.page_step) + row * ROWB;
       const uint8_t* sb = (value ? kv.vs : kv.ks) + paged_at(pg, kv.scale_step) + row * (HD / 16);
       const uint8_t* zb = (value ? kv.vz : kv.kz) + paged_at(pg, kv.zero_step) + row * (HD / 32);
 #pragma unroll
@@ -121,11 +132,7 @@ __global__ void __launch_bounds__(64 * W, 2)
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int r = krow + i * RPI;
-        copy_lds(base, r * ROWB + 16 * (kc ^ (value ? v_turn<HD>(r) : k_turn<HD>(r))),
-                 lds0 + (value ? 2 * KB : 0) + buf * KB + (16 * wave + i * RPI) * HD * 2);
-      }
+      for (int i = 0; i < KL; ++i) copy(value, place(k0, id), buf, i);
     }
   };
   // What was fetched is in place, with NaN for keys of a page that is not there, and zeros for values
@@ -179,9 +186,9 @@ __global__ void __launch_bounds__(64 * W, 2)
   };
   // One step: softmax of its scores s, their product with its values, and the next step's scores
   // into sn (past the last: of whatever its buffer holds, used by nothing).  The order is written out (the compiler would wait for every operand
-  // where it is used): operands are read RING instructions ahead, and the exponentials stand
-  // between the matrix instructions of Q K^T, which run beneath them.
-  auto step = [&](int k0, pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf) __attribute__((always_inline)) {
+  // where it is used): operands are read RING instructions ahead, and the exponentials, and the
+  // 2 KL copies `beside`, stand between the matrix instructions of Q K^T, which run beneath them.
+  auto step = [&](int k0, pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf, auto beside) __attribute__((always_inline)) {
     const int kw = k0 + 32 * TL * kh;  // this wave's keys
     pu4_t ring[RINGV];
 #pragma unroll
@@ -231,6 +238,8 @@ __global__ void __launch_bounds__(64 * W, 2)
       ring[i % RING] = i + RING < NK ? read_k(buf ^ 1, i + RING) : read_v(buf, i + RING - NK);  // (NK is a multiple of RING)
 #pragma unroll
       for (int j = i * 8 * TL / NK; j < (i + 1) * 8 * TL / NK; ++j) weights(j);
+#pragma unroll
+      for (int j = i * 2 * KL / NK; j < (i + 1) * 2 * KL / NK; ++j) beside(j);
       __builtin_amdgcn_sched_barrier(0);
     }
     // O^T += V^T P^T, 16 keys and 32 dims at a time; keys 16 u + {4 gh + 0 .. 3, 8 + 4 gh + 0 .. 3}
@@ -252,32 +261,39 @@ __global__ void __launch_bounds__(64 * W, 2)
     pf16_t s0[TL], s1[TL];
     int id0 = page_of(k0), id1 = page_of(k0 + KEYS), id2 = page_of(k0 + 2 * KEYS);
     auto wait = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
-    fetch(false, k0, id0, 0, kcodes);
+    Codes kfirst;
+    fetch(false, k0, id0, 0, kfirst);
     fetch(true, k0, id0, 0, vcodes);
-    wait();
-    land(false, k0, id0, 0, kcodes);
-    land(true, k0, id0, 0, vcodes);
     fetch(false, k0 + KEYS, id1, 1, kcodes);
     wait();
+    land(false, k0, id0, 0, kfirst);
+    land(true, k0, id0, 0, vcodes);
     land(false, k0 + KEYS, id1, 1, kcodes);
     __syncthreads();
     product(s0, 0);
     __syncthreads();  // (K of the first step is read: its buffer is free)
+    uint64_t at1 = place(k0 + KEYS, id1);
     auto turn = [&](pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf) __attribute__((always_inline)) {
       const bool more = k0 + KEYS < kend;
-      if (more) {
-        fetch(false, k0 + 2 * KEYS, id2, buf, kcodes);
-        fetch(true, k0 + KEYS, id1, buf ^ 1, vcodes);
+      const uint64_t at2 = place(k0 + 2 * KEYS, id2);
+      if constexpr (Q4) {
+        if (more) {
+          fetch(false, k0 + 2 * KEYS, id2, buf, kcodes);
+          fetch(true, k0 + KEYS, id1, buf ^ 1, vcodes);
+        }
       }
       const int id3 = page_of(k0 + 3 * KEYS);
-      step(k0, s, sn, buf);
+      step(k0, s, sn, buf, [&](int j) __attribute__((always_inline)) {
+        if constexpr (!Q4) copy(j >= KL, j < KL ? at2 : at1, j < KL ? buf : buf ^ 1, j % KL);
+      });
+      wait();  // (the last step's copies, too, which are of whatever comes next: LDS is used again)
       if (!more) return false;
-      wait();
       land(false, k0 + 2 * KEYS, id2, buf, kcodes);
       land(true, k0 + KEYS, id1, buf ^ 1, vcodes);
       __syncthreads();
       id1 = id2;
       id2 = id3;
+      at1 = at2;
       k0 += KEYS;
       return true;
     };
