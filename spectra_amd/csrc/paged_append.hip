@@ -33,7 +33,10 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
                                                                   const float* __restrict__ sin_t, int64_t rope_rows,
                                                                   int heads, int hd, int waves, const PagedKv kv,
                                                                   uint16_t* __restrict__ q_rot) {
-  const int lane = threadIdx.x & 63, wv = sread((int)(blockIdx.x * (kPaThreads / 64) + (threadIdx.x >> 6)));
+  // neighbouring blocks go to different XCDs: an eighth of the tokens each, so that rows beside each
+  // other meet in one L2 (4-bit rows are less than a line)
+  const uint32_t run = gridDim.x < 64 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int lane = threadIdx.x & 63, wv = sread((int)(run * (kPaThreads / 64) + (threadIdx.x >> 6)));
   const int t = wv / waves;  // this wave's token
   if (t >= kv.tokens) return;
   const int it = (wv - t * waves) * 64 + lane;  // item of the token
@@ -87,13 +90,13 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
       *(uint4*)dst = lo;
       *(uint4*)(dst + h2) = hi;
     }
-    if (Q4) {  // (the lanes of a group of 32 dims are four of one head; queries ride along)
+    if (Q4 && hh >= heads) {  // (the lanes of a group of 32 dims are four of one head)
       uint32_t pk[2];
       uint16_t sb[2];
       uint8_t zb[2];
       kv4_quant_chunk(lo, pk[0], sb[0], zb[0]);
       kv4_quant_chunk(hi, pk[1], sb[1], zb[1]);
-      if (hh >= heads && keep) {
+      if (keep) {
         const int64_t hr = ((int64_t)(hh - heads) << kv.page_shift) + r;  // row of the page
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -198,7 +201,8 @@ extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const voi
                       ldqkv % 8 == 0,
                   "operands and qkv rows must be 16-byte aligned");
   int waves = ((heads + kv->kv_heads) * (hd / 16) + kv->kv_heads * (hd / 8) + 63) / 64;
-  const int64_t blocks = (tokens * waves + kPaThreads / 64 - 1) / (kPaThreads / 64);
+  int64_t blocks = (tokens * waves + kPaThreads / 64 - 1) / (kPaThreads / 64);
+  if (blocks >= 64) blocks = (blocks + 7) / 8 * 8;
   SPECTRA_REQUIRE(tokens * waves < (1LL << 31) - 256, "tokens out of range");
   const void* kern = kv->kind == SPECTRA_KV_4BIT ? (const void*)paged_append_kernel<false, true>
                      : kv->kind == SPECTRA_KV_BF16 ? (const void*)paged_append_kernel<true, false>
