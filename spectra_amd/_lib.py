@@ -179,3 +179,17 @@ def check(fn_name: str, status: int) -> None:
         if status == ERR_INVALID:
             raise ValueError(f"{fn_name}: {msg}")
         raise SpectraError(fn_name, status, msg)
+
+
+_ops_module = None
+
+
+def torch_ops_module():
+    """The operator library as a Python module (its functions take the operators' arguments past the
+    dispatcher); loaded once, and raising when it is unavailable."""
+    global _ops_module
+    if _ops_module is None:
+        load_torch_ops()
+        from . import _spectra_torch
+        _ops_module = _spectra_torch
+    return _ops_module

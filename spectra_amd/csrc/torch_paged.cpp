@@ -1,18 +1,29 @@
 // The paged KV cache's operators as registered PyTorch operators: torch.ops.spectra_hip.
 // paged_rope_append and paged_attend (no counterpart in the reference).
 //
-// One dispatcher call each: the checks of shapes, types, strides and devices, the descriptor, the
-// output from the caching allocator and the launch on the current HIP stream of the operands'
-// device.  A single-token step is launch-bound, and the same checks in Python with a ctypes
-// call took 18 us, three times the kernel.  Bad arguments raise ValueError; other failures
-// RuntimeError naming the status.
+// One call each: the checks of shapes, types, strides and devices, the descriptor, the output from
+// the caching allocator and the launch on the current HIP stream of the operands' device.  A
+// single-token step is launch-bound: the same checks in Python with a ctypes call took 18 us, three
+// times the kernel.  Bad arguments raise ValueError; other failures RuntimeError naming the status.
+//
+// The library is a Python module, too, whose two functions take the same arguments and go past the
+// dispatcher (some 2 us a call for this many arguments) where it would only have passed them on:
+// plain tensors, and no mode that wants to see operators.  Otherwise they return NotImplemented, and the
+// caller takes the registered operator, which a compiler traces.
+#include <Python.h>
+
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
+#include <vector>
 
 #include "spectra_hip.h"
 
@@ -221,7 +232,112 @@ void paged_attend_out_meta(const at::Tensor&, const at::Tensor&, const at::Tenso
                            at::TensorList, double, double, int64_t, const OptTensor&, const OptTensor&, const OptTensor&,
                            const at::Tensor&) {}
 
+// ---- the Python functions ----
+struct Arguments {
+  PyObject* const* a;
+  bool plain = true;  // nothing but plain tensors, of a device, where tensors belong
+
+  const at::Tensor* tensor(int i) {
+    plain = plain && THPVariable_CheckExact(a[i]) && THPVariable_Unpack(a[i]).is_cuda();
+    return plain ? &THPVariable_Unpack(a[i]) : nullptr;
+  }
+  OptTensor optional(int i) {
+    if (a[i] == Py_None) return c10::nullopt;
+    const at::Tensor* t = tensor(i);
+    return t != nullptr ? OptTensor(*t) : c10::nullopt;
+  }
+  std::vector<at::Tensor> list(int i) {  // a tensor, or a tuple or list of them
+    std::vector<at::Tensor> r;
+    if (THPVariable_Check(a[i])) {
+      if (const at::Tensor* t = tensor(i)) r.push_back(*t);
+      return r;
+    }
+    if (!(plain = plain && (PyTuple_Check(a[i]) || PyList_Check(a[i])))) return r;
+    PyObject** items = PySequence_Fast_ITEMS(a[i]);
+    for (Py_ssize_t j = 0; j < PySequence_Fast_GET_SIZE(a[i]) && plain; ++j) {
+      plain = THPVariable_CheckExact(items[j]) && THPVariable_Unpack(items[j]).is_cuda();
+      if (plain) r.push_back(THPVariable_Unpack(items[j]));
+    }
+    plain = plain && !r.empty();
+    return r;
+  }
+  double number(int i) {
+    const bool is = PyFloat_Check(a[i]) || PyLong_Check(a[i]);
+    const double v = is ? PyFloat_AsDouble(a[i]) : 0.0;
+    return whole(is, v);
+  }
+  int64_t integer(int i) {
+    const bool is = PyLong_Check(a[i]);
+    return whole(is, is ? (int64_t)PyLong_AsLongLong(a[i]) : 0);
+  }
+
+ private:
+  template <typename T>
+  T whole(bool is, T v) {
+    if (PyErr_Occurred() != nullptr) {  // (out of range: the operator says so)
+      PyErr_Clear();
+      is = false;
+    }
+    plain = plain && is;
+    return v;
+  }
+};
+
+// Something else wants to see the operators: a mode, or a key that the thread includes.
+bool dispatched() {
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+         !(c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty();
+}
+
+PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "paged_rope_append takes 10 arguments");
+  Arguments a{args};
+  const at::Tensor *qkv = a.tensor(0), *lens = a.tensor(1), *starts = a.tensor(2), *table = a.tensor(3);
+  const OptTensor cos = a.optional(4), sin = a.optional(5), out = a.optional(9);
+  const int64_t heads = a.integer(6);
+  const std::vector<at::Tensor> k = a.list(7), v = a.list(8);
+  if (!a.plain || dispatched()) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor q;
+  {
+    pybind11::gil_scoped_release release;
+    q = append(*qkv, *lens, *starts, *table, cos, sin, heads, k, v, out.has_value() ? &*out : nullptr);
+  }
+  return THPVariable_Wrap(q);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 13, "paged_attend takes 13 arguments");
+  Arguments a{args};
+  const at::Tensor *q = a.tensor(0), *lens = a.tensor(1), *starts = a.tensor(2), *table = a.tensor(3);
+  const std::vector<at::Tensor> k = a.list(4), v = a.list(5);
+  const bool usual = args[6] == Py_None;  // 1 / sqrt(d)
+  double scale = usual ? 1.0 : a.number(6);
+  const double cap = a.number(7);
+  const int64_t window = a.integer(8);
+  const OptTensor slopes = a.optional(9), prefix = a.optional(10), workspace = a.optional(11), out = a.optional(12);
+  if (!a.plain || dispatched()) Py_RETURN_NOTIMPLEMENTED;
+  if (usual && q->dim() == 3) scale = 1.0 / std::sqrt((double)q->size(2));
+  at::Tensor o;
+  {
+    pybind11::gil_scoped_release release;
+    o = attend(*q, *lens, *starts, *table, k, v, scale, cap, window, slopes, prefix, workspace, out.has_value() ? &*out : nullptr);
+  }
+  return THPVariable_Wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef kMethods[] = {
+    {"paged_rope_append", (PyCFunction)(void*)py_append, METH_FASTCALL, nullptr},
+    {"paged_attend", (PyCFunction)(void*)py_attend, METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_spectra_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+
 }  // namespace
+
+PyMODINIT_FUNC PyInit__spectra_torch(void) { return PyModule_Create(&kModule); }
 
 TORCH_LIBRARY_FRAGMENT(spectra_hip, m) {
   m.def(

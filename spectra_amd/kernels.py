@@ -736,22 +736,10 @@ def attend_decode_q4(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
 # ---------------------------------------------------------------------------
 # the paged KV cache: a batch of sequences
 # ---------------------------------------------------------------------------
-_PAGED_OPS = {}
-
-
-def _paged_op(name: str, *args):
-    """One registered operator over the C entry (csrc/torch_paged.cpp): its checks raise ValueError,
-    the library's other failures SpectraError."""
-    op = _PAGED_OPS.get(name)
-    if op is None:
-        op = _PAGED_OPS[name] = getattr(L.load_torch_ops(), name).default
-    try:
-        return op(*args)
-    except RuntimeError as e:
-        status = re.search(r"(spectra_\w+) failed \((-\d+)\): (.*)", str(e))
-        if status is None:
-            raise
-        raise L.SpectraError(status[1], int(status[2]), status[3]) from None
+def _paged_error(e: RuntimeError) -> RuntimeError:
+    """The library's failure of a status as SpectraError; other errors as they are."""
+    status = re.search(r"(spectra_\w+) failed \((-\d+)\): (.*)", str(e))
+    return e if status is None else L.SpectraError(status[1], int(status[2]), status[3])
 
 
 def _pages(p) -> List[torch.Tensor]:
@@ -776,11 +764,19 @@ def paged_rope_append(qkv: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.T
     table its queries are NaN); rows behind q_start[-1] are left alone."""
     if not qkv.is_cuda:
         raise ValueError("qkv must be on the GPU")
-    args = (qkv, kv_lens, q_start, block_table, cos, sin, heads, _pages(k_pages), _pages(v_pages))
-    if q_out is None:
-        return _paged_op("paged_rope_append", *args)
-    _paged_op("paged_rope_append_out", *args, q_out)
-    return q_out
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            q = (L._ops_module or L.torch_ops_module()).paged_rope_append(
+                qkv, kv_lens, q_start, block_table, cos, sin, heads, k_pages, v_pages, q_out)
+            if q is not NotImplemented:
+                return q
+        args = (qkv, kv_lens, q_start, block_table, cos, sin, heads, _pages(k_pages), _pages(v_pages))
+        if q_out is None:
+            return torch.ops.spectra_hip.paged_rope_append.default(*args)
+        torch.ops.spectra_hip.paged_rope_append_out.default(*args, q_out)
+        return q_out
+    except RuntimeError as e:
+        raise _paged_error(e) from None
 
 
 def paged_attend_workspace(head_dim: int, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -813,11 +809,17 @@ def paged_attend(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
     one, which costs a small kernel."""
     if not q.is_cuda:
         raise ValueError("q must be on the GPU")
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
-    args = (q, kv_lens, q_start, block_table, _pages(k_pages), _pages(v_pages), scale, cap, window, slopes, prefix,
-            workspace)
-    if out is None:
-        return _paged_op("paged_attend", *args)
-    _paged_op("paged_attend_out", *args, out)
-    return out
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            o = (L._ops_module or L.torch_ops_module()).paged_attend(
+                q, kv_lens, q_start, block_table, k_pages, v_pages, scale, cap, window, slopes, prefix, workspace, out)
+            if o is not NotImplemented:
+                return o
+        args = (q, kv_lens, q_start, block_table, _pages(k_pages), _pages(v_pages),
+                q.shape[-1] ** -0.5 if scale is None else scale, cap, window, slopes, prefix, workspace)
+        if out is None:
+            return torch.ops.spectra_hip.paged_attend.default(*args)
+        torch.ops.spectra_hip.paged_attend_out.default(*args, out)
+        return out
+    except RuntimeError as e:
+        raise _paged_error(e) from None

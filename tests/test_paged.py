@@ -695,3 +695,57 @@ def test_wrapper_refuses_host_tensors():
     with pytest.raises(ValueError, match="GPU"):
         K.paged_rope_append(torch.zeros(1, 8 * 64, dtype=torch.float16), one, torch.tensor([0, 1], dtype=torch.int32),
                             one[:, None], None, None, 4, pages, pages)
+
+
+@pytest.mark.gpu
+def test_registered_operators(hip):
+    """The registered operators give what the functions give, and a whole-graph compilation traces them."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [1, 3], [70, 33], 4, 2, 64, 16, seed=16)
+    ops = L.load_torch_ops()
+    ws = K.paged_attend_workspace(64)
+    args = (b.q, b.kv_lens, b.q_start, b.table, [b.k], [b.v], 0.125, 2.0, 20, None, None, ws)
+    want = b.attend(cap=2.0, window=20)
+    assert torch.equal(ops.paged_attend(*args), want)
+    out = torch.empty_like(want)
+    ops.paged_attend_out(*args, out)
+    assert torch.equal(out, want)
+    qkv = b.rand(b.tokens, 8 * 64)
+    cos, sin = _tables(80, 64)
+    q = K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, cos, sin, 4, b.k, b.v)
+    rows = (b.k.clone(), b.v.clone())
+    assert torch.equal(ops.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, cos, sin, 4, [b.k], [b.v]), q)
+    into = torch.empty_like(q)
+    ops.paged_rope_append_out(qkv, b.kv_lens, b.q_start, b.table, cos, sin, 4, [b.k], [b.v], into)
+    assert torch.equal(into, q) and all(torch.equal(x.view(torch.int16), y.contiguous().view(torch.int16))
+                                        for x, y in zip(rows, (b.k, b.v)))
+
+    def step(qkv, k, v):
+        q = ops.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, cos, sin, 4, [k], [v])
+        return ops.paged_attend(q, b.kv_lens, b.q_start, b.table, [k], [v], 0.125, 0.0, 0, None, None, ws)
+
+    eager = step(qkv, b.k, b.v)
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+    assert torch.equal(compiled(qkv, b.k, b.v), eager)
+
+    def functions(qkv, k, v):
+        q = K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, cos, sin, 4, k, v)
+        return K.paged_attend(q, b.kv_lens, b.q_start, b.table, k, v, workspace=ws)
+
+    assert torch.equal(torch.compile(functions, backend="aot_eager", fullgraph=True)(qkv, b.k, b.v), eager)
+
+
+def test_registered_operators_have_shapes():
+    """The operators' Meta kernels (what a compiler traces with)."""
+    ops = L.load_torch_ops()
+    m = dict(device="meta")
+    q = torch.empty(5, 4, 64, dtype=torch.float16, **m)
+    i32 = lambda *s: torch.empty(*s, dtype=torch.int32, **m)  # noqa: E731
+    pages = [torch.empty(3, 2, 16, 64, dtype=torch.float16, **m)]
+    o = ops.paged_attend(q, i32(2), i32(3), i32(2, 4), pages, pages, 0.1, 0.0, 0, None, None, None)
+    assert o.shape == q.shape and o.dtype == q.dtype
+    q4 = [torch.empty(3, 2, 16, 32, dtype=torch.uint8, **m), torch.empty(3, 2, 16, 2, dtype=torch.float16, **m),
+          torch.empty(3, 2, 16, 2, dtype=torch.uint8, **m)]
+    for p in (pages, q4):
+        r = ops.paged_rope_append(torch.empty(5, 8 * 64, dtype=torch.float16, **m), i32(2), i32(3), i32(2, 4), None, None, 4, p, p)
+        assert r.shape == (5, 4, 64)
