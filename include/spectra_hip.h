@@ -405,7 +405,7 @@ typedef struct spectra_paged_kv {
  * q and k heads of `tokens` fused-QKV rows (row stride ldqkv: heads q heads, kv_heads k heads,
  * kv_heads v heads) at their positions (cos_t, sin_t fp32 [rope_rows, head_dim / 2]; NULL = no
  * rotation), appends k and v, 4-bit pages through the quantizer of spectra_kv4_quantize, and
- * writes q_rot [tokens, heads, head_dim].  A token without a position in [0, rope_rows) appends
+ * writes q_rot [tokens, heads, head_dim] (apart from qkv).  A token without a position in [0, rope_rows) appends
  * nothing and gets NaN queries.  Two tokens never write the same row unless two sequences name
  * the same page for positions they append: such rows then hold either's values, or a mix. */
 int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
@@ -422,7 +422,7 @@ int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int
  * with v; 4-bit values stand for fp16((q - z) * s).  A row that sees no key, or only scores of
  * -inf, is zero; what a row does not see (rows of a page past the length, later tokens) does not
  * reach it, whatever it holds, infinities and NaN included.  q [tokens, heads, head_dim], token
- * stride ldq (a multiple of 8, heads contiguous), out contiguous, both 16-byte aligned; slopes
+ * stride ldq (a multiple of 8, heads contiguous), out contiguous and apart from q, both 16-byte aligned; slopes
  * fp32 [heads] and prefix int32 [batch] may be NULL.
  * workspace: spectra_paged_attend_workspace(head_dim) bytes, 16-byte aligned: arrival counters
  * (SPECTRA_PAGED_COUNTER_BYTES at its start), then partial sums of sequences whose keys are

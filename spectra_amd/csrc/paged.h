@@ -34,6 +34,12 @@ __device__ __forceinline__ uint64_t paged_at(int page, uint32_t step) { return (
 // device form (api side of every paged entry).
 int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, PagedKv* out);
 
+// Whether two runs of bytes overlap (an operand that others still read while it is written).
+inline bool paged_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
 // A sequence's part of the call: its first token, how many, and its keys after them.  Starts
 // are clamped to the call's tokens, lengths to what the table can hold plus one (a position past
 // it is a fault of the caller's that its rows report as NaN).
@@ -176,32 +182,39 @@ class PagedWalk {
  public:
   PagedLine line;
 
-  __device__ __forceinline__ PagedWalk(const PagedKv& kv, int g, int rows, int ks, const PagedScore& sc, int w, int groups, int lane)
-      : kv_(kv), sc_(sc), g_(g), rows_(rows), ks_(ks), lane_(lane), grain_(0), pad_(0), c0_(0), base_(0) {
-    float sum = 0.0f;
-    for (int c0 = 0; c0 < kv.batch; c0 += 64) {
-      take(c0);
-      sum += (float)tiles_ * (float)steps_;
+  // wide: the line may pass 32 bits; tokens: about what a tile has
+  __device__ __forceinline__ PagedWalk(const PagedKv& kv, int g, int rows, int tokens, int ks, const PagedScore& sc, int w, int groups,
+                                       bool wide, int lane)
+      : kv_(kv), sc_(sc), g_(g), rows_(rows), toks_(tokens), ks_(ks), lane_(lane), grain_(0), pad_(0), c0_(0), base_(0) {
+    if (wide) {
+      float sum = 0.0f;
+      for (int c0 = 0; c0 < kv.batch; c0 += 64) {
+        take(c0);
+        sum += (float)tiles_ * (float)steps_;
+      }
+      sum = wave_sum(sum) * (float)kv.kv_heads;  // (the same in every lane and wave)
+      while (sum > 536870912.0f) {               // steps of 2, 4, .. steps
+        sum *= 0.5f;
+        ++grain_;
+      }
     }
-    sum = wave_sum(sum) * (float)kv.kv_heads;  // (the same in every lane and wave)
-    while (sum > 536870912.0f) {  // past 32 bits: steps of 2, 4, .. steps
-      sum *= 0.5f;
-      ++grain_;
-    }
-    if (grain_ > 0) take(0);
+    if (kv.batch <= 64) take(0);
     int total = count();
     line.each = (int)((uint32_t)max(total, 0) / (uint32_t)groups);
     line.more = max(total, 0) - line.each * groups;
     // where the tiles can be cut into as many equal pieces of their own, no share has parts of two
     pad_ = line.each + (line.more > 0);
-    const int padded = pad_ > 0 ? count() : 0;
+    const int padded = pad_ > 1 ? count() : total;
     if (pad_ > 0 && padded >= 0 && padded <= groups * (int64_t)pad_) {
       total = padded;
       line.each = pad_;
       line.more = 0;
     } else {
+      if (kv.batch <= 64 && pad_ > 1) {
+        pad_ = 0;
+        take(0);
+      }
       pad_ = 0;
-      if (kv.batch <= 64) take(0);
     }
     if (kv.batch > 64) take(0);
     scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
@@ -244,7 +257,7 @@ class PagedWalk {
   __device__ __forceinline__ int count() {
     int total = 0;
     for (int c0 = 0; c0 < kv_.batch; c0 += 64) {
-      if (kv_.batch > 64 || pad_ > 0) take(c0);
+      if (kv_.batch > 64 || pad_ > 1) take(c0);
       total += __builtin_amdgcn_readlane(wave_scan(kv_.kv_heads * tiles_ * steps_), 63);
     }
     return total;
@@ -253,13 +266,13 @@ class PagedWalk {
     const int b = min(c0 + lane_, kv_.batch - 1);
     seq_ = paged_seq(kv_.q_start[b], kv_.q_start[b + 1], kv_.lens[b], kv_.tokens);
     tiles_ = c0 + lane_ < kv_.batch ? (seq_.n * g_ + rows_ - 1) / rows_ : 0;
-    steps_ = paged_steps(kv_, sc_, seq_.len, rows_ / g_, ks_);
+    steps_ = paged_steps(kv_, sc_, seq_.len, toks_, ks_);
     steps_ = max((steps_ + (1 << grain_) - 1) >> grain_, 1);
-    if (pad_ > 0) steps_ = (int)((uint32_t)(steps_ + pad_ - 1) / (uint32_t)pad_) * pad_;
+    if (pad_ > 1) steps_ = (int)((uint32_t)(steps_ + pad_ - 1) / (uint32_t)pad_) * pad_;
   }
   const PagedKv& kv_;
   const PagedScore& sc_;
-  int g_, rows_, ks_, lane_, grain_, pad_, c0_, base_, scan_, tiles_, steps_;
+  int g_, rows_, toks_, ks_, lane_, grain_, pad_, c0_, base_, scan_, tiles_, steps_;
   PagedSeq seq_;
 };
 

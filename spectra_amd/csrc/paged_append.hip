@@ -200,6 +200,9 @@ extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const voi
                     reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 16) == 0 &&
                       ldqkv % 8 == 0,
                   "operands and qkv rows must be 16-byte aligned");
+  SPECTRA_REQUIRE(!paged_overlap(qkv, ((tokens - 1) * ldqkv + (int64_t)(heads + 2 * kv->kv_heads) * hd) * 2, q_rot,
+                                 tokens * heads * hd * 2),
+                  "q_rot must not overlap qkv");
   int waves = ((heads + kv->kv_heads) * (hd / 16) + kv->kv_heads * (hd / 8) + 63) / 64;
   int64_t blocks = (tokens * waves + kPaThreads / 64 - 1) / (kPaThreads / 64);
   if (blocks >= 64) blocks = (blocks + 7) / 8 * 8;

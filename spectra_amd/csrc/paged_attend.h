@@ -266,6 +266,7 @@ struct PagedLaunch {
   float* slots;
   hipStream_t stream;
   bool mod;
+  bool wide;  // more key steps than 2^29 are possible
 };
 // Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows, as many
 // workgroups as are resident at once, and two partial tiles each at most.

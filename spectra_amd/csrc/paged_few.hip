@@ -42,7 +42,7 @@ constexpr int few_lds() {
 
 template <int HD, int KIND, int NT, bool MOD>
 __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
-    paged_few_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
+    paged_few_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int tokens, int heads, bool wide,
                      uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
   constexpr int ROWS = 16 * NT, KS = HD / 32, DPL = HD / 16, RS = HD + 4;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
   __shared__ int flag;
   __shared__ uint32_t redo[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), c = lane & 15, q4 = lane >> 4;
-  PagedWalk walk(kv, g, ROWS, kFewKeys, sc, blockIdx.x, gridDim.x, lane);
+  PagedWalk walk(kv, g, ROWS, tokens, kFewKeys, sc, blockIdx.x, gridDim.x, wide, lane);
   PagedPart un;
   if (tid == 0) redo[0] = 0;
   int turn = 1;
@@ -61,7 +61,8 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
   turn ^= 1;
   const PagedSeq sq = un.seq;
   const int r0 = un.tile * ROWS, nrows = min(ROWS, sq.n * g - r0);
-  const int tok0 = sread(r0 / g), tok1 = sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;  // the tile's tokens, position of token 0
+  const bool one = sq.n == 1;  // (its rows are token 0's)
+  const int tok0 = one ? 0 : sread(r0 / g), tok1 = one ? 0 : sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;  // the tile's tokens, position of token 0
   const int capacity = kv.table_width << kv.page_shift, pmask = (1 << kv.page_shift) - 1;
   // keys that some row of the tile sees, and those that every row does
   const PagedRange ra = paged_range(i0 + tok0, sq.len, un.prefix, sc.window);
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
   for (int nt = 0; nt < NT; ++nt) {
     const int r = r0 + 16 * nt + c;
     const bool ok = 16 * nt + c < nrows;
-    const int tok = ok ? r / g : tok0, head = un.kvh * g + (ok ? r - tok * g : 0);
+    const int tok = one ? 0 : ok ? r / g : tok0, head = un.kvh * g + (ok ? r - tok * g : 0);
     rg[nt] = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
     slope2[nt] = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
     fpos[nt] = (float)(i0 + tok);
@@ -385,13 +386,14 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
   const int slot = 2 * (int)blockIdx.x + (x != walk.line.begin);
   float* part = slots + (int64_t)slot * paged_slot<HD>(ROWS);
   auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
-    const int r = r0 + row, tok = r / g, head = un.kvh * g + (r - tok * g);
+    const int r = r0 + row, tok = one ? 0 : r / g, head = un.kvh * g + (r - tok * g);
     const bool past = paged_range(i0 + tok, sq.len, un.prefix, sc.window).hi > capacity;
+    const float inv = past ? NAN : den == 0.0f ? 0.0f : 1.0f / den;
     float y[4];
     bool odd = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      y[e] = past ? NAN : den == 0.0f ? 0.0f : v[e] / den;
+      y[e] = v[e] * inv;
       odd |= !(__builtin_fabsf(y[e]) < INFINITY);
     }
     if (mixed && odd) atomicOr(&redo[turn], 1u << row);
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
 template <int HD, int KIND, int NT, bool MOD>
 static int launch_few(const PagedLaunch& a) {
   paged_few_kernel<HD, KIND, NT, MOD><<<dim3((unsigned)a.units), dim3(kFewThreads), 0, a.stream>>>(
-      a.kv, a.sc, a.q, a.ldq, a.g, a.heads, a.counters, a.slots, a.out);
+      a.kv, a.sc, a.q, a.ldq, a.g, 16 * NT / a.g, a.heads, a.wide, a.counters, a.slots, a.out);
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
 }

@@ -462,6 +462,9 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   SPECTRA_REQUIRE(ldq >= (int64_t)heads * kv->head_dim && ldq % 8 == 0, "q token stride too small or not a multiple of 8");
   SPECTRA_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0,
                   "q and out must be 16-byte aligned");
+  SPECTRA_REQUIRE(!paged_overlap(q, ((tokens - 1) * ldq + (int64_t)heads * kv->head_dim) * 2, out,
+                                 tokens * heads * kv->head_dim * 2),
+                  "out must not overlap q");
   SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(slopes) % 4 == 0 && reinterpret_cast<uintptr_t>(prefix) % 4 == 0,
                   "slopes and prefix must be aligned");
   SPECTRA_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive");
@@ -499,5 +502,6 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
   const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(kv->kind, kv->head_dim, rows), tiles * cuts);
   a.units = (int)units;
+  a.wide = tiles * cuts >= (1LL << 29);
   return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
 }

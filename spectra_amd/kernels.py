@@ -797,7 +797,7 @@ def paged_attend(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
                  workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of a ragged batch over a paged cache (as ``paged_rope_append`` fills it): one
     token a sequence, a few drafted ones, or whole prompts.  ``q`` [T, heads, d] (rows may be a
-    view of wider ones); returns [T, heads, d].
+    view of wider ones); returns [T, heads, d] (``out``: apart from q).
 
     The token at position i of sequence b sees the keys j < kv_lens[b] with j <= i, or
     j < prefix[b] (int32 [batch]), and with ``window`` > 0 only those with i - j < window.  A

@@ -550,6 +550,32 @@ def test_empty_calls(hip):
     b = Batch("fp16", [0, 0], [5, 9], 4, 2, 64, 16, seed=14, pad=3)  # tokens, none of a sequence
     out = torch.full_like(b.q, 7.0)
     assert torch.all(b.attend(out=out) == 7.0)
+    b = Batch("4bit", [0, 0], [5, 9], 4, 2, 64, 16, seed=14, pad=200)  # the same for the prompts' tiles
+    out = torch.full_like(b.q, 7.0)
+    assert torch.all(b.attend(out=out) == 7.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40])
+def test_captured_with_a_workspace_of_its_own(hip, n):
+    """No workspace given: the call's own, also in a graph, whose replays follow the lengths."""
+    b = Batch("fp16", [n, n], [3000, 700], 4, 2, 64, 16, seed=17)
+    lens = b.kv_lens.clone()
+    b.attend()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b.attend()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b.attend()
+    for step in range(4):
+        b.kv_lens.copy_(lens - 100 * step)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, b.attend())
 
 
 @pytest.mark.gpu
@@ -642,7 +668,8 @@ def test_descriptor_refusals(bad, msg):
     (dict(tokens=1 << 31), L.ERR_INVALID, "tokens"), (dict(scale=float("nan")), L.ERR_INVALID, "scale"),
     (dict(cap=float("inf")), L.ERR_INVALID, "cap"), (dict(window=-3), L.ERR_INVALID, "window"),
     (dict(ws=None), L.ERR_WORKSPACE, "workspace"), (dict(size=1 << 20), L.ERR_WORKSPACE, "workspace"),
-    (dict(ws=0x60008), L.ERR_INVALID, "workspace")])
+    (dict(ws=0x60008), L.ERR_INVALID, "workspace"), (dict(q=0x50000), L.ERR_INVALID, "overlap"),
+    (dict(q=0x50000 - 16), L.ERR_INVALID, "overlap"), (dict(q=0x50000 + 5 * 4 * 64 * 2 - 16), L.ERR_INVALID, "overlap")])
 def test_attend_refusals(change, status, msg):
     lib = L.load()
     a = dict(q=0x40000, ldq=4 * 64, tokens=5, scale=0.125, cap=0.0, window=0, ws=0x60000, size=1 << 40)
@@ -656,7 +683,7 @@ def test_attend_refusals(change, status, msg):
 @pytest.mark.parametrize("change,msg", [
     (dict(qkv=None), "NULL"), (dict(ld=8 * 64 - 8), "stride"), (dict(ld=8 * 64 + 4), "16-byte"), (dict(cos=0x70000), "both"),
     (dict(cos=0x70000, sin=0x80000, rows=0), "rope_rows"), (dict(cos=0x70004, sin=0x80000, rows=9), "16-byte"),
-    (dict(tokens=0), "tokens")])
+    (dict(tokens=0), "tokens"), (dict(qkv=0x50000), "overlap")])
 def test_append_refusals(change, msg):
     lib = L.load()
     a = dict(qkv=0x40000, ld=8 * 64, tokens=5, cos=None, sin=None, rows=0)
