@@ -277,11 +277,15 @@ class PagedWalk {
 };
 
 // The u-th unit, worked out by every wave from the lengths themselves, so that ragged batches are
-// shared out evenly with no plan on the host: the tiles' key steps (of `ks` keys) are counted,
-// and tiles of more steps than target units would get each (and than min_steps) are cut into pieces.  At most
-// tiles + target units; pieces' partial results take slots, at most 2 target of them (a cut tile
-// has fewer than twice its steps over the steps of a piece).  Lengths that did not fit in
-// max_slots would leave a tile in one piece.  false: u is past the last unit.
+// shared out evenly with no plan on the host: the tiles' key steps (of `ks` keys) are counted, and
+// tiles of more steps than target units would get each (and than min_steps) are cut into pieces.  A
+// piece costs about 8 steps beside its own (its partial sums, and the join: 4 pieces of 8 steps, 23 us,
+// 2 of 16, 27, but 2 of 5 steps 23.5, where the tile in one takes 13.4), so tiles of up to twice
+// min_steps stay whole.  Pieces are rounded up where that is 2 or 3 (2 of 64 steps 85 us, 1 of 128
+// 113) and down past that, where a unit that finds every compute unit taken costs more (6 of 11
+// steps 36 us, 5 of 13 31).  At most tiles + target units; pieces' partial results take slots, less than
+// 2 target of them (a cut tile has fewer than twice its steps over the steps of a piece).
+// Lengths that did not fit in max_slots would leave a tile in one piece.  false: u is past the last unit.
 __device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, int ks, int min_steps, int target,
                                            int max_slots,
                                            const PagedScore& sc, int u, int lane, PagedUnit& un) {
@@ -303,7 +307,8 @@ __device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, i
   int base = 0, slot0 = 0;
   for (int c0 = 0; c0 < kv.batch; c0 += 64) {
     if (kv.batch > 64) take(c0);
-    const int pieces = min((steps + piece_steps - 1) / piece_steps, kPagedPieces);
+    const int up = steps < 3 * piece_steps ? piece_steps - 1 : 0;
+    const int pieces = steps <= 2 * min_steps ? 1 : min((steps + up) / piece_steps, kPagedPieces);
     const int units = kv.kv_heads * tiles * pieces;
     const int end = base + wave_scan(units), slots = pieces > 1 ? units : 0, send = slot0 + wave_scan(slots);
     const uint64_t past = __ballot(end > u);

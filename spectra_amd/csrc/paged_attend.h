@@ -212,10 +212,10 @@ __device__ __forceinline__ float2 load_dev2(const float* p) {
   return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
 }
 
-// A row's pieces (slot_of(p) the p-th's record) joined in their order, whatever order they arrived in: dims d .. d + 3 of the sum
-// of weight times value, and the total.
+// A row's pieces (slot_of(p) the p-th's record) joined in their order, whatever order they arrived in:
+// four dims of the sum of weight times value (two at `at` in the records, two at `next`), and the total.
 template <int HD, int ROWS, int U, typename F>
-__device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
+__device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, int pieces, int row, int at, int next, float (&v)[4]) {
   float mm = -INFINITY, den = 0.0f;
   v[0] = v[1] = v[2] = v[3] = 0.0f;
   for (int p0 = 0; p0 < pieces; p0 += U) {  // U in flight
@@ -224,8 +224,8 @@ __device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, in
     for (int u = 0; u < U; ++u) {
       const float* p = slots + (int64_t)slot_of(min(p0 + u, pieces - 1)) * paged_slot<HD>(ROWS);
       ml[u] = load_dev2(p + ROWS * HD + 2 * row);
-      x[u][0] = load_dev2(p + row * HD + d);
-      x[u][1] = load_dev2(p + row * HD + d + 2);
+      x[u][0] = load_dev2(p + at);
+      x[u][1] = load_dev2(p + next);
     }
     float mn = mm;
 #pragma unroll
@@ -250,8 +250,9 @@ __device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, in
 }
 template <int HD, int ROWS, typename F>
 __device__ __forceinline__ float paged_join(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
-  return pieces <= 4 ? paged_join_by<HD, ROWS, 4>(slots, slot_of, pieces, row, d, v)
-                     : paged_join_by<HD, ROWS, 16>(slots, slot_of, pieces, row, d, v);
+  const int at = row * HD + d;
+  return pieces <= 4 ? paged_join_by<HD, ROWS, 4>(slots, slot_of, pieces, row, at, at + 2, v)
+                     : paged_join_by<HD, ROWS, 16>(slots, slot_of, pieces, row, at, at + 2, v);
 }
 
 // The host side of a launch, shared by the kernels' translation units.

@@ -375,23 +375,24 @@ __global__ void __launch_bounds__(64 * W, 2)
   } else {
     const int first = un.slot - un.piece;
     if (tid < QH) redo[tid] = 0;
-    if (ok && kh == 0) {
+    if (ok && kh == 0) {  // (a record's sums as the lanes hold them: pairs of dims, a wave's beside each other)
       float* p = slots + (int64_t)un.slot * paged_slot<HD>(ROWS);
-      float* row = p + (32 * qh + ln) * HD;
+      float* at = p + qh * 32 * HD + 2 * lane;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          store_dev2(row + 32 * d + 8 * r + 4 * gh, o[d][4 * r], o[d][4 * r + 1]);
-          store_dev2(row + 32 * d + 8 * r + 4 * gh + 2, o[d][4 * r + 2], o[d][4 * r + 3]);
-        }
+      for (int i = 0; i < 4 * DT; ++i) {
+        store_dev2(at + 256 * i, o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1]);
+        store_dev2(at + 256 * i + 128, o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+      }
       if (gh == 0) store_dev2(p + ROWS * HD + 2 * (32 * qh + ln), m, l);
     }
     if (!paged_arrive(counters + first, un.pieces, &flag)) return;
-    for (int it = tid; it < nrows * (HD / 4); it += THREADS) {
-      const int row = it / (HD / 4), d = 4 * (it % (HD / 4)), r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g);
+    for (int it = tid; it < ROWS * (HD / 4); it += THREADS) {
+      const int part = it >> 6, d = 8 * (part % (4 * DT)) + 4 * gh, row = 32 * (part / (4 * DT)) + ln;
+      if (row >= nrows) continue;
+      const int r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g);
       float v[4], y[4];
-      const float den = paged_join_by<HD, ROWS, 4>(slots, [&](int p) { return first + p; }, un.pieces, row, d, v);
+      const float den = paged_join_by<HD, ROWS, 4>(slots, [&](int p) { return first + p; }, un.pieces, row, 256 * part + 2 * lane,
+                                                   256 * part + 128 + 2 * lane, v);
       const bool past = paged_range(i0 + t, sq.len, un.prefix, sc.window).hi > capacity;
       bool odd = false;
 #pragma unroll
