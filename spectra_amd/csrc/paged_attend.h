@@ -281,8 +281,7 @@ constexpr int kFewSlotRows = 2 * 512 * 32;  // the most: two records each, of 51
 static_assert(2 * few_groups(kKv4, 128, 16) * 16 <= kFewSlotRows && 2 * few_groups(kKv4, 64, 32) * 32 <= kFewSlotRows, "");
 int launch_paged_few(const PagedLaunch& a, int rows);
 // Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.
-constexpr int many_waves(int rows) { return 4; }
-constexpr int many_keys(int waves) { return 16 * waves; }  // of a step
+constexpr int kManyWaves = 4, kManyKeys = 16 * kManyWaves;  // keys of a step: a wave copies 16
 constexpr int kManyBig = 512, kManyMinKeys = 512, kManyTarget = 256, kManySlots = 2 * kManyTarget;
 int launch_paged_many(const PagedLaunch& a, int rows);
 

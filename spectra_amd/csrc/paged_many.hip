@@ -20,9 +20,9 @@ namespace spectra {
 // The buffers of keys, then of values: two each, a row of 16-byte chunks a key.  Chunk c of key r lies
 // at c ^ k_turn(r) in K's rows (16 rows' equal chunks, which lanes read at once, on different banks)
 // and at c ^ v_turn(r) in V's (four rows' 64 bytes, read transposed, on different banks).
-template <int HD, int W>
+template <int HD>
 constexpr int many_lds() {
-  return 4 * many_keys(W) * HD * 2;
+  return 4 * kManyKeys * HD * 2;
 }
 template <int HD>
 __device__ __forceinline__ int k_turn(int r) {
@@ -41,13 +41,13 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4_t*)(lds_t)p));
 }
 
-template <int HD, int KIND, bool MOD, int QH, int W>
-__global__ void __launch_bounds__(64 * W, 2)
+template <int HD, int KIND, bool MOD, int QH>
+__global__ void __launch_bounds__(64 * kManyWaves, 2)
     paged_many_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                       uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
   constexpr int CH = HD / 8, KS = HD / 16, DT = HD / 32;  // 8-dim chunks, 16-dim steps, 32-dim tiles
-  constexpr int KEYS = many_keys(W), THREADS = 64 * W;    // keys of a step
+  constexpr int W = kManyWaves, KEYS = kManyKeys, THREADS = 64 * W;
   constexpr int KL = KEYS * CH / THREADS;                 // K chunks a thread copies
   constexpr int KH = W / QH;                              // waves that share a step's keys
   constexpr int ROWS = 32 * QH, TL = KEYS / (32 * KH);    // 32-key tiles of a step that a wave takes
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(64 * W, 2)
   const int rr = r0 + min(32 * qh + ln, nrows - 1), tok = rr / g, head = un.kvh * g + (rr - tok * g);
   const PagedRange rg = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
   const float slope2 = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
-  const float fpos = (float)(i0 + tok - 4 * gh);
+  const int pos = i0 + tok - 4 * gh;
   pu4_t qf[KS];
   {
     const uint16_t* qr = q + (int64_t)(sq.q0 + tok) * ldq + head * HD + 8 * gh;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(64 * W, 2)
     for (int i = 0; i < RING; ++i) ring[i] = read_k(buf ^ 1, i);
     __builtin_amdgcn_sched_barrier(0);
     float mul = sc.mul;
-    if constexpr (MOD) mul = paged_scores<TL, 16>(s, sc, slope2, fpos - (float)kw, [](int r) { return 8 * (r >> 2) + (r & 3); });
+    if constexpr (MOD) mul = paged_scores<TL, 16>(s, sc, slope2, (float)(pos - kw), [](int r) { return 8 * (r >> 2) + (r & 3); });
     if (kw < alo || kw + 32 * TL > ahi) {
       const int from = rg.lo - kw - 4 * gh, to = min(rg.hi, capacity) - kw - 4 * gh;
 #pragma unroll
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(64 * W, 2)
   if constexpr (KH > 1) {  // the waves that shared the keys meet
     float4* red = (float4*)lds;  // [wave past the first QH][4 DT][lane]
     float2* ml = (float2*)(lds + (W - QH) * 16 * DT * 64 * 4);
-    static_assert((W - QH) * (16 * DT * 64 * 4 + 64 * 8) <= many_lds<HD, W>(), "their sums fit the buffers");
+    static_assert((W - QH) * (16 * DT * 64 * 4 + 64 * 8) <= many_lds<HD>(), "their sums fit the buffers");
     __syncthreads();
     if (kh > 0) {
       const int at = wave - QH;
@@ -411,19 +411,19 @@ __global__ void __launch_bounds__(64 * W, 2)
     paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + 32 * qh + __builtin_ctz(r), out);
 }
 
-template <int HD, int KIND, bool MOD, int QH, int W>
+template <int HD, int KIND, bool MOD, int QH>
 static int launch_many(const PagedLaunch& a) {
-  const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD, QH, W>;
+  const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD, QH>;
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
-  paged_many_kernel<HD, KIND, MOD, QH, W><<<dim3((unsigned)a.units), dim3(64 * W), many_lds<HD, W>(), a.stream>>>(
+  paged_many_kernel<HD, KIND, MOD, QH><<<dim3((unsigned)a.units), dim3(64 * kManyWaves), many_lds<HD>(), a.stream>>>(
       a.kv, a.sc, a.q, a.ldq, a.g, a.heads, a.counters, a.slots, a.out);
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
 }
 template <int HD, int KIND>
 static int launch_many_of(const PagedLaunch& a, int rows) {
-  if (rows == 64) return a.mod ? launch_many<HD, KIND, true, 2, many_waves(64)>(a) : launch_many<HD, KIND, false, 2, many_waves(64)>(a);
-  return a.mod ? launch_many<HD, KIND, true, 4, many_waves(128)>(a) : launch_many<HD, KIND, false, 4, many_waves(128)>(a);
+  if (rows == 64) return a.mod ? launch_many<HD, KIND, true, 2>(a) : launch_many<HD, KIND, false, 2>(a);
+  return a.mod ? launch_many<HD, KIND, true, 4>(a) : launch_many<HD, KIND, false, 4>(a);
 }
 int launch_paged_many(const PagedLaunch& a, int rows) {
   if (a.hd == 64)
@@ -477,6 +477,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   constexpr double log2e = 1.4426950408889634;
   a.sc.mul = (float)(cap > 0.0f ? 2.0 * log2e * scale / cap : log2e * scale);
   a.sc.cap2 = (float)(cap * log2e);
+  SPECTRA_REQUIRE(a.sc.mul > 0.0f && a.sc.mul < 1e30f && a.sc.cap2 < 1e30f, "scale or cap out of range");
   a.sc.slopes = slopes;
   a.sc.prefix = prefix;
   a.sc.window = window < (1 << 30) ? window : 0;  // (no sequence is longer)
@@ -496,7 +497,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   const int64_t all = tokens * a.g, seqs = tokens < kv->batch ? tokens : kv->batch;
   const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv->kv_heads * all <= 128 * kManyBig ? 64 : 128;
   const bool many = rows >= 64;
-  const int keys = many ? many_keys(many_waves(rows)) : kFewKeys;
+  const int keys = many ? kManyKeys : kFewKeys;
   // at most this many tiles, each of at most as many key steps as its table has
   const int64_t tiles = kv->kv_heads * (all / rows + seqs);
   const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;

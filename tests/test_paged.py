@@ -212,6 +212,63 @@ def test_long_caches_split(hip, kind, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_distances_of_far_positions(hip, n, prefix):
+    """Positions past 2^24, which fp32 does not hold: the distances, which the bias takes, are small.  The long
+    sequence names the same few pages over and over, and a window leaves its last keys."""
+    from spectra_amd import kernels as K
+    g, page, d, window, m = _gen(n), 4096, 64, 48, (1 << 27) + 77
+    k, v = (torch.randn(4, 1, page, d, generator=g, device="cuda").half() for _ in range(2))
+    table = (torch.arange(m // page + 1, device="cuda") % 4).int()[None]
+    q = torch.randn(n, 2, d, generator=g, device="cuda").half()
+    slopes = torch.tensor([0.5, 0.125], device="cuda")
+    got = K.paged_attend(q, torch.tensor([m], dtype=torch.int32, device="cuda"),
+                         torch.tensor([0, n], dtype=torch.int32, device="cuda"), table, k, v, window=window, slopes=slopes,
+                         prefix=torch.tensor([m], dtype=torch.int32, device="cuda") if prefix else None)
+    i = torch.arange(m - n, m, device="cuda")[:, None]
+    j = torch.arange(m - n - window, m, device="cuda")[None]
+    see = (i - j < window) & ((j <= i) | prefix)
+    kk, vv = (x[table[0, j[0] // page].long(), 0, j[0] % page].double() for x in (k, v))
+    for h in range(2):
+        bias = float(slopes[h]) * (i - j).abs()
+        qh = q[:, h].double()
+        delta = d * 2.0 ** -24 * (qh.abs() @ kk.abs().T / 8).amax(-1, keepdim=True) + 2.0 ** -22 * bias.amax()
+        p = torch.softmax((qh @ kk.T / 8 - bias).masked_fill(~see, -math.inf), -1)
+        want, a = p @ vv, p @ vv.abs()
+        tol = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2 * delta + 2.0 ** -20) * a + 2.0 ** -25 * (1 + see.double() @ vv.abs())
+        assert torch.all((got[:, h].double() - want).abs() <= tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [[1, 1], [3, 4], [70, 40]])
+def test_pages_gigabytes_apart(hip, kind, n):
+    """Offsets past 32 bits, in elements and in bytes: the same rows in pages that lie 3 GiB apart give the same bits."""
+    from spectra_amd import kernels as K
+    b = Batch(kind, n, [90, 75], 4, 2, 64, 64, seed=31)
+    heads, kv, d = b.heads, b.kv, b.d
+
+    def apart(x):
+        step = 3 * (1 << 30) // x.element_size() if x.dtype != torch.half or kind != "4bit" else 1 << 30
+        far = torch.empty(step * (x.shape[0] - 1) + x[0].numel(), dtype=x.dtype, device="cuda")
+        far = far.as_strided(x.shape, (step,) + tuple(x.stride()[1:]))
+        far.copy_(x)
+        return far
+
+    near = b.check()
+    held = b.k, b.v
+    b.k, b.v = (tuple(apart(t) for t in c) if kind == "4bit" else apart(c) for c in held)
+    assert torch.equal(b.attend()[: sum(n)], near[: sum(n)])
+    qkv = b.rand(b.tokens, (heads + 2 * kv) * d)
+    for c in (held, (b.k, b.v)):
+        K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, None, None, heads, *c)
+    for x, y in zip(held, (b.k, b.v)):
+        for s, t in zip(x, y) if kind == "4bit" else [(x, y)]:
+            assert torch.equal(torch.nan_to_num(s.float(), 99.0), torch.nan_to_num(t.float(), 99.0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batch", [65, 200])
 def test_many_sequences(hip, batch):
     g = torch.Generator().manual_seed(batch)
@@ -692,6 +749,14 @@ def test_append_refusals(change, msg):
     st = lib.spectra_paged_rope_append(ctypes.byref(p), a["qkv"], a["ld"], a["tokens"], a["cos"], a["sin"], a["rows"], 4,
                                        0x50000, None)
     assert st == L.ERR_INVALID and msg in lib.spectra_last_error().decode()
+
+
+@pytest.mark.parametrize("scale,cap", [(3e38, 0.0), (1.0, 1e-38), (1.0, 3e38), (0.0, 0.0)])
+def test_scales_out_of_range(scale, cap):
+    lib, p = L.load(), _desc()
+    st = lib.spectra_paged_attend(ctypes.byref(p), 0x40000, 4 * 64, 5, 4, scale, cap, 0, None, None, 0x60000, 1 << 40, 0x50000,
+                                  None)
+    assert st == L.ERR_INVALID and "scale" in lib.spectra_last_error().decode()
 
 
 def test_descriptor_layout_matches_c(tmp_path):
