@@ -280,7 +280,9 @@ constexpr int few_groups(int kind, int hd, int rows) { return 256 * few_resident
 constexpr int kFewSlotRows = 2 * 512 * 32;  // the most: two records each, of 512 workgroups of 32 rows
 static_assert(2 * few_groups(kKv4, 128, 16) * 16 <= kFewSlotRows && 2 * few_groups(kKv4, 64, 32) * 32 <= kFewSlotRows, "");
 int launch_paged_few(const PagedLaunch& a, int rows);
-// Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.
+// Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.  Tiles of more
+// than 2 kManyMinKeys keys may be cut where there are few: into kManyTarget pieces in all (1024: 1536 tokens 67 us,
+// not 30, as every piece writes and joins its sums).
 constexpr int kManyWaves = 4, kManyKeys = 16 * kManyWaves;  // keys of a step: a wave copies 16
 constexpr int kManyBig = 512, kManyMinKeys = 512, kManyTarget = 256, kManySlots = 2 * kManyTarget;
 int launch_paged_many(const PagedLaunch& a, int rows);

@@ -1,21 +1,33 @@
 // Attention over a paged KV cache for many rows a sequence: prompts, and chunks of them on their
-// context, in tiles of 128 rows (the tokens' query heads of one KV head beside each other, so the
-// heads that share keys share their loads).
+// context, in tiles of 64 or 128 rows (the tokens' query heads of one KV head beside each other, so the
+// heads that share keys share their loads).  The mathematics is the few rows' kernel's: one pass with a running
+// maximum, scores transposed, S^T = K Q^T (32 x 32 x 16: K rows as A, the lane's row as B), so a lane holds 16
+// scores of one row a tile, maxima cross only to the lane 32 away, and the exponentials are already the B
+// operand of O^T = V^T P^T when the contraction takes the keys in the accumulator's order.
 //
-// Bound by the matrix cores and the exponentials between them: 4 head_dim flops and one
-// exponential a score.  A workgroup of 4 waves, 32 rows each; steps of 64 keys staged through
-// LDS, two buffers, the rows of the next step in registers while this one computes.  Scores are computed
-// transposed, S^T = K Q^T (32 x 32 x 16: K rows as A, the lane's row as B), so a lane holds 16 scores
-// of one row a tile: maxima cross only to the lane 32 away, and the exponentials are already the
-// B operand of O^T = V^T P^T when the contraction takes the keys in the accumulator's order.  V is
-// transposed, and 4-bit pages expanded, on the way into LDS.
+// Bound by the matrix cores and the exponentials between them (4 head_dim flops and one exponential a score,
+// 8 cycles a wave, a quarter of a 32 x 32 x 16 matrix instruction): a prompt of 8192 tokens
+// (24 heads of 128) does 412 GFLOP in 405 to 423 us, 975 to 1019 TFLOP/s where a large matrix product reaches
+// 1145; there the matrix cores are busy half of the time at a clock that their power lowers.  With a cap (two
+// exponentials and a reciprocal a score) 700 TFLOP/s; 4-bit pages with a bias and heads of 64 276.  A prompt of
+// 777 tokens takes 18 us: 13 key steps one after another for its last rows, and fewer tiles than would
+// hide their latencies.
+//
+// A workgroup is 4 waves of 32 rows each, or for 64 rows two pairs that take the halves of a step's keys; steps
+// are 64 keys, in two buffers each of K and V.  16-bit rows go from memory to LDS directly, with no
+// register between (8192 tokens: 439 us, 498 through registers), K's and V's chunks turned so that what
+// lanes read at once lies on different banks (no conflicts are counted); V is read transposed by the LDS
+// itself.  4-bit rows are expanded on the way, once for all rows.  The loop runs one step ahead: the next
+// step's Q K^T stands beside this step's exponentials, the copies between them (777 tokens 18.6 us, 19.8 with
+// the copies before them).
+//
+// Roundings: as the few rows' kernel.
 #include <algorithm>
 #include <cmath>
 
 #include "paged_attend.h"
 
 namespace spectra {
-
 
 // The buffers of keys, then of values: two each, a row of 16-byte chunks a key.  Chunk c of key r lies
 // at c ^ k_turn(r) in K's rows (16 rows' equal chunks, which lanes read at once, on different banks)
@@ -185,8 +197,8 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
     for (int i = 0; i < NK; ++i) s[i / KS] = mfma32<BF>(read_k(buf, i), qf[i % KS], i % KS == 0 ? zero : s[i / KS]);
   };
   // One step: softmax of its scores s, their product with its values, and the next step's scores
-  // into sn (past the last: of whatever its buffer holds, used by nothing).  The order is written out (the compiler would wait for every operand
-  // where it is used): operands are read RING instructions ahead, and the exponentials, and the
+  // into sn (past the last: of whatever its buffer holds, used by nothing).  The order is written out
+  // (the compiler would wait for every operand where it is used): operands are read RING instructions ahead, and the exponentials, and the
   // 2 KL copies `beside`, stand between the matrix instructions of Q K^T, which run beneath them.
   auto step = [&](int k0, pf16_t (&s)[TL], pf16_t (&sn)[TL], int buf, auto beside) __attribute__((always_inline)) {
     const int kw = k0 + 32 * TL * kh;  // this wave's keys
@@ -492,8 +504,11 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   a.counters = (uint32_t*)workspace;
   a.slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
   a.stream = (hipStream_t)stream;
-  // Rows a sequence has on average pick the tile: 16 or 32 rows of the few, 64 or 128 of the many
-  // (64, whose key steps two waves share, while 128 would leave compute units idle).
+  // Rows a sequence has on average pick the tile, the least that holds them: 16 or 32 rows of the few (32
+  // sequences of 2048 keys, 24 heads of 128 on 8: 18 rows 29.5 us, as two tiles of 16 43; on 4-bit pages 30 rows
+  // 37.8, of 64 52), or of the many (60 rows 30 us, as two tiles of 32 58).  Tiles of 64, whose key steps two
+  // pairs of waves share, while 128 would leave compute units idle: up to kManyBig tiles of 128 (777 tokens: 64
+  // rows 17.4 us, 128 20.2; four such prompts: 39.5 and 33.0).
   const int64_t all = tokens * a.g, seqs = tokens < kv->batch ? tokens : kv->batch;
   const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv->kv_heads * all <= 128 * kManyBig ? 64 : 128;
   const bool many = rows >= 64;
