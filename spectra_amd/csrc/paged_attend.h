@@ -213,19 +213,25 @@ __device__ __forceinline__ float2 load_dev2(const float* p) {
 }
 
 // A row's pieces (slot_of(p) the p-th's record) joined in their order, whatever order they arrived in:
-// four dims of the sum of weight times value (two at `at` in the records, two at `next`), and the total.
-template <int HD, int ROWS, int U, typename F>
-__device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, int pieces, int row, int at, int next, float (&v)[4]) {
+// NI times four dims of the sum of weight times value (two at `at` in the records, two `next` after them; the
+// n-th four n `step` after the first), and the total.  The loads of U pieces are in flight together.
+template <int HD, int ROWS, int U, int NI, typename F>
+__device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, int pieces, int row, int at, int next, int step,
+                                               float (&v)[NI][4]) {
   float mm = -INFINITY, den = 0.0f;
-  v[0] = v[1] = v[2] = v[3] = 0.0f;
-  for (int p0 = 0; p0 < pieces; p0 += U) {  // U in flight
-    float2 ml[U], x[U][2];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+  for (int p0 = 0; p0 < pieces; p0 += U) {
+    float2 ml[U], x[U][NI][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float* p = slots + (int64_t)slot_of(min(p0 + u, pieces - 1)) * paged_slot<HD>(ROWS);
       ml[u] = load_dev2(p + ROWS * HD + 2 * row);
-      x[u][0] = load_dev2(p + at);
-      x[u][1] = load_dev2(p + next);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        x[u][i][0] = load_dev2(p + at + i * step);
+        x[u][i][1] = load_dev2(p + at + i * step + next);
+      }
     }
     float mn = mm;
 #pragma unroll
@@ -233,26 +239,25 @@ __device__ __forceinline__ float paged_join_by(const float* slots, F slot_of, in
     const float corr = paged_weight(mm, den, mn);
     den *= corr;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= corr;
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] *= corr;
     mm = mn;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (p0 + u >= pieces) continue;
       const float f = paged_weight(ml[u].x, ml[u].y, mm);
       den += f * ml[u].y;
-      v[0] += f * x[u][0].x;
-      v[1] += f * x[u][0].y;
-      v[2] += f * x[u][1].x;
-      v[3] += f * x[u][1].y;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        v[i][0] += f * x[u][i][0].x;
+        v[i][1] += f * x[u][i][0].y;
+        v[i][2] += f * x[u][i][1].x;
+        v[i][3] += f * x[u][i][1].y;
+      }
     }
   }
   return den;
-}
-template <int HD, int ROWS, typename F>
-__device__ __forceinline__ float paged_join(const float* slots, F slot_of, int pieces, int row, int d, float (&v)[4]) {
-  const int at = row * HD + d;
-  return pieces <= 4 ? paged_join_by<HD, ROWS, 4>(slots, slot_of, pieces, row, at, at + 2, v)
-                     : paged_join_by<HD, ROWS, 16>(slots, slot_of, pieces, row, at, at + 2, v);
 }
 
 // The host side of a launch, shared by the kernels' translation units.

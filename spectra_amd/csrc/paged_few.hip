@@ -461,9 +461,10 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
       if (paged_arrive(counters + first, pieces, &flag)) {  // the last to arrive joins them
         for (int it = tid; it < nrows * (HD / 4); it += kFewThreads) {
           const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
-          float v[4];
-          const float den = paged_join<HD, ROWS>(slots, slot_of, pieces, row, d, v);
-          write(row, d, v, den);
+          float v[1][4];
+          const float den = pieces <= 4 ? paged_join_by<HD, ROWS, 4, 1>(slots, slot_of, pieces, row, row * HD + d, 2, 0, v)
+                                        : paged_join_by<HD, ROWS, 16, 1>(slots, slot_of, pieces, row, row * HD + d, 2, 0, v);
+          write(row, d, v[0], den);
         }
       }
     }

@@ -398,22 +398,28 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
       if (gh == 0) store_dev2(p + ROWS * HD + 2 * (32 * qh + ln), m, l);
     }
     if (!paged_arrive(counters + first, un.pieces, &flag)) return;
-    for (int it = tid; it < ROWS * (HD / 4); it += THREADS) {
-      const int part = it >> 6, d = 8 * (part % (4 * DT)) + 4 * gh, row = 32 * (part / (4 * DT)) + ln;
-      if (row >= nrows) continue;
-      const int r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g);
-      float v[4], y[4];
-      const float den = paged_join_by<HD, ROWS, 4>(slots, [&](int p) { return first + p; }, un.pieces, row, 256 * part + 2 * lane,
-                                                   256 * part + 128 + 2 * lane, v);
+    // a wave: NI parts of four dims of each 32 rows, whose loads are in flight together (one part after another
+    // would be a round trip past the L2 each)
+    constexpr int NI = 4 * DT / W;
+    for (int row = ln; row < nrows; row += 32) {
+      const int r = r0 + row, t = r / g, h = un.kvh * g + (r - t * g), part = (row >> 5) * 4 * DT + wave;
+      float v[NI][4];
+      const float den = paged_join_by<HD, ROWS, 4, NI>(slots, [&](int p) { return first + p; }, un.pieces, row, 256 * part + 2 * lane,
+                                                       128, 256 * W, v);
       const bool past = paged_range(i0 + t, sq.len, un.prefix, sc.window).hi > capacity;
       bool odd = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = past ? NAN : den == 0.0f ? 0.0f : v[e] / den;
-        odd |= !(__builtin_fabsf(y[e]) < INFINITY);
+      for (int i = 0; i < NI; ++i) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = past ? NAN : den == 0.0f ? 0.0f : v[i][e] / den;
+          odd |= !(__builtin_fabsf(y[e]) < INFINITY);
+        }
+        const int d = 8 * (wave + W * i) + 4 * gh;
+        *(uint2*)(out + ((int64_t)(sq.q0 + t) * heads + h) * HD + d) = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
       }
       if (odd) atomicOr(&redo[row >> 5], 1u << (row & 31));
-      *(uint2*)(out + ((int64_t)(sq.q0 + t) * heads + h) * HD + d) = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
     }
     __syncthreads();
     again = kh == 0 ? redo[qh] : 0;
