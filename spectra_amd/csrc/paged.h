@@ -279,9 +279,9 @@ class PagedWalk {
 // The u-th unit, worked out by every wave from the lengths themselves, so that ragged batches are
 // shared out evenly with no plan on the host: the tiles' key steps (of `ks` keys) are counted, and
 // tiles of more steps than target units would get each (and than min_steps) are cut into pieces.  A
-// piece costs about 8 steps beside its own (its partial sums, and the join: 4 pieces of 8 steps, 23 us,
-// 2 of 16, 27, but 2 of 5 steps 23.5, where the tile in one takes 13.4), so tiles of up to twice
-// min_steps stay whole.  Pieces are rounded up where that is 2 or 3 (2 of 64 steps 85 us, 1 of 128
+// piece costs some 5 steps beside its own (its partial sums, and the join), so tiles of up to half as many again as
+// min_steps stay whole (16 steps: 17.6 us, 23.6 on 4-bit pages in two pieces, 17.7 and 30.2 in one; 9 steps: 13.4 whole).
+// Pieces are rounded up where that is 2 or 3 (2 of 64 steps 80 us, 1 of 128
 // 113) and down past that, where a unit that finds every compute unit taken costs more (6 of 11
 // steps 36 us, 5 of 13 31).  At most tiles + target units; pieces' partial results take slots, less than
 // 2 target of them (a cut tile has fewer than twice its steps over the steps of a piece).
@@ -308,7 +308,7 @@ __device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, i
   for (int c0 = 0; c0 < kv.batch; c0 += 64) {
     if (kv.batch > 64) take(c0);
     const int up = steps < 3 * piece_steps ? piece_steps - 1 : 0;
-    const int pieces = steps <= 2 * min_steps ? 1 : min((steps + up) / piece_steps, kPagedPieces);
+    const int pieces = 2 * steps <= 3 * min_steps ? 1 : min((steps + up) / piece_steps, kPagedPieces);
     const int units = kv.kv_heads * tiles * pieces;
     const int end = base + wave_scan(units), slots = pieces > 1 ? units : 0, send = slot0 + wave_scan(slots);
     const uint64_t past = __ballot(end > u);

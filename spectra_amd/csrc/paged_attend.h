@@ -286,8 +286,8 @@ constexpr int kFewSlotRows = 2 * 512 * 32;  // the most: two records each, of 51
 static_assert(2 * few_groups(kKv4, 128, 16) * 16 <= kFewSlotRows && 2 * few_groups(kKv4, 64, 32) * 32 <= kFewSlotRows, "");
 int launch_paged_few(const PagedLaunch& a, int rows);
 // Many rows a sequence (prompts): tiles of 128 rows, or of 64 up to kManyBig tiles of 128.  Tiles of more
-// than 2 kManyMinKeys keys may be cut where there are few: into kManyTarget pieces in all (1024: 1536 tokens 67 us,
-// not 30, as every piece writes and joins its sums).
+// than 1.5 kManyMinKeys keys may be cut where there are few: into about kManyTarget pieces in all (four times as many,
+// when a join cost twice what it does: 1536 tokens 67 us, not 30; twice: 512 tokens on 32768 345, not 279).
 constexpr int kManyWaves = 4, kManyKeys = 16 * kManyWaves;  // keys of a step: a wave copies 16
 constexpr int kManyBig = 512, kManyMinKeys = 512, kManyTarget = 256, kManySlots = 2 * kManyTarget;
 int launch_paged_many(const PagedLaunch& a, int rows);
