@@ -269,6 +269,32 @@ def test_pages_gigabytes_apart(hip, kind, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [[1, 1, 1], [4, 2, 4], [50, 64, 30]])
+def test_sequences_that_share_pages(hip, kind, n):
+    """A common beginning held once, and a whole sequence named twice."""
+    b = Batch(kind, n, [150, 170, 150], 6, 2, 64, 16, seed=23)
+    b.table[1, :6] = b.table[0, :6]
+    b.table[2] = b.table[0]
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "4bit"])
+@pytest.mark.parametrize("kw", [dict(), dict(window=700, cap=20.0), dict(prefix=True)])
+def test_cut_prompts(hip, kind, kw):
+    """Chunks on long contexts, few enough that their keys are cut: 13 key steps (the least that are), 16, and many; a last
+    tile that is not full, rows of a cut tile that see different keys."""
+    lens = [780, 1024, 5003]
+    b = Batch(kind, [30, 43, 77], lens, 6, 2, 128, 32, seed=29)
+    if "prefix" in kw:
+        kw = dict(kw, prefix=torch.tensor([0, 1024, 4000], dtype=torch.int32, device="cuda"))
+    b.check(**kw)
+    alone = Batch(kind, [40], [1000], 3, 1, 64, 64, seed=30)
+    alone.check(**dict(kw, prefix=torch.tensor([990], dtype=torch.int32, device="cuda")))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batch", [65, 200])
 def test_many_sequences(hip, batch):
     g = torch.Generator().manual_seed(batch)
