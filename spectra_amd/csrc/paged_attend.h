@@ -96,13 +96,13 @@ __device__ __forceinline__ T load_from(const void* base, uint32_t lane_off, int 
 // 64 lanes' 16 bytes at base + off (a lane's own), or 16 or 4 bytes at a lane's address, to LDS at
 // `to` + 16 (4) lane, with no register between.  Nothing waits for them but an s_waitcnt vmcnt.
 __device__ __forceinline__ void copy_lds(const uint8_t* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void copy_lds16(const uint8_t* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory", "m0");
 }
 __device__ __forceinline__ void copy_lds4(const uint8_t* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(p) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(p) : "memory", "m0");
 }
 typedef __attribute__((address_space(3))) uint8_t* lds_t;
 
