@@ -277,10 +277,12 @@ struct PagedLaunch {
 // Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows, as many
 // workgroups as are resident at once, and two partial tiles each at most.
 constexpr int kFewKeys = 128;
-// workgroups a compute unit, by their registers: 4-bit keys of 128 dims fit three in (48 users 121 us, two 127); those
-// of 64 dims keep more in flight as two (65536 keys 25.7 us, as three, with spills, 31.3)
+// workgroups a compute unit, by their registers: 4-bit keys of 128 dims fit three in (48 users 121 us; two, from
+// registers, 127); those of 64 dims keep more in flight as two (65536 keys 25.7 us, as three, with spills, 31.3); with
+// tiles of 32 rows two, but for 16-bit keys of 128 dims, whose tiles in flight take the registers of two
+// (48 sequences of 8 drafted tokens on 8192 keys: 4 bits 153 us, one workgroup 199; 16 bits 290, at the memory's rate)
 constexpr int few_resident(int kind, int hd, int rows) {
-  return rows == 32 ? (hd == 128 ? 1 : 2) : kind == kKv4 && hd == 128 ? 3 : 2;
+  return rows == 32 ? (hd == 128 && kind != kKv4 ? 1 : 2) : kind == kKv4 && hd == 128 ? 3 : 2;
 }
 constexpr int few_groups(int kind, int hd, int rows) { return 256 * few_resident(kind, hd, rows); }
 constexpr int kFewSlotRows = 2 * 512 * 32;  // the most: two records each, of 512 workgroups of 32 rows

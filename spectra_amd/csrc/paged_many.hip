@@ -523,7 +523,12 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   const int64_t tiles = kv->kv_heads * (all / rows + seqs);
   const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;
   SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
-  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : (int64_t)few_groups(kv->kind, kv->head_dim, rows), tiles * cuts);
+  // the few rows' workgroups: as many a compute unit as are resident, but past one only as long as a tile's join,
+  // which is one workgroup's, has no more than some 1024 rows of partial sums (drafts of 24 rows on 8192 4-bit keys: 256
+  // workgroups 32 us, 512 48; 48 such sequences: 199 and 153)
+  const int64_t joined = tiles * 1024 / std::min<int64_t>(rows, (all + seqs - 1) / seqs);
+  const int64_t groups = std::min<int64_t>(few_groups(kv->kind, kv->head_dim, rows), 256 * std::max<int64_t>(1, joined / 256));
+  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : groups, tiles * cuts);
   a.units = (int)units;
   a.wide = tiles * cuts >= (1LL << 29);
   return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
