@@ -150,11 +150,42 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Key steps that a tile of about `tokens` tokens may have.
-__device__ __forceinline__ int paged_steps(const PagedKv& kv, const PagedScore& sc, int len, int tokens, int ks) {
-  int span = min(len, kv.table_width << kv.page_shift);
-  if (sc.window > 0 && sc.prefix == nullptr) span = (int)min((int64_t)span, (int64_t)sc.window + tokens + 16);
-  return (span + ks - 1) / ks;
+// What the plans need of a wave, an Int being one value a lane: on the GPU a register, in a test on the host an
+// array of 64.
+struct Wave {
+  typedef int Int;
+  static __device__ __forceinline__ int read(const int* p, int at) { return p[at]; }   // a lane's own element
+  static __device__ __forceinline__ int load(const int* p) { return sread(sload(p)); }  // the same in every lane
+  static __device__ __forceinline__ int uniform(int v) { return sread(v); }             // (known to be so)
+  static __device__ __forceinline__ int least(int a, int b) { return min(a, b); }
+  static __device__ __forceinline__ int most(int a, int b) { return max(a, b); }
+  static __device__ __forceinline__ int select(bool c, int a, int b) { return c ? a : b; }
+  static __device__ __forceinline__ int quotient(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
+  static __device__ __forceinline__ uint64_t above(int a, int b) { return __ballot(a > b); }
+  static __device__ __forceinline__ int of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  static __device__ __forceinline__ int scan(int v) { return wave_scan(v); }  // sums up to each lane
+  static __device__ __forceinline__ float product(int a, int b) { return wave_sum((float)a * (float)b); }  // their sum
+};
+
+// 64 sequences' parts of the call, a lane each: their tiles of `rows` rows, and a tile's key steps.
+template <typename W>
+struct PagedTake {
+  typename W::Int q0, n, len, tiles, steps;
+};
+template <typename W>
+__host__ __device__ __forceinline__ PagedTake<W> paged_take(const PagedKv& kv, const PagedScore& sc, int g, int rows, int tokens,
+                                                            int ks, int c0, typename W::Int lane) {
+  typedef typename W::Int Int;
+  const Int b = W::least(lane + c0, kv.batch - 1);
+  PagedTake<W> t;
+  t.q0 = W::least(W::most(W::read(kv.q_start, b), 0), kv.tokens);
+  t.n = W::least(W::most(W::read(kv.q_start, b + 1), t.q0), kv.tokens) - t.q0;
+  t.len = W::most(W::read(kv.lens, b), 0);
+  t.tiles = W::select(lane + c0 < kv.batch, (t.n * g + (rows - 1)) / rows, 0);
+  Int span = W::least(t.len, kv.table_width << kv.page_shift);
+  if (sc.window > 0 && sc.prefix == nullptr) span = W::least(span, sc.window + tokens + 16);
+  t.steps = (span + (ks - 1)) / ks;
+  return t;
 }
 
 // A batch's tiles and their key steps in one line, the steps of a tile beside each other, and one of
@@ -166,11 +197,23 @@ struct PagedLine {
   int total, each, more;  // the line's length; shares hold `each` steps, the first `more` of them one more
   int begin, end;         // this share
 
-  __device__ __forceinline__ int start(int w) const { return w * each + min(w, more); }
-  __device__ __forceinline__ int owner(int x) const {  // the share that holds step x
+  __host__ __device__ __forceinline__ int start(int w) const { return w * each + (w < more ? w : more); }
+  __host__ __device__ __forceinline__ int owner(int x) const {  // the share that holds step x
     const int big = more * (each + 1);
     return (int)(x < big ? (uint32_t)x / (uint32_t)(each + 1) : more + (uint32_t)(x - big) / (uint32_t)each);
   }
+  // Records of partial sums: two a share, of the part that it begins with and of a later one.
+  __host__ __device__ __forceinline__ int record(int w, int x) const { return 2 * w + (x != begin); }
+};
+// A tile whose steps several shares hold: the parts' records, in the order of their keys.
+struct PagedCut {
+  int first, share, pieces;
+  __host__ __device__ __forceinline__ PagedCut(const PagedLine& ln, int t0, int steps) {
+    share = ln.owner(t0);
+    pieces = ln.owner(t0 + steps - 1) - share + 1;
+    first = 2 * share + (ln.start(share) != t0);
+  }
+  __host__ __device__ __forceinline__ int record(int p) const { return p == 0 ? first : 2 * (share + p); }
 };
 struct PagedPart {
   PagedSeq seq;
@@ -178,102 +221,112 @@ struct PagedPart {
   int t0, steps;  // the tile's place in the line, its steps
   int from, to;   // this part of them
 };
+template <typename W>
 class PagedWalk {
  public:
+  typedef typename W::Int Int;
   PagedLine line;
 
   // wide: the line may pass 32 bits; tokens: about what a tile has
-  __device__ __forceinline__ PagedWalk(const PagedKv& kv, int g, int rows, int tokens, int ks, const PagedScore& sc, int w, int groups,
-                                       bool wide, int lane)
+  __host__ __device__ __forceinline__ PagedWalk(const PagedKv& kv, int g, int rows, int tokens, int ks, const PagedScore& sc, int w,
+                                                int groups, bool wide, Int lane)
       : kv_(kv), sc_(sc), g_(g), rows_(rows), toks_(tokens), ks_(ks), lane_(lane), grain_(0), pad_(0), c0_(0), base_(0) {
     if (wide) {
-      float sum = 0.0f;
+      float sum = 0.0f;  // (the same in every lane and wave)
       for (int c0 = 0; c0 < kv.batch; c0 += 64) {
         take(c0);
-        sum += (float)tiles_ * (float)steps_;
+        sum += W::product(t_.tiles, t_.steps);
       }
-      sum = wave_sum(sum) * (float)kv.kv_heads;  // (the same in every lane and wave)
-      while (sum > 536870912.0f) {               // steps of 2, 4, .. steps
+      sum *= (float)kv.kv_heads;
+      while (sum > 536870912.0f) {  // steps of 2, 4, .. steps
         sum *= 0.5f;
         ++grain_;
       }
     }
     if (kv.batch <= 64) take(0);
-    int total = count();
-    line.each = (int)((uint32_t)max(total, 0) / (uint32_t)groups);
-    line.more = max(total, 0) - line.each * groups;
-    // where the tiles can be cut into as many equal pieces of their own, no share has parts of two
+    int tiles = 0, total = count(tiles);
+    total = total > 0 ? total : 0;
+    line.each = (int)((uint32_t)total / (uint32_t)groups);
+    line.more = total - line.each * groups;
+    // Where the tiles can be cut into as many equal pieces of their own, no share has parts of two.  Not with more
+    // tiles than shares, each of a piece at least; so what is summed is at most 2 groups pad_, twice the line: more
+    // tiles than that, each of pad_ steps, would pass 32 bits and could come round to a sum that seems to fit.
     pad_ = line.each + (line.more > 0);
-    const int padded = pad_ > 1 ? count() : total;
-    if (pad_ > 0 && padded >= 0 && padded <= groups * (int64_t)pad_) {
+    const bool tried = pad_ > 1 && tiles <= groups;
+    const int padded = tried ? count(tiles) : total;
+    if (pad_ == 1 || (tried && padded <= groups * (int64_t)pad_)) {
       total = padded;
       line.each = pad_;
       line.more = 0;
     } else {
-      if (kv.batch <= 64 && pad_ > 1) {
-        pad_ = 0;
-        take(0);
-      }
       pad_ = 0;
+      if (kv.batch <= 64 && tried) take(0);
     }
     if (kv.batch > 64) take(0);
-    scan_ = wave_scan(kv.kv_heads * tiles_ * steps_);
-    line.total = max(total, 0);
-    line.begin = sread(min(line.start(w), line.total));
-    line.end = sread(min(line.start(w + 1), line.total));
+    scan_ = W::scan(t_.tiles * t_.steps * kv.kv_heads);
+    line.total = total;
+    line.begin = W::uniform(least(line.start(w), total));
+    line.end = W::uniform(least(line.start(w + 1), total));
   }
 
   // The part of the share that begins at x; x never goes back.  false: there is none.
-  __device__ __forceinline__ bool part(int x, PagedPart& p) {
+  __host__ __device__ __forceinline__ bool part(int x, PagedPart& p) {
     uint64_t past;
-    while ((past = __ballot(base_ + scan_ > x)) == 0) {
-      base_ += __builtin_amdgcn_readlane(scan_, 63);
+    while ((past = W::above(scan_ + base_, x)) == 0) {
+      base_ += W::of(scan_, 63);
       c0_ += 64;
       if (c0_ >= kv_.batch) return false;
       take(c0_);
-      scan_ = wave_scan(kv_.kv_heads * tiles_ * steps_);
+      scan_ = W::scan(t_.tiles * t_.steps * kv_.kv_heads);
     }
     const int at = __builtin_ctzll(past);
-    auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
-    const int steps = of(steps_), nt = of(tiles_), r = x - (base_ + of(scan_ - kv_.kv_heads * tiles_ * steps_));
+    const int steps = W::of(t_.steps, at), nt = W::of(t_.tiles, at);
+    const int r = x - (base_ + W::of(scan_ - t_.tiles * t_.steps * kv_.kv_heads, at));
     if (r < 0 || steps <= 0 || nt <= 0) return false;  // (starts that never were a batch: sums that wrapped)
     const int t = r / steps, from = r - t * steps;
     if ((int64_t)x - from + steps > line.total) return false;
     // (the same in every lane, told to the compiler: addresses made of them stay scalar)
-    p.seq = {sread(of(seq_.q0)), sread(of(seq_.n)), sread(of(seq_.len))};
-    p.b = sread(c0_ + at);
-    p.kvh = sread(t / nt);
-    p.tile = sread(t % nt);
-    p.steps = sread(steps);
-    p.from = sread(from);
-    p.t0 = sread(x - from);
-    p.to = sread(min(steps, from + line.end - x));
-    p.prefix = sc_.prefix != nullptr ? max(sread(sload(sc_.prefix + p.b)), 0) : 0;
+    p.seq = {W::uniform(W::of(t_.q0, at)), W::uniform(W::of(t_.n, at)), W::uniform(W::of(t_.len, at))};
+    p.b = W::uniform(c0_ + at);
+    p.kvh = W::uniform(t / nt);
+    p.tile = W::uniform(t % nt);
+    p.steps = W::uniform(steps);
+    p.from = W::uniform(from);
+    p.t0 = W::uniform(x - from);
+    p.to = W::uniform(least(steps, from + line.end - x));
+    p.prefix = 0;
+    if (sc_.prefix != nullptr) {
+      p.prefix = W::load(sc_.prefix + p.b);
+      p.prefix = p.prefix > 0 ? p.prefix : 0;
+    }
     return p.kvh < kv_.kv_heads;
   }
 
  private:
-  // The line's length, with tiles of whole pad_ steps where there is one.
-  __device__ __forceinline__ int count() {
+  static __host__ __device__ __forceinline__ int least(int a, int b) { return a < b ? a : b; }
+  // The line's length, with tiles of whole pad_ steps where there is one; and how many tiles.
+  __host__ __device__ __forceinline__ int count(int& tiles) {
     int total = 0;
+    tiles = 0;
     for (int c0 = 0; c0 < kv_.batch; c0 += 64) {
       if (kv_.batch > 64 || pad_ > 1) take(c0);
-      total += __builtin_amdgcn_readlane(wave_scan(kv_.kv_heads * tiles_ * steps_), 63);
+      total += W::of(W::scan(t_.tiles * t_.steps * kv_.kv_heads), 63);
+      tiles += W::of(W::scan(t_.tiles * kv_.kv_heads), 63);
     }
     return total;
   }
-  __device__ __forceinline__ void take(int c0) {
-    const int b = min(c0 + lane_, kv_.batch - 1);
-    seq_ = paged_seq(kv_.q_start[b], kv_.q_start[b + 1], kv_.lens[b], kv_.tokens);
-    tiles_ = c0 + lane_ < kv_.batch ? (seq_.n * g_ + rows_ - 1) / rows_ : 0;
-    steps_ = paged_steps(kv_, sc_, seq_.len, toks_, ks_);
-    steps_ = max((steps_ + (1 << grain_) - 1) >> grain_, 1);
-    if (pad_ > 1) steps_ = (int)((uint32_t)(steps_ + pad_ - 1) / (uint32_t)pad_) * pad_;
+  __host__ __device__ __forceinline__ void take(int c0) {
+    t_ = paged_take<W>(kv_, sc_, g_, rows_, toks_, ks_, c0, lane_);
+    t_.steps = W::most((t_.steps + ((1 << grain_) - 1)) >> grain_, 1);
+    if (pad_ > 1) t_.steps = W::quotient(t_.steps + (pad_ - 1), pad_) * pad_;
   }
   const PagedKv& kv_;
   const PagedScore& sc_;
-  int g_, rows_, toks_, ks_, lane_, grain_, pad_, c0_, base_, scan_, tiles_, steps_;
-  PagedSeq seq_;
+  int g_, rows_, toks_, ks_;
+  Int lane_;
+  int grain_, pad_, c0_, base_;
+  Int scan_;
+  PagedTake<W> t_;
 };
 
 // The u-th unit, worked out by every wave from the lengths themselves, so that ragged batches are
@@ -286,59 +339,60 @@ class PagedWalk {
 // steps 36 us, 5 of 13 31).  At most tiles + target units; pieces' partial results take slots, less than
 // 2 target of them (a cut tile has fewer than twice its steps over the steps of a piece).
 // Lengths that did not fit in max_slots would leave a tile in one piece.  false: u is past the last unit.
-__device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, int ks, int min_steps, int target,
-                                           int max_slots,
-                                           const PagedScore& sc, int u, int lane, PagedUnit& un) {
-  PagedSeq sq;
-  int tiles, steps;
+template <typename W>
+__host__ __device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, int rows, int ks, int min_steps, int target,
+                                                    int max_slots, const PagedScore& sc, int u, typename W::Int lane,
+                                                    PagedUnit& un) {
+  typedef typename W::Int Int;
+  PagedTake<W> t;
   auto take = [&](int c0) __attribute__((always_inline)) {
-    const int b = min(c0 + lane, kv.batch - 1);
-    sq = paged_seq(kv.q_start[b], kv.q_start[b + 1], kv.lens[b], kv.tokens);
-    tiles = c0 + lane < kv.batch ? (sq.n * g + rows - 1) / rows : 0;
-    steps = max(paged_steps(kv, sc, sq.len, rows / g, ks), 1);
+    t = paged_take<W>(kv, sc, g, rows, rows / g, ks, c0, lane);
+    t.steps = W::most(t.steps, 1);
   };
-  float work = 0.0f;
+  float work = 0.0f;  // (the same in every lane and wave)
   for (int c0 = 0; c0 < kv.batch; c0 += 64) {
     take(c0);
-    work += (float)tiles * (float)steps;
+    work += W::product(t.tiles, t.steps);
   }
-  work = wave_sum(work) * (float)kv.kv_heads;  // (the same in every lane and wave)
-  const int piece_steps = (int)fminf(fmaxf(ceilf(work / (float)target), (float)min_steps), 1e9f);
+  work *= (float)kv.kv_heads;
+  const int piece_steps = (int)__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(work / (float)target), (float)min_steps), 1e9f);
   int base = 0, slot0 = 0;
   for (int c0 = 0; c0 < kv.batch; c0 += 64) {
     if (kv.batch > 64) take(c0);
-    const int up = steps < 3 * piece_steps ? piece_steps - 1 : 0;
-    const int pieces = 2 * steps <= 3 * min_steps ? 1 : min((steps + up) / piece_steps, kPagedPieces);
-    const int units = kv.kv_heads * tiles * pieces;
-    const int end = base + wave_scan(units), slots = pieces > 1 ? units : 0, send = slot0 + wave_scan(slots);
-    const uint64_t past = __ballot(end > u);
+    const Int up = W::select(t.steps < 3 * piece_steps, piece_steps - 1, 0);
+    const Int pieces = W::select(t.steps * 2 <= 3 * min_steps, 1, W::least((t.steps + up) / piece_steps, kPagedPieces));
+    const Int units = t.tiles * pieces * kv.kv_heads, slots = W::select(pieces > 1, units, 0);
+    const Int end = W::scan(units) + base, send = W::scan(slots) + slot0;
+    const uint64_t past = W::above(end, u);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
-      un.b = c0 + at;
-      un.seq = {of(sq.q0), of(sq.n), of(sq.len)};
+      auto of = [&](Int v) __attribute__((always_inline)) { return W::uniform(W::of(v, at)); };
+      const int nt = of(t.tiles), first = of(send - slots), begin = of(end - units);
+      int r = u - begin;
+      // (the same in every lane, told to the compiler: addresses made of them stay scalar)
+      un.seq = {of(t.q0), of(t.n), of(t.len)};
+      un.b = W::uniform(c0 + at);
       un.pieces = of(pieces);
-      const int nt = of(tiles), first = of(send - slots);
-      int r = u - of(end - units);
-      un.kvh = r % kv.kv_heads;
+      un.kvh = W::uniform(r % kv.kv_heads);
       r /= kv.kv_heads;
-      un.piece = r % un.pieces;
-      un.tile = nt - 1 - r / un.pieces;  // (causal tiles: the longest first)
-      if (u < of(end - units) || un.tile < 0) return false;  // (starts that never were a batch: sums that wrapped)
+      un.piece = W::uniform(r % un.pieces);
+      un.tile = W::uniform(nt - 1 - r / un.pieces);  // (causal tiles: the longest first)
+      if (u < begin || un.tile < 0) return false;    // (starts that never were a batch: sums that wrapped)
       const int slot = first + (un.kvh * nt + un.tile) * un.pieces;
       if (un.pieces > 1 && (slot < 0 || slot > max_slots - un.pieces)) {
         if (un.piece > 0) return false;
         un.pieces = 1;
       }
-      un.slot = slot + un.piece;
-      un.prefix = sc.prefix != nullptr ? max(sload(sc.prefix + un.b), 0) : 0;
-      // (the same in every lane, told to the compiler: addresses made of them stay scalar)
-      un = {{sread(un.seq.q0), sread(un.seq.n), sread(un.seq.len)}, sread(un.b), sread(un.kvh), sread(un.tile),
-            sread(un.piece), sread(un.pieces), sread(un.slot), sread(un.prefix)};
+      un.slot = W::uniform(slot + un.piece);
+      un.prefix = 0;
+      if (sc.prefix != nullptr) {
+        un.prefix = W::load(sc.prefix + un.b);
+        un.prefix = un.prefix > 0 ? un.prefix : 0;
+      }
       return true;
     }
-    base = __builtin_amdgcn_readlane(end, 63);
-    slot0 = __builtin_amdgcn_readlane(send, 63);
+    base = W::of(end, 63);
+    slot0 = W::of(send, 63);
   }
   return false;
 }

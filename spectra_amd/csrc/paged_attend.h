@@ -2,6 +2,8 @@
 // row-by-row path.
 #pragma once
 
+#include <algorithm>
+
 #include "kv4.h"
 #include "paged.h"
 
@@ -294,5 +296,36 @@ int launch_paged_few(const PagedLaunch& a, int rows);
 constexpr int kManyWaves = 4, kManyKeys = 16 * kManyWaves;  // keys of a step: a wave copies 16
 constexpr int kManyBig = 512, kManyMinKeys = 512, kManyTarget = 256, kManySlots = 2 * kManyTarget;
 int launch_paged_many(const PagedLaunch& a, int rows);
+
+// The tile and the grid of a call.
+struct PagedGrid {
+  int rows;       // of a tile
+  int64_t tiles;  // at most this many
+  int64_t units;  // workgroups
+  bool wide;      // the tiles' key steps may be more than 2^29
+};
+// Rows a sequence has on average pick the tile, the least that holds them: 16 or 32 rows of the few (32
+// sequences of 2048 keys, 24 heads of 128 on 8: 18 rows 29.5 us, as two tiles of 16 43; on 4-bit pages 30 rows
+// 37.8, of 64 52), or of the many (60 rows 30 us, as two tiles of 32 58).  Tiles of 64, whose key steps two
+// pairs of waves share, while 128 would leave compute units idle: up to kManyBig tiles of 128 (777 tokens: 64
+// rows 17.4 us, 128 20.2; four such prompts: 39.5 and 33.0).
+inline PagedGrid paged_grid(const PagedKv& kv, int64_t tokens, int g, int kind, int hd) {
+  PagedGrid grid;
+  const int64_t all = tokens * g, seqs = std::min<int64_t>(tokens, kv.batch);
+  grid.rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv.kv_heads * all <= 128 * kManyBig ? 64 : 128;
+  const bool many = grid.rows >= 64;
+  const int keys = many ? kManyKeys : kFewKeys;
+  // each tile of at most as many key steps as its table has
+  grid.tiles = kv.kv_heads * (all / grid.rows + seqs);
+  const int64_t cuts = (((int64_t)kv.table_width << kv.page_shift) + keys - 1) / keys;
+  // the few rows' workgroups: as many a compute unit as are resident, but past one only as long as a tile's join,
+  // which is one workgroup's, has no more than some 1024 rows of partial sums (drafts of 24 rows on 8192 4-bit keys: 256
+  // workgroups 32 us, 512 48; 48 such sequences: 199 and 153)
+  const int64_t joined = grid.tiles * 1024 / std::min<int64_t>(grid.rows, (all + seqs - 1) / seqs);
+  const int64_t groups = std::min<int64_t>(few_groups(kind, hd, std::min(grid.rows, 32)), 256 * std::max<int64_t>(1, joined / 256));
+  grid.units = std::min(many ? grid.tiles + kManyTarget + 16 : groups, grid.tiles * cuts);
+  grid.wide = grid.tiles * cuts >= (1LL << 29);
+  return grid;
+}
 
 }  // namespace spectra

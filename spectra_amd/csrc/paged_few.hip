@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
   __shared__ int flag;
   __shared__ uint32_t redo[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), c = lane & 15, q4 = lane >> 4;
-  PagedWalk walk(kv, g, ROWS, tokens, kFewKeys, sc, blockIdx.x, gridDim.x, wide, lane);
+  PagedWalk<Wave> walk(kv, g, ROWS, tokens, kFewKeys, sc, blockIdx.x, gridDim.x, wide, lane);
   PagedPart un;
   if (tid == 0) redo[0] = 0;
   int turn = 1;
@@ -399,8 +399,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
     }
     const bool mixed = tok1 > tok0;  // rows that see different keys
     // this share's parts of tiles that others hold the rest of: one may come first, one last
-    const int slot = 2 * (int)blockIdx.x + (x != walk.line.begin);
-    float* part = slots + (int64_t)slot * paged_slot<HD>(ROWS);
+    float* part = slots + (int64_t)walk.line.record((int)blockIdx.x, x) * paged_slot<HD>(ROWS);
     auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
       const int r = r0 + row, tok = one ? 0 : r / g, head = un.kvh * g + (r - tok * g);
       const bool past = paged_range(i0 + tok, sq.len, un.prefix, sc.window).hi > capacity;
@@ -454,11 +453,10 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
       }
     }
     if (!whole) {
-      const PagedLine& ln = walk.line;
-      const int w0 = ln.owner(un.t0), pieces = ln.owner(un.t0 + un.steps - 1) - w0 + 1;
-      const int first = 2 * w0 + (ln.start(w0) != un.t0);
-      auto slot_of = [&](int p) __attribute__((always_inline)) { return p == 0 ? first : 2 * (w0 + p); };
-      if (paged_arrive(counters + first, pieces, &flag)) {  // the last to arrive joins them
+      const PagedCut cut(walk.line, un.t0, un.steps);
+      const int pieces = cut.pieces;
+      auto slot_of = [&](int p) __attribute__((always_inline)) { return cut.record(p); };
+      if (paged_arrive(counters + cut.first, pieces, &flag)) {  // the last to arrive joins them
         for (int it = tid; it < nrows * (HD / 4); it += kFewThreads) {
           const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
           float v[1][4];

@@ -22,7 +22,6 @@
 // the copies before them).
 //
 // Roundings: as the few rows' kernel.
-#include <algorithm>
 #include <cmath>
 
 #include "paged_attend.h"
@@ -70,7 +69,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), gh = lane >> 5, ln = lane & 31;
   const int qh = wave % QH, kh = wave / QH;  // the wave's 32 rows, and its share of a step's keys
   PagedUnit un;
-  if (!paged_unit(kv, g, ROWS, KEYS, kManyMinKeys / KEYS, kManyTarget, kManySlots, sc, blockIdx.x, lane, un)) return;
+  if (!paged_unit<Wave>(kv, g, ROWS, KEYS, kManyMinKeys / KEYS, kManyTarget, kManySlots, sc, blockIdx.x, lane, un)) return;
   const PagedSeq sq = un.seq;
   const int r0 = un.tile * ROWS, nrows = min(ROWS, sq.n * g - r0);
   const int tok0 = sread(r0 / g), tok1 = sread((r0 + nrows - 1) / g), i0 = sq.len - sq.n;
@@ -510,26 +509,9 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   a.counters = (uint32_t*)workspace;
   a.slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
   a.stream = (hipStream_t)stream;
-  // Rows a sequence has on average pick the tile, the least that holds them: 16 or 32 rows of the few (32
-  // sequences of 2048 keys, 24 heads of 128 on 8: 18 rows 29.5 us, as two tiles of 16 43; on 4-bit pages 30 rows
-  // 37.8, of 64 52), or of the many (60 rows 30 us, as two tiles of 32 58).  Tiles of 64, whose key steps two
-  // pairs of waves share, while 128 would leave compute units idle: up to kManyBig tiles of 128 (777 tokens: 64
-  // rows 17.4 us, 128 20.2; four such prompts: 39.5 and 33.0).
-  const int64_t all = tokens * a.g, seqs = tokens < kv->batch ? tokens : kv->batch;
-  const int rows = all <= 16 * seqs ? 16 : all <= 32 * seqs ? 32 : kv->kv_heads * all <= 128 * kManyBig ? 64 : 128;
-  const bool many = rows >= 64;
-  const int keys = many ? kManyKeys : kFewKeys;
-  // at most this many tiles, each of at most as many key steps as its table has
-  const int64_t tiles = kv->kv_heads * (all / rows + seqs);
-  const int64_t cuts = ((int64_t)kv->table_width * kv->page_size + keys - 1) / keys;
-  SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
-  // the few rows' workgroups: as many a compute unit as are resident, but past one only as long as a tile's join,
-  // which is one workgroup's, has no more than some 1024 rows of partial sums (drafts of 24 rows on 8192 4-bit keys: 256
-  // workgroups 32 us, 512 48; 48 such sequences: 199 and 153)
-  const int64_t joined = tiles * 1024 / std::min<int64_t>(rows, (all + seqs - 1) / seqs);
-  const int64_t groups = std::min<int64_t>(few_groups(kv->kind, kv->head_dim, rows), 256 * std::max<int64_t>(1, joined / 256));
-  const int64_t units = std::min(many ? tiles + kManyTarget + 16 : groups, tiles * cuts);
-  a.units = (int)units;
-  a.wide = tiles * cuts >= (1LL << 29);
-  return many ? launch_paged_many(a, rows) : launch_paged_few(a, rows);
+  const PagedGrid grid = paged_grid(a.kv, tokens, a.g, a.kind, a.hd);
+  SPECTRA_REQUIRE(grid.tiles < (1LL << 28), "tokens out of range");
+  a.units = (int)grid.units;
+  a.wide = grid.wide;
+  return grid.rows >= 64 ? launch_paged_many(a, grid.rows) : launch_paged_few(a, grid.rows);
 }

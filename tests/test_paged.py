@@ -306,6 +306,58 @@ def test_many_sequences(hip, batch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "4bit"])
+def test_large_batch(hip, kind):
+    """So many tiles that a sum of padded ones would be 2^32: 65536 sequences, which share the pages of 64."""
+    from spectra_amd import kernels as K
+    times = 1024
+    few = Batch(kind, [1] * 64, [1024 - 2 * b for b in range(64)], 8, 8, 64, 64, seed=37)
+    want, tol = few.reference()
+    got = torch.full((64 * times, 8, 64), 7.0, dtype=few.q.dtype, device="cuda")
+    K.paged_attend(few.q.repeat(times, 1, 1), few.kv_lens.repeat(times), torch.arange(64 * times + 1, dtype=torch.int32, device="cuda"),
+                   few.table.repeat(times, 1), few.k, few.v, out=got)
+    for part in got.view(times, 64, 8, 64).split(64):
+        assert torch.all((part.double() - want).abs() <= tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("far", [False, True])
+def test_tables_past_32_bits(hip, kind, n, far):
+    """Tables of so many key steps in all that shares are counted in steps of several: with short sequences, and with
+    long ones of which a window leaves the last keys (their lengths are counted whole beside a prefix)."""
+    from spectra_amd import kernels as K
+    g, page, d, kv, heads, batch, window = _gen(n), 65536, 64, 4, 8, 72, 300
+    pool = lambda: torch.randn(3, kv, page, d, generator=g, device="cuda").to(_DT[kind])  # noqa: E731
+    k, v = pool(), pool()
+    if kind == "4bit":
+        k, v = (tuple(t.view(3, kv, page, -1) for t in K.kv4_quantize(x.view(3 * kv, page, d))) for x in (k, v))
+    table = (torch.arange(batch * 8193, device="cuda") % 3).int().view(batch, -1)
+    lens = [((1 << 29) - 77 * b if far else 20 + 11 * b) for b in range(batch)]
+    q = torch.randn(batch * n, heads, d, generator=g, device="cuda").to(_DT[kind])
+    got = K.paged_attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                         torch.arange(0, batch * n + 1, n, dtype=torch.int32, device="cuda"), table, k, v, window=window,
+                         prefix=torch.zeros(batch, dtype=torch.int32, device="cuda"))
+    u, sub = torch.finfo(_DT[kind]).eps / 2, 2.0 ** -25 if kind != "bf16" else 0.0
+    for b, m in enumerate(lens):
+        i = torch.arange(m - n, m, device="cuda")[:, None]
+        j = torch.arange(max(0, m - n - window), m, device="cuda")[None]
+        see = (i - j < window) & (j <= i)
+        at = table[b, j[0] // page].long(), slice(None), j[0] % page
+        kk, vv = (_values(tuple(t[at] for t in c) if kind == "4bit" else c[at], kind) for c in (k, v))
+        for h in range(heads):
+            qh, kh, vh = q[b * n: b * n + n, h].double(), kk[:, h * kv // heads], vv[:, h * kv // heads]
+            delta = d * 2.0 ** -24 * (qh.abs() @ kh.abs().T / 8).amax(-1, keepdim=True)
+            x = (qh @ kh.T / 8).masked_fill(~see, -math.inf)
+            p = torch.softmax(x, -1)
+            total = torch.exp(x - x.amax(-1, keepdim=True)).sum(-1, keepdim=True)
+            want, a = p @ vh, p @ vh.abs()
+            tol = u * want.abs() + (u + 2 * delta + 2.0 ** -20) * a + sub * (1 + (see.double() @ vh.abs()) / total)
+            assert torch.all((got[b * n: b * n + n, h].double() - want).abs() <= tol), (b, h)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 def test_rows_without_keys(hip, kind):
     """More tokens than keys (positions below zero), and scores that are all -inf: zeros."""
