@@ -77,9 +77,15 @@ __device__ __forceinline__ int paged_find(const int* q_start, int batch, int t, 
 
 // What turns products x = q . k into scores in log2 units, up to a constant of the row (softmax
 // knows none): mul x, or with a cap
-//   cap2 tanh(t x / 2) = cap2 (1 - 2 / (1 + 2^(t2 x)))  ->  2 cap2 (-1 / (1 + 2^(t2 x)))
-// (t2 = 2 log2(e) scale / cap, cap2 = cap log2(e)); less slope2 |i - j|, which for keys up to the row's
-// position is slope2 (j - i).
+//   cap2 tanh(y) = cap2 (1 - 2 / (1 + 2^(t2 x)))  ->  2 cap2 (-1 / (1 + 2^(t2 x)))
+// (y = scale x / cap, t2 = 2 log2(e) scale / cap, cap2 = cap log2(e)); less slope2 |i - j|, which for keys up to the
+// row's position is slope2 (j - i).  That form's error is some 2^-22 of the cap whatever the score: up to kPagedCap a
+// tenth of a weight's rounding to fp16 (a cap of 256: weights off by 4e-5; of 1e6, by 15 %).  Past it, where |y| < 1/4
+// (the subtraction would cancel), tanh(y) is y times the Taylor polynomial of tanh(y) / y in y^2, whose next term is
+// below 2^-26: an error of 2^-19 of the score at most.
+// It has kernels of its own: as a branch beside the other form its registers made chunks with a cap of 50 2 % slower.
+constexpr float kPagedCap = 256.0f * 1.44269504f;  // of cap2
+enum { kModNone, kMod, kModLargeCap };             // what becomes of scores
 struct PagedScore {
   float mul;           // scale log2(e); with a cap t2
   float cap2;          // 0: no cap
@@ -91,10 +97,21 @@ struct PagedScore {
 // Applies cap and bias to T tiles of N products; far: the row's position less the first key's, at(n):
 // the n-th product's key after it (tiles 32 or 16 N / 4 keys apart).  The scores are the result's
 // factor times what is left in s.
-template <int T, int N, typename V, typename F>
+template <int MOD, int T, int N, typename V, typename F>
 __device__ __forceinline__ float paged_scores(V (&s)[T], const PagedScore& sc, float slope2, float far, F at) {
   float mul = sc.mul;
-  if (sc.cap2 > 0.0f) {
+  if constexpr (MOD == kModLargeCap) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float y = s[t][n] * (0.34657359f * mul), z = y * y;  // (ln(2) / 2)
+        const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(62.0f / 2835.0f, z, -17.0f / 315.0f), z, 2.0f / 15.0f), z, -1.0f / 3.0f), z, 1.0f);
+        const float r = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[t][n] * mul));
+        s[t][n] = __builtin_fabsf(y) < 0.25f ? y * p : __builtin_fmaf(2.0f, r, 1.0f);
+      }
+    mul = sc.cap2;
+  } else if (sc.cap2 > 0.0f) {
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll

@@ -126,7 +126,7 @@ __device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int p
 // One row by itself, every key that it does not see left out: the path of rows that came out
 // infinite or NaN beside rows that see other keys (a weight of zero times an infinity is NaN in the
 // matrix product).  A wave a row: lane = key for the scores, lane = HD / 64 dims for the sums.
-template <int HD, int KIND, bool MOD, typename U>
+template <int HD, int KIND, int MOD, typename U>
 __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& sc, const U& un, int g,
                                        const uint16_t* q, int64_t ldq, int heads, int row, uint16_t* out) {
   constexpr bool BF = KIND == kKvBf16;
@@ -136,7 +136,7 @@ __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& s
   const uint16_t* qr = q + (int64_t)(un.seq.q0 + tok) * ldq + head * HD;
   const PagedRange rg = paged_range(i, un.seq.len, un.prefix, sc.window);
   const int capacity = kv.table_width << kv.page_shift, mask = (1 << kv.page_shift) - 1;
-  const float slope2 = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
+  const float slope2 = MOD != kModNone && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
   float m = -INFINITY, l = 0.0f, acc[DL] = {};
   for (int j0 = rg.lo; j0 < min(rg.hi, capacity); j0 += 64) {
     const int j = j0 + lane;
@@ -150,7 +150,7 @@ __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& s
       for (int d = 0; d < HD; ++d) x += (BF ? bf2f(qr[d]) : h2f(qr[d])) * paged_elem<HD, KIND>(kv, false, bad ? 0 : page, r, d);
       pf4_t one[1] = {{x, x, x, x}};
       float mul = sc.mul;
-      if constexpr (MOD) mul = paged_scores<1, 4>(one, sc, slope2, (float)(i - j), [](int) { return 0; });
+      if constexpr (MOD != kModNone) mul = paged_scores<MOD, 1, 4>(one, sc, slope2, (float)(i - j), [](int) { return 0; });
       x = bad ? NAN : one[0][0] * mul;
     }
     const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.0f : mn;
@@ -273,7 +273,7 @@ struct PagedLaunch {
   uint32_t* counters;
   float* slots;
   hipStream_t stream;
-  bool mod;
+  int mod;
   bool wide;  // more key steps than 2^29 are possible
 };
 // Few rows a sequence (drafted tokens times heads of a KV head): tiles of 16 or 32 rows, as many

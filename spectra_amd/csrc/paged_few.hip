@@ -54,7 +54,7 @@ constexpr int few_lds() {
   return red > ring ? red : ring;
 }
 
-template <int HD, int KIND, int NT, bool MOD>
+template <int HD, int KIND, int NT, int MOD>
 __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
     paged_few_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int tokens,
                      int heads, bool wide, uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
       const bool ok = 16 * nt + c < nrows;
       const int tok = one ? 0 : ok ? r / g : tok0, head = un.kvh * g + (ok ? r - tok * g : 0);
       rg[nt] = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
-      slope2[nt] = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
+      slope2[nt] = MOD != kModNone && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
       pos[nt] = i0 + tok;
       const uint16_t* qr = q + (int64_t)(sq.q0 + tok) * ldq + head * HD;
 #pragma unroll
@@ -232,8 +232,8 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
       for (int nt = 0; nt < NT; ++nt) {
         // scores of the keys key0 + 16 (e / 4) + 4 q4 + e % 4
         float x[8], mn = m[nt], mul = sc.mul;
-        if constexpr (MOD)
-          mul = paged_scores<2, 4>(s[nt], sc, slope2[nt], (float)(pos[nt] - (key0 + 4 * q4)), [](int n) { return n; });
+        if constexpr (MOD != kModNone)
+          mul = paged_scores<MOD, 2, 4>(s[nt], sc, slope2[nt], (float)(pos[nt] - (key0 + 4 * q4)), [](int n) { return n; });
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[nt][e >> 2][e & 3] * mul;
         if (part) {
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
   }
 }
 
-template <int HD, int KIND, int NT, bool MOD>
+template <int HD, int KIND, int NT, int MOD>
 static int launch_few(const PagedLaunch& a) {
   paged_few_kernel<HD, KIND, NT, MOD><<<dim3((unsigned)a.units), dim3(kFewThreads), 0, a.stream>>>(
       a.kv, a.sc, a.q, a.ldq, a.g, 16 * NT / a.g, a.heads, a.wide, a.counters, a.slots, a.out);
@@ -484,8 +484,9 @@ static int launch_few(const PagedLaunch& a) {
 }
 template <int HD, int KIND>
 static int launch_few_of(const PagedLaunch& a, int rows) {
-  if (rows == 16) return a.mod ? launch_few<HD, KIND, 1, true>(a) : launch_few<HD, KIND, 1, false>(a);
-  return a.mod ? launch_few<HD, KIND, 2, true>(a) : launch_few<HD, KIND, 2, false>(a);
+  if (a.mod == kModLargeCap) return rows == 16 ? launch_few<HD, KIND, 1, kModLargeCap>(a) : launch_few<HD, KIND, 2, kModLargeCap>(a);
+  if (rows == 16) return a.mod ? launch_few<HD, KIND, 1, kMod>(a) : launch_few<HD, KIND, 1, kModNone>(a);
+  return a.mod ? launch_few<HD, KIND, 2, kMod>(a) : launch_few<HD, KIND, 2, kModNone>(a);
 }
 int launch_paged_few(const PagedLaunch& a, int rows) {
   if (a.hd == 64)

@@ -52,7 +52,7 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4_t*)(lds_t)p));
 }
 
-template <int HD, int KIND, bool MOD, int QH>
+template <int HD, int KIND, int MOD, int QH>
 __global__ void __launch_bounds__(64 * kManyWaves, 2)
     paged_many_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                       uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
   const bool ok = 32 * qh + ln < nrows;
   const int rr = r0 + min(32 * qh + ln, nrows - 1), tok = rr / g, head = un.kvh * g + (rr - tok * g);
   const PagedRange rg = paged_range(i0 + tok, sq.len, un.prefix, sc.window);
-  const float slope2 = MOD && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
+  const float slope2 = MOD != kModNone && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
   const int pos = i0 + tok - 4 * gh;
   pu4_t qf[KS];
   {
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
     for (int i = 0; i < RING; ++i) ring[i] = read_k(buf ^ 1, i);
     __builtin_amdgcn_sched_barrier(0);
     float mul = sc.mul;
-    if constexpr (MOD) mul = paged_scores<TL, 16>(s, sc, slope2, (float)(pos - kw), [](int r) { return 8 * (r >> 2) + (r & 3); });
+    if constexpr (MOD != kModNone) mul = paged_scores<MOD, TL, 16>(s, sc, slope2, (float)(pos - kw), [](int r) { return 8 * (r >> 2) + (r & 3); });
     if (kw < alo || kw + 32 * TL > ahi) {
       const int from = rg.lo - kw - 4 * gh, to = min(rg.hi, capacity) - kw - 4 * gh;
 #pragma unroll
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
     paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + 32 * qh + __builtin_ctz(r), out);
 }
 
-template <int HD, int KIND, bool MOD, int QH>
+template <int HD, int KIND, int MOD, int QH>
 static int launch_many(const PagedLaunch& a) {
   const void* kern = (const void*)paged_many_kernel<HD, KIND, MOD, QH>;
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
@@ -439,8 +439,9 @@ static int launch_many(const PagedLaunch& a) {
 }
 template <int HD, int KIND>
 static int launch_many_of(const PagedLaunch& a, int rows) {
-  if (rows == 64) return a.mod ? launch_many<HD, KIND, true, 2>(a) : launch_many<HD, KIND, false, 2>(a);
-  return a.mod ? launch_many<HD, KIND, true, 4>(a) : launch_many<HD, KIND, false, 4>(a);
+  if (a.mod == kModLargeCap) return rows == 64 ? launch_many<HD, KIND, kModLargeCap, 2>(a) : launch_many<HD, KIND, kModLargeCap, 4>(a);
+  if (rows == 64) return a.mod ? launch_many<HD, KIND, kMod, 2>(a) : launch_many<HD, KIND, kModNone, 2>(a);
+  return a.mod ? launch_many<HD, KIND, kMod, 4>(a) : launch_many<HD, KIND, kModNone, 4>(a);
 }
 int launch_paged_many(const PagedLaunch& a, int rows) {
   if (a.hd == 64)
@@ -498,7 +499,7 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   a.sc.slopes = slopes;
   a.sc.prefix = prefix;
   a.sc.window = window < (1 << 30) ? window : 0;  // (no sequence is longer)
-  a.mod = cap > 0.0f || slopes != nullptr;
+  a.mod = a.sc.cap2 > kPagedCap ? kModLargeCap : cap > 0.0f || slopes != nullptr ? kMod : kModNone;
   a.q = (const uint16_t*)q;
   a.ldq = ldq;
   a.out = (uint16_t*)out;

@@ -199,6 +199,36 @@ def test_scores_and_masks(hip, kind, n, mods):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [[1, 1, 1], [3, 2, 4], [150, 40, 77]])
+@pytest.mark.parametrize("cap,scale", [(200.0, 0.125), (300.0, 0.125), (1e5, 0.125), (1e6, 0.3), (1e8, 0.125), (3e29, 0.125),
+                                       (300.0, 30.0), (2000.0, 400.0)])
+def test_large_caps(hip, kind, n, cap, scale):
+    """Caps far above the scores, and large ones that the scores reach.  A cap's error: 2^-20 of it up to 256 (its form is a
+    constant plus the score); past that 2^-19 of the score, whatever the cap: 10 roundings of 2^-24 where tanh is a
+    polynomial, and where it is 1 - 2 / (1 + 2^t), at least 0.24, 6 of 2^-24 in all (exp2 and the reciprocal are off by a
+    unit)."""
+    b = Batch(kind, n, [200, 333, 150], 6, 2, 64, 16, seed=41)
+    got, u, at = b.attend(cap=cap, scale=scale), torch.finfo(_DT[kind]).eps / 2, 0
+    sub = 2.0 ** -25 if kind != "bf16" else 0.0
+    for s, (t, m) in enumerate(zip(b.n, b.lens)):
+        k, v = b.rows(s)
+        see = torch.arange(m, device="cuda")[None] <= torch.arange(m - t, m, device="cuda")[:, None]
+        for h in range(6):
+            qh, kh, vh = b.q[at: at + t, h].double(), k[h // 3], v[h // 3]
+            x = cap * torch.tanh(qh @ kh.T * scale / cap)
+            delta = 64 * 2.0 ** -24 * (qh.abs() @ kh.abs().T * scale).amax(-1, keepdim=True)
+            delta = delta + (2.0 ** -20 * cap if cap <= 256 else 2.0 ** -19 * x.abs().amax(-1, keepdim=True))
+            x = x.masked_fill(~see, -math.inf)
+            p = torch.softmax(x, -1)
+            total = torch.exp(x - x.amax(-1, keepdim=True)).sum(-1, keepdim=True)
+            want, a = p @ vh, p @ vh.abs()
+            tol = u * want.abs() + (u + 2 * delta + 2.0 ** -20) * a + sub * (1 + (see.double() @ vh.abs()) / total)
+            assert torch.all((got[at: at + t, h].double() - want).abs() <= tol)
+        at += t
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["fp16", "4bit"])
 @pytest.mark.parametrize("n", [1, 6, 40])
 def test_long_caches_split(hip, kind, n):
