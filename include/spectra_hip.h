@@ -385,6 +385,8 @@ int spectra_greedy_finish(void* argmax_key, int64_t* token, int64_t* history, in
  * q_start[batch] (a padded batch) are left alone.  All three are read on the device: a captured
  * step follows them.  A page id outside [0, num_pages) or a position past the table is never
  * read or written: appending skips it, and attention gives NaN to every row that sees it.
+ * What a call writes (pages that it appends to, outputs, the workspace) must not overlap anything
+ * else that it is given; memory between pages is nobody's.
  */
 typedef enum { SPECTRA_KV_F16 = 0, SPECTRA_KV_BF16 = 1, SPECTRA_KV_4BIT = 2 } spectra_kv_kind_t;
 

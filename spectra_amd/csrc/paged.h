@@ -11,6 +11,8 @@
 // outside the table are never turned into addresses.
 #pragma once
 
+#include <initializer_list>
+
 #include "common.h"
 
 namespace spectra {
@@ -34,11 +36,50 @@ __device__ __forceinline__ uint64_t paged_at(int page, uint32_t step) { return (
 // device form (api side of every paged entry).
 int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, PagedKv* out);
 
-// Whether two runs of bytes overlap (an operand that others still read while it is written).
-inline bool paged_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+// An operand in memory: n runs of `bytes` bytes, `step` bytes from one to the next (pages of a pool, rows of a wider
+// matrix: what lies between them is not the operand's).
+struct PagedRegion {
+  const char* name;
+  const void* at;
+  int64_t bytes, step, n;
+};
+// Whether some run of a and some run of b share a byte.
+inline bool paged_meet(const PagedRegion& a, const PagedRegion& b) {
+  typedef __int128 wide;
+  if (a.at == nullptr || b.at == nullptr || a.bytes == 0 || b.bytes == 0) return false;
+  const wide x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  const int64_t as = a.n > 1 ? a.step : 0, bs = b.n > 1 ? b.step : 0;
+  if (x + (wide)(a.n - 1) * as + a.bytes <= y || y + (wide)(b.n - 1) * bs + b.bytes <= x) return false;
+  if (a.n > 1 && b.n > 1 && as != bs) {  // (pools that lie among each other with other strides)
+    const PagedRegion &few = a.n < b.n ? a : b, &all = a.n < b.n ? b : a;
+    for (int64_t i = 0; i < few.n; ++i)
+      if (paged_meet({few.name, (const uint8_t*)few.at + i * few.step, few.bytes, 0, 1}, all)) return true;
+    return false;
+  }
+  // Run j of b lies y - x + k step after run i of a, k = j - i if both have that step: the least k for which it does not
+  // end before a's begins.
+  const int64_t step = a.n > 1 ? as : bs;
+  wide k = 1 - a.n;
+  if (step > 0) {
+    const wide past = x - y - b.bytes, floor = past / step - (past % step < 0);
+    k = floor + 1 > k ? floor + 1 : k;
+  }
+  return k < b.n && y - x + k * step > -(wide)b.bytes && y - x + k * step < a.bytes;
 }
+// Refuses a call that writes memory which another of its operands has too: each region written against the others
+// written and those read.
+int paged_apart(std::initializer_list<PagedRegion> written, std::initializer_list<PagedRegion> read);
+// The caches' regions, keys and values of pages, scales and zero points (of no bytes where there are none).
+struct PagedPools {
+  PagedRegion k, v, ks, vs, kz, vz;
+};
+PagedPools paged_pools(const spectra_paged_kv_t* kv);
+// The block table, the lengths and the starts.
+inline PagedRegion paged_table(const spectra_paged_kv_t* kv) {
+  return {"block_table", kv->block_table, 4LL * kv->table_width, 4 * kv->table_stride, kv->batch};
+}
+inline PagedRegion paged_lens(const spectra_paged_kv_t* kv) { return {"kv_lens", kv->kv_lens, 4LL * kv->batch, 0, 1}; }
+inline PagedRegion paged_starts(const spectra_paged_kv_t* kv) { return {"q_start", kv->q_start, 4LL * (kv->batch + 1), 0, 1}; }
 
 // A sequence's part of the call: its first token, how many, and its keys after them.  Starts
 // are clamped to the call's tokens, lengths to what the table can hold plus one (a position past

@@ -13,6 +13,8 @@
 // thousand bf16 tokens (32 heads of 128 on 8) read and write 199 MB in 34 us, 5.8 TB/s.
 // Roundings: the rotated values to their 16 bits, once, from fp32 products and sums; 4-bit rows as the
 // quantizer rounds.
+#include <algorithm>
+
 #include "kv4.h"
 #include "paged.h"
 
@@ -185,6 +187,28 @@ int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, Page
   return SPECTRA_OK;
 }
 
+PagedPools paged_pools(const spectra_paged_kv_t* kv) {
+  const bool q4 = kv->kind == SPECTRA_KV_4BIT;
+  const int64_t rows = (int64_t)kv->kv_heads * kv->page_size, d = kv->head_dim, n = kv->num_pages;
+  const int64_t row = q4 ? d / 2 : 2 * d, step = kv->page_stride * (q4 ? 1 : 2), sb = q4 ? rows * (d / 32) * 2 : 0, zb = sb / 2;
+  return {{"the key pages", kv->k, rows * row, step, n},
+          {"the value pages", kv->v, rows * row, step, n},
+          {"the keys' scales", kv->k_scales, sb, kv->scale_stride * 2, n},
+          {"the values' scales", kv->v_scales, sb, kv->scale_stride * 2, n},
+          {"the keys' zero points", kv->k_zeros, zb, kv->zero_stride, n},
+          {"the values' zero points", kv->v_zeros, zb, kv->zero_stride, n}};
+}
+
+int paged_apart(std::initializer_list<PagedRegion> written, std::initializer_list<PagedRegion> read) {
+  for (const PagedRegion* w = written.begin(); w != written.end(); ++w) {
+    for (const PagedRegion* o = written.begin(); o != w; ++o)
+      if (paged_meet(*w, *o)) return fail(SPECTRA_ERR_INVALID, std::string(w->name) + " must not overlap " + o->name);
+    for (const PagedRegion& o : read)
+      if (paged_meet(*w, o)) return fail(SPECTRA_ERR_INVALID, std::string(w->name) + " must not overlap " + o.name);
+  }
+  return SPECTRA_OK;
+}
+
 }  // namespace spectra
 
 using namespace spectra;
@@ -203,9 +227,17 @@ extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const voi
                     reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 16) == 0 &&
                       ldqkv % 8 == 0,
                   "operands and qkv rows must be 16-byte aligned");
-  SPECTRA_REQUIRE(!paged_overlap(qkv, ((tokens - 1) * ldqkv + (int64_t)(heads + 2 * kv->kv_heads) * hd) * 2, q_rot,
-                                 tokens * heads * hd * 2),
-                  "q_rot must not overlap qkv");
+  const PagedPools pools = paged_pools(kv);
+  const int64_t turned = 2 * std::min<int64_t>(rope_rows, 1LL << 31) * hd;  // bytes of each table that positions name
+  if (int st = paged_apart({{"q_rot", q_rot, tokens * heads * hd * 2, 0, 1}, pools.k, pools.v, pools.ks, pools.vs, pools.kz, pools.vz},
+                           {{"qkv", qkv, (int64_t)(heads + 2 * kv->kv_heads) * hd * 2, ldqkv * 2, tokens},
+                            {"cos", cos_t, turned, 0, 1},
+                            {"sin", sin_t, turned, 0, 1},
+                            paged_table(kv),
+                            paged_lens(kv),
+                            paged_starts(kv)});
+      st != SPECTRA_OK)
+    return st;
   int waves = ((heads + kv->kv_heads) * (hd / 16) + kv->kv_heads * (hd / 8) + 63) / 64;
   int64_t blocks = (tokens * waves + kPaThreads / 64 - 1) / (kPaThreads / 64);
   if (blocks >= 64) blocks = (blocks + 7) / 8 * 8;

@@ -481,9 +481,6 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   SPECTRA_REQUIRE(ldq >= (int64_t)heads * kv->head_dim && ldq % 8 == 0, "q token stride too small or not a multiple of 8");
   SPECTRA_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0,
                   "q and out must be 16-byte aligned");
-  SPECTRA_REQUIRE(!paged_overlap(q, ((tokens - 1) * ldq + (int64_t)heads * kv->head_dim) * 2, out,
-                                 tokens * heads * kv->head_dim * 2),
-                  "out must not overlap q");
   SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(slopes) % 4 == 0 && reinterpret_cast<uintptr_t>(prefix) % 4 == 0,
                   "slopes and prefix must be aligned");
   SPECTRA_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive");
@@ -492,6 +489,16 @@ extern "C" int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q,
   if (workspace == nullptr || workspace_bytes < spectra_paged_attend_workspace(kv->head_dim))
     return fail(SPECTRA_ERR_WORKSPACE, "workspace missing or smaller than spectra_paged_attend_workspace bytes");
   SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  const PagedPools pools = paged_pools(kv);
+  if (int st = paged_apart({{"out", out, tokens * heads * kv->head_dim * 2, 0, 1},
+                            {"the workspace", workspace, (int64_t)spectra_paged_attend_workspace(kv->head_dim), 0, 1}},
+                           {{"q", q, (int64_t)heads * kv->head_dim * 2, ldq * 2, tokens},
+                            pools.k, pools.v, pools.ks, pools.vs, pools.kz, pools.vz,
+                            paged_table(kv), paged_lens(kv), paged_starts(kv),
+                            {"slopes", slopes, 4LL * heads, 0, 1},
+                            {"prefix", prefix, 4LL * kv->batch, 0, 1}});
+      st != SPECTRA_OK)
+    return st;
   constexpr double log2e = 1.4426950408889634;
   a.sc.mul = (float)(cap > 0.0f ? 2.0 * log2e * scale / cap : log2e * scale);
   a.sc.cap2 = (float)(cap * log2e);

@@ -2,6 +2,7 @@
 // Reads a call (heads, head size, page, table, lengths) and checks that the shares, or units, cover every key step of
 // every tile once, and that partial sums have records of their own.
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <map>
 #include <tuple>
@@ -184,7 +185,35 @@ static int check_many(const Call& c, const PagedGrid& grid, const Lanes& lane) {
   return 0;
 }
 
-int main() {
+// Regions of random runs in a small memory, against marks of their bytes.
+static int check_meet(unsigned seed) {
+  auto next = [&](int n) { return (int)(((seed = seed * 1664525u + 1013904223u) >> 8) % (unsigned)n); };
+  int both[2] = {0, 0};
+  for (int it = 0; it < 200000; ++it) {
+    PagedRegion r[2];
+    const int64_t one = 1 + next(24);
+    uint8_t marks[2][1024] = {};
+    for (int i = 0; i < 2; ++i) {
+      const int64_t step = next(3) ? one + 8 : 1 + next(40), n = 1 + next(12);
+      r[i] = {"", (const void*)(uintptr_t)(64 + next(200)), 1 + next((int)step), next(8) ? step : 0, n};
+      if (r[i].step == 0) r[i].n = 1;
+      for (int64_t j = 0; j < r[i].n; ++j)
+        for (int64_t k = 0; k < r[i].bytes; ++k) marks[i][(uintptr_t)r[i].at + j * r[i].step + k] = 1;
+    }
+    bool want = false;
+    for (int k = 0; k < 1024; ++k) want |= marks[0][k] && marks[1][k];
+    CHECK(paged_meet(r[0], r[1]) == want && paged_meet(r[1], r[0]) == want, "%zu + %lld of %lld x %lld, %zu + %lld of %lld x %lld",
+          (size_t)r[0].at, (long long)r[0].bytes, (long long)r[0].step, (long long)r[0].n, (size_t)r[1].at, (long long)r[1].bytes,
+          (long long)r[1].step, (long long)r[1].n);
+    ++both[want];
+  }
+  CHECK(both[0] > 10000 && both[1] > 10000, "%d apart, %d not", both[0], both[1]);
+  printf("ok\n");
+  return 0;
+}
+
+int main(int argc, char** argv) {
+  if (argc > 1) return check_meet((unsigned)atoi(argv[1]));
   Call c = {};
   int kvh, page, batch, width, pad;
   if (scanf("%d %d %d %d %d %d %d %d %d", &c.kind, &c.heads, &kvh, &c.hd, &page, &width, &batch, &pad, &c.window) != 9) return 2;

@@ -859,6 +859,100 @@ def test_append_refusals(change, msg):
     assert st == L.ERR_INVALID and msg in lib.spectra_last_error().decode()
 
 
+_POOL = 10 * 2 * 16 * 64 * 2  # bytes of the descriptor's pools
+
+
+def _desc4(**kw):
+    """4-bit pages, all operands apart."""
+    d = dict(kind=L.KV_4BIT, page_stride=2 * 16 * 32, k_scales=0x90000, v_scales=0x94000, k_zeros=0x98000, v_zeros=0x9c000,
+             scale_stride=2 * 16 * 2, zero_stride=2 * 16 * 2)
+    return _desc(**{**d, **kw})
+
+
+@pytest.mark.parametrize("what", ["k", "v", "k end", "table", "lens", "starts", "workspace", "slopes", "prefix", "4-bit scales",
+                                  "4-bit zeros", "workspace on k", "workspace on q", "workspace on lens"])
+def test_attend_refuses_outputs_in_other_operands(what):
+    lib, p, out, ws, sl, pre, q = L.load(), _desc(), 0x50000, 0x100000, None, None, 0x40000
+    if what.startswith("4-bit"):
+        p = _desc4()
+        out = 0x94000 + 9 * 2 * 16 * 2 * 2 if "scales" in what else 0x9c000
+    elif what in ("k", "v", "k end"):
+        out = {"k": 0x10000, "v": 0x20000 + _POOL - 16, "k end": 0x10000 - 5 * 4 * 64 * 2 + 16}[what]
+    elif what in ("table", "lens", "starts"):
+        setattr(p, {"table": "block_table", "lens": "kv_lens", "starts": "q_start"}[what], out + 64)
+    elif what == "workspace":
+        out = ws + 4096
+    elif what == "slopes":
+        sl = out + 16
+    elif what == "prefix":
+        pre = out + 5 * 4 * 64 * 2 - 4
+    else:
+        ws = {"workspace on k": 0x10000 - 4096, "workspace on q": 0x40000, "workspace on lens": 0x31000 - 4096}[what]
+    st = lib.spectra_paged_attend(ctypes.byref(p), q, 4 * 64, 5, 4, 0.125, 0.0, 0, sl, pre, ws, 1 << 40, out, None)
+    assert st == L.ERR_INVALID and "must not overlap" in lib.spectra_last_error().decode()
+
+
+@pytest.mark.parametrize("what", ["q on k", "q on v", "q on cos", "q on table", "k on v", "k on qkv", "v on lens", "k on sin",
+                                  "k on scales", "scales on zeros", "zeros on keys' zeros", "strides"])
+def test_append_refuses_operands_that_it_writes_twice(what):
+    lib, p, q, qkv, cos, sin = L.load(), _desc4() if "scales" in what or "zeros" in what else _desc(), 0x50000, 0x40000, 0x70000, 0x80000
+    if what == "q on k":
+        q = 0x10000 + _POOL - 16
+    elif what == "q on v":
+        q = 0x20000 - 16
+    elif what == "q on cos":
+        q = cos + 9 * 32 * 4 - 16
+    elif what == "q on table":
+        p.block_table = q
+    elif what == "k on v":
+        p.v = p.k
+    elif what == "k on qkv":
+        qkv = 0x10000 + 32
+    elif what == "v on lens":
+        p.kv_lens = 0x20000 + 12
+    elif what == "k on sin":
+        sin = 0x10000 + _POOL - 16
+    elif what == "k on scales":
+        p.k_scales = 0x10000 + 16
+    elif what == "scales on zeros":
+        p.v_zeros = p.k_scales + 32
+    elif what == "zeros on keys' zeros":
+        p.v_zeros = p.k_zeros
+    else:  # 4-bit scales between the codes' pages, but farther apart: the second lies in a page
+        p = _desc4(page_stride=2 * 16 * 32 + 128, k_scales=0x10000 + 2 * 16 * 32, scale_stride=2 * 16 * 2 + 576)
+    st = lib.spectra_paged_rope_append(ctypes.byref(p), qkv, 8 * 64, 5, cos, sin, 9, 4, q, None)
+    assert st == L.ERR_INVALID and "must not overlap" in lib.spectra_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [[1, 1], [40, 70]])
+def test_pools_among_each_other(hip, kind, n):
+    """Keys and values (and scales and zero points) of a page beside each other in one allocation, the outputs between
+    the last ones: apart, and the same results."""
+    from spectra_amd import kernels as K
+    b = Batch(kind, n, [90, 75], 4, 2, 64, 16, seed=43)
+    parts = [t for c in zip(b.k, b.v) for t in c] if kind == "4bit" else [b.k, b.v]
+    sizes = [t[0].numel() * t.element_size() for t in parts]
+    pages, rest = parts[0].shape[0], b.q.numel() * 2
+    step = sum(sizes) + 64
+    room = torch.zeros(pages * step + 2 * rest, dtype=torch.uint8, device="cuda")
+    views, at = [], 0
+    for t, size in zip(parts, sizes):
+        x = room[at:].view(t.dtype).as_strided(t.shape, (step // t.element_size(),) + t.stride()[1:])
+        x.copy_(t)
+        views.append(x)
+        at += size
+    ends = [room[pages * step + i * rest:][:rest].view(b.q.dtype).view(b.q.shape) for i in (0, 1)]
+    qkv = b.rand(b.tokens, 8 * 64)
+    near = K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, None, None, 4, b.k, b.v)
+    want = b.attend()
+    c = (tuple(views[0::2]), tuple(views[1::2])) if kind == "4bit" else views
+    q = K.paged_rope_append(qkv, b.kv_lens, b.q_start, b.table, None, None, 4, *c, q_out=ends[0])
+    assert torch.equal(q, near)
+    assert torch.equal(K.paged_attend(b.q, b.kv_lens, b.q_start, b.table, *c, out=ends[1]), want)
+
+
 @pytest.mark.parametrize("scale,cap", [(3e38, 0.0), (1.0, 1e-38), (1.0, 3e38), (0.0, 0.0)])
 def test_scales_out_of_range(scale, cap):
     lib, p = L.load(), _desc()

@@ -13,22 +13,32 @@ F16, Q4 = 0, 2
 
 
 @pytest.fixture(scope="session")
-def plan(tmp_path_factory):
+def program(tmp_path_factory):
     exe = str(tmp_path_factory.mktemp("plan") / "paged_plan")
     r = subprocess.run([shutil.which("hipcc") or "/opt/rocm/bin/hipcc", "-x", "hip", "--offload-host-only",
                         "--offload-arch=gfx950", "-O2", "-std=c++17", "-w", f"-I{ROOT}/spectra_amd/csrc", f"-I{ROOT}/include",
                         os.path.join(ROOT, "tests", "paged_plan.cpp"), "-o", exe], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+    return exe
 
+
+@pytest.fixture(scope="session")
+def plan(program):
     def run(n, lens, heads=8, kv_heads=8, d=64, page=64, kind=F16, width=0, pad=0, window=0, prefix=None):
         """``width``: pages a sequence that the table holds (0: what the longest needs)."""
         head = f"{kind} {heads} {kv_heads} {d} {page} {width} {len(n)} {pad} {window}\n"
         rows = "\n".join(f"{a} {b} {-1 if prefix is None else prefix[i]}" for i, (a, b) in enumerate(zip(n, lens)))
-        r = subprocess.run([exe], input=head + rows + "\n", capture_output=True, text=True, timeout=300)
+        r = subprocess.run([program], input=head + rows + "\n", capture_output=True, text=True, timeout=300)
         assert r.returncode == 0, r.stdout + r.stderr
         return r.stdout
 
     return run
+
+
+def test_regions_that_meet(program):
+    """Which operands share memory, runs with gaps between them included (what lies between pages is not the pool's)."""
+    r = subprocess.run([program, "7"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout
 
 
 # sums of padded steps of exactly 2^32, of a little more, and past it without a wrap to something small
