@@ -8,13 +8,15 @@
 //
 // The library is a Python module, too, whose two functions take the same arguments and go past the
 // dispatcher (some 2 us a call for this many arguments) where it would only have passed them on:
-// plain tensors, and no mode that wants to see operators.  Otherwise they return NotImplemented, and the
-// caller takes the registered operator, which a compiler traces.
+// plain tensors that nothing is differentiated by, and no mode that wants to see operators.  Otherwise they return
+// NotImplemented, and the caller takes the registered operator, which a compiler traces and whose result says, when a
+// gradient is asked of it, that there is none.
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
@@ -233,12 +235,23 @@ void paged_attend_out_meta(const at::Tensor&, const at::Tensor&, const at::Tenso
                            const at::Tensor&) {}
 
 // ---- the Python functions ----
+
+// A tensor of a device that the dispatcher would do nothing about.
+bool plain_tensor(PyObject* o) {
+  if (!THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  static const c10::DispatchKeySet views({c10::DispatchKey::Negative, c10::DispatchKey::Conjugate, c10::DispatchKey::ZeroTensor,
+                                          c10::DispatchKey::Functionalize, c10::DispatchKey::Python});
+  return t.is_cuda() && !t.key_set().has_any(views) && !(t.requires_grad() && c10::GradMode::is_enabled()) &&
+         !t._fw_grad(/*level=*/0).defined();
+}
+
 struct Arguments {
   PyObject* const* a;
-  bool plain = true;  // nothing but plain tensors, of a device, where tensors belong
+  bool plain = true;  // nothing but plain tensors where tensors belong
 
   const at::Tensor* tensor(int i) {
-    plain = plain && THPVariable_CheckExact(a[i]) && THPVariable_Unpack(a[i]).is_cuda();
+    plain = plain && plain_tensor(a[i]);
     return plain ? &THPVariable_Unpack(a[i]) : nullptr;
   }
   OptTensor optional(int i) {
@@ -255,7 +268,7 @@ struct Arguments {
     if (!(plain = plain && (PyTuple_Check(a[i]) || PyList_Check(a[i])))) return r;
     PyObject** items = PySequence_Fast_ITEMS(a[i]);
     for (Py_ssize_t j = 0; j < PySequence_Fast_GET_SIZE(a[i]) && plain; ++j) {
-      plain = THPVariable_CheckExact(items[j]) && THPVariable_Unpack(items[j]).is_cuda();
+      plain = plain_tensor(items[j]);
       if (plain) r.push_back(THPVariable_Unpack(items[j]));
     }
     plain = plain && !r.empty();

@@ -1029,6 +1029,33 @@ def test_registered_operators(hip):
     assert torch.equal(torch.compile(functions, backend="aot_eager", fullgraph=True)(qkv, b.k, b.v), eager)
 
 
+@pytest.mark.gpu
+def test_operands_that_gradients_are_asked_of(hip):
+    """There is no derivative: the results are the registered operators', which say so when one is asked for."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [1, 3], [70, 33], 4, 2, 64, 16, seed=16)
+    ws, want = K.paged_attend_workspace(64), b.attend()
+    qkv = b.rand(b.tokens, 8 * 64)
+    batch = b.kv_lens, b.q_start, b.table
+    rows = K.paged_rope_append(qkv, *batch, None, None, 4, b.k, b.v)
+    want = b.attend()
+    q = b.q.clone().requires_grad_()
+    got = [K.paged_attend(q, *batch, b.k, b.v, workspace=ws), K.paged_attend(b.q, *batch, b.k, b.v.clone().requires_grad_()),
+           K.paged_attend(b.q, *batch, b.k, b.v, slopes=torch.zeros(4, device="cuda", requires_grad=True))]
+    for o in got:
+        assert o.requires_grad and torch.equal(o, want)
+        with pytest.warns(UserWarning, match="autograd kernel was not registered"):
+            o.sum().backward()
+    r = K.paged_rope_append(qkv.clone().requires_grad_(), *batch, None, None, 4, b.k, b.v)
+    assert r.requires_grad and torch.equal(r, rows)
+    with torch.no_grad():
+        assert not K.paged_attend(q, *batch, b.k, b.v, workspace=ws).requires_grad
+    # a negated view of one number, which only the dispatcher would resolve
+    one = Batch("fp16", [1], [40], 1, 1, 64, 16, seed=17)
+    slope = torch.complex(torch.zeros(1), torch.full((1,), -0.25)).cuda().conj().imag
+    assert slope.is_neg() and torch.equal(one.attend(slopes=slope), one.attend(slopes=torch.full((1,), 0.25, device="cuda")))
+
+
 def test_registered_operators_have_shapes():
     """The operators' Meta kernels (what a compiler traces with)."""
     ops = L.load_torch_ops()
