@@ -160,12 +160,21 @@ void paged_rope_append_out(const at::Tensor& qkv, const at::Tensor& kv_lens, con
                            at::TensorList k, at::TensorList v, const at::Tensor& q_out) {
   append(qkv, kv_lens, q_start, block_table, cos, sin, heads, k, v, &q_out);
 }
+// What the results' shapes are made of, for a call without memory.
+void check_meta(const at::Tensor& x, int64_t dims, at::TensorList k, at::TensorList v) {
+  TORCH_CHECK_VALUE(x.dim() == dims && (k.size() == 1 || k.size() == 3) && v.size() == k.size() && k[0].dim() == 4,
+                    "k_pages and v_pages must be [pages, kv_heads, page, d], or (codes, scales, zeros) of that, for ", dims,
+                    "-dimensional activations");
+}
 at::Tensor paged_rope_append_meta(const at::Tensor& qkv, const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                                  const OptTensor&, const OptTensor&, int64_t heads, at::TensorList k, at::TensorList) {
+                                  const OptTensor&, const OptTensor&, int64_t heads, at::TensorList k, at::TensorList v) {
+  check_meta(qkv, 2, k, v);
   return at::empty_symint({qkv.sym_size(0), heads, k[0].sym_size(3) * (k.size() == 3 ? 2 : 1)}, qkv.options());
 }
-void paged_rope_append_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
-                                const OptTensor&, int64_t, at::TensorList, at::TensorList, const at::Tensor&) {}
+void paged_rope_append_out_meta(const at::Tensor& qkv, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                                const OptTensor&, int64_t, at::TensorList k, at::TensorList v, const at::Tensor&) {
+  check_meta(qkv, 2, k, v);
+}
 
 // ---- attention ----
 at::Tensor attend(const at::Tensor& q_in, const at::Tensor& kv_lens, const at::Tensor& q_start,
@@ -225,14 +234,17 @@ void paged_attend_out(const at::Tensor& q, const at::Tensor& kv_lens, const at::
                       const at::Tensor& out) {
   attend(q, kv_lens, q_start, block_table, k, v, scale, cap, window, slopes, prefix, workspace, &out);
 }
-at::Tensor paged_attend_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::TensorList,
-                             at::TensorList, double, double, int64_t, const OptTensor&, const OptTensor&,
+at::Tensor paged_attend_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::TensorList k,
+                             at::TensorList v, double, double, int64_t, const OptTensor&, const OptTensor&,
                              const OptTensor&) {
+  check_meta(q, 3, k, v);
   return at::empty_symint(q.sym_sizes(), q.options());
 }
-void paged_attend_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::TensorList,
-                           at::TensorList, double, double, int64_t, const OptTensor&, const OptTensor&, const OptTensor&,
-                           const at::Tensor&) {}
+void paged_attend_out_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::TensorList k,
+                           at::TensorList v, double, double, int64_t, const OptTensor&, const OptTensor&, const OptTensor&,
+                           const at::Tensor&) {
+  check_meta(q, 3, k, v);
+}
 
 // ---- the Python functions ----
 

@@ -1070,3 +1070,21 @@ def test_registered_operators_have_shapes():
     for p in (pages, q4):
         r = ops.paged_rope_append(torch.empty(5, 8 * 64, dtype=torch.float16, **m), i32(2), i32(3), i32(2, 4), None, None, 4, p, p)
         assert r.shape == (5, 4, 64)
+
+
+@pytest.mark.parametrize("out", [False, True])
+@pytest.mark.parametrize("what", ["none", "two", "values"])
+def test_registered_operators_refuse_other_lists(out, what):
+    """Lists of no pages, or of neither one tensor nor three, without memory: an error, also for a tracing compiler."""
+    ops = L.load_torch_ops()
+    m = dict(device="meta")
+    i32 = lambda *s: torch.empty(*s, dtype=torch.int32, **m)  # noqa: E731
+    p = torch.empty(3, 2, 16, 64, dtype=torch.float16, **m)
+    k, v = {"none": ([], []), "two": ([p, p], [p, p]), "values": ([p], [])}[what]
+    q, qkv = torch.empty(5, 4, 64, dtype=torch.float16, **m), torch.empty(5, 8 * 64, dtype=torch.float16, **m)
+    append = (qkv, i32(2), i32(3), i32(2, 4), None, None, 4, k, v)
+    attend = (q, i32(2), i32(3), i32(2, 4), k, v, 0.1, 0.0, 0, None, None, None)
+    with pytest.raises(ValueError, match="k_pages"):
+        ops.paged_rope_append_out(*append, q) if out else ops.paged_rope_append(*append)
+    with pytest.raises(ValueError, match="k_pages"):
+        ops.paged_attend_out(*attend, q) if out else ops.paged_attend(*attend)
