@@ -123,6 +123,14 @@ __device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int p
   }
 }
 
+// The running maximum lags: sums are rescaled only where a score passes the maximum they refer to by
+// kPagedSlack (so hardly ever after the first steps).  Weights are 2^(score - maximum + raise): in fp16's range at
+// most 2^15, with its subnormals 2^-21 below the largest (values are at most 65504, so 2^30 of them fit fp32's sums);
+// in bf16, whose values reach fp32's last power of two, at most 2^-16, so that sums of 65536 of the largest do not pass it.
+constexpr float kPagedSlack = 8.0f;
+template <bool BF>
+constexpr float kPagedRaise = BF ? -24.0f : 7.0f;
+
 // One row by itself, every key that it does not see left out: the path of rows that came out
 // infinite or NaN beside rows that see other keys (a weight of zero times an infinity is NaN in the
 // matrix product).  A wave a row: lane = key for the scores, lane = HD / 64 dims for the sums.
@@ -154,7 +162,7 @@ __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& s
       x = bad ? NAN : one[0][0] * mul;
     }
     const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.0f : mn;
-    const float corr = __builtin_amdgcn_exp2f(m - mu), e = see ? __builtin_amdgcn_exp2f(x - mu) : 0.0f;
+    const float corr = __builtin_amdgcn_exp2f(m - mu), e = see ? __builtin_amdgcn_exp2f(x - mu + kPagedRaise<BF>) : 0.0f;
     m = mn;
     l = l * corr + wave_sum(e);
 #pragma unroll
@@ -188,11 +196,6 @@ __device__ __forceinline__ bool paged_arrive(uint32_t* counter, int pieces, int*
   __syncthreads();
   return *flag != 0;
 }
-
-// The running maximum lags: sums are rescaled only where a score passes the maximum they refer to by
-// kPagedSlack (so hardly ever after the first steps), and weights are 2^(score - maximum +
-// kPagedRaise), at most 2^15: inside fp16's range, with its subnormals 2^-21 below the largest.
-constexpr float kPagedSlack = 8.0f, kPagedRaise = 7.0f;
 
 // The factor that brings sums of maximum m and total l to the maximum mm.  Without keys (-inf and
 // 0): 0; a total of NaN (NaN scores do not show in a maximum): 1.

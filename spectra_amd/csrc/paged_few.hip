@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
             for (int i = 0; i < 4; ++i) o[nt][j][i] *= corr;
           m[nt] = mn;
         }
-        const float mu = m[nt] == -INFINITY ? 0.0f : m[nt] - kPagedRaise;
+        const float mu = m[nt] == -INFINITY ? 0.0f : m[nt] - kPagedRaise<BF>;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           x[e] = __builtin_amdgcn_exp2f(x[e] - mu);

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
         for (int r = 0; r < 16; ++r) o[d][r] *= corr;
       m = mn;
     }
-    const float mu = m == -INFINITY ? 0.0f : m - kPagedRaise;
+    const float mu = m == -INFINITY ? 0.0f : m - kPagedRaise<BF>;
     pu4_t pf[TL][2];
     auto weights = [&](int i) __attribute__((always_inline)) {  // the i-th pair
       const int t = i >> 3, r = 2 * (i & 7);

@@ -388,6 +388,18 @@ def test_tables_past_32_bits(hip, kind, n, far):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [[1, 1], [3, 4], [70, 40]])
+@pytest.mark.parametrize("size", [7e37, 1e-24])
+def test_values_at_the_ends_of_the_range(hip, n, size):
+    """bf16 values whose unweighted sums pass fp32's range, and tiny ones."""
+    b = Batch("bf16", n, [90, 3000], 6, 2, 128, 32, seed=47)
+    b.v = (b.v.float().clamp(-4.0, 4.0) * size).bfloat16()
+    assert torch.all(torch.isfinite(b.check()[: sum(n)]))
+    b.q.zero_()  # (all weights alike)
+    assert torch.all(torch.isfinite(b.check()[: sum(n)]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 def test_rows_without_keys(hip, kind):
     """More tokens than keys (positions below zero), and scores that are all -inf: zeros."""
