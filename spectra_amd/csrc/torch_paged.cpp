@@ -254,8 +254,9 @@ bool plain_tensor(PyObject* o) {
   const at::Tensor& t = THPVariable_Unpack(o);
   static const c10::DispatchKeySet views({c10::DispatchKey::Negative, c10::DispatchKey::Conjugate, c10::DispatchKey::ZeroTensor,
                                           c10::DispatchKey::Functionalize, c10::DispatchKey::Python});
-  return t.is_cuda() && !t.key_set().has_any(views) && !(t.requires_grad() && c10::GradMode::is_enabled()) &&
-         !t._fw_grad(/*level=*/0).defined();
+  if (!t.is_cuda() || t.key_set().has_any(views)) return false;
+  return t.unsafeGetTensorImpl()->autograd_meta() == nullptr ||
+         (!(t.requires_grad() && c10::GradMode::is_enabled()) && !t._fw_grad(/*level=*/0).defined());
 }
 
 struct Arguments {
