@@ -108,20 +108,77 @@ __device__ __forceinline__ void copy_lds4(const uint8_t* p, uint32_t to) {
 }
 typedef __attribute__((address_space(3))) uint8_t* lds_t;
 
-// One element of the pages (the row-by-row path's reads).
+// Eight dims 8 c .. of a row of the pages (the row-by-row path's reads).
 template <int HD, int KIND>
-__device__ __forceinline__ float paged_elem(const PagedKv& kv, bool value, int page, int64_t row, int d) {
+__device__ __forceinline__ void paged_eight(const PagedKv& kv, bool value, int page, int64_t row, int c, float (&x)[8]) {
   const uint8_t* p = (value ? kv.v : kv.k) + paged_at(page, kv.page_step);
   if constexpr (KIND == kKv4) {
-    const uint32_t c = (p[row * (HD / 2) + d / 2] >> (4 * (d & 1))) & 15u;
-    const float s = h2f(*(const uint16_t*)((value ? kv.vs : kv.ks) + paged_at(page, kv.scale_step) + 2 * (row * (HD / 32) + d / 32)));
-    const float z = (float)(value ? kv.vz : kv.kz)[paged_at(page, kv.zero_step) + row * (HD / 32) + d / 32];
-    return h2f(f2h(((float)c - z) * s));
+    const uint32_t w = *(const uint32_t*)(p + row * (HD / 2) + 4 * c);
+    const float s = h2f(*(const uint16_t*)((value ? kv.vs : kv.ks) + paged_at(page, kv.scale_step) + 2 * (row * (HD / 32) + c / 4)));
+    const float z = (float)(value ? kv.vz : kv.kz)[paged_at(page, kv.zero_step) + row * (HD / 32) + c / 4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = h2f(f2h(((float)((w >> (4 * e)) & 15u) - z) * s));
   } else {
-    const uint16_t h = ((const uint16_t*)p)[row * HD + d];
-    return KIND == kKvBf16 ? bf2f(h) : h2f(h);
+    const pu4_t u = *(const pu4_t*)(p + (row * HD + 8 * c) * 2);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t h = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+      x[e] = KIND == kKvBf16 ? bf2f(h) : h2f(h);
+    }
   }
 }
+
+// What values that are not finite do to a tile whose rows see different keys: in the product a weight of zero times such
+// a value is NaN, so they reach the rows that do not see them.  Those keys lie at the tile's ragged ends, which the wave
+// looks over: the first in [klo, alo) and the last in [ahi - 1, khi), and the first in the latter whose values
+// are NaN in every dim (rows that see it are NaN in any case).
+struct PagedSpoiled {
+  int low, high, full;
+  // Whether a row that sees [lo, hi) has to be computed by itself.
+  __device__ __forceinline__ bool reaches(const PagedRange& r) const {
+    return (low < r.lo || high >= r.hi) && !(r.lo <= full && full < r.hi);
+  }
+};
+template <int HD, int KIND, typename U>
+__device__ __forceinline__ PagedSpoiled paged_spoiled(const PagedKv& kv, const PagedScore& sc, const U& un, int g, int r0, int nrows) {
+  PagedSpoiled sp = {0x7fffffff, -1, 0x7fffffff};
+  const int i0 = un.seq.len - un.seq.n, capacity = kv.table_width << kv.page_shift;
+  const PagedRange ra = paged_range(i0 + r0 / g, un.seq.len, un.prefix, sc.window);
+  const PagedRange rb = paged_range(i0 + (r0 + nrows - 1) / g, un.seq.len, un.prefix, sc.window);
+  const int klo = ra.lo, alo = rb.lo, ahi = ra.hi, khi = min(rb.hi, capacity);
+  const int lane = __lane_id(), mask = (1 << kv.page_shift) - 1;
+#pragma unroll 1
+  for (int end = 0; end < 2; ++end) {
+    const int from = end ? max(ahi - 1, klo) : klo, to = end ? khi : min(alo, khi);
+#pragma unroll 1
+    for (int j0 = from; j0 < to; j0 += 64) {
+      const int j = min(j0 + lane, to - 1);
+      int page = kv.table[un.b * kv.table_stride + (j >> kv.page_shift)];
+      if ((uint32_t)page >= (uint32_t)kv.num_pages) page = 0;  // (the rows that stood in for it)
+      const int64_t r = ((int64_t)un.kvh << kv.page_shift) + (j & mask);
+      uint32_t most = 0, least = ~0u;  // of the magnitudes' bits: infinity's 0x7f800000, NaNs' past it
+#pragma unroll 4
+      for (int c = 0; c < HD / 8; ++c) {
+        float x[8];
+        paged_eight<HD, KIND>(kv, true, page, r, c, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t bits = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu;
+          most = max(most, bits);
+          least = min(least, bits);
+        }
+      }
+      const uint64_t some = __ballot(most >= 0x7f800000u), every = __ballot(least > 0x7f800000u);
+      if (end == 0 && some != 0) sp.low = min(sp.low, j0 + __builtin_ctzll(some));
+      if (end == 1 && some != 0) sp.high = min(j0 + 63 - __builtin_clzll(some), to - 1);
+      if (end == 1 && every != 0) sp.full = min(sp.full, j0 + __builtin_ctzll(every));
+    }
+  }
+  return sp;
+}
+
+// odd, or NaN where y is infinite or NaN.
+__device__ __forceinline__ float paged_odd(float odd, float y) { return __builtin_fmaf(y, 0.0f, odd); }
 
 // The running maximum lags: sums are rescaled only where a score passes the maximum they refer to by
 // kPagedSlack (so hardly ever after the first steps).  Weights are 2^(score - maximum + raise): in fp16's range at
@@ -131,31 +188,38 @@ constexpr float kPagedSlack = 8.0f;
 template <bool BF>
 constexpr float kPagedRaise = BF ? -24.0f : 7.0f;
 
-// One row by itself, every key that it does not see left out: the path of rows that came out
-// infinite or NaN beside rows that see other keys (a weight of zero times an infinity is NaN in the
-// matrix product).  A wave a row: lane = key for the scores, lane = HD / 64 dims for the sums.
+// One row by itself, every key that it does not see left out: the path of rows that values reach which they do not
+// see (PagedSpoiled), rows of at most the two tiles of a sequence's KV head that such a key lies at an end of.  A wave a row:
+// lane = key for the scores; for the sums each lane has 8 dims of every G-th key.
 template <int HD, int KIND, int MOD, typename U>
 __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& sc, const U& un, int g,
                                        const uint16_t* q, int64_t ldq, int heads, int row, uint16_t* out) {
   constexpr bool BF = KIND == kKvBf16;
-  constexpr int DL = HD / 64;
-  const int lane = threadIdx.x & 63;
+  constexpr int CH = HD / 8, G = 64 / CH;
+  const int lane = __lane_id(), kc = lane % CH, kg = lane / CH;  // (made anew: the loop before this has no register for it)
   const int tok = row / g, head = un.kvh * g + row % g, i = un.seq.len - un.seq.n + tok;
   const uint16_t* qr = q + (int64_t)(un.seq.q0 + tok) * ldq + head * HD;
   const PagedRange rg = paged_range(i, un.seq.len, un.prefix, sc.window);
-  const int capacity = kv.table_width << kv.page_shift, mask = (1 << kv.page_shift) - 1;
+  const int capacity = kv.table_width << kv.page_shift, mask = (1 << kv.page_shift) - 1, end = min(rg.hi, capacity);
   const float slope2 = MOD != kModNone && sc.slopes ? sc.slopes[head] * 1.4426950408889634f : 0.0f;
-  float m = -INFINITY, l = 0.0f, acc[DL] = {};
-  for (int j0 = rg.lo; j0 < min(rg.hi, capacity); j0 += 64) {
+  float m = -INFINITY, l = 0.0f, acc[8] = {};
+#pragma unroll 1
+  for (int j0 = rg.lo; j0 < end; j0 += 64) {
     const int j = j0 + lane;
-    const bool see = j < min(rg.hi, capacity);
+    const bool see = j < end;
     const int page = see ? kv.table[un.b * kv.table_stride + (j >> kv.page_shift)] : 0;
     const bool bad = (uint32_t)page >= (uint32_t)kv.num_pages;
     const int64_t r = ((int64_t)un.kvh << kv.page_shift) + (j & mask);
     float x = -INFINITY;
     if (see) {
       x = 0.0f;
-      for (int d = 0; d < HD; ++d) x += (BF ? bf2f(qr[d]) : h2f(qr[d])) * paged_elem<HD, KIND>(kv, false, bad ? 0 : page, r, d);
+#pragma unroll 4
+      for (int c = 0; c < CH; ++c) {
+        float k[8];
+        paged_eight<HD, KIND>(kv, false, bad ? 0 : page, r, c, k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x += (BF ? bf2f(qr[8 * c + e]) : h2f(qr[8 * c + e])) * k[e];
+      }
       pf4_t one[1] = {{x, x, x, x}};
       float mul = sc.mul;
       if constexpr (MOD != kModNone) mul = paged_scores<MOD, 1, 4>(one, sc, slope2, (float)(i - j), [](int) { return 0; });
@@ -166,20 +230,30 @@ __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& s
     m = mn;
     l = l * corr + wave_sum(e);
 #pragma unroll
-    for (int d = 0; d < DL; ++d) acc[d] *= corr;
-    for (int n = 0; n < 64 && j0 + n < min(rg.hi, capacity); ++n) {
-      const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), n));
-      const int pg = __builtin_amdgcn_readlane(bad ? 0 : page, n);
-      const int64_t rn = ((int64_t)un.kvh << kv.page_shift) + ((j0 + n) & mask);
+    for (int d = 0; d < 8; ++d) acc[d] *= corr;
+#pragma unroll 4
+    for (int n0 = 0; n0 < 64; n0 += G) {
+      const int n = n0 + kg;
+      const float p = __shfl(e, n, 64);
+      const int pg = __shfl(bad ? 0 : page, n, 64);
+      if (j0 + n < end) {
+        float v[8];
+        paged_eight<HD, KIND>(kv, true, pg, ((int64_t)un.kvh << kv.page_shift) + ((j0 + n) & mask), kc, v);
 #pragma unroll
-      for (int d = 0; d < DL; ++d) acc[d] += p * paged_elem<HD, KIND>(kv, true, pg, rn, DL * lane + d);
+        for (int d = 0; d < 8; ++d) acc[d] += p * v[d];
+      }
     }
   }
-  if (rg.hi > capacity) l = NAN;
 #pragma unroll
-  for (int d = 0; d < DL; ++d) {
-    const float v = l == 0.0f ? 0.0f : acc[d] / l;
-    out[((int64_t)(un.seq.q0 + tok) * heads + head) * HD + DL * lane + d] = BF ? f2bf(v) : f2h(v);
+  for (int d = 0; d < 8; ++d)
+#pragma unroll
+    for (int off = CH; off < 64; off *= 2) acc[d] += __shfl_xor(acc[d], off, 64);
+  if (kg == 0) {
+    uint32_t w[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      w[d] = pack2<BF>(l == 0.0f ? 0.0f : acc[2 * d] / l, l == 0.0f ? 0.0f : acc[2 * d + 1] / l);
+    *(uint4*)(out + ((int64_t)(un.seq.q0 + tok) * heads + head) * HD + 8 * kc) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 

@@ -403,15 +403,16 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
     auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
       const int r = r0 + row, tok = one ? 0 : r / g, head = un.kvh * g + (r - tok * g);
       const bool past = paged_range(i0 + tok, sq.len, un.prefix, sc.window).hi > capacity;
-      const float inv = past ? NAN : den == 0.0f ? 0.0f : 1.0f / den;
+      const float inv = past ? NAN : 1.0f / den;
       float y[4];
-      bool odd = false;
+      float odd = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        y[e] = v[e] * inv;
-        odd |= !(__builtin_fabsf(y[e]) < INFINITY);
+        y[e] = den == 0.0f && !past ? 0.0f : v[e] * inv;
+        odd = paged_odd(odd, y[e]);
       }
-      if (mixed && odd) atomicOr(&redo[turn], 1u << row);
+      // (where the total is NaN the row's own scores are)
+      if (mixed && odd != odd && den == den && !past) atomicOr(&redo[turn], 1u << row);
       const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
       *(uint2*)(out + ((int64_t)(sq.q0 + tok) * heads + head) * HD + d) = w;
     };
@@ -467,11 +468,14 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
       }
     }
     __syncthreads();  // (rows to be done over are known, and LDS is free for the next part)
-    if (mixed)
+    if (mixed && redo[turn] != 0) {
+      const PagedSpoiled sp = paged_spoiled<HD, KIND>(kv, sc, un, g, r0, nrows);
       for (uint32_t r = redo[turn]; r != 0; r &= r - 1) {
         const int row = __builtin_ctz(r);
-        if ((row & 3) == wave) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + row, out);
+        if ((row & 3) != wave || !sp.reaches(paged_range(i0 + (r0 + row) / g, sq.len, un.prefix, sc.window))) continue;
+        paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + row, out);
       }
+    }
   }
 }
 

@@ -364,8 +364,15 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
   uint32_t again = 0;              // this wave's rows to be done over
   if (un.pieces == 1) {
     const bool past = rg.hi > capacity;
-    const float inv = past ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
-    bool odd = false;
+    if (__ballot(l == 0.0f) != 0) {  // rows without keys or scores, whatever the values are
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = l == 0.0f ? 0.0f : o[d][r];
+      l = l == 0.0f ? 1.0f : l;
+    }
+    const float inv = past ? NAN : 1.0f / l;
+    float odd = 0.0f;
     if (ok && kh == 0) {
       uint16_t* orow = out + ((int64_t)(sq.q0 + tok) * heads + head) * HD;
 #pragma unroll
@@ -376,12 +383,12 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             y[e] = o[d][4 * r + e] * inv;
-            odd |= !(__builtin_fabsf(y[e]) < INFINITY);
+            odd = paged_odd(odd, y[e]);
           }
           *(uint2*)(orow + 32 * d + 8 * r + 4 * gh) = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
         }
     }
-    const uint64_t b = __ballot(odd);
+    const uint64_t b = __ballot(odd != odd && l == l && !past);  // (where the total is NaN the row's own scores are)
     again = (uint32_t)(b | (b >> 32));
   } else {
     const int first = un.slot - un.piece;
@@ -406,26 +413,30 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
       const float den = paged_join_by<HD, ROWS, 4, NI>(slots, [&](int p) { return first + p; }, un.pieces, row, 256 * part + 2 * lane,
                                                        128, 256 * W, v);
       const bool past = paged_range(i0 + t, sq.len, un.prefix, sc.window).hi > capacity;
-      bool odd = false;
+      float odd = 0.0f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           y[e] = past ? NAN : den == 0.0f ? 0.0f : v[i][e] / den;
-          odd |= !(__builtin_fabsf(y[e]) < INFINITY);
+          odd = paged_odd(odd, y[e]);
         }
         const int d = 8 * (wave + W * i) + 4 * gh;
         *(uint2*)(out + ((int64_t)(sq.q0 + t) * heads + h) * HD + d) = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
       }
-      if (odd) atomicOr(&redo[row >> 5], 1u << (row & 31));
+      if (odd != odd && den == den && !past) atomicOr(&redo[row >> 5], 1u << (row & 31));
     }
     __syncthreads();
     again = kh == 0 ? redo[qh] : 0;
   }
-  if (!mixed) return;
-  for (uint32_t r = sread(again); r != 0; r &= r - 1)
-    paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, r0 + 32 * qh + __builtin_ctz(r), out);
+  again = sread(again);
+  if (!mixed || again == 0) return;
+  const PagedSpoiled sp = paged_spoiled<HD, KIND>(kv, sc, un, g, r0, nrows);
+  for (uint32_t r = again; r != 0; r &= r - 1) {
+    const int row = r0 + 32 * qh + __builtin_ctz(r);
+    if (sp.reaches(paged_range(i0 + row / g, sq.len, un.prefix, sc.window))) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, row, out);
+  }
 }
 
 template <int HD, int KIND, int MOD, int QH>

@@ -464,6 +464,87 @@ def test_what_a_row_does_not_see_stays_out(hip, kind, n, lens, what):
         at += t
 
 
+def _least_us(f):
+    f()
+    least = math.inf
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        least = min(least, 1e3 * a.elapsed_time(b))
+    return least
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,lens", [([2500], [2500]), ([400, 300], [9000, 300]), ([5] * 9, [4000] * 9)])
+@pytest.mark.parametrize("what", ["value", "values", "key", "page"])
+def test_what_is_not_finite_costs_little(hip, kind, n, lens, what):
+    """A value, all values, a key that are not finite, or a page that is missing, where every row sees it: no row is computed
+    by itself for that, and the call takes about as long as with finite ones.  (One by one the prompt's rows took
+    some hundred times as long.)"""
+    b = Batch(kind, n, lens, 6, 2, 128, 16, seed=51)
+    from spectra_amd import kernels as K
+    ws = K.paged_attend_workspace(128)
+    out = torch.empty_like(b.q)
+    clean = _least_us(lambda: b.attend(workspace=ws, out=out))
+    row, first = b.table[:, 0].long(), (slice(None), 3)
+    if what == "page":
+        b.table[:, 0] = -1
+    else:
+        x = (b.k if what == "key" else b.v)
+        x = x[1] if kind == "4bit" else x
+        x[(slice(None),) * 3 if what == "values" else (row, *first)] = float("nan")
+    spoilt = _least_us(lambda: b.attend(workspace=ws, out=out))
+    at = 0
+    for t, m in zip(n, lens):
+        pos = torch.arange(m - t, m, device="cuda")
+        sees = pos >= (0 if what in ("values", "page") else 3)
+        lost = torch.isnan(out[at: at + t]).all(-1).all(-1)
+        assert torch.equal(lost, sees) and torch.all(torch.isfinite(out[at: at + t][~sees]))
+        at += t
+    assert spoilt < 4 * clean + 100, (clean, spoilt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("n", [[1, 1], [3, 4], [40, 130]])
+def test_infinite_values_where_every_score_is(hip, kind, n):
+    """Rows that see only scores of -inf are zero, whatever the values are."""
+    b = Batch(kind, n, [40, 300], 4, 2, 64, 16, seed=53)
+    b.k[:] = float("inf")
+    b.q[:] = -1.0
+    for what in (float("inf"), float("nan")):
+        b.v[:] = what
+        assert torch.all(b.attend()[: sum(n)] == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=5.0, slopes=True), dict(cap=1e4), dict(window=30, prefix=True)])
+def test_rows_computed_by_themselves(hip, kind, d, kw):
+    """One value of the last tokens that is not finite: the rows of its tile that do not see it are as without it."""
+    kw = dict(kw)
+    if "slopes" in kw:
+        kw["slopes"] = torch.exp2(-torch.arange(1, 7, device="cuda").float())
+    if "prefix" in kw:
+        kw["prefix"] = torch.tensor([10, 0, 60], dtype=torch.int32, device="cuda")
+    b = Batch(kind, [4, 50, 140], [90, 77, 500], 6, 2, d, 16, seed=57)
+    want, tol = b.reference(**kw)
+    for s, (t, m) in enumerate(zip(b.n, b.lens)):
+        x = b.v[1] if kind == "4bit" else b.v
+        x[b.table[s, (m - 2) // 16].long(), :, (m - 2) % 16, 0] = float("inf")
+    out, at = b.attend(**kw), 0
+    for t, m in zip(b.n, b.lens):
+        x, keep = out[at: at + t].double(), slice(0, t - 2)
+        assert torch.all((x[keep] - want[at: at + t][keep]).abs() <= tol[at: at + t][keep])
+        assert not torch.any(torch.isfinite(x[t - 2:]).all(-1))
+        at += t
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("n", [1, 3, 100])
