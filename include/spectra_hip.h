@@ -422,7 +422,7 @@ int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int
  * j is visible when j < kv_lens[b], j <= i or j < prefix[b], and i - j < window or window is 0.
  * fp32 scores, softmax and sums (a cap up to 256 adds at most 2^-20 of itself to a score's error, a larger
  * one 2^-19 of the score); weights rounded to the activations' 16 bits for the product
- * with v; 4-bit values stand for fp16((q - z) * s).  A row that sees no key, or only scores of
+ * with v; 4-bit values stand for fp16((q - z) * s) (bf16 in the contiguous cache).  A row that sees no key, or only scores of
  * -inf, is zero; what a row does not see (rows of a page past the length, later tokens) does not
  * reach it, whatever it holds, infinities and NaN included.  q [tokens, heads, head_dim], token
  * stride ldq (a multiple of 8, heads contiguous), out contiguous and apart from q, both 16-byte aligned; slopes

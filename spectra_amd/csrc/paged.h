@@ -81,9 +81,9 @@ inline PagedRegion paged_table(const spectra_paged_kv_t* kv) {
 inline PagedRegion paged_lens(const spectra_paged_kv_t* kv) { return {"kv_lens", kv->kv_lens, 4LL * kv->batch, 0, 1}; }
 inline PagedRegion paged_starts(const spectra_paged_kv_t* kv) { return {"q_start", kv->q_start, 4LL * (kv->batch + 1), 0, 1}; }
 
-// A sequence's part of the call: its first token, how many, and its keys after them.  Starts
-// are clamped to the call's tokens, lengths to what the table can hold plus one (a position past
-// it is a fault of the caller's that its rows report as NaN).
+// A sequence's part of the call: its first token, how many, and its keys after them.  Starts are clamped to the
+// call's tokens, lengths at zero.  (Lengths past what the table holds stay: rows that would see such positions are NaN,
+// and no position past it is read.)
 struct PagedSeq {
   int q0, n, len;
 };

@@ -26,7 +26,8 @@
 // length, more of them than fit at once: 131071 keys 125 us, not 113, 64 users 206, not 200.)
 //
 // Roundings: the weights to the activations' 16 bits, which the product with V takes (half a unit each, in
-// sums that stay fp32), the 4-bit values to fp16 (what the dequantizer gives), the output.
+// sums that stay fp32), the 4-bit values to fp16 (which the products take; three bits more than the bf16 that
+// kv4_dequantize and the contiguous 4-bit cache's attention round them to), the output.
 #include "paged_attend.h"
 
 namespace spectra {
@@ -364,10 +365,8 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
       __syncthreads();  // (the waves' sums go where the codes were)
     } else if (key < kend) {
       Tile ta, tb;
-      int a0 = page_of(key), a1 = page_of(key + 16), b0 = 0, b1 = 0;
-      load(ta, key, a0, a1);
-      b0 = page_of(key + kFewKeys);
-      b1 = page_of(key + kFewKeys + 16);
+      load(ta, key, page_of(key), page_of(key + 16));
+      int b0 = page_of(key + kFewKeys), b1 = page_of(key + kFewKeys + 16);
       while (true) {
         if (key + kFewKeys < kend) load(tb, key + kFewKeys, b0, b1);
         int n0 = page_of(key + 2 * kFewKeys), n1 = page_of(key + 2 * kFewKeys + 16);
@@ -375,8 +374,6 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
         key += kFewKeys;
         if (key >= kend) break;
         if (key + kFewKeys < kend) load(ta, key + kFewKeys, n0, n1);
-        a0 = n0;
-        a1 = n1;
         n0 = page_of(key + 2 * kFewKeys);
         n1 = page_of(key + 2 * kFewKeys + 16);
         compute(tb, key, tb.bad[0], tb.bad[1]);

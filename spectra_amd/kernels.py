@@ -803,9 +803,9 @@ def paged_attend(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
     j < prefix[b] (int32 [batch]), and with ``window`` > 0 only those with i - j < window.  A
     score is scale q.k (1/sqrt(d) by default), capped as cap * tanh(. / cap) when ``cap`` > 0,
     less slopes[h] |i - j| (fp32 [heads]).  fp32 scores and softmax; the weights are rounded to q's
-    type for the product with v; 4-bit values stand for fp16((q - z) * s).  A row that sees no key
-    is zero; one that would need a page outside the pool or past the table is NaN; rows behind
-    q_start[-1] are left alone.  ``workspace``: ``paged_attend_workspace(d)``; by default a fresh
+    type for the product with v; 4-bit values stand for fp16((q - z) * s) (``attend_decode_q4`` takes
+    them as bf16).  A row that sees no key is zero; one that would need a page outside the pool or past the
+    table is NaN; rows behind q_start[-1] are left alone.  ``workspace``: ``paged_attend_workspace(d)``; by default a fresh
     one, which costs a small kernel."""
     if not q.is_cuda:
         raise ValueError("q must be on the GPU")

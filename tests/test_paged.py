@@ -771,6 +771,42 @@ def test_against_the_contiguous_kernels(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,d,m", [(24, 8, 128, 700), (8, 2, 64, 90)])
+def test_against_the_contiguous_4bit_cache(hip, heads, kv, d, m):
+    """The same codes in the contiguous 4-bit cache stand for bf16 values there, and for fp16 ones on pages: the two differ
+    by that rounding and their kernels', no more."""
+    from spectra_amd import kernels as K
+    w, page = 16, 64
+    b = Batch("4bit", [1], [m], heads, kv, d, page, seed=61)
+    g = _gen(62)
+    # the newest rows, which the contiguous cache takes from qkv: exact in 4 bits (every group holds codes 0 and 15)
+    code = torch.randint(0, 16, (2, kv, d // 32, 32), generator=g, device="cuda")
+    code[..., 0], code[..., 1] = 0, 15
+    new = ((code - 6) * 0.125).half().view(2, kv, d)
+    at = (int(b.table[0, (m - 1) // page]), slice(None), (m - 1) % page)
+    for c, x in zip((b.k, b.v), new):
+        for t, y in zip(c, K.kv4_quantize(x.view(kv, 1, d).contiguous())):
+            t[at] = y.view(kv, -1)
+    ids = b.table[0, : -(-m // page)].long()
+    codes = [tuple(t[ids].transpose(0, 1).reshape(kv, -1, t.shape[-1])[:, :m].contiguous() for t in c) for c in (b.k, b.v)]
+    rows = b.rows(0)
+    ring = [torch.zeros(kv, w, d, dtype=torch.float16, device="cuda") for _ in rows]  # the window: the same values
+    last = torch.arange(m - w, m, device="cuda")
+    for r, x in zip(ring, rows):
+        r[:, last % w] = x[:, last].half()
+    one, zero = torch.ones(m, d // 2, device="cuda"), torch.zeros(m, d // 2, device="cuda")
+    qkv = torch.cat([b.q.reshape(-1), new.reshape(-1)])
+    old = K.attend_decode_q4(qkv, torch.tensor([m - 1], device="cuda"), one, zero, heads, kv, *ring, *codes)
+    want, tol = b.reference()
+    u, g = 2.0 ** -8 + 2.0 ** -11, heads // kv
+    k, v = (x.repeat_interleave(g, 0) for x in rows)
+    size = (b.q[0].double().abs()[:, None] @ k.abs().transpose(1, 2)).squeeze(1) / math.sqrt(d)
+    p = torch.softmax((b.q[0].double()[:, None] @ k.transpose(1, 2)).squeeze(1) / math.sqrt(d), -1)
+    a = (p[:, None] @ v.abs()).squeeze(1)
+    assert torch.all((old.double() - b.attend()[0].double()).abs() <= 2 * tol[0] + u * (1 + 2 * size.amax(-1, keepdim=True)) * a)
+
+
+@pytest.mark.gpu
 def test_strided_queries_and_streams(hip):
     """Queries inside wider rows, and calls on another stream than the current default, with a workspace each."""
     from spectra_amd import kernels as K
