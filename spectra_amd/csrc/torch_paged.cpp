@@ -125,8 +125,8 @@ at::Tensor append(const at::Tensor& qkv_in, const at::Tensor& kv_lens, const at:
   if (cos.has_value())
     for (const at::Tensor* t : {&*cos, &*sin})
       TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == cos->size(0) &&
-                            t->size(1) == d / 2 && t->is_contiguous() && t->device() == qkv.device(),
-                        "cos and sin must be contiguous fp32 [rows, d / 2] on ", qkv.device());
+                            t->size(0) > 0 && t->size(1) == d / 2 && t->is_contiguous() && t->device() == qkv.device(),
+                        "cos and sin must be contiguous fp32 [rows, d / 2], at least a row, on ", qkv.device());
   const c10::DeviceGuard guard(qkv.device());
   // rows are read 16 bytes at a time
   if (qkv.stride(1) != 1 || (tokens > 1 && (qkv.stride(0) < width || qkv.stride(0) % 8 != 0)) ||

@@ -925,6 +925,17 @@ def test_refusals(hip):
         K.paged_rope_append(*args[:4], torch.ones(40, 16, device="cuda"), torch.ones(40, 16, device="cuda"), *args[6:])
 
 
+@pytest.mark.gpu
+def test_rope_tables_without_rows(hip):
+    """Not the same as no tables: no position has an angle."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [1], [4], 2, 2, 64, 16, seed=15)
+    none = torch.empty(0, 32, device="cuda")
+    with pytest.raises(ValueError, match="at least a row"):
+        K.paged_rope_append(torch.zeros(1, 6 * 64, dtype=torch.float16, device="cuda"), b.kv_lens, b.q_start, b.table, none, none, 2,
+                            b.k, b.v)
+
+
 # -- the C entries' refusals, without a GPU -------------------------------------------------------
 def _desc(**kw):
     p = L.PagedKv()
