@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
     }
   }
   const bool mixed = tok1 > tok0;  // rows that see different keys
-  uint32_t again = 0;              // this wave's rows to be done over
+  uint32_t again = 0;              // rows that came out infinite or NaN
   if (un.pieces == 1) {
     const bool past = rg.hi > capacity;
     if (__ballot(l == 0.0f) != 0) {  // rows without keys or scores, whatever the values are
@@ -428,14 +428,19 @@ __global__ void __launch_bounds__(64 * kManyWaves, 2)
       if (odd != odd && den == den && !past) atomicOr(&redo[row >> 5], 1u << (row & 31));
     }
     __syncthreads();
-    again = kh == 0 ? redo[qh] : 0;
+#pragma unroll
+    for (int h = 0; h < QH; ++h) again |= redo[h];
   }
   again = sread(again);
   if (!mixed || again == 0) return;
   const PagedSpoiled sp = paged_spoiled<HD, KIND>(kv, sc, un, g, r0, nrows);
-  for (uint32_t r = again; r != 0; r &= r - 1) {
-    const int row = r0 + 32 * qh + __builtin_ctz(r);
-    if (sp.reaches(paged_range(i0 + row / g, sq.len, un.prefix, sc.window))) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, row, out);
+#pragma unroll 1
+  for (int h = 0; h < QH; ++h) {  // (a joined tile's rows by all waves)
+    uint32_t r = un.pieces == 1 ? (h == qh ? again : 0) : redo[h] & (0x11111111u << wave);
+    for (r = sread(r); r != 0; r &= r - 1) {
+      const int row = r0 + 32 * h + __builtin_ctz(r);
+      if (sp.reaches(paged_range(i0 + row / g, sq.len, un.prefix, sc.window))) paged_row<HD, KIND, MOD>(kv, sc, un, g, q, ldq, heads, row, out);
+    }
   }
 }
 
