@@ -407,7 +407,7 @@ typedef struct spectra_paged_kv {
  * q and k heads of `tokens` fused-QKV rows (row stride ldqkv: heads q heads, kv_heads k heads,
  * kv_heads v heads) at their positions (cos_t, sin_t fp32 [rope_rows, head_dim / 2]; NULL = no
  * rotation), appends k and v, 4-bit pages through the quantizer of spectra_kv4_quantize, and
- * writes q_rot [tokens, heads, head_dim] (apart from qkv).  A token without a position in [0, rope_rows) appends
+ * writes q_rot [tokens, heads, head_dim].  A token without a position in [0, rope_rows) appends
  * nothing and gets NaN queries.  Two tokens never write the same row unless two sequences name
  * the same page for positions they append: such rows then hold either's values, or a mix. */
 int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
@@ -420,13 +420,13 @@ int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int
  *               f(scale q[t, h] . k_j) - slopes[h] |i - j|,   f(x) = cap tanh(x / cap), or x
  *                                                             when cap is 0
  * j is visible when j < kv_lens[b], j <= i or j < prefix[b], and i - j < window or window is 0.
- * fp32 scores, softmax and sums (a cap up to 256 adds at most 2^-20 of itself to a score's error, a larger
- * one 2^-19 of the score); weights rounded to the activations' 16 bits for the product
- * with v; 4-bit values stand for fp16((q - z) * s) (bf16 in the contiguous cache).  A row that sees no key, or only scores of
- * -inf, is zero; what a row does not see (rows of a page past the length, later tokens) does not
- * reach it, whatever it holds, infinities and NaN included.  q [tokens, heads, head_dim], token
- * stride ldq (a multiple of 8, heads contiguous), out contiguous and apart from q, both 16-byte aligned; slopes
- * fp32 [heads] and prefix int32 [batch] may be NULL.
+ * fp32 scores, softmax and sums (a cap up to 256 adds at most 2^-20 of itself to a score's error, a
+ * larger one 2^-19 of the score); weights rounded to the activations' 16 bits for the product with
+ * v; 4-bit values stand for fp16((q - z) * s) (bf16 in the contiguous cache).  A row that sees no
+ * key, or only scores of -inf, is zero; what a row does not see (rows of a page past the length,
+ * later tokens) does not reach it, whatever it holds, infinities and NaN included.  q [tokens,
+ * heads, head_dim], token stride ldq (a multiple of 8, heads contiguous), out contiguous, both
+ * 16-byte aligned; slopes fp32 [heads] and prefix int32 [batch] may be NULL.
  * workspace: spectra_paged_attend_workspace(head_dim) bytes, 16-byte aligned: arrival counters
  * (SPECTRA_PAGED_COUNTER_BYTES at its start), then partial sums of sequences whose keys are
  * split.  ZERO the counters before its first use; every complete call leaves them at zero, so a
