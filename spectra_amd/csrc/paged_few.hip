@@ -6,9 +6,9 @@
 // of every workgroup that holds some of a tile's keys ends with such sums of its own, and sums of maxima m and
 // m' are brought together by the factors 2^(m - max(m, m')).
 //
-// Bound by reading the cache once: 64 users with 0 to 8191 keys read 1.11 GB in 201 us, 5.5 TB/s (a copy reaches
-// 5.0 both ways), 131071 bf16 keys 537 MB in 112 us, 4.8 TB/s, 48 users on 4-bit pages 455 MB in 121 us, 3.8 TB/s
-// (there the expansion's vector instructions are as much as the loads); 96 keys take 6.8 us, of which an
+// Bound by reading the cache once: 64 users with 0 to 8191 keys read 1.11 GB in 200 us, 5.5 TB/s (a copy reaches
+// 5.0 both ways), 131071 bf16 keys 537 MB in 109 us, 4.9 TB/s, 48 users on 4-bit pages 455 MB in 110 to 122 us, 3.7 to
+// 4.1 TB/s (there the expansion's vector instructions are as much as the loads); 96 keys take 6.7 us, of which an
 // empty launch is most.  So 16-bit rows do not go through LDS: a wave takes 32 keys at a
 // time straight into the registers that the matrix instructions read, the next 32 in flight
 // behind them.  Scores are computed transposed, S^T = K Q^T (16 x 16 x 32): a lane's 16 bytes of a key

@@ -7,9 +7,9 @@
 //
 // Bound by the matrix cores and the exponentials between them (4 head_dim flops and one exponential a score,
 // 8 cycles a wave, a quarter of a 32 x 32 x 16 matrix instruction): a prompt of 8192 tokens
-// (24 heads of 128) does 412 GFLOP in 405 to 423 us, 975 to 1019 TFLOP/s where a large matrix product reaches
+// (24 heads of 128) does 412 GFLOP in 403 to 430 us, 960 to 1022 TFLOP/s where a large matrix product reaches
 // 1145; there the matrix cores are busy half of the time at a clock that their power lowers.  With a cap (two
-// exponentials and a reciprocal a score) 700 TFLOP/s; 4-bit pages with a bias and heads of 64 276.  A prompt of
+// exponentials and a reciprocal a score) 670 to 720 TFLOP/s; 4-bit pages with a bias and heads of 64 250 to 280.  A prompt of
 // 777 tokens takes 18 us: 13 key steps one after another for its last rows, and fewer tiles than would
 // hide their latencies.
 //
