@@ -261,12 +261,12 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(KIND, HD, 16 * NT))
         }
         const float mu = m[nt] == -INFINITY ? 0.0f : m[nt] - kPagedRaise<BF>;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(x[e] - mu);
-          l[nt] += x[e];
-        }
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - mu);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pf[nt][e] = pack2<BF>(x[2 * e], x[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) {  // (the total is of the weights as rounded, so that a mean of values lies among them)
+          pf[nt][e] = pack2<BF>(x[2 * e], x[2 * e + 1]);
+          l[nt] = add2<BF>(pf[nt][e], l[nt]);
+        }
       }
       // O^T += V^T P^T, dims DPL (l % 16) + j at step j: the 8 keys' values of a dim, in pairs of keys
       uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};

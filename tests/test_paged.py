@@ -400,6 +400,36 @@ def test_values_at_the_ends_of_the_range(hip, n, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("n", [[1] * 40, [3, 4] * 20, [70, 40]])
+def test_means_of_the_largest_value(hip, kind, n):
+    """Values that are all the type's largest: so is their mean, whatever the weights' roundings."""
+    b = Batch(kind, n, [90 + 7 * s for s in range(len(n))], 6, 2, 128, 32, seed=63)
+    b.q *= 3
+    most = torch.finfo(b.q.dtype).max
+    for sign in (1, -1):
+        b.v[:] = sign * most
+        assert torch.all(b.attend()[: sum(n)] == sign * most)
+    b.v[:] = 0.75  # (and of another: half a unit in the last place, and the sums' own roundings, away at most)
+    assert torch.all((b.attend()[: sum(n)].float() - 0.75).abs() <= torch.finfo(b.q.dtype).eps / 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 30])
+def test_weights_that_round_alike(hip, kind, n):
+    """One key, and others whose weights are one number each time and round up or down together: the mean of the type's
+    largest value is that value."""
+    b = Batch(kind, [n], [32], 6, 2, 128, 32, seed=67)
+    most = torch.finfo(b.q.dtype).max
+    b.v[:], b.k[:], b.q[:] = most, 0, 0
+    b.q[..., 0] = 1
+    b.k[:, :, 0, 0] = 1
+    for j in range(1, 400):
+        assert torch.all(b.attend(scale=math.log(2) * (1 - j / 1000)) == most), j
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 def test_rows_without_keys(hip, kind):
     """More tokens than keys (positions below zero), and scores that are all -inf: zeros."""
