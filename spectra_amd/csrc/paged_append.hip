@@ -146,6 +146,7 @@ int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, Page
   const bool q4 = kv->kind == SPECTRA_KV_4BIT;
   const int d = kv->head_dim;
   SPECTRA_REQUIRE(kv->kv_heads > 0 && heads > 0 && heads % kv->kv_heads == 0, "heads must be a multiple of kv_heads");
+  SPECTRA_REQUIRE(heads <= (1 << 20), "heads out of range");
   if (d != 64 && d != 128) return fail(SPECTRA_ERR_UNSUPPORTED, "paged KV head_dim must be 64 or 128");
   SPECTRA_REQUIRE(kv->page_size >= 16 && kv->page_size <= 65536 && is_pow2(kv->page_size),
                   "page_size must be a power of two, at least 16");
@@ -156,6 +157,9 @@ int paged_args(const spectra_paged_kv_t* kv, int64_t tokens, int32_t heads, Page
   SPECTRA_REQUIRE(tokens > 0 && tokens < (1LL << 31) && tokens * (heads / kv->kv_heads) < (1LL << 30),
                   "tokens out of range");
   SPECTRA_REQUIRE(kv->k && kv->v && kv->block_table && kv->kv_lens && kv->q_start, "NULL pointer");
+  SPECTRA_REQUIRE((reinterpret_cast<uintptr_t>(kv->block_table) | reinterpret_cast<uintptr_t>(kv->kv_lens) |
+                   reinterpret_cast<uintptr_t>(kv->q_start)) % 4 == 0,
+                  "block table, lengths and starts must be aligned");
   const int64_t rows = (int64_t)kv->kv_heads * kv->page_size;
   const int64_t row = q4 ? d / 2 : 2 * d;
   SPECTRA_REQUIRE(rows * row < (1LL << 31), "page too large");

@@ -997,6 +997,19 @@ def test_descriptor_refusals(bad, msg):
     assert st in (L.ERR_INVALID, L.ERR_UNSUPPORTED) and msg in lib.spectra_last_error().decode()
 
 
+@pytest.mark.parametrize("bad,heads,msg", [(dict(block_table=0x30002), 4, "aligned"), (dict(kv_lens=0x31001), 4, "aligned"),
+                                           (dict(q_start=0x32002), 4, "aligned"), (dict(kv_heads=1), 1 << 25, "range")])
+def test_descriptor_refusals_of_addresses_and_heads(bad, heads, msg):
+    """Integers that lie across words, which scalar loads would read elsewhere, and heads past 32-bit offsets of a row."""
+    lib = L.load()
+    p = _desc(**bad)
+    st = lib.spectra_paged_rope_append(ctypes.byref(p), 0x40000, (1 << 26) * 64, 5, None, None, 0, heads, 0x50000, None)
+    assert st == L.ERR_INVALID and msg in lib.spectra_last_error().decode()
+    st = lib.spectra_paged_attend(ctypes.byref(p), 0x40000, (1 << 26) * 64, 5, heads, 0.125, 0.0, 0, None, None, 0x60000, 1 << 40,
+                                  0x50000, None)
+    assert st == L.ERR_INVALID and msg in lib.spectra_last_error().decode()
+
+
 @pytest.mark.parametrize("change,status,msg", [
     (dict(q=None), L.ERR_INVALID, "NULL"), (dict(q=0x40008), L.ERR_INVALID, "16-byte"), (dict(ldq=100), L.ERR_INVALID, "stride"),
     (dict(ldq=4 * 64 + 4), L.ERR_INVALID, "stride"), (dict(tokens=0), L.ERR_INVALID, "tokens"),
