@@ -190,8 +190,8 @@ constexpr float kPagedRaise = BF ? -24.0f : 7.0f;
 
 // One row by itself, every key that it does not see left out: the path of rows that values reach which they do not
 // see (PagedSpoiled), rows of at most the two tiles of a sequence's KV head that such a key lies at an end of.  A wave a row:
-// lane = key for the scores; for the sums each lane has 8 dims of every G-th key.  Its loops are not unrolled: that made it
-// 8 % faster and prompts that never come here 2 % slower (biased 4-bit ones 49.0 to 50.0 us).
+// lane = key for the scores; for the sums each lane has 8 dims of every G-th key.  Its loops are not unrolled: four times
+// made it 8 % faster, and prompts that never come here 2 % slower (biased 4-bit ones 49.0 to 50.0 us).
 template <int HD, int KIND, int MOD, typename U>
 __device__ __forceinline__ void paged_row(const PagedKv& kv, const PagedScore& sc, const U& un, int g,
                                        const uint16_t* q, int64_t ldq, int heads, int row, uint16_t* out) {

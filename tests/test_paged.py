@@ -431,6 +431,22 @@ def test_weights_that_round_alike(hip, kind, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ones,chunk", [(64, 300), (30, 150), (16, 700)])
+def test_single_tokens_beside_a_chunk(hip, kind, ones, chunk):
+    """One call, as a serving loop makes it: users' next tokens and a part of a new prompt, in tiles of the few rows' kernel
+    (the first two) and of the many rows'."""
+    r = torch.Generator().manual_seed(ones)
+    lens = torch.randint(1, 900, (ones,), generator=r).tolist()
+    n = [1] * (ones // 2) + [chunk] + [1] * (ones - ones // 2)
+    lens[ones // 2: ones // 2] = [chunk + 250]
+    b = Batch(kind, n, lens, 6, 2, 128, 32, seed=71, pad=1)
+    first = b.check()
+    assert torch.equal(b.attend(out=torch.full_like(b.q, 7.0)), first)
+    b.check(cap=20.0, window=300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
 def test_rows_without_keys(hip, kind):
     """More tokens than keys (positions below zero), and scores that are all -inf: zeros."""
     b = Batch(kind, [4, 2, 150], [2, 0, 100], 4, 2, 64, 16, seed=1)
