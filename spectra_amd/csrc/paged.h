@@ -413,7 +413,8 @@ __host__ __device__ __forceinline__ bool paged_unit(const PagedKv& kv, int g, in
     work += W::product(t.tiles, t.steps);
   }
   work *= (float)kv.kv_heads;
-  const int piece_steps = (int)__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(work / (float)target), (float)min_steps), 1e9f);
+  // (2^25: more steps than any tile has, and three times as many fit in 32 bits)
+  const int piece_steps = (int)__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(work / (float)target), (float)min_steps), 33554432.0f);
   int base = 0, slot0 = 0;
   for (int c0 = 0; c0 < kv.batch; c0 += 64) {
     if (kv.batch > 64) take(c0);

@@ -446,6 +446,41 @@ def test_single_tokens_beside_a_chunk(hip, kind, ones, chunk):
 
 
 @pytest.mark.gpu
+def test_many_prompts_at_far_positions(hip):
+    """Prompts whose key steps, counted whole beside a prefix, are more for each unit of work than a tile can have; a window
+    leaves the last keys."""
+    from spectra_amd import kernels as K
+    g, page, d, kv, batch, n, window = _gen(73), 65536, 64, 8, 64, 5500, 300
+    k, v = (torch.randn(3, kv, page, d, generator=g, device="cuda").half() for _ in range(2))
+    table = (torch.arange(batch * 8193, device="cuda") % 3).int().view(batch, -1)
+    lens = [(1 << 29) - 999 * b for b in range(batch)]
+    q = torch.randn(batch * n, kv, d, generator=g, device="cuda", dtype=torch.float16)
+    out = torch.full_like(q, 7.0)
+    K.paged_attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                   torch.arange(0, batch * n + 1, n, dtype=torch.int32, device="cuda"), table, k, v, window=window,
+                   prefix=torch.zeros(batch, dtype=torch.int32, device="cuda"), out=out)
+    assert not torch.any((out == 7.0).all(-1)), "rows were left as they were"
+    for b in (0, 31, 63):
+        m = lens[b]
+        for at in (0, 2741, n - 40):  # 40 rows
+            i = torch.arange(m - n + at, m - n + at + 40, device="cuda")[:, None]
+            j = torch.arange(int(i[0]) - window, int(i[-1]) + 1, device="cuda")[None]
+            see = (i - j < window) & (j <= i)
+            rows = table[b, j[0] // page].long(), slice(None), j[0] % page
+            kk, vv = k[rows].double(), v[rows].double()
+            for h in range(kv):
+                qh = q[b * n + at: b * n + at + 40, h].double()
+                delta = d * 2.0 ** -24 * (qh.abs() @ kk[:, h].abs().T / 8).amax(-1, keepdim=True)
+                x = (qh @ kk[:, h].T / 8).masked_fill(~see, -math.inf)
+                p = torch.softmax(x, -1)
+                total = torch.exp(x - x.amax(-1, keepdim=True)).sum(-1, keepdim=True)
+                want, a = p @ vv[:, h], p @ vv[:, h].abs()
+                tol = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2 * delta + 2.0 ** -20) * a + \
+                    2.0 ** -25 * (1 + (see.double() @ vv[:, h].abs()) / total)
+                assert torch.all((out[b * n + at: b * n + at + 40, h].double() - want).abs() <= tol), (b, at, h)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 def test_rows_without_keys(hip, kind):
     """More tokens than keys (positions below zero), and scores that are all -inf: zeros."""

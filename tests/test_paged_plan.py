@@ -62,6 +62,17 @@ def test_lines_past_32_bits(plan, lens, kv_heads):
     plan([1] * len(lens), lens, window=48, prefix=[0] * len(lens), **kw)
 
 
+@pytest.mark.parametrize("batch,chunk,kv_heads", [(33, 1800, 64), (129, 2600, 32), (3000, 30, 32), (64, 900, 8)])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_many_tiles_of_long_caches(plan, batch, chunk, kv_heads, prefix):
+    """So much work that a share of it has more steps than any tile: none is cut, and none is lost."""
+    r = random.Random(batch)
+    lens = [r.randint(1 << 28, (1 << 30) - 70000) for _ in range(batch)]
+    out = plan([chunk - b % 7 for b in range(batch)], lens, heads=6 * kv_heads, kv_heads=kv_heads, page=4096,
+               window=300 if prefix else 0, prefix=[0] * batch if prefix else None)
+    assert "ok many" in out
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_ragged_batches(plan, seed):
     r = random.Random(seed)
