@@ -30,6 +30,10 @@
  *                           <- spectra/engine.py:614-700 the 4-bit KV cache
  *   spectra_paged_rope_append, spectra_paged_attend
  *                           <- no counterpart: the caches above for a batch of sequences
+ *   spectra_paged_rope_axes_append, spectra_paged_key_bounds, spectra_paged_select,
+ *   spectra_paged_attend_blocks, spectra_adjust_logits, spectra_next_tokens
+ *                           <- no counterpart: positions of several axes, attention over selected pages
+ *                              and constrained choices for such a batch
  */
 #ifndef SPECTRA_HIP_H_
 #define SPECTRA_HIP_H_
@@ -437,6 +441,105 @@ size_t spectra_paged_attend_workspace(int32_t head_dim);
 int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q, int64_t ldq, int64_t tokens, int32_t heads,
                          float scale, float cap, int32_t window, const float* slopes, const int32_t* prefix,
                          void* workspace, size_t workspace_bytes, void* out, spectra_stream_t stream);
+
+/* spectra_paged_rope_append with rotary positions of several axes (images and video: time, height
+ * and width): pair i of a head (dims i and i + head_dim / 2) of token t turns by row
+ * positions[axis[i] * ldpos + t] of the tables.  positions int32, axes (1 to 4) rows of `tokens`; axis
+ * uint8 [head_dim / 2], 8-byte aligned; a pair whose axis is `axes` or more does not turn.  cos_t and sin_t are required.  The rows that
+ * the cache gets stay those of the sequences' positions.  A token with a position of any axis
+ * outside [0, rope_rows) appends nothing and gets NaN queries. */
+int spectra_paged_rope_axes_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
+                                   const int32_t* positions, int64_t ldpos, int32_t axes, const uint8_t* axis,
+                                   const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads, void* q_rot,
+                                   spectra_stream_t stream);
+
+/* Bounds of the keys of each page (sparse attention selects by them): codes int8 [pages, kv_heads,
+ * 2, head_dim], first the greatest, then the least value of each dim over the page's rows, scales
+ * fp32 [pages, kv_heads]; code_stride and scale_stride: elements from page to page.  With A the largest
+ * magnitude of a page's keys and inv = 127 / A (fp32, each operation rounded): codes ceil(max inv) and
+ * floor(min inv) within +-127, scale A / 127; A < 2^-100: codes and scale 0; a key that is not
+ * finite: codes 0, scale +inf. */
+typedef struct spectra_paged_bounds {
+  int8_t* codes; int64_t code_stride;
+  float* scales; int64_t scale_stride;
+} spectra_paged_bounds_t;
+
+/* Works out anew the bounds of every page that a token of the call lies in, over the rows of
+ * positions below kv_lens: to be called after each append, by the same lengths and starts.  Other
+ * pages' bounds, and those of ids outside the pool, are left alone.  The descriptor's values (v..)
+ * are not read. */
+int spectra_paged_key_bounds(const spectra_paged_kv_t* kv, int64_t tokens, const spectra_paged_bounds_t* bounds,
+                             spectra_stream_t stream);
+/* out [pages, kv_heads, 2, head_dim] (F16 / BF16 / F32, 16-byte aligned): code times scale, +-inf where
+ * the scale is. */
+int spectra_paged_bounds_values(const spectra_paged_bounds_t* bounds, int64_t num_pages, int32_t kv_heads, int32_t head_dim,
+                                void* out, int32_t out_dtype, spectra_stream_t stream);
+
+/* Selection of pages: blocks int32 [tokens, kv_heads, count], contiguous: for the token at position i of
+ * its sequence the `count` of the visible blocks j <= i / page_size to attend to, ascending, then -1.  The
+ * first `sink` and the last `local` (>= 1, sink + local <= count) visible blocks are among them, the
+ * others have the largest scores, the lowest block on ties:
+ *   c_h = rint(q_h 127 / A), A = the largest magnitude of the KV head's query heads
+ *   score_j = scale_j max_h sum_d (max(c_hd, 0) codes[j, 0, d] + min(c_hd, 0) codes[j, 1, d])
+ * whole numbers, exact, and one product in fp32.  (A not finite or below 2^-100: c = 0.)  Blocks
+ * with a scale of +inf or of a page outside the pool come before all scores.  q [tokens, heads,
+ * head_dim], act_dtype F16 or BF16, token stride ldq (a multiple of 8), 16-byte aligned.  Of kv
+ * only the sizes, the table, the lengths and the starts are read (kv_lens count the call's tokens,
+ * whose bounds are there: spectra_paged_key_bounds).  Rows behind the last sequence are left alone.  Tables of
+ * up to 32768 pages (SPECTRA_ERR_UNSUPPORTED otherwise).  workspace: NULL, or
+ * spectra_paged_select_workspace() bytes, 16-byte aligned, by which few tokens with long tables are shared
+ * among workgroups.  ZERO it before its first use; every complete call leaves its counters at zero; calls
+ * sharing one must not overlap. */
+size_t spectra_paged_select_workspace(void);
+int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_paged_bounds_t* bounds, const void* q, int64_t ldq,
+                         int32_t act_dtype, int64_t tokens, int32_t heads, int32_t count, int32_t sink, int32_t local,
+                         void* workspace, size_t workspace_bytes, int32_t* blocks, spectra_stream_t stream);
+
+/* spectra_paged_attend over listed blocks: the token at position i sees, in KV head n, the keys j <= i
+ * of the blocks (of the sequence) in blocks[token, n, :] (int32 [tokens, kv_heads, count],
+ * contiguous); negative entries, and ones past the table, name nothing, one named twice counts twice.  Scores, cap, roundings and the
+ * workspace are spectra_paged_attend's.  A row that sees no key is zero; one that sees a key of a page
+ * outside the pool, or whose position lies past the table, is NaN. */
+int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const void* q, int64_t ldq, int64_t tokens, int32_t heads,
+                                const int32_t* blocks, int32_t count, float scale, float cap, void* workspace,
+                                size_t workspace_bytes, void* out, spectra_stream_t stream);
+
+/* A batch's logits [rows, vocab] (dtype, row stride ld) and what is to be done to them; every pointer but
+ * logits may be NULL.  Strides in elements; rows of 2-D operands contiguous. */
+typedef struct spectra_logits {
+  const void* logits; int64_t ld;
+  int32_t dtype;                 /* F16, BF16 or F32 */
+  int32_t rows;                  /* 1 .. 65535 */
+  int64_t vocab;
+  const int64_t* history; int64_t history_ld, history_width; /* tokens so far, prompt first */
+  const int32_t* history_lens;   /* [rows]: how many of a row count; NULL: all */
+  const int32_t* prompt_lens;    /* [rows]: how many of those are the prompt's; NULL: none */
+  const float *repetition, *presence, *frequency; /* [rows] */
+  const int64_t* bias_ids; int64_t bias_ids_ld;   /* [rows, biases]; an id outside [0, vocab) names nothing */
+  const float* bias; int64_t bias_ld;             /* [rows, biases] */
+  int32_t biases;
+  int32_t states;
+  const int32_t* allowed; int64_t allowed_ld;     /* [states, (vocab + 31) / 32]: bit v % 32 of word v / 32 */
+  const int32_t* state;          /* [rows]: the row's mask; outside [0, states): none; NULL: its own */
+} spectra_logits_t;
+
+/* out [rows, vocab] of the logits' type, row stride ldo (out may be the logits themselves), rounded
+ * once from fp32 (each operation rounded):
+ *   x = logit;  seen in the history:  x > 0 ? x / repetition : x * repetition
+ *   c times in it after the prompt:   x -= frequency c;  c > 0:  x -= presence
+ *   biased:                           x += bias (of an id given twice, the last)
+ *   not allowed:                      -inf
+ * A history without penalties is not read; ids outside [0, vocab) count nothing. */
+int spectra_adjust_logits(const spectra_logits_t* l, void* out, int64_t ldo, spectra_stream_t stream);
+
+/* tokens[row] = the largest x of the above (in fp32, nothing stored): the lowest token on ties, NaN
+ * counts as largest; -1 when every x is -inf.  At most SPECTRA_NEXT_TOKENS_ROWS rows.  workspace:
+ * spectra_next_tokens_workspace() bytes, 16-byte aligned.  ZERO it before its first use; every complete call
+ * leaves it at zero; calls sharing one must not overlap. */
+#define SPECTRA_NEXT_TOKENS_ROWS 4096
+size_t spectra_next_tokens_workspace(void);
+int spectra_next_tokens(const spectra_logits_t* l, int64_t* tokens, void* workspace, size_t workspace_bytes,
+                        spectra_stream_t stream);
 
 /* Measurement only (no counterpart in the reference): the fixed cost of one launch and
  * the time of a plain HBM stream, the floor and ceiling a one-launch GEMV is held against.

@@ -19,8 +19,8 @@ INCLUDE = os.path.join(ROOT, "include")
 OBJDIR = os.path.join(PKG, "_obj")
 LIB = os.path.join(PKG, "libspectra_hip.so")
 TORCH_OPS_LIB = os.path.join(PKG, "_spectra_torch.so")
-TORCH_OPS_SOURCES = ["torch_ops.cpp", "torch_paged.cpp"]
-SOURCES = ["api.hip", "quant.hip", "dequant.hip", "gemv.hip", "gemv_f16.hip", "gemv_bf16.hip", "gemv_stream_f16.hip", "gemv_stream_bf16.hip", "gemv_rows_plain.hip", "gemv_rows_pro.hip", "gemv_rows_lm.hip", "gemv_rows_multi_f16.hip", "gemv_rows_multi_bf16.hip", "gemm.hip", "mid.hip", "prefill.hip", "skinny.hip", "outliers.hip", "decode.hip", "attend_prefill.hip", "paged_append.hip", "paged_few.hip", "paged_many.hip", "measure.hip"]
+TORCH_OPS_SOURCES = ["torch_ops.cpp", "torch_paged.cpp", "torch_batch.cpp"]
+SOURCES = ["api.hip", "quant.hip", "dequant.hip", "gemv.hip", "gemv_f16.hip", "gemv_bf16.hip", "gemv_stream_f16.hip", "gemv_stream_bf16.hip", "gemv_rows_plain.hip", "gemv_rows_pro.hip", "gemv_rows_lm.hip", "gemv_rows_multi_f16.hip", "gemv_rows_multi_bf16.hip", "gemm.hip", "mid.hip", "prefill.hip", "skinny.hip", "outliers.hip", "decode.hip", "attend_prefill.hip", "paged_append.hip", "paged_few.hip", "paged_many.hip", "paged_bounds.hip", "paged_select.hip", "paged_blocks.hip", "logits.hip", "measure.hip"]
 ARCH = "gfx950"
 
 COMMON_FLAGS = [
@@ -51,7 +51,7 @@ def _compile(src: str) -> str:
 
 
 def build_torch_ops(verbose: bool = True) -> str:
-    """The operator registrations (csrc/torch_ops.cpp, csrc/torch_paged.cpp): host C++ only, compiled with the host
+    """The operator registrations (csrc/torch_ops.cpp, torch_paged.cpp, torch_batch.cpp): host C++ only, compiled with the host
     compiler against the installed torch's headers and linked to libspectra_hip.so, which it
     finds next to itself (rpath $ORIGIN)."""
     import torch

@@ -65,6 +65,25 @@ class PagedKv(ctypes.Structure):
                 ("kv_lens", c_void_p), ("q_start", c_void_p)]
 
 
+class PagedBounds(ctypes.Structure):
+    """Mirror of ``spectra_paged_bounds_t``."""
+    _fields_ = [("codes", c_void_p), ("code_stride", c_int64), ("scales", c_void_p), ("scale_stride", c_int64)]
+
+
+NEXT_TOKENS_ROWS = 4096  # SPECTRA_NEXT_TOKENS_ROWS
+
+
+class Logits(ctypes.Structure):
+    """Mirror of ``spectra_logits_t``."""
+    _fields_ = [("logits", c_void_p), ("ld", c_int64), ("dtype", c_int32), ("rows", c_int32), ("vocab", c_int64),
+                ("history", c_void_p), ("history_ld", c_int64), ("history_width", c_int64),
+                ("history_lens", c_void_p), ("prompt_lens", c_void_p),
+                ("repetition", c_void_p), ("presence", c_void_p), ("frequency", c_void_p),
+                ("bias_ids", c_void_p), ("bias_ids_ld", c_int64), ("bias", c_void_p), ("bias_ld", c_int64),
+                ("biases", c_int32), ("states", c_int32), ("allowed", c_void_p), ("allowed_ld", c_int64),
+                ("state", c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/spectra_hip.h declares
 SIGNATURES = {
     "spectra_version": (c_char_p, []),
@@ -119,6 +138,22 @@ SIGNATURES = {
     "spectra_paged_attend": (c_int32, [ctypes.POINTER(PagedKv), c_void_p, c_int64, c_int64, c_int32, ctypes.c_float,
                                        ctypes.c_float, c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
                                        c_void_p]),
+    "spectra_paged_rope_axes_append": (c_int32, [ctypes.POINTER(PagedKv), c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                                 c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p,
+                                                 c_void_p]),
+    "spectra_paged_key_bounds": (c_int32, [ctypes.POINTER(PagedKv), c_int64, ctypes.POINTER(PagedBounds), c_void_p]),
+    "spectra_paged_bounds_values": (c_int32, [ctypes.POINTER(PagedBounds), c_int64, c_int32, c_int32, c_void_p, c_int32,
+                                              c_void_p]),
+    "spectra_paged_select_workspace": (c_size_t, []),
+    "spectra_paged_select": (c_int32, [ctypes.POINTER(PagedKv), ctypes.POINTER(PagedBounds), c_void_p, c_int64, c_int32,
+                                       c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_size_t, c_void_p,
+                                       c_void_p]),
+    "spectra_paged_attend_blocks": (c_int32, [ctypes.POINTER(PagedKv), c_void_p, c_int64, c_int64, c_int32, c_void_p,
+                                              c_int32, ctypes.c_float, ctypes.c_float, c_void_p, c_size_t, c_void_p,
+                                              c_void_p]),
+    "spectra_adjust_logits": (c_int32, [ctypes.POINTER(Logits), c_void_p, c_int64, c_void_p]),
+    "spectra_next_tokens_workspace": (c_size_t, []),
+    "spectra_next_tokens": (c_int32, [ctypes.POINTER(Logits), c_void_p, c_void_p, c_size_t, c_void_p]),
     "spectra_measure_empty": (c_int32, [c_int32, c_int32, c_void_p]),
     "spectra_measure_read": (c_int32, [c_void_p, c_size_t, c_int32, c_int32, c_void_p, c_void_p]),
 }

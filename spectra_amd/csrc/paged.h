@@ -74,6 +74,10 @@ struct PagedPools {
   PagedRegion k, v, ks, vs, kz, vz;
 };
 PagedPools paged_pools(const spectra_paged_kv_t* kv);
+// The bounds of a pool's keys: checks of the descriptor, and its regions.
+int paged_bounds_args(const spectra_paged_bounds_t* b, int64_t num_pages, int32_t kv_heads, int32_t hd);
+PagedRegion paged_bound_codes(const spectra_paged_bounds_t* b, int64_t num_pages, int32_t kv_heads, int32_t hd);
+PagedRegion paged_bound_scales(const spectra_paged_bounds_t* b, int64_t num_pages, int32_t kv_heads);
 // The block table, the lengths and the starts.
 inline PagedRegion paged_table(const spectra_paged_kv_t* kv) {
   return {"block_table", kv->block_table, 4LL * kv->table_width, 4 * kv->table_stride, kv->batch};

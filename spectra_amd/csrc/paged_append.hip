@@ -6,6 +6,10 @@
 // end); a 4-bit pool takes the rows through the 4-bit quantizer, scale and zero point beside the
 // codes.
 //
+// With axes (AXES) the pairs of a head turn by positions of their own: pair i by row positions[axis[i]][t] of the tables
+// (images and video: time, height and width), while the cache's row stays the sequence's position.  A lane's 8 pairs
+// mostly have one axis and so one run of the table; where they do not, the angles are gathered.
+//
 // A pass over the rows: 8 rotation pairs (two 16-byte loads and stores) or 8 values of v a lane.
 // The waves of a token are its own, so its sequence, position and page are found once a wave, by
 // scalar loads behind a search of the starts that the row's loads overlap.  Bound by that chain
@@ -21,6 +25,7 @@
 namespace spectra {
 
 constexpr int kPaThreads = 256;
+constexpr int kPagedAxes = 4;  // most axes
 
 template <bool BF>
 __device__ __forceinline__ void unpack8t(const uint4& u, float (&f)[8]) {
@@ -32,12 +37,20 @@ __device__ __forceinline__ void unpack8t(const uint4& u, float (&f)[8]) {
   }
 }
 
-template <bool BF, bool Q4>
+// Positions of the rotation by axis, and the axis of every pair (AXES only).
+struct PagedAxes {
+  const int* pos;  // [axes][tokens], rows `stride` apart
+  int64_t stride;
+  const uint8_t* axis;  // [head_dim / 2]; a pair of an axis past the last stays as it is
+  int axes;
+};
+
+template <bool BF, bool Q4, bool AXES>
 __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t* __restrict__ qkv, int64_t ldqkv,
                                                                   const float* __restrict__ cos_t,
                                                                   const float* __restrict__ sin_t, int64_t rope_rows,
                                                                   int heads, int hd, int waves, const PagedKv kv,
-                                                                  uint16_t* __restrict__ q_rot) {
+                                                                  uint16_t* __restrict__ q_rot, const PagedAxes ax) {
   // neighbouring blocks go to different XCDs: an eighth of the tokens each, so that rows beside each
   // other meet in one L2 (4-bit rows are less than a line)
   const uint32_t run = gridDim.x < 64 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
@@ -61,7 +74,16 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
   if (seq >= kv.batch) return;  // behind the last sequence: left alone
   const PagedSeq sq = paged_seq(sload(kv.q_start + seq), sload(kv.q_start + seq + 1), sload(kv.lens + seq), kv.tokens);
   const int pos = sq.len - sq.n + (t - sq.q0);
-  const bool turn = cos_t == nullptr || (pos >= 0 && pos < rope_rows);
+  int at[kPagedAxes];  // the token's rows of the tables
+  bool turn = cos_t == nullptr || (pos >= 0 && pos < rope_rows);
+  if constexpr (AXES) {
+    turn = true;
+#pragma unroll
+    for (int a = 0; a < kPagedAxes; ++a) {
+      at[a] = a < ax.axes ? sload(ax.pos + a * ax.stride + t) : 0;
+      turn = turn && at[a] >= 0 && at[a] < rope_rows;
+    }
+  }
   int page = -1;
   if (turn && pos >= 0 && (pos >> kv.page_shift) < kv.table_width)
     page = sload(kv.table + seq * kv.table_stride + (pos >> kv.page_shift));
@@ -71,16 +93,45 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
     uint4 lo = a, hi = b;
     if (cos_t != nullptr && turn) {
       float c[8], s[8], x[8], y[8];
-      *(float4*)c = *(const float4*)(cos_t + (int64_t)pos * h2 + i);
-      *(float4*)(c + 4) = *(const float4*)(cos_t + (int64_t)pos * h2 + i + 4);
-      *(float4*)s = *(const float4*)(sin_t + (int64_t)pos * h2 + i);
-      *(float4*)(s + 4) = *(const float4*)(sin_t + (int64_t)pos * h2 + i + 4);
+      int64_t from = pos;
+      bool run = true;     // the pairs' angles are one run of the table
+      uint32_t still = 0;  // pairs that do not turn (not by an angle of 0: its product with an infinite partner is NaN)
+      if constexpr (AXES) {
+        const uint2 ids = *(const uint2*)(ax.axis + i);
+        const uint32_t first = ids.x & 255u;
+        run = ids.x == first * 0x01010101u && ids.y == ids.x && first < (uint32_t)ax.axes;
+        from = at[0];
+#pragma unroll
+        for (int a = 1; a < kPagedAxes; ++a) from = first == (uint32_t)a ? at[a] : from;
+        if (!run) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t id = ((e < 4 ? ids.x : ids.y) >> (8 * (e & 3))) & 255u;
+            int64_t row = at[0];
+#pragma unroll
+            for (int a = 1; a < kPagedAxes; ++a) row = id == (uint32_t)a ? at[a] : row;
+            c[e] = cos_t[row * h2 + i + e];
+            s[e] = sin_t[row * h2 + i + e];
+            still |= (id < (uint32_t)ax.axes ? 0u : 1u) << e;
+          }
+        }
+      }
+      if (run) {
+        *(float4*)c = *(const float4*)(cos_t + from * h2 + i);
+        *(float4*)(c + 4) = *(const float4*)(cos_t + from * h2 + i + 4);
+        *(float4*)s = *(const float4*)(sin_t + from * h2 + i);
+        *(float4*)(s + 4) = *(const float4*)(sin_t + from * h2 + i + 4);
+      }
       unpack8t<BF>(a, x);
       unpack8t<BF>(b, y);
       uint32_t lw[4] = {0, 0, 0, 0}, hw[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float u = x[e] * c[e] - y[e] * s[e], w = y[e] * c[e] + x[e] * s[e];
+        float u = x[e] * c[e] - y[e] * s[e], w = y[e] * c[e] + x[e] * s[e];
+        if (AXES && (still >> e & 1)) {
+          u = x[e];
+          w = y[e];
+        }
         lw[e >> 1] |= (uint32_t)(BF ? f2bf(u) : f2h(u)) << (16 * (e & 1));
         hw[e >> 1] |= (uint32_t)(BF ? f2bf(w) : f2h(w)) << (16 * (e & 1));
       }
@@ -231,9 +282,10 @@ int paged_apart(std::initializer_list<PagedRegion> written, std::initializer_lis
 
 using namespace spectra;
 
-extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
-                                         const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads,
-                                         void* q_rot, spectra_stream_t stream) {
+namespace {
+// Both entries: positions of the sequences, or of axes of their own.
+int append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens, const PagedAxes* axes,
+           const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads, void* q_rot, spectra_stream_t stream) {
   PagedKv p;
   if (int st = paged_args(kv, tokens, heads, &p); st != SPECTRA_OK) return st;
   SPECTRA_REQUIRE(qkv && q_rot, "NULL pointer");
@@ -245,12 +297,23 @@ extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const voi
                     reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 16) == 0 &&
                       ldqkv % 8 == 0,
                   "operands and qkv rows must be 16-byte aligned");
+  PagedAxes ax{};
+  if (axes != nullptr) {
+    ax = *axes;
+    SPECTRA_REQUIRE(ax.pos && ax.axis && cos_t, "NULL pointer");
+    SPECTRA_REQUIRE(ax.axes >= 1 && ax.axes <= kPagedAxes, "one to four axes");
+    SPECTRA_REQUIRE(ax.stride >= tokens || ax.axes == 1, "positions' row stride too small");
+    SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(ax.pos) % 4 == 0 && reinterpret_cast<uintptr_t>(ax.axis) % 8 == 0,
+                    "positions must be aligned, the pairs' axes to 8 bytes");
+  }
   const PagedPools pools = paged_pools(kv);
   const int64_t turned = 2 * std::min<int64_t>(rope_rows, 1LL << 31) * hd;  // bytes of each table that positions name
   if (int st = paged_apart({{"q_rot", q_rot, tokens * heads * hd * 2, 0, 1}, pools.k, pools.v, pools.ks, pools.vs, pools.kz, pools.vz},
                            {{"qkv", qkv, (int64_t)(heads + 2 * kv->kv_heads) * hd * 2, ldqkv * 2, tokens},
                             {"cos", cos_t, turned, 0, 1},
                             {"sin", sin_t, turned, 0, 1},
+                            {"positions", ax.pos, 4 * tokens, 4 * ax.stride, ax.axes},
+                            {"axis", ax.axis, hd / 2, 0, 1},
                             paged_table(kv),
                             paged_lens(kv),
                             paged_starts(kv)});
@@ -260,13 +323,32 @@ extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const voi
   int64_t blocks = (tokens * waves + kPaThreads / 64 - 1) / (kPaThreads / 64);
   if (blocks >= 64) blocks = (blocks + 7) / 8 * 8;
   SPECTRA_REQUIRE(tokens * waves < (1LL << 31) - 256, "tokens out of range");
-  const void* kern = kv->kind == SPECTRA_KV_4BIT ? (const void*)paged_append_kernel<false, true>
-                     : kv->kind == SPECTRA_KV_BF16 ? (const void*)paged_append_kernel<true, false>
-                                                   : (const void*)paged_append_kernel<false, false>;
+  const bool q4 = kv->kind == SPECTRA_KV_4BIT, bf = kv->kind == SPECTRA_KV_BF16;
+  const void* kern = axes == nullptr ? (q4   ? (const void*)paged_append_kernel<false, true, false>
+                                        : bf ? (const void*)paged_append_kernel<true, false, false>
+                                             : (const void*)paged_append_kernel<false, false, false>)
+                     : q4 ? (const void*)paged_append_kernel<false, true, true>
+                     : bf ? (const void*)paged_append_kernel<true, false, true>
+                          : (const void*)paged_append_kernel<false, false, true>;
   int hdv = hd;
   void* args[] = {(void*)&qkv, (void*)&ldqkv, (void*)&cos_t, (void*)&sin_t, (void*)&rope_rows, (void*)&heads,
-                  (void*)&hdv, (void*)&waves, (void*)&p, (void*)&q_rot};
+                  (void*)&hdv, (void*)&waves, (void*)&p, (void*)&q_rot, (void*)&ax};
   SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)blocks), dim3(kPaThreads), args, 0, (hipStream_t)stream));
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
+}
+}  // namespace
+
+extern "C" int spectra_paged_rope_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
+                                         const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads,
+                                         void* q_rot, spectra_stream_t stream) {
+  return append(kv, qkv, ldqkv, tokens, nullptr, cos_t, sin_t, rope_rows, heads, q_rot, stream);
+}
+
+extern "C" int spectra_paged_rope_axes_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
+                                              const int32_t* positions, int64_t ldpos, int32_t axes, const uint8_t* axis,
+                                              const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads,
+                                              void* q_rot, spectra_stream_t stream) {
+  const PagedAxes ax = {positions, ldpos, axis, axes};
+  return append(kv, qkv, ldqkv, tokens, &ax, cos_t, sin_t, rope_rows, heads, q_rot, stream);
 }

@@ -1,0 +1,471 @@
+// Attention over listed pages of a paged KV cache: each token and KV head has pages of its own (as paged_select.hip chooses
+// them), of which it sees the keys up to its position.
+//
+//   out = sum_j p_j v_j / sum_j p_j,   p_j = 2^(score_j - m),   scores in log2 units (PagedScore),
+// one pass over the listed keys with the running maximum m, the sums rescaled where it rises (paged_few.hip, whose
+// operand layouts these are: scores transposed, S^T = K Q^T, so that the weights are the next product's operand where
+// they lie; V turned by byte permutes; 4-bit pages through LDS).  All rows of a tile, up to 16 query heads of one token
+// and KV head, see the same keys, so none has to be computed by itself.
+//
+// Tiles have `count` pages at most, the same for all, so the line of their key steps (128 keys) is shared out by
+// arithmetic: as many workgroups as are resident at once take equal runs of it, whole tiles and at most two parts; the
+// parts of a tile meet in the workspace, where the last to arrive joins them in the order of their keys.
+//
+// Bound by reading the listed pages.  Roundings: the weights to the activations' 16 bits for the product with V, 4-bit
+// values to fp16, the output.
+#include "paged_attend.h"
+
+namespace spectra {
+
+constexpr int kBlkThreads = 256, kBlkKeys = 128;
+
+// 32 keys of 16-bit K and V as they lie.
+template <int HD>
+struct BlkTile {
+  pu4_t k[2][HD / 32];
+  uint32_t v[2][4][HD / 32];
+};
+// 32 keys of 4-bit K and V in LDS, a wave's own: codes, scales and zero points of both.
+template <int HD>
+struct BlkCodes {
+  static constexpr int kCodes = 16 * HD, kScales = 2 * HD, kZeros = HD;  // bytes of 32 keys
+  static constexpr int kV = kCodes, kS = 2 * kCodes, kZ = kS + 2 * kScales, kBytes = kZ + 2 * kZeros;
+  static constexpr int kCopies = HD == 128 ? 7 : 4;  // instructions that bring them
+};
+template <int HD, int KIND>
+constexpr int blk_lds() {
+  const int red = 4 * 16 * (HD + 4) * 4, ring = KIND == kKv4 ? 4 * 2 * BlkCodes<HD>::kBytes : 0;
+  return red > ring ? red : ring;
+}
+// Sixteen keys of one page: the position of the first, and how many of them the row sees; where they lie (page 0 for a
+// page that is not there, or for nothing).
+struct BlkHalf {
+  int page, seen;
+  bool bad;
+};
+
+template <int HD, int KIND, int MOD>
+__global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
+    paged_blocks_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
+                        const int* __restrict__ blocks, int count, int tiles_a_token, int64_t steps_a_tile, PagedLine line0,
+                        uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
+  constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
+  constexpr int ROWS = 16, KS = HD / 32, DPL = HD / 16, RS = HD + 4;
+  constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;  // bytes of a row of a page
+  __shared__ __align__(16) uint8_t pool[blk_lds<HD, KIND>()];  // 4-bit keys on their way; at the end the waves' sums
+  float* red = (float*)pool;
+  __shared__ float wm[4][ROWS], wl[4][ROWS];
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), c = lane & 15, q4 = lane >> 4;
+  const int S = (int)steps_a_tile;
+  PagedLine line = line0;
+  line.begin = line.start(blockIdx.x);
+  line.end = line.start(blockIdx.x + 1);
+  const int pmask = (1 << kv.page_shift) - 1;
+  for (int x = line.begin; x < line.end;) {
+    const int tile = (int)((uint32_t)x / (uint32_t)S), from = x - tile * S, t0 = x - from;
+    const int to = min(S, from + line.end - x);
+    const bool whole = from == 0 && to == S;
+    const int tok = sread(tile / tiles_a_token), ht = tile - tok * tiles_a_token;  // (heads of a token beside each other)
+    const int groups = (g + 15) / 16, kvh = sread(ht / groups), h0 = sread(kvh * g + 16 * (ht - kvh * groups));
+    const int nrows = min(16, (kvh + 1) * g - h0);
+    x += to - from;
+    const int seq = paged_find(kv.q_start, kv.batch, tok, lane);
+    if (seq >= kv.batch) continue;  // behind the last sequence: left alone
+    const PagedSeq sq = paged_seq(sload(kv.q_start + seq), sload(kv.q_start + seq + 1), sload(kv.lens + seq), kv.tokens);
+    const int pos = sq.len - sq.n + (tok - sq.q0);  // the row's position: it sees the keys up to that
+    const bool past = pos >= kv.table_width << kv.page_shift;
+
+    // the lane's row (column c): its queries, B operands
+    const float slope2 = 0.0f;
+    pu4_t qf[KS];
+    {
+      const uint16_t* qr = q + (int64_t)tok * ldq + (int64_t)(h0 + min(c, nrows - 1)) * HD;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        pu4_t y = *(const pu4_t*)(qr + (Q4 ? (HD / 4) * q4 + 8 * s : 32 * s + 8 * q4));
+        if (Q4)  // pairs in the order of the expanded codes: dims n, n + 4
+          y = (pu4_t){__builtin_amdgcn_perm(y[2], y[0], 0x05040100u), __builtin_amdgcn_perm(y[2], y[0], 0x07060302u),
+                      __builtin_amdgcn_perm(y[3], y[1], 0x05040100u), __builtin_amdgcn_perm(y[3], y[1], 0x07060302u)};
+        qf[s] = y;
+      }
+    }
+
+    // ---- loads: the list's entries two tiles ahead of their rows, page ids one, rows a tile ahead of their use
+    const int* list = blocks + ((int64_t)tok * kv.kv_heads + kvh) * count;
+    const int* tab = kv.table + seq * kv.table_stride;
+    const int last = count - 1;
+    auto listed = [&](int key) __attribute__((always_inline)) { return sread(sload(list + min(key >> kv.page_shift, last))); };
+    // the 16 keys from `key` of the list on, in block b of the sequence
+    auto half_of = [&](int key, int b) __attribute__((always_inline)) {
+      BlkHalf h;
+      const bool there = (key >> kv.page_shift) <= last && (uint32_t)b < (uint32_t)kv.table_width;
+      const int id = sread(sload(tab + (there ? b : 0)));
+      h.seen = there ? min(max(pos + 1 - ((b << kv.page_shift) + (key & pmask)), 0), 16) : 0;
+      h.bad = (uint32_t)id >= (uint32_t)kv.num_pages;
+      h.page = h.bad || !there ? 0 : id;
+      return h;
+    };
+    typedef BlkTile<HD> Tile;
+    const uint32_t koff = (uint32_t)(c * ROWB + 16 * q4), voff = (uint32_t)(4 * q4 * ROWB + c * (ROWB / 16));
+    auto load = [&](Tile& t, int key0, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = (kvh << kv.page_shift) + ((key0 + 16 * h) & pmask);
+        const uint64_t at = paged_at(hf[h].page, kv.page_step) + row * ROWB;
+        const uint8_t *kb = kv.k + at, *vb = kv.v + at;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) t.k[h][s] = __builtin_bit_cast(pu4_t, load_from<uint4>(kb, koff, 64 * s));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (HD == 128) {
+            const uint4 y = load_from<uint4>(vb, voff, i * ROWB);
+            t.v[h][i][0] = y.x;
+            t.v[h][i][1] = y.y;
+            t.v[h][i][2] = y.z;
+            t.v[h][i][3] = y.w;
+          } else {
+            const uint2 y = load_from<uint2>(vb, voff, i * ROWB);
+            t.v[h][i][0] = y.x;
+            t.v[h][i][1] = y.y;
+          }
+        }
+      }
+    };
+    // 4 bits: to LDS at `to`, whose last reads are complete
+    typedef BlkCodes<HD> C;
+    auto fetch = [&](uint32_t at, int key0, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const int row0 = (kvh << kv.page_shift) + (key0 & pmask), row1 = (kvh << kv.page_shift) + ((key0 + 16) & pmask);
+      const int p0 = hf[0].page, p1 = hf[1].page;
+      const uint64_t a0 = paged_at(p0, kv.page_step) + row0 * ROWB, a1 = paged_at(p1, kv.page_step) + row1 * ROWB;
+      const uint64_t s0 = paged_at(p0, kv.scale_step) + row0 * (HD / 16), s1 = paged_at(p1, kv.scale_step) + row1 * (HD / 16);
+      const uint64_t z0 = paged_at(p0, kv.zero_step) + row0 * (HD / 32), z1 = paged_at(p1, kv.zero_step) + row1 * (HD / 32);
+      if constexpr (HD == 128) {
+        const uint32_t off = 16 * lane;
+        copy_lds(kv.k + a0, off, at);
+        copy_lds(kv.k + a1, off, at + 1024);
+        copy_lds(kv.v + a0, off, at + C::kV);
+        copy_lds(kv.v + a1, off, at + C::kV + 1024);
+        const uint64_t s = (lane < 32 ? s0 : s1) + 4 * (lane & 31);
+        copy_lds4(kv.ks + s, at + C::kS);
+        copy_lds4(kv.vs + s, at + C::kS + C::kScales);
+        copy_lds4((lane < 32 ? kv.kz : kv.vz) + ((lane & 16) == 0 ? z0 : z1) + 4 * (lane & 15), at + C::kZ);
+      } else {
+        const uint64_t a = (lane < 32 ? a0 : a1) + 16 * (lane & 31);
+        copy_lds16(kv.k + a, at);
+        copy_lds16(kv.v + a, at + C::kV);
+        copy_lds4((lane < 32 ? kv.ks : kv.vs) + ((lane & 16) == 0 ? s0 : s1) + 4 * (lane & 15), at + C::kS);
+        if (lane < 32) copy_lds4((lane < 16 ? kv.kz : kv.vz) + ((lane & 8) == 0 ? z0 : z1) + 4 * (lane & 7), at + C::kZ);
+      }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    pf4_t o[DPL];
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) o[j] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    // t: the tile's registers, or its place in LDS
+    auto compute = [&](const auto& t, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
+      pf4_t s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (Q4) {
+          const int key = 16 * h + c, kg = HD == 128 ? q4 : q4 >> 1;  // group of the lane's dims
+          const uint32_t zb = t[C::kZ + key * (HD / 32) + kg], sb = *(const uint16_t*)(t + C::kS + 2 * (key * (HD / 32) + kg));
+          const Kv4Zero z = kv4_zero(zb | zb << 16);
+          const ph2_t sf = __builtin_bit_cast(ph2_t, sb | sb << 16);
+          uint32_t w[KS];
+          if constexpr (HD == 128) {
+            const pu4_t y = *(const pu4_t*)(t + key * ROWB + 16 * q4);
+#pragma unroll
+            for (int st = 0; st < KS; ++st) w[st] = y[st];
+          } else {
+            const uint2 y = *(const uint2*)(t + key * ROWB + 8 * q4);
+            w[0] = y.x;
+            w[1] = y.y;
+          }
+#pragma unroll
+          for (int st = 0; st < KS; ++st) s[h] = mfma16<BF>(kv4_pairs(w[st], z, sf), qf[st], s[h]);
+        } else {
+#pragma unroll
+          for (int st = 0; st < KS; ++st) s[h] = mfma16<BF>(t.k[h][st], qf[st], s[h]);
+        }
+      }
+      const bool part = hf[0].seen < 16 || hf[1].seen < 16;  // keys that the row does not see: their values must not reach the product
+      // scores of the keys 16 (e / 4) + 4 q4 + e % 4
+      float y[8], mn = m, mul = sc.mul;
+      if constexpr (MOD != kModNone) mul = paged_scores<MOD, 2, 4>(s, sc, slope2, 0.0f, [](int n) { return n; });
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3] * mul;
+      if (part || hf[0].bad || hf[1].bad) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (hf[e >> 2].bad) y[e] = NAN;
+          if (4 * q4 + (e & 3) >= hf[e >> 2].seen) y[e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mn = fmaxf(mn, y[e]);
+      mn = fmaxf(mn, lane_xor<16>(mn, lane));
+      mn = fmaxf(mn, lane_xor<32>(mn, lane));
+      if (__ballot(mn > m + kPagedSlack) != 0) {
+        const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+        l *= corr;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[j][i] *= corr;
+        m = mn;
+      }
+      const float mu = m == -INFINITY ? 0.0f : m - kPagedRaise<BF>;
+      pu4_t pf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(y[e] - mu);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // (the total is of the weights as rounded, so that a mean of values lies among them)
+        pf[e] = pack2<BF>(y[2 * e], y[2 * e + 1]);
+        l = add2<BF>(pf[e], l);
+      }
+      // O^T += V^T P^T, dims DPL (l % 16) + j at step j: the 8 keys' values of a dim, in pairs of keys
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (part) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int key = 4 * q4 + 2 * (p & 1), n = hf[p >> 1].seen;
+          keep[p] = (key < n ? 0xffffu : 0u) | (key + 1 < n ? 0xffff0000u : 0u);
+        }
+      }
+      if constexpr (Q4) {
+        constexpr int HALF = HD / 64;  // codes of 4 dims each
+        const int vg = c * DPL / 32;   // group of the lane's dims
+        Kv4Zero z2[4];
+        ph2_t s2[4];
+        uint32_t v0[4], v1[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int key = 16 * (p >> 1) + 4 * q4 + 2 * (p & 1);  // and the next
+          const uint8_t* zp = t + C::kZ + C::kZeros + key * (HD / 32) + vg;
+          z2[p] = kv4_zero((uint32_t)zp[0] | (uint32_t)zp[HD / 32] << 16);
+          const uint8_t* sp = t + C::kS + C::kScales + 2 * (key * (HD / 32) + vg);
+          s2[p] = __builtin_bit_cast(ph2_t, ((uint32_t)*(const uint16_t*)sp | (uint32_t)*(const uint16_t*)(sp + HD / 16) << 16) & keep[p]);
+          const uint8_t* vp = t + C::kV + key * ROWB + c * (ROWB / 16);
+          if constexpr (HD == 128) {
+            v0[p] = *(const uint32_t*)vp;
+            v1[p] = *(const uint32_t*)(vp + ROWB);
+          } else {
+            v0[p] = *(const uint16_t*)vp;
+            v1[p] = *(const uint16_t*)(vp + ROWB);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < HALF; ++u) {
+          pu4_t a[4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const pu4_t w = kv4_pairs(__builtin_amdgcn_perm(v1[p], v0[p], u ? 0x07060302u : 0x05040100u), z2[p], s2[p]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) a[n][p] = w[n];
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) o[4 * u + n] = mfma16<BF>(a[n], pf, o[4 * u + n]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) {
+          pu4_t a;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            a[p] = __builtin_amdgcn_perm(t.v[p >> 1][2 * (p & 1) + 1][j >> 1], t.v[p >> 1][2 * (p & 1)][j >> 1],
+                                         (j & 1) ? 0x07060302u : 0x05040100u);
+            if (part) a[p] &= keep[p];
+          }
+          o[j] = mfma16<BF>(a, pf, o[j]);
+        }
+      }
+    };
+
+    const int kend = min(to * kBlkKeys, count << kv.page_shift);  // (of the list's keys)
+    int key = from * kBlkKeys + 32 * wave;
+    if (key < kend) {
+      int l0 = listed(key), l1 = listed(key + 16);
+      BlkHalf h0_[2] = {half_of(key, l0), half_of(key + 16, l1)}, h1_[2];
+      l0 = listed(key + kBlkKeys);
+      l1 = listed(key + kBlkKeys + 16);
+      // the next tile's halves, and the list's entries after them
+      auto next = [&](BlkHalf (&hf)[2], int k) __attribute__((always_inline)) {
+        hf[0] = half_of(k, l0);
+        hf[1] = half_of(k + 16, l1);
+        l0 = listed(k + kBlkKeys);
+        l1 = listed(k + kBlkKeys + 16);
+      };
+      if constexpr (Q4) {
+        uint8_t* mine = pool + wave * 2 * C::kBytes;
+        const uint32_t at0 = (uint32_t)(uintptr_t)(lds_t)mine;
+        fetch(at0, key, h0_);
+        next(h1_, key + kBlkKeys);
+        for (int turn = 0;; turn ^= 1) {
+          if (key + kBlkKeys < kend) {
+            fetch(at0 + (turn ^ 1) * C::kBytes, key + kBlkKeys, h1_);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::kCopies) : "memory");  // all but the next tile's
+          } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          }
+          compute(mine + turn * C::kBytes, h0_);
+          key += kBlkKeys;
+          if (key >= kend) break;
+          h0_[0] = h1_[0];
+          h0_[1] = h1_[1];
+          next(h1_, key + kBlkKeys);
+        }
+      } else {
+        Tile ta, tb;
+        load(ta, key, h0_);
+        next(h1_, key + kBlkKeys);
+        while (true) {
+          if (key + kBlkKeys < kend) load(tb, key + kBlkKeys, h1_);
+          compute(ta, h0_);
+          next(h0_, key + 2 * kBlkKeys);
+          key += kBlkKeys;
+          if (key >= kend) break;
+          if (key + kBlkKeys < kend) load(ta, key + kBlkKeys, h0_);
+          compute(tb, h1_);
+          next(h1_, key + 2 * kBlkKeys);
+          key += kBlkKeys;
+          if (key >= kend) break;
+        }
+      }
+    }
+    if constexpr (Q4) __syncthreads();  // (the waves' sums go where the codes were)
+
+    // ---- the waves meet, in LDS
+    l += lane_xor<16>(l, lane);
+    l += lane_xor<32>(l, lane);
+    if (q4 == 0) {
+      wm[wave][c] = m;
+      wl[wave][c] = l;
+    }
+    float* part = slots + (int64_t)line.record((int)blockIdx.x, t0 + from) * paged_slot<HD>(ROWS);
+    auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
+      const float inv = past ? NAN : 1.0f / den;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = den == 0.0f && !past ? 0.0f : v[e] * inv;
+      const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
+      *(uint2*)(out + ((int64_t)tok * heads + h0 + row) * HD + d) = w;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < DPL; j += 4)
+        *(float4*)(red + (wave * 16 + c) * RS + DPL * (4 * q4 + i) + j) =
+            make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
+    __syncthreads();
+    for (int it = tid; it < nrows * (HD / 4); it += kBlkThreads) {
+      const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
+      float mm = -INFINITY, den = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, wm[w][row]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = paged_weight(wm[w][row], wl[w][row], mm);
+        const float4 y = *(const float4*)(red + (w * 16 + row) * RS + d);
+        den += f * wl[w][row];
+        v[0] += f * y.x;
+        v[1] += f * y.y;
+        v[2] += f * y.z;
+        v[3] += f * y.w;
+      }
+      if (whole) {
+        write(row, d, v, den);
+      } else {
+        store_dev2(part + row * HD + d, v[0], v[1]);
+        store_dev2(part + row * HD + d + 2, v[2], v[3]);
+        if (d == 0) store_dev2(part + ROWS * HD + 2 * row, mm, den);
+      }
+    }
+    if (!whole) {
+      const PagedCut cut(line, t0, S);
+      const int pieces = cut.pieces;
+      auto slot_of = [&](int p) __attribute__((always_inline)) { return cut.record(p); };
+      if (paged_arrive(counters + cut.first, pieces, &flag)) {  // the last to arrive joins them
+        for (int it = tid; it < nrows * (HD / 4); it += kBlkThreads) {
+          const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
+          float v[1][4];
+          const float den = pieces <= 4 ? paged_join_by<HD, ROWS, 4, 1>(slots, slot_of, pieces, row, row * HD + d, 2, 0, v)
+                                        : paged_join_by<HD, ROWS, 16, 1>(slots, slot_of, pieces, row, row * HD + d, 2, 0, v);
+          write(row, d, v[0], den);
+        }
+      }
+    }
+    __syncthreads();  // (LDS is free for the next part)
+  }
+}
+
+template <int HD, int KIND>
+static const void* blocks_of(int mod) {
+  return mod == kModNone ? (const void*)paged_blocks_kernel<HD, KIND, kModNone>
+         : mod == kMod   ? (const void*)paged_blocks_kernel<HD, KIND, kMod>
+                         : (const void*)paged_blocks_kernel<HD, KIND, kModLargeCap>;
+}
+template <int HD>
+static const void* blocks_of(int kind, int mod) {
+  return kind == kKv4 ? blocks_of<HD, kKv4>(mod) : kind == kKvBf16 ? blocks_of<HD, kKvBf16>(mod) : blocks_of<HD, kKvF16>(mod);
+}
+
+}  // namespace spectra
+
+using namespace spectra;
+
+extern "C" int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const void* q, int64_t ldq, int64_t tokens,
+                                           int32_t heads, const int32_t* blocks, int32_t count, float scale, float cap,
+                                           void* workspace, size_t workspace_bytes, void* out, spectra_stream_t stream) {
+  PagedKv p;
+  if (int st = paged_args(kv, tokens, heads, &p); st != SPECTRA_OK) return st;
+  const int hd = kv->head_dim, g = heads / kv->kv_heads;
+  SPECTRA_REQUIRE(q && out && blocks, "NULL pointer");
+  SPECTRA_REQUIRE(ldq >= (int64_t)heads * hd && ldq % 8 == 0, "q token stride too small or not a multiple of 8");
+  SPECTRA_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(blocks) % 4 == 0,
+                  "q and out must be 16-byte aligned, blocks aligned");
+  SPECTRA_REQUIRE(count >= 1 && (int64_t)count * kv->page_size < (1LL << 30), "count out of range");
+  SPECTRA_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive");
+  SPECTRA_REQUIRE(cap >= 0.0f && cap < INFINITY, "cap must be 0 (none) or positive");
+  if (workspace == nullptr || workspace_bytes < spectra_paged_attend_workspace(hd))
+    return fail(SPECTRA_ERR_WORKSPACE, "workspace missing or smaller than spectra_paged_attend_workspace bytes");
+  SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  const PagedPools pools = paged_pools(kv);
+  if (int st = paged_apart({{"out", out, tokens * heads * hd * 2, 0, 1},
+                            {"the workspace", workspace, (int64_t)spectra_paged_attend_workspace(hd), 0, 1}},
+                           {{"q", q, (int64_t)heads * hd * 2, ldq * 2, tokens},
+                            {"blocks", blocks, tokens * kv->kv_heads * count * 4, 0, 1},
+                            pools.k, pools.v, pools.ks, pools.vs, pools.kz, pools.vz,
+                            paged_table(kv), paged_lens(kv), paged_starts(kv)});
+      st != SPECTRA_OK)
+    return st;
+  constexpr double log2e = 1.4426950408889634;
+  PagedScore sc{};
+  sc.mul = (float)(cap > 0.0f ? 2.0 * log2e * scale / cap : log2e * scale);
+  sc.cap2 = (float)(cap * log2e);
+  SPECTRA_REQUIRE(sc.mul > 0.0f && sc.mul < 1e30f && sc.cap2 < 1e30f, "scale or cap out of range");
+  const int mod = sc.cap2 > kPagedCap ? kModLargeCap : cap > 0.0f ? kMod : kModNone;
+  // the line of the tiles' steps, and its equal shares
+  int tiles_a_token = kv->kv_heads * ((g + 15) / 16);
+  int64_t steps = ((int64_t)count * kv->page_size + kBlkKeys - 1) / kBlkKeys;
+  const int64_t total = tokens * tiles_a_token * steps;
+  SPECTRA_REQUIRE(total < (1LL << 30), "tokens times listed keys out of range");
+  const int64_t groups = std::min<int64_t>(total, few_groups(kv->kind, hd, 16));
+  PagedLine line{};
+  line.total = (int)total;
+  line.each = (int)(total / groups);
+  line.more = (int)(total % groups);
+  uint32_t* counters = (uint32_t*)workspace;
+  float* slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
+  int gv = g, hv = heads, cv = count;
+  const void* kern = hd == 64 ? blocks_of<64>(kv->kind, mod) : blocks_of<128>(kv->kind, mod);
+  void* args[] = {(void*)&p, (void*)&sc, (void*)&q, (void*)&ldq, (void*)&gv, (void*)&hv, (void*)&blocks, (void*)&cv,
+                  (void*)&tiles_a_token, (void*)&steps, (void*)&line, (void*)&counters, (void*)&slots, (void*)&out};
+  SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)groups), dim3(kBlkThreads), args, 0, (hipStream_t)stream));
+  SPECTRA_HIP_CHECK(hipGetLastError());
+  return SPECTRA_OK;
+}

@@ -1,0 +1,360 @@
+// Selection of pages for sparse attention: for each token and KV head the pages whose bounds allow the largest products.
+//
+// The token's g query heads of the KV head become whole numbers of one scale, A = max |q|, c = rint(q 127 / A) (both
+// operations fp32 as written), and page j scores
+//   s_j = scale_j max_h sum_d (max(c_hd, 0) M_jd + min(c_hd, 0) m_jd)
+// (M, m, scale: paged_bounds.hip): whole numbers below 2^23 summed exactly, one rounding by the product with the scale.
+// So a score is the same whatever order it is summed in, and the choice among near scores, too: the largest scores,
+// the lowest page on ties.  A scale of infinity, or a page that is not in the pool, is taken before all scores: the
+// attention then shows what is wrong.  The first `sink` and the last `local` pages of the visible are always taken.
+//
+// Scores are matrix products (16 x 16 x 64 of bytes): rows are query heads, padded to 4, 8 or 16 a token by copies of the
+// last one, so that a token's maximum lies in a lane's registers and at most two exchanges; columns are 16 pages, whose
+// 2 d bytes a lane reads as they lie.  Scores are kept in LDS as 32-bit keys in the scores' order; the `count`-th largest
+// is found by bisection of the keys between their least and largest (some 20 counts), ties by the order of the pages,
+// and the chosen are written in that order.
+// A workgroup has one token (drafts and prompts: as many as fill the rows, whose pages are read once) and one KV head.
+// Few such units with long tables are split: workgroups score a run of pages each, and the last of a unit to arrive
+// chooses from the keys of all in the workspace.
+#include <algorithm>
+
+#include "paged_attend.h"
+
+namespace spectra {
+
+typedef int pi4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kSelMost = 32768;            // pages of a table
+constexpr int kSelLds = 160 * 1024 - 256;  // codes and keys of a workgroup
+constexpr int kSelSplit = 64;              // units whose pages are split among workgroups: at most as many
+constexpr size_t kSelCounters = 4 * kSelSplit;
+constexpr uint32_t kSelForced = ~0u, kSelOdd = ~0u - 1;
+constexpr float kSelLeast = 7.8886091e-31f;  // 2^-100
+
+struct PagedSelect {
+  const int8_t* codes;  // [pages][kv_heads][2][hd]
+  const float* scales;  // [pages][kv_heads]
+  int64_t code_step, scale_step;
+  int count, sink, local;
+  int pitch;  // keys a row in LDS
+  // units whose pages are split among `chunks` workgroups (of `chunk` pages): their arrivals, and the keys that meet
+  int chunks, chunk;
+  uint32_t *counters, *keys;
+};
+
+// A score as an unsigned key of the same order.
+__device__ __forceinline__ uint32_t sel_key(float s) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, s + 0.0f);
+  return u ^ (u >> 31 ? ~0u : 0x80000000u);
+}
+
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_least(uint32_t v) {
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) v = min(v, (uint32_t)__shfl_xor((int)v, off, 64));
+  return v;
+}
+
+__device__ __forceinline__ void store_dev1(uint32_t* p, uint32_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint32_t load_dev1(const uint32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// What the waves that work on one row of keys tell each other: one wave by itself, or all of a workgroup, each with a
+// part of the keys.
+struct SelAlone {
+  static constexpr int parts = 1, part = 0;
+  __device__ __forceinline__ int sum(int v) { return v; }
+  __device__ __forceinline__ int before(int, int) { return 0; }
+  __device__ __forceinline__ uint32_t most(uint32_t v) { return v; }
+  __device__ __forceinline__ uint32_t least(uint32_t v) { return v; }
+};
+struct SelTogether {
+  int parts, part;
+  uint32_t* box;  // [2][16]
+  int turn = 0;
+  // every wave's value, in lanes 0 .. parts - 1
+  __device__ __forceinline__ uint32_t all(uint32_t v, uint32_t none) {
+    uint32_t* b = box + 16 * turn;
+    turn ^= 1;  // (a wave that is a step ahead writes the other half)
+    if (__lane_id() == 0) b[part] = v;
+    __syncthreads();
+    const int lane = __lane_id();
+    return lane < parts ? b[lane & 15] : none;
+  }
+  __device__ __forceinline__ int sum(int v) {
+    const int s = wave_scan((int)all((uint32_t)v, 0));
+    return __builtin_amdgcn_readlane(s, 63);
+  }
+  __device__ __forceinline__ int before(int v, int) {
+    const int s = wave_scan((int)all((uint32_t)v, 0));
+    return __builtin_amdgcn_readlane(s, part) - v;
+  }
+  __device__ __forceinline__ uint32_t most(uint32_t v) { return wave_most(all(v, 0)); }
+  __device__ __forceinline__ uint32_t least(uint32_t v) { return wave_least(all(v, ~0u)); }
+};
+
+// The `count` largest of n > count keys, the first on ties, written in their order.
+template <typename W>
+__device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, int* out, W w) {
+  const int lane = __lane_id();
+  const int each = ((n + w.parts - 1) / w.parts + 63) & ~63;
+  const int from = min(each * w.part, n), to = min(from + each, n);
+  uint32_t hi = 0, lo = ~0u;
+  for (int j = from + lane; j < to; j += 64) {
+    hi = max(hi, key[j]);
+    lo = min(lo, key[j]);
+  }
+  hi = w.most(wave_most(hi));
+  lo = w.least(wave_least(lo));
+  auto at_least = [&](uint32_t t) __attribute__((always_inline)) {
+    int c = 0;
+    for (int j = from; j < to; j += 64) c += __builtin_popcountll(__ballot(j + lane < to && key[min(j + lane, to - 1)] >= t));
+    return w.sum(c);
+  };
+  // the largest t that at least `count` keys reach: lo is one that they do, hi one that they do not
+  if (at_least(hi) >= count) {
+    lo = hi;
+  } else {
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int c = at_least(mid);
+      if (c >= count) lo = mid;
+      else hi = mid;
+      if (c == count) break;
+    }
+  }
+  int above = 0, equal = 0;
+  for (int j = from; j < to; j += 64) {
+    const uint32_t k = key[min(j + lane, to - 1)];
+    above += __builtin_popcountll(__ballot(j + lane < to && k > lo));
+    equal += __builtin_popcountll(__ballot(j + lane < to && k == lo));
+  }
+  const int spare = count - w.sum(above);  // how many of the equal are taken
+  int a = w.before(above, 0), e = w.before(equal, 0);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int j = from; j < to; j += 64) {
+    const uint32_t k = key[min(j + lane, to - 1)];
+    const uint64_t ab = __ballot(j + lane < to && k > lo), eb = __ballot(j + lane < to && k == lo);
+    const int ea = e + __builtin_popcountll(eb & below);
+    if ((ab >> lane & 1) || ((eb >> lane & 1) && ea < spare)) out[a + __builtin_popcountll(ab & below) + min(ea, spare)] = j + lane;
+    a += __builtin_popcountll(ab);
+    e += __builtin_popcountll(eb);
+  }
+}
+
+// GP: rows a token takes of a tile of 16 (its heads, rounded up to 4, 8, 16); more than 16 heads take several tiles.
+template <int HD, bool BF, int GP>
+__global__ void __launch_bounds__(1024) paged_select_kernel(const PagedKv kv, const PagedSelect sel,
+                                                            const uint16_t* __restrict__ q, int64_t ldq, int heads, int g,
+                                                            int tokens_a_group, int* __restrict__ blocks) {
+  constexpr int KS = 2 * HD / 64;  // matrix instructions of a tile
+  constexpr int TOK = 16 / GP;     // tokens of a tile
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint32_t box[32];
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), waves = sread((int)(blockDim.x >> 6));
+  const int c16 = lane & 15, q4 = lane >> 4;
+  const int tiles = (g + 15) / 16;  // of a token's heads (GP 16)
+  uint8_t* qc = smem;               // [rows][2 hd] codes of the queries
+  uint32_t* keys = (uint32_t*)(smem + 16 * tiles * 2 * HD);
+  uint32_t* mine = sel.keys + (int64_t)blockIdx.x * tokens_a_group * sel.pitch;  // (split units only)
+  const int kvh = blockIdx.x % kv.kv_heads, first = (blockIdx.x / kv.kv_heads) * tokens_a_group;
+  const int past = min(first + tokens_a_group, kv.tokens);
+  for (int t0 = first; t0 < past;) {
+    const int seq = paged_find(kv.q_start, kv.batch, t0, lane);
+    if (seq >= kv.batch) return;  // behind the last sequence: left alone
+    const PagedSeq sq = paged_seq(sload(kv.q_start + seq), sload(kv.q_start + seq + 1), sload(kv.lens + seq), kv.tokens);
+    const int n = max(min(min(sq.q0 + sq.n, past) - t0, TOK), 1);  // tokens of this step (starts that are no batch's: one)
+    const int i0 = sq.len - sq.n + (t0 - sq.q0);           // position of the first
+    const int most = min((i0 + n - 1 >> kv.page_shift) + 1, kv.table_width);  // pages that the last sees
+    int* to = blocks + ((int64_t)t0 * kv.kv_heads + kvh) * sel.count;
+    const int64_t row = (int64_t)kv.kv_heads * sel.count;  // from a token's to the next one's
+    if (most <= sel.count && blockIdx.y > 0) return;
+    auto visible = [&](int t) __attribute__((always_inline)) {
+      return i0 + t < 0 ? 0 : min((i0 + t >> kv.page_shift) + 1, kv.table_width);
+    };
+    if (most > sel.count) {
+      // ---- the queries' codes: a wave a token
+      for (int t = wave; t < TOK; t += waves) {
+        const uint16_t* qr = q + (int64_t)(t0 + min(t, n - 1)) * ldq + (int64_t)kvh * g * HD;
+        uint32_t big = 0;
+        for (int x = 8 * lane; x < g * HD; x += 512) {
+          const uint4 u = *(const uint4*)(qr + x);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t m = w[e] & 0x7fff7fffu;
+            big = max(big, max(m & 0xffffu, m >> 16));
+          }
+        }
+        big = wave_most(big);
+        const float a = BF ? bf2f((uint16_t)big) : h2f((uint16_t)big);
+        const float inv = big >= (BF ? 0x7f80u : 0x7c00u) || a < kSelLeast ? 0.0f : 127.0f / a;
+        for (int x = lane; x < GP * tiles * (HD / 8); x += 64) {  // eight dims of a row
+          const int r = x / (HD / 8), d = 8 * (x % (HD / 8));
+          const uint4 u = *(const uint4*)(qr + min(r, g - 1) * HD + d);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          uint32_t up[2] = {0, 0}, dn[2] = {0, 0};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            const int c = inv == 0.0f ? 0 : (int)rintf((BF ? bf2f(h) : h2f(h)) * inv);
+            up[e >> 2] |= (uint32_t)(max(c, 0) & 255) << (8 * (e & 3));
+            dn[e >> 2] |= (uint32_t)(min(c, 0) & 255) << (8 * (e & 3));
+          }
+          uint8_t* dst = qc + (t * GP + r) * 2 * HD + d;
+          *(uint2*)dst = make_uint2(up[0], up[1]);
+          *(uint2*)(dst + HD) = make_uint2(dn[0], dn[1]);
+        }
+      }
+      __syncthreads();
+      // ---- scores: 16 pages a wave and step
+      pi4_t qa[KS];
+      auto rows = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qa[s] = *(const pi4_t*)(qc + (16 * tile + c16) * 2 * HD + 64 * s + 16 * q4);
+      };
+      rows(0);
+      const int* tab = kv.table + seq * kv.table_stride;
+      const int begin = blockIdx.y * sel.chunk, end = min(most, begin + sel.chunk);
+      for (int j0 = begin + 16 * wave; j0 < end; j0 += 16 * waves) {
+        const int j = j0 + c16;
+        int page = tab[min(j, most - 1)];
+        const bool bad = (uint32_t)page >= (uint32_t)kv.num_pages;
+        page = bad ? 0 : page;
+        const int8_t* at = sel.codes + page * sel.code_step + (int64_t)kvh * 2 * HD + 16 * q4;
+        pi4_t b[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) b[s] = *(const pi4_t*)(at + 64 * s);
+        const float scale = sel.scales[page * sel.scale_step + kvh];
+        int m = -0x7fffffff;
+        for (int tile = 0; tile < tiles; ++tile) {
+          if (tiles > 1) rows(tile);
+          pi4_t acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[s], b[s], acc, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m = max(m, acc[r]);
+        }
+        if (GP >= 8) m = max(m, __shfl_xor(m, 16, 64));
+        if (GP >= 16) m = max(m, __shfl_xor(m, 32, 64));
+        const int t = q4 * 4 / GP;  // the token of the lane's rows
+        if (q4 % (GP / 4) == 0 && t < n && j < most) {
+          const int cur = i0 + t >> kv.page_shift;
+          uint32_t k = bad || scale == INFINITY ? kSelOdd : min(sel_key((float)m * scale), kSelOdd - 1);
+          if (j < sel.sink || j > min(cur, kv.table_width - 1) - sel.local) k = kSelForced;
+          if (sel.chunks > 1) store_dev1(mine + t * sel.pitch + j, k);
+          else keys[t * sel.pitch + j] = k;
+        }
+      }
+      if (sel.chunks > 1) {  // (a unit of one step) the last to arrive chooses
+        if (!paged_arrive(sel.counters + blockIdx.x, sel.chunks, &flag)) return;
+        for (int t = 0; t < n; ++t)
+          for (int j = tid; j < most; j += blockDim.x) keys[t * sel.pitch + j] = load_dev1(mine + t * sel.pitch + j);
+      }
+      __syncthreads();
+    }
+    // ---- the choice
+    if (n == 1 && most > sel.count) {
+      sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, box});
+    } else {
+      for (int t = wave; t < n; t += waves) {
+        const int v = visible(t);
+        if (v > sel.count) {
+          sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{});
+        } else {
+          for (int x = lane; x < sel.count; x += 64) to[t * row + x] = x < v ? x : -1;
+        }
+      }
+    }
+    t0 += n;
+    if (t0 < past) __syncthreads();  // (codes and keys are read)
+  }
+}
+
+template <int HD, bool BF>
+static const void* select_of(int gp) {
+  return gp == 4   ? (const void*)paged_select_kernel<HD, BF, 4>
+         : gp == 8 ? (const void*)paged_select_kernel<HD, BF, 8>
+                   : (const void*)paged_select_kernel<HD, BF, 16>;
+}
+
+}  // namespace spectra
+
+using namespace spectra;
+
+extern "C" size_t spectra_paged_select_workspace(void) { return kSelCounters + (size_t)kSelSplit * kSelLds; }
+
+extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_paged_bounds_t* bounds, const void* q,
+                                    int64_t ldq, int32_t act_dtype, int64_t tokens, int32_t heads, int32_t count, int32_t sink,
+                                    int32_t local, void* workspace, size_t workspace_bytes, int32_t* blocks,
+                                    spectra_stream_t stream) {
+  SPECTRA_REQUIRE(kv != nullptr, "paged KV descriptor is NULL");
+  spectra_paged_kv_t d = *kv;  // (neither keys nor values are read, nor need they be given)
+  d.kind = SPECTRA_KV_4BIT;
+  d.k = d.v = d.k_scales = d.v_scales = d.k_zeros = d.v_zeros = (void*)16;
+  d.page_stride = d.scale_stride = d.zero_stride = 1LL << 32;
+  kv = &d;
+  PagedKv p;
+  if (int st = paged_args(kv, tokens, heads, &p); st != SPECTRA_OK) return st;
+  const int hd = kv->head_dim, g = heads / kv->kv_heads;
+  if (int st = paged_bounds_args(bounds, kv->num_pages, kv->kv_heads, hd); st != SPECTRA_OK) return st;
+  SPECTRA_REQUIRE(act_dtype == SPECTRA_F16 || act_dtype == SPECTRA_BF16, "q must be fp16 or bf16");
+  SPECTRA_REQUIRE(q && blocks, "NULL pointer");
+  SPECTRA_REQUIRE(ldq >= (int64_t)heads * hd && ldq % 8 == 0, "q token stride too small or not a multiple of 8");
+  SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(blocks) % 4 == 0,
+                  "q must be 16-byte aligned, blocks aligned");
+  SPECTRA_REQUIRE(sink >= 0 && local >= 1 && count >= 1 && (int64_t)sink + local <= count,
+                  "count must hold the first `sink` and the last `local` (at least one) blocks");
+  SPECTRA_REQUIRE(count <= kSelMost && tokens * kv->kv_heads * count < (1LL << 40), "count out of range");
+  if (kv->table_width > kSelMost) return fail(SPECTRA_ERR_UNSUPPORTED, "block tables of more than 32768 pages");
+  const int pitch = (kv->table_width + 63) & ~63, rows = 16 * ((g + 15) / 16);
+  if (g > 256 || rows * 2 * hd + 4 * pitch > kSelLds)
+    return fail(SPECTRA_ERR_UNSUPPORTED, "too many query heads a KV head, with a block table of this width");
+  if (workspace != nullptr) {
+    if (workspace_bytes < spectra_paged_select_workspace())
+      return fail(SPECTRA_ERR_WORKSPACE, "workspace smaller than spectra_paged_select_workspace bytes");
+    SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  }
+  if (int st = paged_apart({{"blocks", blocks, tokens * kv->kv_heads * count * 4, 0, 1},
+                            {"the workspace", workspace, (int64_t)spectra_paged_select_workspace(), 0, 1}},
+                           {{"q", q, (int64_t)heads * hd * 2, ldq * 2, tokens},
+                            paged_bound_codes(bounds, kv->num_pages, kv->kv_heads, hd),
+                            paged_bound_scales(bounds, kv->num_pages, kv->kv_heads),
+                            paged_table(kv), paged_lens(kv), paged_starts(kv)});
+      st != SPECTRA_OK)
+    return st;
+  const bool one = kv->num_pages == 1;
+  PagedSelect sel = {bounds->codes, bounds->scales, one ? 0 : bounds->code_stride, one ? 0 : bounds->scale_stride,
+                     count, sink, local, pitch, 1, kSelMost, nullptr, nullptr};
+  int gp = g <= 4 ? 4 : g <= 8 ? 8 : 16, gv = g, hv = heads;
+  // tokens a workgroup takes: one where sequences have one each, a tile's rows otherwise
+  const int64_t seqs = std::min<int64_t>(tokens, kv->batch);
+  int group = tokens < 2 * seqs ? 1 : 16 / gp;
+  while (rows * 2 * hd + 4 * group * pitch > kSelLds) group /= 2;
+  const int64_t groups = (tokens + group - 1) / group * kv->kv_heads;
+  SPECTRA_REQUIRE(groups < (1LL << 31), "tokens out of range");
+  const int lds = rows * 2 * hd + 4 * group * pitch;
+  // units of one step each, few of them, and pages enough for several workgroups
+  if (workspace != nullptr && groups <= kSelSplit && kv->table_width >= 1024 && (group == 1 || kv->batch == 1)) {
+    sel.chunks = (int)std::min<int64_t>(256 / groups, (kv->table_width + 255) / 256);
+    sel.chunk = ((kv->table_width + sel.chunks - 1) / sel.chunks + 15) & ~15;
+    sel.counters = (uint32_t*)workspace;
+    sel.keys = (uint32_t*)((uint8_t*)workspace + kSelCounters);
+  }
+  const int threads = kv->table_width <= 512 ? 256 : kv->table_width <= 1024 ? 512 : 1024;
+  const void* kern = hd == 64 ? (act_dtype == SPECTRA_BF16 ? select_of<64, true>(gp) : select_of<64, false>(gp))
+                              : (act_dtype == SPECTRA_BF16 ? select_of<128, true>(gp) : select_of<128, false>(gp));
+  if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
+  void* args[] = {(void*)&p, (void*)&sel, (void*)&q, (void*)&ldq, (void*)&hv, (void*)&gv, (void*)&group, (void*)&blocks};
+  SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)groups, (unsigned)sel.chunks), dim3(threads), args, lds, (hipStream_t)stream));
+  SPECTRA_HIP_CHECK(hipGetLastError());
+  return SPECTRA_OK;
+}

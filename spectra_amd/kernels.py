@@ -21,7 +21,7 @@ import ctypes
 import re
 import weakref
 from collections import OrderedDict
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -32,6 +32,8 @@ __all__ = ["fused_w4a16_gemv_hdsq", "batched_w4a16_gemm", "w4a16_linear", "w4_de
            "attend_workspace_bytes", "attend_prefill", "silu_mul", "greedy_next", "argmax_slots", "greedy_finish",
            "w4a16_gemv_fused", "kv4_quantize",
            "kv4_dequantize", "attend_decode_q4", "paged_rope_append", "paged_attend", "paged_attend_workspace",
+           "rope_axes", "paged_rope_axes_append", "paged_bounds", "paged_key_bounds", "paged_bounds_values", "paged_select",
+           "paged_select_workspace", "paged_attend_blocks", "adjust_logits", "next_tokens", "next_tokens_workspace",
            "validate_outliers"]
 
 GEMV_MAX_M = 4  # rows served by the GEMV family; larger batches go to the MFMA GEMM
@@ -820,6 +822,233 @@ def paged_attend(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
         if out is None:
             return torch.ops.spectra_hip.paged_attend.default(*args)
         torch.ops.spectra_hip.paged_attend_out.default(*args, out)
+        return out
+    except RuntimeError as e:
+        raise _paged_error(e) from None
+
+
+# ---------------------------------------------------------------------------
+# a served batch's step around the paged cache
+# ---------------------------------------------------------------------------
+def rope_axes(sections: Sequence[int], head_dim: int, interleaved: bool = False,
+              device: Optional[torch.device] = None) -> torch.Tensor:
+    """The axis of every rotation pair (uint8 [head_dim / 2]) for ``paged_rope_axes_append``: ``sections[a]`` pairs of axis
+    a one after another, or ``interleaved``: pair i is axis i % n's (n axes) while i < n * sections[i % n], and axis 0's
+    after that.  Pairs behind all sections (and pairs that a caller sets to n or more) do not turn."""
+    n, half = len(sections), head_dim // 2
+    if not 1 <= n <= 4 or min(sections) < 0 or sum(sections) > half:
+        raise ValueError(f"one to four sections of at most {half} pairs together, got {tuple(sections)}")
+    if interleaved:
+        if sum(sections) != half:
+            raise ValueError(f"interleaved sections must hold the head's {half} pairs, got {tuple(sections)}")
+        axis = [i % n if i < n * sections[i % n] else 0 for i in range(half)]
+    else:
+        axis = [a for a, c in enumerate(sections) for _ in range(c)]
+        axis += [255] * (half - len(axis))
+    return torch.tensor(axis, dtype=torch.uint8, device=device or torch.device("cuda"))
+
+
+def paged_rope_axes_append(qkv: torch.Tensor, positions: torch.Tensor, axis: torch.Tensor, kv_lens: torch.Tensor,
+                           q_start: torch.Tensor, block_table: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                           heads: int, k_pages, v_pages, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_rope_append`` with rotary positions of several axes (time, height and width of images and video beside
+    text): pair i of a head turns by row ``positions[axis[i], t]`` of ``cos`` / ``sin``, while the rows that the cache gets
+    stay those of the sequences' positions.  ``positions`` int32 [axes, T], one to four axes; ``axis`` uint8 [d / 2]
+    (``rope_axes``), a pair whose axis is past the last does not turn.  A token with a position of any axis outside the
+    tables appends nothing and gets NaN queries; everything else is as there."""
+    if not qkv.is_cuda:
+        raise ValueError("qkv must be on the GPU")
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            q = (L._ops_module or L.torch_ops_module()).paged_rope_axes_append(
+                qkv, positions, axis, kv_lens, q_start, block_table, cos, sin, heads, k_pages, v_pages, q_out)
+            if q is not NotImplemented:
+                return q
+        args = (qkv, positions, axis, kv_lens, q_start, block_table, cos, sin, heads, _pages(k_pages), _pages(v_pages))
+        if q_out is None:
+            return torch.ops.spectra_hip.paged_rope_axes_append.default(*args)
+        torch.ops.spectra_hip.paged_rope_axes_append_out.default(*args, q_out)
+        return q_out
+    except RuntimeError as e:
+        raise _paged_error(e) from None
+
+
+def paged_bounds(k_pages) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Room for the bounds of a pool's keys (``paged_key_bounds``): codes int8 [pages, kv, 2, d] and scales fp32
+    [pages, kv], zero."""
+    k = _pages(k_pages)
+    pages, kv, _, d = k[0].shape
+    return (torch.zeros(pages, kv, 2, d * (2 if len(k) == 3 else 1), dtype=torch.int8, device=k[0].device),
+            torch.zeros(pages, kv, dtype=torch.float32, device=k[0].device))
+
+
+def paged_key_bounds(tokens: int, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor, k_pages,
+                     bounds: Tuple[torch.Tensor, torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Works out anew the 8-bit ``bounds`` (``paged_bounds``) of every page that one of a call's ``tokens`` tokens lies in,
+    over its rows below ``kv_lens``: to be called after each append, with its lengths and starts; ``paged_select`` reads
+    them.  With A the largest magnitude of a page's keys of a head: codes ceil(max 127 / A) and floor(min 127 / A) of each
+    dim within +-127, scale A / 127; all zero where A < 2^-100; codes 0 and scale infinity where a key is not finite.
+    Other pages' bounds stay.  Returns ``bounds``."""
+    codes, scales = bounds
+    if not codes.is_cuda:
+        raise ValueError("bounds must be on the GPU")
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            r = (L._ops_module or L.torch_ops_module()).paged_key_bounds(tokens, kv_lens, q_start, block_table, k_pages,
+                                                                         codes, scales)
+            if r is not NotImplemented:
+                return bounds
+        torch.ops.spectra_hip.paged_key_bounds.default(tokens, kv_lens, q_start, block_table, _pages(k_pages), codes, scales)
+        return bounds
+    except RuntimeError as e:
+        raise _paged_error(e) from None
+
+
+def paged_bounds_values(bounds: Tuple[torch.Tensor, torch.Tensor], out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """What ``bounds`` stand for: [pages, kv, 2, d], the greatest, then the least value of each dim, rounded outwards to
+    whole steps of the scale (+-infinity where a key is not finite)."""
+    codes, scales = bounds
+    if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 4 or codes.shape[2] != 2 or not codes[0].is_contiguous():
+        raise ValueError("codes must be int8 [pages, kv, 2, d] on the GPU, each page contiguous")
+    pages, kv, _, d = codes.shape
+    if scales.dtype != torch.float32 or scales.shape != (pages, kv) or scales.stride(1) != 1 or scales.device != codes.device:
+        raise ValueError(f"scales must be fp32 [{pages}, {kv}] with contiguous rows on {codes.device}")
+    out = torch.empty(codes.shape, device=codes.device, dtype=out_dtype)
+    b = L.PagedBounds(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
+    with torch.cuda.device(codes.device):
+        L.check("spectra_paged_bounds_values", L.load().spectra_paged_bounds_values(
+            ctypes.byref(b), pages, kv, d, out.data_ptr(), _dtype_code(out, _DT.keys(), "out_dtype"), _stream(codes.device)))
+    return out
+
+
+def paged_select_workspace(device: Optional[torch.device] = None) -> torch.Tensor:
+    """A workspace for ``paged_select`` calls of any shape, ready for use: one may serve every layer and step of a stream,
+    but calls that overlap need one each."""
+    return torch.zeros(int(L.load().spectra_paged_select_workspace()), dtype=torch.uint8, device=device or torch.device("cuda"))
+
+
+def paged_select(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
+                 bounds: Tuple[torch.Tensor, torch.Tensor], page: int, count: int, *, sink: int = 1, local: int = 2,
+                 workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The blocks (pages of a sequence) that each token attends to in each KV head, for ``paged_attend_blocks``: int32
+    [T, kv, count], ascending, then -1.
+
+    Of the blocks that the token at position i of its sequence sees (j <= i // page) the first ``sink`` and the last
+    ``local`` (at least one: its own) are always taken, then those with the largest scores, the lowest block on ties.  A
+    score bounds the largest product of any of the KV head's query heads with any key of the block: the heads of ``q``
+    [T, heads, d] (fp16 or bf16) rounded to 8 bits of one scale, times the ``bounds`` of ``paged_key_bounds`` in whole
+    numbers, exact, so the choice depends on nothing else.  Blocks whose bounds are infinite, and pages outside the pool, come
+    first.  Lengths, starts and the table are ``paged_attend``'s; rows behind q_start[-1] are left alone.  ``workspace``
+    (``paged_select_workspace``): shares one long sequence among more of the card; without one the result is the same."""
+    if not q.is_cuda:
+        raise ValueError("q must be on the GPU")
+    codes, scales = bounds
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            o = (L._ops_module or L.torch_ops_module()).paged_select(
+                q, kv_lens, q_start, block_table, codes, scales, page, count, sink, local, workspace, out)
+            if o is not NotImplemented:
+                return o
+        args = (q, kv_lens, q_start, block_table, codes, scales, page, count, sink, local, workspace)
+        if out is None:
+            return torch.ops.spectra_hip.paged_select.default(*args)
+        torch.ops.spectra_hip.paged_select_out.default(*args, out)
+        return out
+    except RuntimeError as e:
+        raise _paged_error(e) from None
+
+
+def paged_attend_blocks(q: torch.Tensor, blocks: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor,
+                        block_table: torch.Tensor, k_pages, v_pages, *, scale: Optional[float] = None, cap: float = 0.0,
+                        workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attend`` over listed blocks: the token at position i sees, in KV head n, the keys j <= i of the blocks of
+    its sequence in ``blocks[t, n]`` (int32 [T, kv, count], as ``paged_select`` leaves them).  Negative entries and ones
+    past the table name nothing; a block named twice counts twice.  Scores, ``cap``, roundings and the ``workspace``
+    (``paged_attend_workspace``) are ``paged_attend``'s.  A row that sees no key is zero; one that sees a key of a page
+    outside the pool, or whose position lies past the table, is NaN; rows behind q_start[-1] are left alone."""
+    if not q.is_cuda:
+        raise ValueError("q must be on the GPU")
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            o = (L._ops_module or L.torch_ops_module()).paged_attend_blocks(
+                q, blocks, kv_lens, q_start, block_table, k_pages, v_pages, scale, cap, workspace, out)
+            if o is not NotImplemented:
+                return o
+        args = (q, blocks, kv_lens, q_start, block_table, _pages(k_pages), _pages(v_pages),
+                q.shape[-1] ** -0.5 if scale is None else scale, cap, workspace)
+        if out is None:
+            return torch.ops.spectra_hip.paged_attend_blocks.default(*args)
+        torch.ops.spectra_hip.paged_attend_blocks_out.default(*args, out)
+        return out
+    except RuntimeError as e:
+        raise _paged_error(e) from None
+
+
+def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                  prompt_lens: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                  presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
+                  bias_ids: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                  allowed: Optional[torch.Tensor] = None, allowed_rows: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A batch's ``logits`` [B, V] (fp16, bf16 or fp32) with penalties for repeated tokens, biases and grammar masks, in
+    their type (``out`` may be ``logits``).  In fp32, each operation rounded, the result once:
+
+    * tokens in the row's ``history`` (int64 [B, L], the first ``lens[b]`` count, all by default): x / ``repetition`` where
+      x > 0, x * ``repetition`` otherwise; of the history's tokens behind the first ``prompt_lens[b]`` (0 by default), the answer, c
+      times there: x - ``frequency`` c, then x - ``presence``.  Each fp32 [B], or None; ids outside [0, V) count nothing;
+    * x + ``bias`` (fp32 [B, n]) for the tokens ``bias_ids`` (int64 [B, n]; of an id given twice the last counts, ids
+      outside [0, V), as -1, are filling);
+    * -infinity where the row's mask has no bit: ``allowed`` int32 [M, ceil(V / 32)], token v's bit v % 32 of word v // 32;
+      row b's mask is ``allowed_rows[b]`` (int32 [B], no mask where it is not a row; its own by default).
+
+    ``lens``, ``prompt_lens`` and ``allowed_rows`` are int32 [B].  All are read on the device: a captured step follows
+    them, and nothing is kept between calls."""
+    if not logits.is_cuda:
+        raise ValueError("logits must be on the GPU")
+    more = (history, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, allowed, allowed_rows)
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            o = (L._ops_module or L.torch_ops_module()).adjust_logits(logits, *more, out)
+            if o is not NotImplemented:
+                return o
+        if out is None:
+            return torch.ops.spectra_hip.adjust_logits.default(logits, *more)
+        if out is logits:
+            torch.ops.spectra_hip.adjust_logits_.default(logits, *more)
+        else:
+            torch.ops.spectra_hip.adjust_logits_out.default(logits, *more, out)
+        return out
+    except RuntimeError as e:
+        raise _paged_error(e) from None
+
+
+def next_tokens_workspace(device: Optional[torch.device] = None) -> torch.Tensor:
+    """A workspace for ``next_tokens``, ready for use: one may serve every step of a stream, but calls that overlap need
+    one each."""
+    return torch.zeros(int(L.load().spectra_next_tokens_workspace()), dtype=torch.uint8, device=device or torch.device("cuda"))
+
+
+def next_tokens(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                prompt_lens: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
+                bias_ids: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                allowed: Optional[torch.Tensor] = None, allowed_rows: Optional[torch.Tensor] = None,
+                workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``greedy_next`` for a batch under ``adjust_logits``' penalties, biases and masks, without writing the logits: int64
+    [B], the token with the largest adjusted logit in fp32 (the lowest on ties, NaN counts as largest, as torch.argmax), or
+    -1 where every one is -infinity.  At most 4096 rows.  ``workspace``: ``next_tokens_workspace()``; by default a fresh
+    one, which costs a small kernel."""
+    if not logits.is_cuda:
+        raise ValueError("logits must be on the GPU")
+    more = (history, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, allowed, allowed_rows, workspace)
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            o = (L._ops_module or L.torch_ops_module()).next_tokens(logits, *more, out)
+            if o is not NotImplemented:
+                return o
+        if out is None:
+            return torch.ops.spectra_hip.next_tokens.default(logits, *more)
+        torch.ops.spectra_hip.next_tokens_out.default(logits, *more, out)
         return out
     except RuntimeError as e:
         raise _paged_error(e) from None
