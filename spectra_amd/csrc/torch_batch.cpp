@@ -96,6 +96,23 @@ void key_bounds(int64_t tokens, const at::Tensor& kv_lens, const at::Tensor& q_s
   check_paged("spectra_paged_key_bounds", spectra_paged_key_bounds(&p, tokens, &b, stream_of(dev)));
 }
 
+// dtype: SPECTRA_F16, BF16 or F32
+at::ScalarType type_of(int64_t dtype) {
+  TORCH_CHECK_VALUE(dtype == SPECTRA_F16 || dtype == SPECTRA_BF16 || dtype == SPECTRA_F32, "unknown dtype ", dtype);
+  return dtype == SPECTRA_F16 ? at::kHalf : dtype == SPECTRA_BF16 ? at::kBFloat16 : at::kFloat;
+}
+at::Tensor bounds_values(const at::Tensor& codes, const at::Tensor& scales, int64_t dtype) {
+  const auto dev = codes.device();
+  const spectra_paged_bounds_t b = describe_bounds(codes, scales, -1, -1, -1, dev);
+  const c10::DeviceGuard guard(dev);
+  at::Tensor out = at::detail::empty_cuda(codes.sizes(), type_of(dtype), dev, c10::nullopt);
+  TORCH_CHECK_VALUE(codes.size(1) <= 65536 && codes.size(3) <= 65536, "sizes out of range");
+  check_paged("spectra_paged_bounds_values",
+              spectra_paged_bounds_values(&b, codes.size(0), (int32_t)codes.size(1), (int32_t)codes.size(3), out.data_ptr(),
+                                          (int32_t)dtype, stream_of(dev)));
+  return out;
+}
+
 // ---- selection ----
 at::Tensor select(const at::Tensor& q_in, const at::Tensor& kv_lens, const at::Tensor& q_start, const at::Tensor& block_table,
                   const at::Tensor& codes, const at::Tensor& scales, int64_t page, int64_t count, int64_t sink, int64_t local,
@@ -351,6 +368,10 @@ void key_bounds_meta(int64_t, const at::Tensor&, const at::Tensor&, const at::Te
   TORCH_CHECK_VALUE(k.size() == 1 || k.size() == 3, "k_pages must be [pages, kv_heads, page, d], or (codes, scales, zeros) of that");
 }
 
+at::Tensor bounds_values_meta(const at::Tensor& codes, const at::Tensor&, int64_t dtype) {
+  return at::empty_symint(codes.sym_sizes(), codes.options().dtype(type_of(dtype)));
+}
+
 at::Tensor select_op(const at::Tensor& q, const at::Tensor& kv_lens, const at::Tensor& q_start, const at::Tensor& block_table,
                      const at::Tensor& codes, const at::Tensor& scales, int64_t page, int64_t count, int64_t sink, int64_t local,
                      const OptTensor& workspace) {
@@ -475,6 +496,17 @@ PyObject* py_key_bounds(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_bounds_values(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 3, "paged_bounds_values takes 3 arguments");
+  Arguments a{args};
+  const at::Tensor *codes = a.tensor(0), *scales = a.tensor(1);
+  const int64_t dtype = a.integer(2);
+  if (!a.plain || dispatched()) Py_RETURN_NOTIMPLEMENTED;
+  return THPVariable_Wrap(released([&] { return bounds_values(*codes, *scales, dtype); }));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 12, "paged_select takes 12 arguments");
@@ -543,6 +575,7 @@ TORCH_LIBRARY_FRAGMENT(spectra_hip, m) {
   m.def(("paged_rope_axes_append(" + axes + ") -> Tensor").c_str());
   m.def(("paged_rope_axes_append_out(" + axes + ", Tensor(c!) q_out) -> ()").c_str());
   m.def(("paged_key_bounds(int tokens, " + batch + "Tensor[] k_pages, Tensor(a!) codes, Tensor(b!) scales) -> ()").c_str());
+  m.def("paged_bounds_values(Tensor codes, Tensor scales, int dtype) -> Tensor");
   const std::string sel = "Tensor q, " + batch + "Tensor codes, Tensor scales, int page, int count, int sink, int local, Tensor(a!)? workspace";
   m.def(("paged_select(" + sel + ") -> Tensor").c_str());
   m.def(("paged_select_out(" + sel + ", Tensor(b!) out) -> ()").c_str());
@@ -563,6 +596,7 @@ TORCH_LIBRARY_IMPL(spectra_hip, CUDA, m) {
   m.impl("paged_rope_axes_append", &axes_append_op);
   m.impl("paged_rope_axes_append_out", &axes_append_out_op);
   m.impl("paged_key_bounds", &key_bounds);
+  m.impl("paged_bounds_values", &bounds_values);
   m.impl("paged_select", &select_op);
   m.impl("paged_select_out", &select_out_op);
   m.impl("paged_attend_blocks", &attend_blocks_op);
@@ -578,6 +612,7 @@ TORCH_LIBRARY_IMPL(spectra_hip, Meta, m) {
   m.impl("paged_rope_axes_append", &axes_append_meta);
   m.impl("paged_rope_axes_append_out", &axes_append_out_meta);
   m.impl("paged_key_bounds", &key_bounds_meta);
+  m.impl("paged_bounds_values", &bounds_values_meta);
   m.impl("paged_select", &select_meta);
   m.impl("paged_select_out", &select_out_meta);
   m.impl("paged_attend_blocks", &attend_blocks_meta);

@@ -7,6 +7,7 @@ namespace spectra_torch {
 
 PyObject* py_axes_append(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_key_bounds(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* py_bounds_values(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_select(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_attend_blocks(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n);

@@ -193,6 +193,7 @@ PyMethodDef kMethods[] = {
     {"paged_attend", (PyCFunction)(void*)py_attend, METH_FASTCALL, nullptr},
     {"paged_rope_axes_append", (PyCFunction)(void*)py_axes_append, METH_FASTCALL, nullptr},
     {"paged_key_bounds", (PyCFunction)(void*)py_key_bounds, METH_FASTCALL, nullptr},
+    {"paged_bounds_values", (PyCFunction)(void*)py_bounds_values, METH_FASTCALL, nullptr},
     {"paged_select", (PyCFunction)(void*)py_select, METH_FASTCALL, nullptr},
     {"paged_attend_blocks", (PyCFunction)(void*)py_attend_blocks, METH_FASTCALL, nullptr},
     {"adjust_logits", (PyCFunction)(void*)py_adjust_logits, METH_FASTCALL, nullptr},

@@ -908,17 +908,18 @@ def paged_bounds_values(bounds: Tuple[torch.Tensor, torch.Tensor], out_dtype: to
     """What ``bounds`` stand for: [pages, kv, 2, d], the greatest, then the least value of each dim, rounded outwards to
     whole steps of the scale (+-infinity where a key is not finite)."""
     codes, scales = bounds
-    if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 4 or codes.shape[2] != 2 or not codes[0].is_contiguous():
-        raise ValueError("codes must be int8 [pages, kv, 2, d] on the GPU, each page contiguous")
-    pages, kv, _, d = codes.shape
-    if scales.dtype != torch.float32 or scales.shape != (pages, kv) or scales.stride(1) != 1 or scales.device != codes.device:
-        raise ValueError(f"scales must be fp32 [{pages}, {kv}] with contiguous rows on {codes.device}")
-    out = torch.empty(codes.shape, device=codes.device, dtype=out_dtype)
-    b = L.PagedBounds(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
-    with torch.cuda.device(codes.device):
-        L.check("spectra_paged_bounds_values", L.load().spectra_paged_bounds_values(
-            ctypes.byref(b), pages, kv, d, out.data_ptr(), _dtype_code(out, _DT.keys(), "out_dtype"), _stream(codes.device)))
-    return out
+    if not codes.is_cuda:
+        raise ValueError("bounds must be on the GPU")
+    if out_dtype not in _DT:
+        raise ValueError(f"out_dtype must be one of {[str(a) for a in _DT]}, got {out_dtype}")
+    try:
+        if not torch.compiler.is_dynamo_compiling():
+            o = (L._ops_module or L.torch_ops_module()).paged_bounds_values(codes, scales, _DT[out_dtype])
+            if o is not NotImplemented:
+                return o
+        return torch.ops.spectra_hip.paged_bounds_values.default(codes, scales, _DT[out_dtype])
+    except RuntimeError as e:
+        raise _paged_error(e) from None
 
 
 def paged_select_workspace(device: Optional[torch.device] = None) -> torch.Tensor:
