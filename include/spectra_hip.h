@@ -445,9 +445,9 @@ int spectra_paged_attend(const spectra_paged_kv_t* kv, const void* q, int64_t ld
 /* spectra_paged_rope_append with rotary positions of several axes (images and video: time, height
  * and width): pair i of a head (dims i and i + head_dim / 2) of token t turns by row
  * positions[axis[i] * ldpos + t] of the tables.  positions int32, axes (1 to 4) rows of `tokens`; axis
- * uint8 [head_dim / 2], 8-byte aligned; a pair whose axis is `axes` or more does not turn.  cos_t and sin_t are required.  The rows that
- * the cache gets stay those of the sequences' positions.  A token with a position of any axis
- * outside [0, rope_rows) appends nothing and gets NaN queries. */
+ * uint8 [head_dim / 2]; a pair whose axis is `axes` or more does not turn.  cos_t and sin_t are
+ * required.  The rows that the cache gets stay those of the sequences' positions.  A token with a
+ * position of any axis outside [0, rope_rows) appends nothing and gets NaN queries. */
 int spectra_paged_rope_axes_append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t tokens,
                                    const int32_t* positions, int64_t ldpos, int32_t axes, const uint8_t* axis,
                                    const float* cos_t, const float* sin_t, int64_t rope_rows, int32_t heads, void* q_rot,

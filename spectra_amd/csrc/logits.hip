@@ -9,18 +9,19 @@
 //   the row's grammar state does not allow v:              x = -inf
 // and the choice is the largest x, the lowest v on ties, NaN before all (as torch.argmax); -1 when every x is -inf.
 //
-// A workgroup takes a slice of a row's vocabulary and keeps the slice's counts in LDS: the row's tokens are read once a
-// slice (from L2), those of the slice counted by LDS atomics on whole numbers, whose order changes nothing, and the
-// logits pass once, 16 bytes a lane.  So nothing is kept between steps, and the history may change in any way.  The choice
-// meets over a row's slices in 64-bit maxima of (value, token) in the workspace, whose last arrival writes the token.
+// A workgroup takes a slice of a row's vocabulary, 8 or 16 logits a lane, which are asked for first and stay in registers.
+// The row's tokens are read once a slice (from L2); those of the slice are counted in LDS, a word a token, by atomics on
+// whole numbers, whose order changes nothing, and a bit each says which words there are to look at: most logits pass
+// without.  So nothing is kept between steps, and the history may change in any way.  The choice meets over a row's slices
+// in 64-bit maxima of (value, token) in the workspace, whose last arrival writes the token.
 #include <algorithm>
 
 #include "paged.h"
 
 namespace spectra {
 
-constexpr int kLgThreads = 256;
 constexpr int kLgRows = SPECTRA_NEXT_TOKENS_ROWS;  // rows whose slices meet in the workspace
+constexpr int kLgApart = 256;  // bytes of a row there: the best so far, and from kLgApart / 2 on how many slices have arrived
 
 struct LogitsArgs {
   const void* x;
@@ -40,7 +41,6 @@ struct LogitsArgs {
   int64_t ldallowed;
   int states;
   const int* state;  // or NULL: the row's number
-  int slice;         // tokens of a slice, a multiple of 2048
 };
 
 // fp32 as an unsigned number of the same order, NaN above all.
@@ -82,136 +82,202 @@ struct LgType<SPECTRA_F32> {
   static __device__ __forceinline__ T put(float v) { return v; }
 };
 
-template <int DT, bool PICK>
-__global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsArgs a, void* __restrict__ out, int64_t ldo,
-                                                            int64_t* __restrict__ tokens, int slices,
-                                                            unsigned long long* __restrict__ best, uint32_t* __restrict__ arrived) {
+// A token's word: in its lower half how often it is in the answer, the half's top bit for the prompt; in the upper half 1
+// + the place of its bias.  Of 32 bits, or of 64 where a history or a list of biases is longer than the halves hold.
+template <typename W>
+struct LgWord {
+  static constexpr int half = 4 * sizeof(W);
+  static constexpr W prompt = W(1) << (half - 1), count = prompt - 1, low = (W(1) << half) - 1;
+};
+// A slice's words, its map of bits and its list of tokens in LDS; of these the first two start at zero.
+constexpr size_t lg_zero(int slice, size_t word) { return slice / 8 + slice * word; }
+
+// TH: threads of a workgroup; C: chunks of 8 logits a lane; W: the words' type.
+template <int DT, bool PICK, int TH, int C, typename W>
+__global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* __restrict__ out, int64_t ldo,
+                                                    int64_t* __restrict__ tokens, int slices, uint8_t* __restrict__ meeting) {
   typedef typename LgType<DT>::T T;
-  extern __shared__ __align__(16) uint32_t seen[];  // [slice]: bit 31 said at all, below it how often in the answer; then
-  __shared__ lg_key_t meet[kLgThreads / 64];        // [slice]: 1 + the place of its bias
+  typedef LgWord<W> Word;
+  constexpr int S = 8 * TH * C, U = 2048 / TH > 4 ? 8 : 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ lg_key_t meet[TH / 64];
+  __shared__ float held[TH];  // the first biases
+  __shared__ int listed;
   const int tid = threadIdx.x, row = blockIdx.y;
-  const int64_t begin = (int64_t)blockIdx.x * a.slice;
-  const int n = (int)min((int64_t)a.slice, a.vocab - begin);
+  const int64_t begin = (int64_t)blockIdx.x * S;
+  const int n = (int)min((int64_t)S, a.vocab - begin);
   const bool counts = a.history != nullptr, biased = a.biases > 0;
-  uint32_t* where = seen + (counts ? a.slice : 0);
-  if (counts || biased) {
-    for (int i = 4 * tid; i < (counts && biased ? 2 : 1) * a.slice; i += 4 * kLgThreads) *(uint4*)(seen + i) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-  }
-  float rep = 1.0f, pres = 0.0f, freq = 0.0f;
-  if (counts) {
-    if (a.repetition != nullptr) rep = a.repetition[row];
-    if (a.presence != nullptr) pres = a.presence[row];
-    if (a.frequency != nullptr) freq = a.frequency[row];
-    const int64_t* h = a.history + row * a.ldh;
-    const int len = a.lens != nullptr ? min(max(a.lens[row], 0), a.hist) : a.hist;
-    const int prompt = a.prompts != nullptr ? a.prompts[row] : 0;
-    constexpr int U = 8;
-    for (int i0 = tid; i0 < len; i0 += U * kLgThreads) {
-      int64_t id[U];
+  const T* x = (const T*)a.x + row * a.ldx + begin;
+  T* y = (T*)out + row * ldo + begin;
+  // ---- the lane's logits; of a chunk that the row ends in, one by one
+  LgEight<T> u[C];
 #pragma unroll
-      for (int u = 0; u < U; ++u) id[u] = h[min(i0 + u * kLgThreads, len - 1)];
+  for (int k = 0; k < C; ++k) {
+    const int i = 8 * (tid + k * TH);
+    if (i + 8 <= n) {
+      u[k] = *(const LgEight<T>*)(x + i);
+    } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kLgThreads;
-        const uint64_t at = (uint64_t)(id[u] - begin);
-        if (i < len && at < (uint64_t)n) {
-          if (i < prompt) atomicOr(&seen[at], 0x80000000u);
-          else atomicAdd(&seen[at], 1u);
-        }
-      }
+      for (int e = 0; e < 8; ++e) u[k].v[e] = i + e < n ? x[i + e] : T(0);
     }
   }
-  if (biased) {
-    const int64_t* ids = a.bias_ids + row * a.ldid;
-    for (int i = tid; i < a.biases; i += kLgThreads) {
-      const uint64_t at = (uint64_t)(ids[i] - begin);
-      if (at < (uint64_t)n) atomicMax(&where[at], (uint32_t)i + 1);
-    }
-  }
-  if (counts || biased) __syncthreads();
   const uint8_t* mask = nullptr;
   if (a.allowed != nullptr) {
     const int s = a.state != nullptr ? a.state[row] : row;
     if (s >= 0 && s < a.states) mask = (const uint8_t*)(a.allowed + s * a.ldallowed) + begin / 8;
   }
+  // ---- the tokens that are adjusted
+  uint32_t* map = (uint32_t*)smem;
+  W* words = (W*)(smem + S / 8);
+  uint16_t* list = (uint16_t*)(smem + lg_zero(S, sizeof(W)));
+  float rep = 1.0f, pres = 0.0f, freq = 0.0f;
   const float* bias = a.bias + row * a.ldbias;
-  const T* x = (const T*)a.x + row * a.ldx + begin;
-  T* y = (T*)out + row * ldo + begin;
-  float top = 0.0f;  // the best of this lane, whose tokens come in order
-  uint32_t at = 0;
-  bool any = false;
-  auto adjusted = [&](float v, int i, bool ok) __attribute__((always_inline)) {
+  if (counts || biased) {
+    const int64_t* h = a.history + row * a.ldh;
+    const int64_t* ids = a.bias_ids + row * a.ldid;
+    // (the first of both are on their way while the words are cleared; a row's history is there beyond its length)
+    int64_t id[U], bid = -1;
+    int len = 0, prompt = 0;
     if (counts) {
-      const uint32_t s = seen[i];
-      if (s != 0) {
-        const uint32_t c = s & 0x7fffffffu;
+#pragma unroll
+      for (int k = 0; k < U; ++k) id[k] = h[min(tid + k * TH, a.hist - 1)];
+      len = a.lens != nullptr ? min(max(a.lens[row], 0), a.hist) : a.hist;
+      prompt = a.prompts != nullptr ? a.prompts[row] : 0;
+      if (a.repetition != nullptr) rep = a.repetition[row];
+      if (a.presence != nullptr) pres = a.presence[row];
+      if (a.frequency != nullptr) freq = a.frequency[row];
+    }
+    if (biased && tid < a.biases) {
+      bid = ids[tid];
+      held[tid] = bias[tid];
+    }
+    for (int i = tid; i < (int)(lg_zero(S, sizeof(W)) / 16); i += TH) *(uint4*)(smem + 16 * i) = make_uint4(0, 0, 0, 0);
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    auto enlist = [&](uint32_t at) __attribute__((always_inline)) {
+      list[atomicAdd(&listed, 1)] = (uint16_t)at;
+      atomicOr(&map[at >> 5], 1u << (at & 31));
+    };
+    for (int i0 = tid; i0 < len; i0 += U * TH) {
+      if (i0 >= U * TH) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) id[k] = h[min(i0 + k * TH, a.hist - 1)];
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * TH;
+        const uint64_t at = (uint64_t)(id[k] - begin);
+        if (i < len && at < (uint64_t)n) {
+          const W was = i < prompt ? atomicOr(&words[at], Word::prompt) : atomicAdd(&words[at], W(1));
+          if (was == 0) enlist((uint32_t)at);
+        }
+      }
+    }
+    if (biased) {
+      __syncthreads();  // (lower halves are what they will be)
+      for (int i = tid; i < a.biases; i += TH) {
+        if (i >= TH) bid = ids[i];
+        const uint64_t at = (uint64_t)(bid - begin);
+        if (at < (uint64_t)n) {
+          if (atomicMax(&words[at], (W)(i + 1) << Word::half | (words[at] & Word::low)) == 0) enlist((uint32_t)at);
+        }
+      }
+    }
+    __syncthreads();
+    for (int p = tid; p < listed; p += TH) {
+      const int at = list[p];
+      const W s = words[at], c = s & Word::count;
+      float v = LgType<DT>::get(x[at]);
+      if ((s & Word::low) != 0) {
         v = v > 0.0f ? v / rep : v * rep;
         v = v - freq * (float)c;
         if (c != 0) v = v - pres;
       }
+      const int place = (int)(s >> Word::half);
+      if (place != 0) v = v + (place <= TH ? held[place - 1] : bias[place - 1]);
+      words[at] = __builtin_bit_cast(uint32_t, v);
     }
-    if (biased) {
-      const uint32_t p = where[i];
-      if (p != 0) v = v + bias[p - 1];
-    }
-    return ok ? v : -INFINITY;
-  };
-  auto take = [&](float v, int i) __attribute__((always_inline)) {
-    if (!any || (v > top && !(top != top)) || (v != v && !(top != top))) {
-      top = v;
-      at = (uint32_t)i;
-      any = true;
-    }
-  };
-  for (int i = 8 * tid; i < n; i += 8 * kLgThreads) {
-    const uint32_t bits = mask != nullptr ? mask[i / 8] : 255u;
-    if (i + 8 <= n) {
-      const LgEight<T> u = *(const LgEight<T>*)(x + i);
-      LgEight<T> w;
+    __syncthreads();
+  }
+  // ---- all of them
+  float top = -INFINITY;  // the best of this lane, whose tokens come in order
+  int at = -1;
+  bool odd = false;       // it is NaN
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int i = 8 * (tid + k * TH);
+    if (i >= n) continue;
+    const uint32_t ok = mask != nullptr ? mask[i / 8] : 255u;
+    const uint32_t own = counts || biased ? ((const uint8_t*)map)[i / 8] : 0u;
+    float z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = LgType<DT>::get(u[k].v[e]);
+    if (own != 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = adjusted(LgType<DT>::get(u.v[e]), i + e, bits >> e & 1);
-        if (PICK) take(v, i + e);
-        else w.v[e] = LgType<DT>::put(v);
+        const float v = __builtin_bit_cast(float, (uint32_t)words[i + e]);
+        z[e] = own >> e & 1 ? v : z[e];
       }
-      if (!PICK) *(LgEight<T>*)(y + i) = w;
-    } else {
-      for (int e = 0; i + e < n; ++e) {
-        const float v = adjusted(LgType<DT>::get(x[i + e]), i + e, bits >> e & 1);
-        if (PICK) take(v, i + e);
-        else y[i + e] = LgType<DT>::put(v);
+    }
+    LgEight<T> w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v = z[e];
+      if (!(ok >> e & 1)) v = -INFINITY;
+      if (PICK) {
+        if (i + e < n && !odd && !(v <= top)) {
+          top = v;
+          at = i + e;
+          odd = v != v;
+        }
+      } else {
+        w.v[e] = LgType<DT>::put(v);
+      }
+    }
+    if (!PICK) {
+      if (i + 8 <= n) {
+        *(LgEight<T>*)(y + i) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < n) y[i + e] = w.v[e];
       }
     }
   }
   if (PICK) {
-    lg_key_t k = any ? (lg_key_t)lg_order(top) << 32 | (uint32_t)~(uint32_t)(begin + at) : 0;
+    lg_key_t k = at >= 0 ? (lg_key_t)lg_order(top) << 32 | (uint32_t)~(uint32_t)(begin + at) : 0;
 #pragma unroll
     for (int off = 1; off < 64; off *= 2) k = lg_most(k, (lg_key_t)__shfl_xor((unsigned long long)k, off, 64));
     if ((tid & 63) == 0) meet[tid >> 6] = k;
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-      for (int w = 1; w < kLgThreads / 64; ++w) k = lg_most(k, meet[w]);
+      for (int w = 1; w < TH / 64; ++w) k = lg_most(k, meet[w]);
       if (slices > 1) {
-        __hip_atomic_fetch_max(best + row, (unsigned long long)k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __builtin_amdgcn_s_waitcnt(0);
-        // (the maximum has happened before the arrival is counted)
-        if (__hip_atomic_fetch_add(arrived + row, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) != (uint32_t)slices - 1) return;
-        k = __hip_atomic_load(best + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(best + row, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // The maximum has happened before the arrival is counted, both where all of the card sees them.  (An ordered atomic
+        // would write back and drop the L2 for it: 53 us, not 16, with 2048 workgroups; rows beside each other in memory
+        // have their atomics wait for each other: 64 rows of 128256 took 23 us, not 9.7.)
+        unsigned long long* best = (unsigned long long*)(meeting + row * kLgApart);
+        uint32_t* arrived = (uint32_t*)(meeting + row * kLgApart + kLgApart / 2);
+        __hip_atomic_fetch_max(best, (unsigned long long)k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (__hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (uint32_t)slices - 1) return;
+        asm volatile("" ::: "memory");
+        k = __hip_atomic_load(best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(best, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       tokens[row] = lg_token(k);
     }
   }
 }
 
-// Slices: of 8192 tokens, whose counts leave room for four workgroups a compute unit; of 2048 while the batch has too few
-// of those to fill the card.
-int logits_slice(int64_t rows, int64_t vocab) { return rows * ((vocab + 8191) / 8192) >= 512 ? 8192 : 2048; }
+// Slices of 16384 logits by 1024 threads: a row's history is read by few workgroups, of which two fill a compute unit (64
+// rows of 128256 with 4096 tokens each: 15.0 us, in slices of 4096 by 256 threads 17.9); of 2048 by 256 while the batch has
+// too few of those for the card.
+bool logits_large(int64_t rows, int64_t vocab) { return rows * ((vocab + 16383) / 16384) >= 256; }
 
-int logits_args(const spectra_logits_t* l, LogitsArgs* out, size_t* lds) {
+int logits_args(const spectra_logits_t* l, LogitsArgs* out, size_t* lds, int* threads, int* slices, bool* wide) {
   SPECTRA_REQUIRE(l != nullptr && l->logits, "NULL pointer");
   SPECTRA_REQUIRE(l->dtype == SPECTRA_F16 || l->dtype == SPECTRA_BF16 || l->dtype == SPECTRA_F32, "unknown dtype");
   SPECTRA_REQUIRE(l->rows > 0 && l->rows <= 65535 && l->vocab > 0 && l->vocab < (1LL << 31), "rows or vocab out of range");
@@ -255,8 +321,14 @@ int logits_args(const spectra_logits_t* l, LogitsArgs* out, size_t* lds) {
   a.ldallowed = l->allowed_ld;
   a.states = l->states;
   a.state = l->state;
-  a.slice = logits_slice(l->rows, l->vocab);
-  *lds = (size_t)a.slice * 4 * ((counts ? 1 : 0) + (a.biases > 0 ? 1 : 0));
+  const bool large = logits_large(l->rows, l->vocab);
+  const int slice = large ? 16384 : 2048;
+  *threads = large ? 1024 : 256;
+  *slices = (int)((l->vocab + slice - 1) / slice);
+  *wide = a.hist > (int)LgWord<uint32_t>::count || a.biases >= 65535;
+  *lds = 0;
+  if (counts || a.biases > 0)
+    *lds = lg_zero(slice, *wide ? 8 : 4) + 2 * std::min<int64_t>(slice, (int64_t)a.hist + a.biases);
   *out = a;
   return SPECTRA_OK;
 }
@@ -278,11 +350,16 @@ int logits_apart(const spectra_logits_t* l, const PagedRegion& written, const Pa
                       {"allowed_rows", l->state, 4LL * l->rows, 0, 1}});
 }
 
-template <bool PICK>
+template <bool PICK, int TH, int C, typename W>
 static const void* logits_of(int dtype) {
-  return dtype == SPECTRA_F16    ? (const void*)logits_kernel<SPECTRA_F16, PICK>
-         : dtype == SPECTRA_BF16 ? (const void*)logits_kernel<SPECTRA_BF16, PICK>
-                                 : (const void*)logits_kernel<SPECTRA_F32, PICK>;
+  return dtype == SPECTRA_F16    ? (const void*)logits_kernel<SPECTRA_F16, PICK, TH, C, W>
+         : dtype == SPECTRA_BF16 ? (const void*)logits_kernel<SPECTRA_BF16, PICK, TH, C, W>
+                                 : (const void*)logits_kernel<SPECTRA_F32, PICK, TH, C, W>;
+}
+template <bool PICK>
+static const void* logits_of(int dtype, int threads, bool wide) {
+  if (wide) return threads == 256 ? logits_of<PICK, 256, 1, unsigned long long>(dtype) : logits_of<PICK, 1024, 2, unsigned long long>(dtype);
+  return threads == 256 ? logits_of<PICK, 256, 1, uint32_t>(dtype) : logits_of<PICK, 1024, 2, uint32_t>(dtype);
 }
 
 }  // namespace spectra
@@ -292,31 +369,33 @@ using namespace spectra;
 extern "C" int spectra_adjust_logits(const spectra_logits_t* l, void* out, int64_t ldo, spectra_stream_t stream) {
   LogitsArgs a;
   size_t lds;
-  if (int st = logits_args(l, &a, &lds); st != SPECTRA_OK) return st;
+  int threads, slices;
+  bool wide;
+  if (int st = logits_args(l, &a, &lds, &threads, &slices, &wide); st != SPECTRA_OK) return st;
   const int es = elem_size(l->dtype);
   SPECTRA_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % es == 0, "out missing or not aligned");
   SPECTRA_REQUIRE(ldo >= l->vocab || l->rows == 1, "out's row stride too small");
   const bool in_place = out == l->logits && (ldo == l->ld || l->rows == 1);
   if (int st = logits_apart(l, {"out", out, l->vocab * es, ldo * es, l->rows}, {"", nullptr, 0, 0, 1}, in_place); st != SPECTRA_OK) return st;
-  const void* kern = logits_of<false>(l->dtype);
+  const void* kern = logits_of<false>(l->dtype, threads, wide);
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
-  int slices = (int)((l->vocab + a.slice - 1) / a.slice);
   int64_t* tokens = nullptr;
-  unsigned long long* best = nullptr;
-  uint32_t* arrived = nullptr;
-  void* args[] = {(void*)&a, (void*)&out, (void*)&ldo, (void*)&tokens, (void*)&slices, (void*)&best, (void*)&arrived};
-  SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)slices, (unsigned)l->rows), dim3(kLgThreads), args, lds, (hipStream_t)stream));
+  uint8_t* meeting = nullptr;
+  void* args[] = {(void*)&a, (void*)&out, (void*)&ldo, (void*)&tokens, (void*)&slices, (void*)&meeting};
+  SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)slices, (unsigned)l->rows), dim3((unsigned)threads), args, lds, (hipStream_t)stream));
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
 }
 
-extern "C" size_t spectra_next_tokens_workspace(void) { return (size_t)kLgRows * 16; }
+extern "C" size_t spectra_next_tokens_workspace(void) { return (size_t)kLgRows * kLgApart; }
 
 extern "C" int spectra_next_tokens(const spectra_logits_t* l, int64_t* tokens, void* workspace, size_t workspace_bytes,
                                    spectra_stream_t stream) {
   LogitsArgs a;
   size_t lds;
-  if (int st = logits_args(l, &a, &lds); st != SPECTRA_OK) return st;
+  int threads, slices;
+  bool wide;
+  if (int st = logits_args(l, &a, &lds, &threads, &slices, &wide); st != SPECTRA_OK) return st;
   SPECTRA_REQUIRE(tokens != nullptr && reinterpret_cast<uintptr_t>(tokens) % 8 == 0, "tokens missing or not aligned");
   SPECTRA_REQUIRE(l->rows <= kLgRows, "too many rows");
   if (workspace == nullptr || workspace_bytes < spectra_next_tokens_workspace())
@@ -326,15 +405,13 @@ extern "C" int spectra_next_tokens(const spectra_logits_t* l, int64_t* tokens, v
                             {"the workspace", workspace, (int64_t)spectra_next_tokens_workspace(), 0, 1}, false);
       st != SPECTRA_OK)
     return st;
-  const void* kern = logits_of<true>(l->dtype);
+  const void* kern = logits_of<true>(l->dtype, threads, wide);
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
-  int slices = (int)((l->vocab + a.slice - 1) / a.slice);
-  unsigned long long* best = (unsigned long long*)workspace;
-  uint32_t* arrived = (uint32_t*)(best + kLgRows);
+  uint8_t* meeting = (uint8_t*)workspace;
   void* out = nullptr;
   int64_t ldo = 0;
-  void* args[] = {(void*)&a, (void*)&out, (void*)&ldo, (void*)&tokens, (void*)&slices, (void*)&best, (void*)&arrived};
-  SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)slices, (unsigned)l->rows), dim3(kLgThreads), args, lds, (hipStream_t)stream));
+  void* args[] = {(void*)&a, (void*)&out, (void*)&ldo, (void*)&tokens, (void*)&slices, (void*)&meeting};
+  SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)slices, (unsigned)l->rows), dim3((unsigned)threads), args, lds, (hipStream_t)stream));
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;
 }

@@ -7,8 +7,8 @@
 // codes.
 //
 // With axes (AXES) the pairs of a head turn by positions of their own: pair i by row positions[axis[i]][t] of the tables
-// (images and video: time, height and width), while the cache's row stays the sequence's position.  A lane's 8 pairs
-// mostly have one axis and so one run of the table; where they do not, the angles are gathered.
+// (images and video: time, height and width), while the cache's row stays the sequence's position.  A wave gathers its
+// token's angles once, a pair a lane, and its heads read them from LDS.
 //
 // A pass over the rows: 8 rotation pairs (two 16-byte loads and stores) or 8 values of v a lane.
 // The waves of a token are its own, so its sequence, position and page are found once a wave, by
@@ -41,7 +41,7 @@ __device__ __forceinline__ void unpack8t(const uint4& u, float (&f)[8]) {
 struct PagedAxes {
   const int* pos;  // [axes][tokens], rows `stride` apart
   int64_t stride;
-  const uint8_t* axis;  // [head_dim / 2]; a pair of an axis past the last stays as it is
+  const uint8_t* axis;  // [head_dim / 2]; a pair whose axis is past the last stays as it is
   int axes;
 };
 
@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
                                                                   const float* __restrict__ sin_t, int64_t rope_rows,
                                                                   int heads, int hd, int waves, const PagedKv kv,
                                                                   uint16_t* __restrict__ q_rot, const PagedAxes ax) {
+  __shared__ __align__(16) float angles[AXES ? kPaThreads / 64 : 1][128];  // a wave's token's cosines and sines
   // neighbouring blocks go to different XCDs: an eighth of the tokens each, so that rows beside each
   // other meet in one L2 (4-bit rows are less than a line)
   const uint32_t run = gridDim.x < 64 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
@@ -70,19 +71,31 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
     a = *(const uint4*)src;
     if (rot) b = *(const uint4*)(src + h2);
   }
+  int axis = 255;  // of the lane's pair
+  if constexpr (AXES) {
+    if (lane < h2) axis = ax.axis[lane];
+  }
   const int seq = paged_find(kv.q_start, kv.batch, t, lane);
   if (seq >= kv.batch) return;  // behind the last sequence: left alone
   const PagedSeq sq = paged_seq(sload(kv.q_start + seq), sload(kv.q_start + seq + 1), sload(kv.lens + seq), kv.tokens);
   const int pos = sq.len - sq.n + (t - sq.q0);
-  int at[kPagedAxes];  // the token's rows of the tables
   bool turn = cos_t == nullptr || (pos >= 0 && pos < rope_rows);
+  uint64_t turned = 0;  // pairs that turn
   if constexpr (AXES) {
     turn = true;
+    int64_t row = 0;  // of the table, the lane's pair's
 #pragma unroll
-    for (int a = 0; a < kPagedAxes; ++a) {
-      at[a] = a < ax.axes ? sload(ax.pos + a * ax.stride + t) : 0;
-      turn = turn && at[a] >= 0 && at[a] < rope_rows;
+    for (int e = 0; e < kPagedAxes; ++e) {
+      const int at = e < ax.axes ? sload(ax.pos + e * ax.stride + t) : 0;
+      turn = turn && at >= 0 && at < rope_rows;
+      row = axis == e ? at : row;
     }
+    turned = __ballot(axis < ax.axes);
+    if (turn && lane < h2) {  // (a wave's own: read back behind the wave's own wait)
+      angles[threadIdx.x >> 6][lane] = cos_t[row * h2 + lane];
+      angles[threadIdx.x >> 6][64 + lane] = sin_t[row * h2 + lane];
+    }
+    __builtin_amdgcn_wave_barrier();
   }
   int page = -1;
   if (turn && pos >= 0 && (pos >> kv.page_shift) < kv.table_width)
@@ -93,34 +106,19 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const uint16_t
     uint4 lo = a, hi = b;
     if (cos_t != nullptr && turn) {
       float c[8], s[8], x[8], y[8];
-      int64_t from = pos;
-      bool run = true;     // the pairs' angles are one run of the table
       uint32_t still = 0;  // pairs that do not turn (not by an angle of 0: its product with an infinite partner is NaN)
       if constexpr (AXES) {
-        const uint2 ids = *(const uint2*)(ax.axis + i);
-        const uint32_t first = ids.x & 255u;
-        run = ids.x == first * 0x01010101u && ids.y == ids.x && first < (uint32_t)ax.axes;
-        from = at[0];
-#pragma unroll
-        for (int a = 1; a < kPagedAxes; ++a) from = first == (uint32_t)a ? at[a] : from;
-        if (!run) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t id = ((e < 4 ? ids.x : ids.y) >> (8 * (e & 3))) & 255u;
-            int64_t row = at[0];
-#pragma unroll
-            for (int a = 1; a < kPagedAxes; ++a) row = id == (uint32_t)a ? at[a] : row;
-            c[e] = cos_t[row * h2 + i + e];
-            s[e] = sin_t[row * h2 + i + e];
-            still |= (id < (uint32_t)ax.axes ? 0u : 1u) << e;
-          }
-        }
-      }
-      if (run) {
-        *(float4*)c = *(const float4*)(cos_t + from * h2 + i);
-        *(float4*)(c + 4) = *(const float4*)(cos_t + from * h2 + i + 4);
-        *(float4*)s = *(const float4*)(sin_t + from * h2 + i);
-        *(float4*)(s + 4) = *(const float4*)(sin_t + from * h2 + i + 4);
+        const float* mine = angles[threadIdx.x >> 6];
+        *(float4*)c = *(const float4*)(mine + i);
+        *(float4*)(c + 4) = *(const float4*)(mine + i + 4);
+        *(float4*)s = *(const float4*)(mine + 64 + i);
+        *(float4*)(s + 4) = *(const float4*)(mine + 64 + i + 4);
+        still = (uint32_t)(turned >> i) & 255u ^ 255u;
+      } else {
+        *(float4*)c = *(const float4*)(cos_t + (int64_t)pos * h2 + i);
+        *(float4*)(c + 4) = *(const float4*)(cos_t + (int64_t)pos * h2 + i + 4);
+        *(float4*)s = *(const float4*)(sin_t + (int64_t)pos * h2 + i);
+        *(float4*)(s + 4) = *(const float4*)(sin_t + (int64_t)pos * h2 + i + 4);
       }
       unpack8t<BF>(a, x);
       unpack8t<BF>(b, y);
@@ -303,8 +301,7 @@ int append(const spectra_paged_kv_t* kv, const void* qkv, int64_t ldqkv, int64_t
     SPECTRA_REQUIRE(ax.pos && ax.axis && cos_t, "NULL pointer");
     SPECTRA_REQUIRE(ax.axes >= 1 && ax.axes <= kPagedAxes, "one to four axes");
     SPECTRA_REQUIRE(ax.stride >= tokens || ax.axes == 1, "positions' row stride too small");
-    SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(ax.pos) % 4 == 0 && reinterpret_cast<uintptr_t>(ax.axis) % 8 == 0,
-                    "positions must be aligned, the pairs' axes to 8 bytes");
+    SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(ax.pos) % 4 == 0, "positions must be aligned");
   }
   const PagedPools pools = paged_pools(kv);
   const int64_t turned = 2 * std::min<int64_t>(rope_rows, 1LL << 31) * hd;  // bytes of each table that positions name

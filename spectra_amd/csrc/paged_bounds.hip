@@ -10,9 +10,12 @@
 // A page with a key that is not finite has codes of 0 and the scale infinity (the selection takes it first, so that the
 // attention shows what is wrong); one whose largest magnitude is below 2^-100, codes and scale of 0.
 //
-// A wave a page and KV head: a row is 16 lanes (head size 128) or 8, so 4 or 8 rows a load of 1 KB, eight
-// loads in flight; rows meet across the lanes at the end.  No LDS, no workspace.
+// A wave a page and KV head: a row is 16 lanes (head size 128) or 8, so 4 or 8 rows a load of 1 KB, four or eight
+// loads in flight; rows meet across the lanes at the end.  Values are compared as pairs of 16-bit integers of the same
+// order (five instructions for two; as fp32 values, eighteen), in which infinities and NaN end up at the ends, so that
+// the maxima show them.  No LDS, no workspace.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attend.h"
 
@@ -20,6 +23,41 @@ namespace spectra {
 
 constexpr int kPbThreads = 256;
 constexpr float kPbLeast = 7.8886091e-31f;  // 2^-100
+
+typedef int16_t ps2_t __attribute__((ext_vector_type(2)));
+
+// A pair of fp16 or bf16 values as integers of their order, and back (its own inverse).
+__device__ __forceinline__ ps2_t pb_order(uint32_t x) {
+  const ps2_t v = __builtin_bit_cast(ps2_t, x);
+  return v ^ ((v >> 15) & (ps2_t){0x7fff, 0x7fff});
+}
+
+// Eight dims 8 c .. of a row: 16-bit values, or codes with their group's zero point and scale.
+struct PbGroup {
+  uint32_t zero, scale;
+};
+template <int HD, int KIND>
+__device__ __forceinline__ uint4 pb_load(const PagedKv& kv, int page, int64_t row, int c, PbGroup& g) {
+  const uint8_t* p = kv.k + paged_at(page, kv.page_step);
+  if constexpr (KIND == kKv4) {
+    g.scale = *(const uint16_t*)(kv.ks + paged_at(page, kv.scale_step) + 2 * (row * (HD / 32) + c / 4));
+    g.zero = kv.kz[paged_at(page, kv.zero_step) + row * (HD / 32) + c / 4];
+    return make_uint4(*(const uint32_t*)(p + row * (HD / 2) + 4 * c), 0, 0, 0);
+  } else {
+    return *(const uint4*)(p + (row * HD + 8 * c) * 2);
+  }
+}
+// Their bits as pairs: 2 e and 2 e + 1, of 4 bits e and e + 4.  (An infinite or NaN scale gives infinities and NaN.)
+template <int KIND>
+__device__ __forceinline__ pu4_t pb_values(const uint4& x, const PbGroup& g) {
+  if constexpr (KIND == kKv4) return kv4_pairs(x.x, kv4_zero(g.zero | g.zero << 16), __builtin_bit_cast(ph2_t, g.scale | g.scale << 16));
+  else return (pu4_t){x.x, x.y, x.z, x.w};
+}
+template <int LB>
+__device__ __forceinline__ void pb_meet(ps2_t& hi, ps2_t& lo, int lane) {
+  hi = __builtin_elementwise_max(hi, __builtin_bit_cast(ps2_t, lane_xor<LB>(__builtin_bit_cast(float, hi), lane)));
+  lo = __builtin_elementwise_min(lo, __builtin_bit_cast(ps2_t, lane_xor<LB>(__builtin_bit_cast(float, lo), lane)));
+}
 
 // Pages that a sequence's tokens of the call lie in: the first, and how many.
 struct PagedTouched {
@@ -36,7 +74,8 @@ template <int HD, int KIND>
 __global__ void __launch_bounds__(kPbThreads) paged_bounds_kernel(const PagedKv kv, int8_t* __restrict__ codes,
                                                                   int64_t code_step, float* __restrict__ scales,
                                                                   int64_t scale_step, int units) {
-  constexpr int CH = HD / 8, G = 64 / CH, U = 8;  // lanes a row, rows a load, loads in flight
+  constexpr int CH = HD / 8, G = 64 / CH;  // lanes a row, rows a load
+  constexpr bool BF = KIND == kKvBf16;
   const int lane = threadIdx.x & 63, c = lane % CH, rg = lane / CH;
   const int u = sread((int)(blockIdx.x * (kPbThreads / 64) + (threadIdx.x >> 6)));
   if (u >= units) return;
@@ -62,46 +101,66 @@ __global__ void __launch_bounds__(kPbThreads) paged_bounds_kernel(const PagedKv 
   const int len = sload(kv.lens + seq), page = sload(kv.table + seq * kv.table_stride + block);
   if ((uint32_t)page >= (uint32_t)kv.num_pages) return;
   const int rows = min(len - (block << kv.page_shift), 1 << kv.page_shift);  // >= 1
-  float hi[8], lo[8];
+  // pairs of 16-bit values as integers of the same order, infinities and NaN at its ends
+  ps2_t hi[4], lo[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    hi[e] = -INFINITY;
-    lo[e] = INFINITY;
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = (ps2_t){-32768, -32768};
+    lo[e] = (ps2_t){32767, 32767};
   }
-  uint32_t most = 0;  // of the magnitudes' bits: infinity's 0x7f800000, NaNs' past it
   const int64_t first = (int64_t)kvh << kv.page_shift;
-  for (int r0 = 0; r0 < rows; r0 += G * U) {
-    float x[U][8];
+  auto take = [&](int r0, auto n) __attribute__((always_inline)) {
+    constexpr int U = decltype(n)::value;
+    uint4 x[U];
+    PbGroup z[U];
 #pragma unroll
     for (int i = 0; i < U; ++i)  // (past the last row: the last once more)
-      paged_eight<HD, KIND>(kv, false, page, first + min(r0 + G * i + rg, rows - 1), c, x[i]);
+      x[i] = pb_load<HD, KIND>(kv, page, first + min(r0 + G * i + rg, rows - 1), c, z[i]);
 #pragma unroll
-    for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i) {
+      const pu4_t y = pb_values<KIND>(x[i], z[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        hi[e] = fmaxf(hi[e], x[i][e]);
-        lo[e] = fminf(lo[e], x[i][e]);
-        most = max(most, __builtin_bit_cast(uint32_t, x[i][e]) & 0x7fffffffu);
+      for (int e = 0; e < 4; ++e) {
+        const ps2_t v = pb_order(y[e]);
+        hi[e] = __builtin_elementwise_max(hi[e], v);
+        lo[e] = __builtin_elementwise_min(lo[e], v);
       }
+    }
+  };
+  if (rows <= 4 * G) {
+    take(0, std::integral_constant<int, 4>());
+  } else {
+    for (int r0 = 0; r0 < rows; r0 += 8 * G) take(r0, std::integral_constant<int, 8>());
   }
 #pragma unroll
-  for (int off = CH; off < 64; off *= 2)
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (CH == 8) pb_meet<8>(hi[e], lo[e], lane);
+    pb_meet<16>(hi[e], lo[e], lane);
+    pb_meet<32>(hi[e], lo[e], lane);
+  }
+  // back to the values' bits; the largest magnitude
+  uint32_t most = 0;
+  uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], off, 64));
-      lo[e] = fminf(lo[e], __shfl_xor(lo[e], off, 64));
-    }
+  for (int e = 0; e < 4; ++e) {
+    h[e] = __builtin_bit_cast(uint32_t, pb_order(__builtin_bit_cast(uint32_t, hi[e])));
+    l[e] = __builtin_bit_cast(uint32_t, pb_order(__builtin_bit_cast(uint32_t, lo[e])));
+    for (const uint32_t m : {h[e] & 0x7fff7fffu, l[e] & 0x7fff7fffu}) most = max(most, max(m & 0xffffu, m >> 16));
+  }
 #pragma unroll
-  for (int off = 1; off < 64; off *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
-  const float a = __builtin_bit_cast(float, most);
-  const bool odd = most >= 0x7f800000u, none = odd || a < kPbLeast;
+  for (int off = 1; off < CH; off *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
+  const float a = BF ? bf2f((uint16_t)most) : h2f((uint16_t)most);
+  const bool odd = most >= (BF ? 0x7f80u : 0x7c00u), none = odd || a < kPbLeast;
   const float inv = none ? 0.0f : 127.0f / a;
   uint32_t up[2] = {0, 0}, dn[2] = {0, 0};
   if (!none) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int m = (int)fminf(fmaxf(__builtin_ceilf(hi[e] * inv), -127.0f), 127.0f);
-      const int n = (int)fminf(fmaxf(__builtin_floorf(lo[e] * inv), -127.0f), 127.0f);
+      const int at = KIND == kKv4 ? e & 3 : e >> 1, half = 16 * (KIND == kKv4 ? e >> 2 : e & 1);
+      const uint16_t hb = (uint16_t)(h[at] >> half), lb = (uint16_t)(l[at] >> half);
+      const float hf = BF ? bf2f(hb) : h2f(hb), lf = BF ? bf2f(lb) : h2f(lb);
+      const int m = (int)fminf(fmaxf(__builtin_ceilf(hf * inv), -127.0f), 127.0f);
+      const int n = (int)fminf(fmaxf(__builtin_floorf(lf * inv), -127.0f), 127.0f);
       up[e >> 2] |= (uint32_t)(m & 255) << (8 * (e & 3));
       dn[e >> 2] |= (uint32_t)(n & 255) << (8 * (e & 3));
     }

@@ -40,13 +40,13 @@ at::Tensor axes_append(const at::Tensor& qkv_in, const at::Tensor& positions_in,
                           t->size(1) == d / 2 && t->is_contiguous() && t->device() == dev,
                       "cos and sin must be contiguous fp32 [rows, d / 2], at least a row, on ", dev);
   const c10::DeviceGuard guard(dev);
-  // rows are read 16 bytes at a time, the pairs' axes 8
+  // rows are read 16 bytes at a time
   if (qkv.stride(1) != 1 || (tokens > 1 && (qkv.stride(0) < width || qkv.stride(0) % 8 != 0)) ||
       reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 != 0)
     qkv = qkv.clone(at::MemoryFormat::Contiguous);
   if ((tokens > 1 && positions.stride(1) != 1) || (positions.size(0) > 1 && positions.stride(0) < tokens))
     positions = positions.clone(at::MemoryFormat::Contiguous);
-  if (axis.stride(0) != 1 || reinterpret_cast<uintptr_t>(axis.data_ptr()) % 8 != 0) axis = axis.clone(at::MemoryFormat::Contiguous);
+  if (axis.stride(0) != 1) axis = axis.clone(at::MemoryFormat::Contiguous);
   at::Tensor q;
   if (q_out != nullptr) {
     check_out(*q_out, qkv, tokens, heads, d, "q_out");
