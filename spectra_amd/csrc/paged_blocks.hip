@@ -7,9 +7,10 @@
 // they lie; V turned by byte permutes; 4-bit pages through LDS).  All rows of a tile, up to 16 query heads of one token
 // and KV head, see the same keys, so none has to be computed by itself.
 //
-// Tiles have `count` pages at most, the same for all, so the line of their key steps (128 keys) is shared out by
-// arithmetic: as many workgroups as are resident at once take equal runs of it, whole tiles and at most two parts; the
-// parts of a tile meet in the workspace, where the last to arrive joins them in the order of their keys.
+// As many workgroups as are resident at once share the tiles' key steps (of 128 keys) evenly (PagedWalk, by the sequences'
+// lengths and `count`): whole tiles and at most two parts each; the parts of a tile meet in the workspace, where the last
+// to arrive joins them in the order of their keys.  (Shares by `count` alone: 64 users of 100 to 2000 keys with room for
+// 4096 took 105 us, not 73.)
 //
 // Bound by reading the listed pages.  Roundings: the weights to the activations' 16 bits for the product with V, 4-bit
 // values to fp16, the output.
@@ -18,6 +19,11 @@
 namespace spectra {
 
 constexpr int kBlkThreads = 256, kBlkKeys = 128;
+
+// Workgroups a compute unit.  (Three fit the registers of the 64-dim kernels and, with spills, of the 4-bit ones: drafts on 4
+// bits 33.0 us, not 28.3, 64 users of 64 dims 116, not 110.)
+constexpr int kBlkResident = 2;
+static_assert(2 * 256 * kBlkResident * 16 <= kFewSlotRows && 8 * 256 * kBlkResident <= SPECTRA_PAGED_COUNTER_BYTES, "two records and counters a workgroup");
 
 // 32 keys of 16-bit K and V as they lie.
 template <int HD>
@@ -45,10 +51,10 @@ struct BlkHalf {
 };
 
 template <int HD, int KIND, int MOD>
-__global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
+__global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     paged_blocks_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
-                        const int* __restrict__ blocks, int count, int tiles_a_token, int64_t steps_a_tile, PagedLine line0,
-                        uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
+                        const int* __restrict__ blocks, int count, bool wide, int apart,
+                         uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
   constexpr int ROWS = 16, KS = HD / 32, DPL = HD / 16, RS = HD + 4;
   constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;  // bytes of a row of a page
@@ -57,24 +63,35 @@ __global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
   __shared__ float wm[4][ROWS], wl[4][ROWS];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), c = lane & 15, q4 = lane >> 4;
-  const int S = (int)steps_a_tile;
-  PagedLine line = line0;
-  line.begin = line.start(blockIdx.x);
-  line.end = line.start(blockIdx.x + 1);
-  const int pmask = (1 << kv.page_shift) - 1;
-  for (int x = line.begin; x < line.end;) {
-    const int tile = (int)((uint32_t)x / (uint32_t)S), from = x - tile * S, t0 = x - from;
-    const int to = min(S, from + line.end - x);
-    const bool whole = from == 0 && to == S;
-    const int tok = sread(tile / tiles_a_token), ht = tile - tok * tiles_a_token;  // (heads of a token beside each other)
-    const int groups = (g + 15) / 16, kvh = sread(ht / groups), h0 = sread(kvh * g + 16 * (ht - kvh * groups));
+  const int pmask = (1 << kv.page_shift) - 1, groups = (g + 15) / 16;
+  // neighbouring workgroups go to different XCDs: an eighth of the line each, so that the tokens of a sequence and KV head,
+  // whose lists have pages in common, meet in one L2
+  const int share = (gridDim.x & 7) != 0 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  PagedKv line = kv;  // (for the walk: rows are tokens, heads their tiles)
+  line.kv_heads = kv.kv_heads * groups;
+  PagedScore most{};
+  most.window = count << kv.page_shift;
+  PagedWalk<Wave> walk(line, 1, 1, -16, kBlkKeys, most, share, gridDim.x, wide, lane);
+  PagedPart un;
+  for (int x = walk.line.begin; x < walk.line.end && walk.part(x, un); x = un.t0 + un.to) {
+    const int tok = un.seq.q0 + un.tile, kvh = sread(un.kvh / groups), h0 = sread(kvh * g + 16 * (un.kvh - kvh * groups));
     const int nrows = min(16, (kvh + 1) * g - h0);
-    x += to - from;
-    const int seq = paged_find(kv.q_start, kv.batch, tok, lane);
-    if (seq >= kv.batch) continue;  // behind the last sequence: left alone
-    const PagedSeq sq = paged_seq(sload(kv.q_start + seq), sload(kv.q_start + seq + 1), sload(kv.lens + seq), kv.tokens);
-    const int pos = sq.len - sq.n + (tok - sq.q0);  // the row's position: it sees the keys up to that
+    const int pos = un.seq.len - un.seq.n + un.tile;  // the row's position: it sees the keys up to that
     const bool past = pos >= kv.table_width << kv.page_shift;
+    const bool whole = un.from == 0 && un.to == un.steps;
+    // the list up to its last entry, and this part of it
+    const int* list = blocks + ((int64_t)tok * kv.kv_heads + kvh) * count;
+    int extent = 0;
+    for (int s0 = 0; s0 < count; s0 += 64) {
+      const uint64_t some = __ballot(s0 + lane < count && list[min(s0 + lane, count - 1)] >= 0);
+      if (some != 0) extent = s0 + 64 - __builtin_clzll(some);
+    }
+    const int keys = extent << kv.page_shift, steps = (keys + kBlkKeys - 1) / kBlkKeys;
+    int sbeg = un.from, send = un.to;
+    if (steps != un.steps) {  // (the line counted by the length)
+      sbeg = sread((int)((uint64_t)(uint32_t)steps * (uint32_t)un.from / (uint32_t)un.steps));
+      send = sread((int)((uint64_t)(uint32_t)steps * (uint32_t)un.to / (uint32_t)un.steps));
+    }
 
     // the lane's row (column c): its queries, B operands
     const float slope2 = 0.0f;
@@ -91,16 +108,17 @@ __global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
       }
     }
 
-    // ---- loads: the list's entries two tiles ahead of their rows, page ids one, rows a tile ahead of their use
-    const int* list = blocks + ((int64_t)tok * kv.kv_heads + kvh) * count;
-    const int* tab = kv.table + seq * kv.table_stride;
-    const int last = count - 1;
-    auto listed = [&](int key) __attribute__((always_inline)) { return sread(sload(list + min(key >> kv.page_shift, last))); };
-    // the 16 keys from `key` of the list on, in block b of the sequence
-    auto half_of = [&](int key, int b) __attribute__((always_inline)) {
+    // ---- loads: rows a tile ahead of their use, the pages' ids two, the list's entries three
+    const int* tab = kv.table + un.b * kv.table_stride;
+    const int last = extent - 1;
+    auto listed = [&](int key) __attribute__((always_inline)) { return sload(list + max(min(key >> kv.page_shift, last), 0)); };
+    auto page_of = [&](int b) __attribute__((always_inline)) {
+      return sload(tab + ((uint32_t)b < (uint32_t)kv.table_width ? b : 0));
+    };
+    // the 16 keys from `key` of the list on, in block b of the sequence, whose page has this id
+    auto half_of = [&](int key, int b, int id) __attribute__((always_inline)) {
       BlkHalf h;
       const bool there = (key >> kv.page_shift) <= last && (uint32_t)b < (uint32_t)kv.table_width;
-      const int id = sread(sload(tab + (there ? b : 0)));
       h.seen = there ? min(max(pos + 1 - ((b << kv.page_shift) + (key & pmask)), 0), 16) : 0;
       h.bad = (uint32_t)id >= (uint32_t)kv.num_pages;
       h.page = h.bad || !there ? 0 : id;
@@ -285,52 +303,67 @@ __global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
       }
     };
 
-    const int kend = min(to * kBlkKeys, count << kv.page_shift);  // (of the list's keys)
-    int key = from * kBlkKeys + 32 * wave;
+    const int kend = min(send * kBlkKeys, keys);  // (of the list's keys)
+    int key = sbeg * kBlkKeys + 32 * wave;
     if (key < kend) {
-      int l0 = listed(key), l1 = listed(key + 16);
-      BlkHalf h0_[2] = {half_of(key, l0), half_of(key + 16, l1)}, h1_[2];
-      l0 = listed(key + kBlkKeys);
-      l1 = listed(key + kBlkKeys + 16);
-      // the next tile's halves, and the list's entries after them
+      // blocks and ids of the next tile's halves, blocks of the one after it
+      int b0 = listed(key), b1 = listed(key + 16), m0 = listed(key + kBlkKeys), m1 = listed(key + kBlkKeys + 16);
+      int id0 = page_of(b0), id1 = page_of(b1);
       auto next = [&](BlkHalf (&hf)[2], int k) __attribute__((always_inline)) {
-        hf[0] = half_of(k, l0);
-        hf[1] = half_of(k + 16, l1);
-        l0 = listed(k + kBlkKeys);
-        l1 = listed(k + kBlkKeys + 16);
+        hf[0] = half_of(k, b0, id0);
+        hf[1] = half_of(k + 16, b1, id1);
       };
+      auto ahead = [&](int k) __attribute__((always_inline)) {  // k: the tile after the next
+        b0 = m0;
+        b1 = m1;
+        id0 = page_of(b0);
+        id1 = page_of(b1);
+        m0 = listed(k + kBlkKeys);
+        m1 = listed(k + kBlkKeys + 16);
+      };
+      BlkHalf ha[2], hb[2];
+      next(ha, key);
       if constexpr (Q4) {
         uint8_t* mine = pool + wave * 2 * C::kBytes;
         const uint32_t at0 = (uint32_t)(uintptr_t)(lds_t)mine;
-        fetch(at0, key, h0_);
-        next(h1_, key + kBlkKeys);
+        fetch(at0, key, ha);
+        ahead(key + kBlkKeys);
         for (int turn = 0;; turn ^= 1) {
           if (key + kBlkKeys < kend) {
-            fetch(at0 + (turn ^ 1) * C::kBytes, key + kBlkKeys, h1_);
+            next(hb, key + kBlkKeys);
+            fetch(at0 + (turn ^ 1) * C::kBytes, key + kBlkKeys, hb);
+            ahead(key + 2 * kBlkKeys);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::kCopies) : "memory");  // all but the next tile's
           } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
           }
-          compute(mine + turn * C::kBytes, h0_);
+          compute(mine + turn * C::kBytes, ha);
           key += kBlkKeys;
           if (key >= kend) break;
-          h0_[0] = h1_[0];
-          h0_[1] = h1_[1];
-          next(h1_, key + kBlkKeys);
+          ha[0] = hb[0];
+          ha[1] = hb[1];
         }
       } else {
+        // (the next tile is asked for behind the last one, too, whose rows it then has again: a branch around the loads would
+        // have the rows before them waited for as if they were the newest, 1.05 GB in 188 us, not 180)
         Tile ta, tb;
-        load(ta, key, h0_);
-        next(h1_, key + kBlkKeys);
+        load(ta, key, ha);
+        ahead(key + kBlkKeys);
+        auto beside = [&](BlkHalf (&hf)[2], const BlkHalf (&now)[2], Tile& t) __attribute__((always_inline)) {
+          const bool more = key + kBlkKeys < kend;
+          next(hf, key + kBlkKeys);
+          hf[0].page = more ? hf[0].page : now[0].page;
+          hf[1].page = more ? hf[1].page : now[1].page;
+          load(t, key + kBlkKeys, hf);
+          ahead(key + 2 * kBlkKeys);
+        };
         while (true) {
-          if (key + kBlkKeys < kend) load(tb, key + kBlkKeys, h1_);
-          compute(ta, h0_);
-          next(h0_, key + 2 * kBlkKeys);
+          beside(hb, ha, tb);
+          compute(ta, ha);
           key += kBlkKeys;
           if (key >= kend) break;
-          if (key + kBlkKeys < kend) load(ta, key + kBlkKeys, h0_);
-          compute(tb, h1_);
-          next(h1_, key + 2 * kBlkKeys);
+          beside(ha, hb, ta);
+          compute(tb, hb);
           key += kBlkKeys;
           if (key >= kend) break;
         }
@@ -345,7 +378,7 @@ __global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
       wm[wave][c] = m;
       wl[wave][c] = l;
     }
-    float* part = slots + (int64_t)line.record((int)blockIdx.x, t0 + from) * paged_slot<HD>(ROWS);
+    float* part = slots + (int64_t)walk.line.record(share, x) * paged_slot<HD>(ROWS);
     auto write = [&](int row, int d, const float (&v)[4], float den) __attribute__((always_inline)) {
       const float inv = past ? NAN : 1.0f / den;
       float y[4];
@@ -385,10 +418,10 @@ __global__ void __launch_bounds__(kBlkThreads, few_resident(KIND, HD, 16))
       }
     }
     if (!whole) {
-      const PagedCut cut(line, t0, S);
+      const PagedCut cut(walk.line, un.t0, un.steps);
       const int pieces = cut.pieces;
       auto slot_of = [&](int p) __attribute__((always_inline)) { return cut.record(p); };
-      if (paged_arrive(counters + cut.first, pieces, &flag)) {  // the last to arrive joins them
+      if (paged_arrive(counters + cut.first * apart, pieces, &flag)) {  // the last to arrive joins them
         for (int it = tid; it < nrows * (HD / 4); it += kBlkThreads) {
           const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
           float v[1][4];
@@ -449,22 +482,21 @@ extern "C" int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const v
   sc.cap2 = (float)(cap * log2e);
   SPECTRA_REQUIRE(sc.mul > 0.0f && sc.mul < 1e30f && sc.cap2 < 1e30f, "scale or cap out of range");
   const int mod = sc.cap2 > kPagedCap ? kModLargeCap : cap > 0.0f ? kMod : kModNone;
-  // the line of the tiles' steps, and its equal shares
-  int tiles_a_token = kv->kv_heads * ((g + 15) / 16);
-  int64_t steps = ((int64_t)count * kv->page_size + kBlkKeys - 1) / kBlkKeys;
-  const int64_t total = tokens * tiles_a_token * steps;
-  SPECTRA_REQUIRE(total < (1LL << 30), "tokens times listed keys out of range");
-  const int64_t groups = std::min<int64_t>(total, few_groups(kv->kind, hd, 16));
-  PagedLine line{};
-  line.total = (int)total;
-  line.each = (int)(total / groups);
-  line.more = (int)(total % groups);
+  // at most as many steps as the lists have
+  const int64_t tiles = tokens * kv->kv_heads * ((g + 15) / 16);
+  const int64_t total = tiles * (((int64_t)count * kv->page_size + kBlkKeys - 1) / kBlkKeys);
+  SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
+  const int64_t groups = std::min<int64_t>(total, 256 * kBlkResident);
+  bool wide = total >= (1LL << 29);
+  // (counters as far apart as there is room: atomics on one line wait for each other)
+  int apart = 1;
+  while (2 * apart * 2 * groups <= SPECTRA_PAGED_COUNTER_BYTES / 4 && apart < 64) apart *= 2;
   uint32_t* counters = (uint32_t*)workspace;
   float* slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
   int gv = g, hv = heads, cv = count;
   const void* kern = hd == 64 ? blocks_of<64>(kv->kind, mod) : blocks_of<128>(kv->kind, mod);
   void* args[] = {(void*)&p, (void*)&sc, (void*)&q, (void*)&ldq, (void*)&gv, (void*)&hv, (void*)&blocks, (void*)&cv,
-                  (void*)&tiles_a_token, (void*)&steps, (void*)&line, (void*)&counters, (void*)&slots, (void*)&out};
+                  (void*)&wide, (void*)&apart, (void*)&counters, (void*)&slots, (void*)&out};
   SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)groups), dim3(kBlkThreads), args, 0, (hipStream_t)stream));
   SPECTRA_HIP_CHECK(hipGetLastError());
   return SPECTRA_OK;

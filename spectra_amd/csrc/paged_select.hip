@@ -11,8 +11,8 @@
 // Scores are matrix products (16 x 16 x 64 of bytes): rows are query heads, padded to 4, 8 or 16 a token by copies of the
 // last one, so that a token's maximum lies in a lane's registers and at most two exchanges; columns are 16 pages, whose
 // 2 d bytes a lane reads as they lie.  Scores are kept in LDS as 32-bit keys in the scores' order; the `count`-th largest
-// is found by bisection of the keys between their least and largest (some 20 counts), ties by the order of the pages,
-// and the chosen are written in that order.
+// is found by counts of the keys in 256 parts of their range, and of the part's range again (two or three rounds), ties by
+// the order of the pages, and the chosen are written in that order.
 // A workgroup has one token (drafts and prompts: as many as fill the rows, whose pages are read once) and one KV head.
 // Few such units with long tables are split: workgroups score a run of pages each, and the last of a unit to arrive
 // chooses from the keys of all in the workspace.
@@ -25,9 +25,11 @@ namespace spectra {
 typedef int pi4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kSelMost = 32768;            // pages of a table
-constexpr int kSelLds = 160 * 1024 - 256;  // codes and keys of a workgroup
+constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;  // parts of a range that keys are counted in
+constexpr int kSelLds = 160 * 1024 - 512;  // codes, keys and counts of a workgroup
 constexpr int kSelSplit = 64;              // units whose pages are split among workgroups: at most as many
-constexpr size_t kSelCounters = 4 * kSelSplit;
+constexpr int kSelApart = 256;             // bytes from one unit's counter to the next one's (atomics on one line wait for each other)
+constexpr size_t kSelCounters = kSelApart * kSelSplit;
 constexpr uint32_t kSelForced = ~0u, kSelOdd = ~0u - 1;
 constexpr float kSelLeast = 7.8886091e-31f;  // 2^-100
 
@@ -48,16 +50,27 @@ __device__ __forceinline__ uint32_t sel_key(float s) {
   return u ^ (u >> 31 ? ~0u : 0x80000000u);
 }
 
+template <int LB>
+__device__ __forceinline__ uint32_t lane_xor_u(uint32_t v, int lane) {
+  return __builtin_bit_cast(uint32_t, lane_xor<LB>(__builtin_bit_cast(float, v), lane));
+}
+template <typename F>
+__device__ __forceinline__ uint32_t wave_meet(uint32_t v, F f) {
+  const int lane = __lane_id();
+  v = f(v, lane_xor_u<32>(v, lane));
+  v = f(v, lane_xor_u<16>(v, lane));
+  v = f(v, lane_xor_u<8>(v, lane));
+  v = f(v, lane_xor_u<4>(v, lane));
+  v = f(v, lane_xor_u<2>(v, lane));
+  return f(v, lane_xor_u<1>(v, lane));
+}
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
-  return v;
+  return wave_meet(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) v = min(v, (uint32_t)__shfl_xor((int)v, off, 64));
-  return v;
+  return wave_meet(v, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 __device__ __forceinline__ void store_dev1(uint32_t* p, uint32_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -70,107 +83,170 @@ __device__ __forceinline__ uint32_t load_dev1(const uint32_t* p) {
 // part of the keys.
 struct SelAlone {
   static constexpr int parts = 1, part = 0;
-  __device__ __forceinline__ int sum(int v) { return v; }
-  __device__ __forceinline__ int before(int, int) { return 0; }
-  __device__ __forceinline__ uint32_t most(uint32_t v) { return v; }
-  __device__ __forceinline__ uint32_t least(uint32_t v) { return v; }
+  uint32_t* bins;  // [2][kSelBins]
+  __device__ __forceinline__ void sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+  template <int N>
+  __device__ __forceinline__ void all(uint32_t (&v)[N], const uint32_t (&none)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __lane_id() == 0 ? v[i] : none[i];
+  }
 };
 struct SelTogether {
   int parts, part;
-  uint32_t* box;  // [2][16]
+  uint32_t* bins;
+  uint32_t* box;  // [2][3][16]
   int turn = 0;
-  // every wave's value, in lanes 0 .. parts - 1
-  __device__ __forceinline__ uint32_t all(uint32_t v, uint32_t none) {
-    uint32_t* b = box + 16 * turn;
-    turn ^= 1;  // (a wave that is a step ahead writes the other half)
-    if (__lane_id() == 0) b[part] = v;
-    __syncthreads();
+  __device__ __forceinline__ void sync() { __syncthreads(); }
+  // every wave's values, in lanes 0 .. parts - 1
+  template <int N>
+  __device__ __forceinline__ void all(uint32_t (&v)[N], const uint32_t (&none)[N]) {
+    uint32_t* b = box + 48 * turn;
+    turn ^= 1;
     const int lane = __lane_id();
-    return lane < parts ? b[lane & 15] : none;
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[16 * i + part] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lane < parts ? b[16 * i + (lane & 15)] : none[i];
   }
-  __device__ __forceinline__ int sum(int v) {
-    const int s = wave_scan((int)all((uint32_t)v, 0));
-    return __builtin_amdgcn_readlane(s, 63);
-  }
-  __device__ __forceinline__ int before(int v, int) {
-    const int s = wave_scan((int)all((uint32_t)v, 0));
-    return __builtin_amdgcn_readlane(s, part) - v;
-  }
-  __device__ __forceinline__ uint32_t most(uint32_t v) { return wave_most(all(v, 0)); }
-  __device__ __forceinline__ uint32_t least(uint32_t v) { return wave_least(all(v, ~0u)); }
 };
 
-// The `count` largest of n > count keys, the first on ties, written in their order.
+// The `count` largest of n > count keys, the first on ties, written in their order.  The range that holds the count-th
+// largest is narrowed by counting the keys in kSelBins equal parts of it; some two rounds leave as many keys as are
+// wanted, or keys that are all the same.
 template <typename W>
 __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, int* out, W w) {
   const int lane = __lane_id();
   const int each = ((n + w.parts - 1) / w.parts + 63) & ~63;
   const int from = min(each * w.part, n), to = min(from + each, n);
-  uint32_t hi = 0, lo = ~0u;
-  for (int j = from + lane; j < to; j += 64) {
-    hi = max(hi, key[j]);
-    lo = min(lo, key[j]);
-  }
-  hi = w.most(wave_most(hi));
-  lo = w.least(wave_least(lo));
-  auto at_least = [&](uint32_t t) __attribute__((always_inline)) {
-    int c = 0;
-    for (int j = from; j < to; j += 64) c += __builtin_popcountll(__ballot(j + lane < to && key[min(j + lane, to - 1)] >= t));
-    return w.sum(c);
+  // f of all keys of this part, a lane's each, the loads of four in flight together
+  auto over = [&](auto f) __attribute__((always_inline)) {
+    constexpr int U = 4;
+    for (int j0 = from; j0 < to; j0 += 64 * U) {
+      uint32_t k[U];
+#pragma unroll
+      for (int e = 0; e < U; ++e) k[e] = key[min(j0 + 64 * e + lane, to - 1)];
+#pragma unroll
+      for (int e = 0; e < U; ++e) f(k[e], j0 + 64 * e + lane < to, j0 + 64 * e + lane);
+    }
   };
-  // the largest t that at least `count` keys reach: lo is one that they do, hi one that they do not
-  if (at_least(hi) >= count) {
-    lo = hi;
-  } else {
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      const int c = at_least(mid);
-      if (c >= count) lo = mid;
-      else hi = mid;
-      if (c == count) break;
+  uint32_t hi = 0, lo = ~0u;
+  int first = 0;  // keys before all scores
+  over([&](uint32_t k, bool there, int) __attribute__((always_inline)) {
+    const bool score = there && k < kSelOdd;
+    first += there && k >= kSelOdd;
+    hi = max(hi, score ? k : 0u);
+    lo = min(lo, score ? k : ~0u);
+  });
+  for (int i = w.part * 64 + lane; i < 2 * kSelBins; i += w.parts * 64) w.bins[i] = 0;
+  uint32_t met[3] = {wave_most(hi), wave_least(lo), (uint32_t)wave_total(first)};
+  w.all(met, {0u, ~0u, 0u});
+  hi = wave_most(met[0]);
+  lo = wave_least(met[1]);
+  int above = wave_total((int)met[2]);  // keys past hi
+  if (above >= count) {
+    above = 0;
+    hi = kSelForced;
+    lo = kSelOdd;
+  }
+  for (int turn = 0;; turn ^= 1) {
+    const int shift = hi - lo < kSelBins ? 0 : 32 - __builtin_clz(hi - lo) - kSelBits;
+    uint32_t* bins = w.bins + turn * kSelBins;
+    if (hi != lo) {
+      over([&](uint32_t k, bool there, int) __attribute__((always_inline)) {
+        if (there && k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1u);
+      });
+      w.sync();
+      // the parts from the last on: lane l has parts 255 - 4 l - 0 .. 3
+      const uint4 c = *(const uint4*)(bins + kSelBins - 4 - 4 * lane);
+      const int mine = (int)(c.x + c.y + c.z + c.w), upto = above + wave_scan(mine);
+      const uint64_t enough = __ballot(upto >= count);
+      const int at = __builtin_ctzll(enough);
+      int before = __builtin_amdgcn_readlane(upto - mine, at), part = kSelBins - 1 - 4 * at, of = 0;
+      const uint32_t v[4] = {(uint32_t)__builtin_amdgcn_readlane((int)c.w, at), (uint32_t)__builtin_amdgcn_readlane((int)c.z, at),
+                             (uint32_t)__builtin_amdgcn_readlane((int)c.y, at), (uint32_t)__builtin_amdgcn_readlane((int)c.x, at)};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (of == 0) {
+          if (before + (int)v[e] >= count) {
+            of = (int)v[e];
+          } else {
+            before += (int)v[e];
+            --part;
+          }
+        }
+      above = before;
+      lo += (uint32_t)part << shift;
+      hi = min(hi, lo + ((1u << shift) - 1));
+      if (shift == 0 || above + of == count) break;
+      // (the counts of the round before this one, which nobody reads any more)
+      for (int i = w.part * 64 + lane; i < kSelBins; i += w.parts * 64) w.bins[(turn ^ 1) * kSelBins + i] = 0;
+      w.sync();
+    } else {
+      break;
     }
   }
-  int above = 0, equal = 0;
-  for (int j = from; j < to; j += 64) {
-    const uint32_t k = key[min(j + lane, to - 1)];
-    above += __builtin_popcountll(__ballot(j + lane < to && k > lo));
-    equal += __builtin_popcountll(__ballot(j + lane < to && k == lo));
-  }
-  const int spare = count - w.sum(above);  // how many of the equal are taken
-  int a = w.before(above, 0), e = w.before(equal, 0);
+  // keys past hi, and the first of those from lo to hi
+  const int spare = count - above;
+  int a = 0, e = 0;
+  over([&](uint32_t k, bool there, int) __attribute__((always_inline)) {
+    a += __builtin_popcountll(__ballot(there && k > hi));
+    e += __builtin_popcountll(__ballot(there && k >= lo && k <= hi));
+  });
+  uint32_t both[2] = {(uint32_t)a, (uint32_t)e};
+  w.all(both, {0u, 0u});
+  a = __builtin_amdgcn_readlane(wave_scan((int)both[0]), w.part) - a;
+  e = __builtin_amdgcn_readlane(wave_scan((int)both[1]), w.part) - e;
   const uint64_t below = (1ull << lane) - 1;
-  for (int j = from; j < to; j += 64) {
-    const uint32_t k = key[min(j + lane, to - 1)];
-    const uint64_t ab = __ballot(j + lane < to && k > lo), eb = __ballot(j + lane < to && k == lo);
+  over([&](uint32_t k, bool there, int j) __attribute__((always_inline)) {
+    const uint64_t ab = __ballot(there && k > hi), eb = __ballot(there && k >= lo && k <= hi);
+    if ((ab | eb) == 0) return;
     const int ea = e + __builtin_popcountll(eb & below);
-    if ((ab >> lane & 1) || ((eb >> lane & 1) && ea < spare)) out[a + __builtin_popcountll(ab & below) + min(ea, spare)] = j + lane;
+    if ((ab >> lane & 1) || ((eb >> lane & 1) && ea < spare)) out[a + __builtin_popcountll(ab & below) + min(ea, spare)] = j;
     a += __builtin_popcountll(ab);
     e += __builtin_popcountll(eb);
-  }
+  });
 }
 
 // GP: rows a token takes of a tile of 16 (its heads, rounded up to 4, 8, 16); more than 16 heads take several tiles.
 template <int HD, bool BF, int GP>
-__global__ void __launch_bounds__(1024) paged_select_kernel(const PagedKv kv, const PagedSelect sel,
+__global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, const PagedSelect sel,
                                                             const uint16_t* __restrict__ q, int64_t ldq, int heads, int g,
                                                             int tokens_a_group, int* __restrict__ blocks) {
   constexpr int KS = 2 * HD / 64;  // matrix instructions of a tile
   constexpr int TOK = 16 / GP;     // tokens of a tile
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ uint32_t box[32];
+  __shared__ uint32_t box[96];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), waves = sread((int)(blockDim.x >> 6));
   const int c16 = lane & 15, q4 = lane >> 4;
   const int tiles = (g + 15) / 16;  // of a token's heads (GP 16)
   uint8_t* qc = smem;               // [rows][2 hd] codes of the queries
-  uint32_t* keys = (uint32_t*)(smem + 16 * tiles * 2 * HD);
+  uint32_t* bins = (uint32_t*)(smem + 16 * tiles * 2 * HD);  // [waves or 1][2][kSelBins]
+  const bool alone = tokens_a_group > 1;                     // (rows of keys are a wave's each)
+  uint32_t* keys = bins + (alone ? waves : 1) * 2 * kSelBins;
   uint32_t* mine = sel.keys + (int64_t)blockIdx.x * tokens_a_group * sel.pitch;  // (split units only)
   const int kvh = blockIdx.x % kv.kv_heads, first = (blockIdx.x / kv.kv_heads) * tokens_a_group;
   const int past = min(first + tokens_a_group, kv.tokens);
+  // A token's heads as a wave holds them: eight dims of a row a lane, the rows of a tile (what a token of more than 16 heads
+  // has beside them is read again).
+  constexpr int NCH = GP * HD / 8 > 64 ? GP * HD / 512 : 1;
+  uint4 u[NCH];
+  auto ask = [&](int token) __attribute__((always_inline)) {
+    const uint16_t* qr = q + (int64_t)token * ldq + (int64_t)kvh * g * HD;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int x = lane + 64 * k, r = x / (HD / 8), d = 8 * (x % (HD / 8));
+      u[k] = *(const uint4*)(qr + min(r, g - 1) * HD + d);
+    }
+  };
+  if (tokens_a_group == 1) ask(first);  // (on their way while the sequence is found)
   for (int t0 = first; t0 < past;) {
-    const int seq = paged_find(kv.q_start, kv.batch, t0, lane);
+    PagedSeq sq;
+    const int seq = paged_where(kv, t0, lane, sq);
     if (seq >= kv.batch) return;  // behind the last sequence: left alone
-    const PagedSeq sq = paged_seq(sload(kv.q_start + seq), sload(kv.q_start + seq + 1), sload(kv.lens + seq), kv.tokens);
     const int n = max(min(min(sq.q0 + sq.n, past) - t0, TOK), 1);  // tokens of this step (starts that are no batch's: one)
     const int i0 = sq.len - sq.n + (t0 - sq.q0);           // position of the first
     const int most = min((i0 + n - 1 >> kv.page_shift) + 1, kv.table_width);  // pages that the last sees
@@ -181,26 +257,56 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const PagedKv kv, co
       return i0 + t < 0 ? 0 : min((i0 + t >> kv.page_shift) + 1, kv.table_width);
     };
     if (most > sel.count) {
+      const int* tab = kv.table + seq * kv.table_stride;
+      const int begin = blockIdx.y * sel.chunk, end = min(most, begin + sel.chunk), step = 16 * waves;
+      // 16 pages a wave and step: ids two steps ahead, bounds one
+      auto page_of = [&](int j0) __attribute__((always_inline)) { return tab[min(j0 + c16, end - 1)]; };
+      struct Bounds {
+        pi4_t b[KS];
+        float scale;
+        bool bad;
+      };
+      auto bounds_of = [&](Bounds& x, int page) __attribute__((always_inline)) {
+        x.bad = (uint32_t)page >= (uint32_t)kv.num_pages;
+        page = x.bad ? 0 : page;
+        const int8_t* at = sel.codes + page * sel.code_step + (int64_t)kvh * 2 * HD + 16 * q4;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x.b[s] = *(const pi4_t*)(at + 64 * s);
+        x.scale = sel.scales[page * sel.scale_step + kvh];
+      };
+      int j0 = begin + 16 * wave;
+      Bounds ba, bb;
+      int pa = 0, pb = 0;
+      if (j0 < end) {
+        pa = page_of(j0);
+        pb = page_of(j0 + step);
+        bounds_of(ba, pa);
+        bounds_of(bb, pb);
+        pa = page_of(j0 + 2 * step);
+        pb = page_of(j0 + 3 * step);
+      }
       // ---- the queries' codes: a wave a token
       for (int t = wave; t < TOK; t += waves) {
+        if (tokens_a_group > 1) ask(t0 + min(t, n - 1));
         const uint16_t* qr = q + (int64_t)(t0 + min(t, n - 1)) * ldq + (int64_t)kvh * g * HD;
         uint32_t big = 0;
-        for (int x = 8 * lane; x < g * HD; x += 512) {
-          const uint4 u = *(const uint4*)(qr + x);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        auto magnitude = [&](const uint4& x) __attribute__((always_inline)) {
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t m = w[e] & 0x7fff7fffu;
             big = max(big, max(m & 0xffffu, m >> 16));
           }
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) magnitude(u[k]);
+        for (int x = 16 * HD + 8 * lane; x < g * HD; x += 512) magnitude(*(const uint4*)(qr + x));
         big = wave_most(big);
         const float a = BF ? bf2f((uint16_t)big) : h2f((uint16_t)big);
         const float inv = big >= (BF ? 0x7f80u : 0x7c00u) || a < kSelLeast ? 0.0f : 127.0f / a;
-        for (int x = lane; x < GP * tiles * (HD / 8); x += 64) {  // eight dims of a row
+        auto codes = [&](const uint4& y, int x) __attribute__((always_inline)) {  // of chunk x of the rows
           const int r = x / (HD / 8), d = 8 * (x % (HD / 8));
-          const uint4 u = *(const uint4*)(qr + min(r, g - 1) * HD + d);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          const uint32_t w[4] = {y.x, y.y, y.z, y.w};
           uint32_t up[2] = {0, 0}, dn[2] = {0, 0};
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -212,63 +318,80 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const PagedKv kv, co
           uint8_t* dst = qc + (t * GP + r) * 2 * HD + d;
           *(uint2*)dst = make_uint2(up[0], up[1]);
           *(uint2*)(dst + HD) = make_uint2(dn[0], dn[1]);
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+          if (lane + 64 * k < GP * HD / 8) codes(u[k], lane + 64 * k);
+        for (int x = 16 * HD / 8 + lane; x < 16 * tiles * (HD / 8); x += 64)
+          codes(*(const uint4*)(qr + min(x / (HD / 8), g - 1) * HD + 8 * (x % (HD / 8))), x);
       }
       __syncthreads();
-      // ---- scores: 16 pages a wave and step
+      // ---- scores
       pi4_t qa[KS];
       auto rows = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) qa[s] = *(const pi4_t*)(qc + (16 * tile + c16) * 2 * HD + 64 * s + 16 * q4);
       };
       rows(0);
-      const int* tab = kv.table + seq * kv.table_stride;
-      const int begin = blockIdx.y * sel.chunk, end = min(most, begin + sel.chunk);
-      for (int j0 = begin + 16 * wave; j0 < end; j0 += 16 * waves) {
+      auto score = [&](const Bounds& x, int j0) __attribute__((always_inline)) {
         const int j = j0 + c16;
-        int page = tab[min(j, most - 1)];
-        const bool bad = (uint32_t)page >= (uint32_t)kv.num_pages;
-        page = bad ? 0 : page;
-        const int8_t* at = sel.codes + page * sel.code_step + (int64_t)kvh * 2 * HD + 16 * q4;
-        pi4_t b[KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) b[s] = *(const pi4_t*)(at + 64 * s);
-        const float scale = sel.scales[page * sel.scale_step + kvh];
         int m = -0x7fffffff;
         for (int tile = 0; tile < tiles; ++tile) {
           if (tiles > 1) rows(tile);
           pi4_t acc = {0, 0, 0, 0};
 #pragma unroll
-          for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[s], b[s], acc, 0, 0, 0);
+          for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[s], x.b[s], acc, 0, 0, 0);
 #pragma unroll
           for (int r = 0; r < 4; ++r) m = max(m, acc[r]);
         }
-        if (GP >= 8) m = max(m, __shfl_xor(m, 16, 64));
-        if (GP >= 16) m = max(m, __shfl_xor(m, 32, 64));
+        if (GP >= 8) m = max(m, (int)lane_xor_u<16>((uint32_t)m, lane));
+        if (GP >= 16) m = max(m, (int)lane_xor_u<32>((uint32_t)m, lane));
         const int t = q4 * 4 / GP;  // the token of the lane's rows
-        if (q4 % (GP / 4) == 0 && t < n && j < most) {
+        if (q4 % (GP / 4) == 0 && t < n && j < end) {
           const int cur = i0 + t >> kv.page_shift;
-          uint32_t k = bad || scale == INFINITY ? kSelOdd : min(sel_key((float)m * scale), kSelOdd - 1);
+          uint32_t k = x.bad || x.scale == INFINITY ? kSelOdd : min(sel_key((float)m * x.scale), kSelOdd - 1);
           if (j < sel.sink || j > min(cur, kv.table_width - 1) - sel.local) k = kSelForced;
           if (sel.chunks > 1) store_dev1(mine + t * sel.pitch + j, k);
           else keys[t * sel.pitch + j] = k;
         }
+      };
+      while (j0 < end) {
+        score(ba, j0);
+        if (j0 + 2 * step < end) {
+          bounds_of(ba, pa);
+          pa = page_of(j0 + 4 * step);
+        }
+        if (j0 + step >= end) break;
+        score(bb, j0 + step);
+        if (j0 + 3 * step < end) {
+          bounds_of(bb, pb);
+          pb = page_of(j0 + 5 * step);
+        }
+        j0 += 2 * step;
       }
       if (sel.chunks > 1) {  // (a unit of one step) the last to arrive chooses
-        if (!paged_arrive(sel.counters + blockIdx.x, sel.chunks, &flag)) return;
+        if (!paged_arrive(sel.counters + blockIdx.x * (kSelApart / 4), sel.chunks, &flag)) return;
+        constexpr int U = 8;  // loads in flight
         for (int t = 0; t < n; ++t)
-          for (int j = tid; j < most; j += blockDim.x) keys[t * sel.pitch + j] = load_dev1(mine + t * sel.pitch + j);
+          for (int j = tid; j < most; j += U * blockDim.x) {
+            uint32_t k[U];
+#pragma unroll
+            for (int e = 0; e < U; ++e) k[e] = load_dev1(mine + t * sel.pitch + min(j + e * (int)blockDim.x, most - 1));
+#pragma unroll
+            for (int e = 0; e < U; ++e)
+              if (j + e * (int)blockDim.x < most) keys[t * sel.pitch + j + e * blockDim.x] = k[e];
+          }
       }
       __syncthreads();
     }
     // ---- the choice
-    if (n == 1 && most > sel.count) {
-      sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, box});
+    if (!alone && most > sel.count) {
+      sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, bins, box});
     } else {
       for (int t = wave; t < n; t += waves) {
         const int v = visible(t);
         if (v > sel.count) {
-          sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{});
+          sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{bins + wave * 2 * kSelBins});
         } else {
           for (int x = lane; x < sel.count; x += 64) to[t * row + x] = x < v ? x : -1;
         }
@@ -316,7 +439,12 @@ extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_
   SPECTRA_REQUIRE(count <= kSelMost && tokens * kv->kv_heads * count < (1LL << 40), "count out of range");
   if (kv->table_width > kSelMost) return fail(SPECTRA_ERR_UNSUPPORTED, "block tables of more than 32768 pages");
   const int pitch = (kv->table_width + 63) & ~63, rows = 16 * ((g + 15) / 16);
-  if (g > 256 || rows * 2 * hd + 4 * pitch > kSelLds)
+  // (64 users of up to 250 pages: 12.6 us with 256 or 512 threads; a chunk of 300 on 30000 keys 21.5 with 256, 24.7 with 512,
+  // 34.6 with 1024; one user of 250 pages 9.0 with 256, 8.4 with 512, 9.7 with 1024)
+  const int threads = tokens * kv->kv_heads >= 512 ? 256 : 512;
+  // codes, counts and keys of a workgroup of `group` tokens
+  auto lds_of = [&](int group) { return rows * 2 * hd + 8 * kSelBins * (group > 1 ? threads / 64 : 1) + 4 * group * pitch; };
+  if (g > 256 || lds_of(1) > kSelLds)
     return fail(SPECTRA_ERR_UNSUPPORTED, "too many query heads a KV head, with a block table of this width");
   if (workspace != nullptr) {
     if (workspace_bytes < spectra_paged_select_workspace())
@@ -335,13 +463,14 @@ extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_
   PagedSelect sel = {bounds->codes, bounds->scales, one ? 0 : bounds->code_stride, one ? 0 : bounds->scale_stride,
                      count, sink, local, pitch, 1, kSelMost, nullptr, nullptr};
   int gp = g <= 4 ? 4 : g <= 8 ? 8 : 16, gv = g, hv = heads;
-  // tokens a workgroup takes: one where sequences have one each, a tile's rows otherwise
+  // tokens a workgroup takes: as many as fill a tile's rows, but one where sequences have less than two tiles (5 drafted
+  // tokens of 12 sequences: one 10.6 us, four 15.4; a chunk of 100 on 30000 keys: 21.9 and 13.3)
   const int64_t seqs = std::min<int64_t>(tokens, kv->batch);
-  int group = tokens < 2 * seqs ? 1 : 16 / gp;
-  while (rows * 2 * hd + 4 * group * pitch > kSelLds) group /= 2;
+  int group = tokens < 32 / gp * seqs ? 1 : 16 / gp;
+  while (lds_of(group) > kSelLds) group /= 2;
   const int64_t groups = (tokens + group - 1) / group * kv->kv_heads;
   SPECTRA_REQUIRE(groups < (1LL << 31), "tokens out of range");
-  const int lds = rows * 2 * hd + 4 * group * pitch;
+  const int lds = lds_of(group);
   // units of one step each, few of them, and pages enough for several workgroups
   if (workspace != nullptr && groups <= kSelSplit && kv->table_width >= 1024 && (group == 1 || kv->batch == 1)) {
     sel.chunks = (int)std::min<int64_t>(256 / groups, (kv->table_width + 255) / 256);
@@ -349,7 +478,6 @@ extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_
     sel.counters = (uint32_t*)workspace;
     sel.keys = (uint32_t*)((uint8_t*)workspace + kSelCounters);
   }
-  const int threads = kv->table_width <= 512 ? 256 : kv->table_width <= 1024 ? 512 : 1024;
   const void* kern = hd == 64 ? (act_dtype == SPECTRA_BF16 ? select_of<64, true>(gp) : select_of<64, false>(gp))
                               : (act_dtype == SPECTRA_BF16 ? select_of<128, true>(gp) : select_of<128, false>(gp));
   if (int st = ensure_lds_limit(kern); st != SPECTRA_OK) return st;
