@@ -11,8 +11,7 @@
 // Scores are matrix products (16 x 16 x 64 of bytes): rows are query heads, padded to 4, 8 or 16 a token by copies of the
 // last one, so that a token's maximum lies in a lane's registers and at most two exchanges; columns are 16 pages, whose
 // 2 d bytes a lane reads as they lie.  Scores are kept in LDS as 32-bit keys in the scores' order; the `count`-th largest
-// is found by counts of the keys in 256 parts of their range, and of the part's range again (two or three rounds), ties by
-// the order of the pages, and the chosen are written in that order.
+// bounds the choice, ties go by the order of the pages, and the chosen are written in that order (sel_pick).
 // A workgroup has one token (drafts and prompts: as many as fill the rows, whose pages are read once) and one KV head.
 // Few such units with long tables are split: workgroups score a run of pages each, and the last of a unit to arrive
 // chooses from the keys of all in the workspace.
@@ -26,7 +25,8 @@ typedef int pi4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kSelMost = 32768;            // pages of a table
 constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;  // parts of a range that keys are counted in
-constexpr int kSelLds = 160 * 1024 - 512;  // codes, keys and counts of a workgroup
+constexpr int kSelWave = 512;                          // keys that one wave chooses from in its registers
+constexpr int kSelLds = 160 * 1024 - 1024;  // codes, keys and counts of a workgroup
 constexpr int kSelSplit = 64;              // units whose pages are split among workgroups: at most as many
 constexpr int kSelApart = 256;             // bytes from one unit's counter to the next one's (atomics on one line wait for each other)
 constexpr size_t kSelCounters = kSelApart * kSelSplit;
@@ -79,11 +79,89 @@ __device__ __forceinline__ uint32_t load_dev1(const uint32_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// K keys a lane, 0 where there is none: the largest t that at least `count` of them reach, or, with `slack`, a t that
+// between count and count + slack reach where bisection meets one on its way.
+template <int K>
+__device__ __forceinline__ uint32_t sel_kth(const uint32_t (&k)[K], int count, int slack) {
+  auto reach = [&](uint32_t t) __attribute__((always_inline)) {
+    int c = 0;
+#pragma unroll
+    for (int r = 0; r < K; ++r) c += __builtin_popcountll(__ballot(k[r] >= t));
+    return c;
+  };
+  uint32_t hi = 0, lo = ~0u;  // of the scores
+#pragma unroll
+  for (int r = 0; r < K; ++r) {
+    const bool score = k[r] != 0 && k[r] < kSelOdd;
+    hi = max(hi, score ? k[r] : 0u);
+    lo = min(lo, score ? k[r] : ~0u);
+  }
+  hi = sread((int)wave_most(hi));
+  lo = sread((int)wave_least(lo));
+  if (reach(kSelForced) >= count) return kSelForced;
+  if (reach(kSelOdd) >= count) return kSelOdd;
+  if (reach(hi) >= count) return hi;
+  // `count` reach lo, but not hi; three places between them at a time, whose counts do not wait for each other
+  while (hi - lo > 1) {
+    const uint32_t q = max((hi - lo) >> 2, 1u), t1 = lo + q, t2 = min(lo + 2 * q, hi), t3 = min(lo + 3 * q, hi);
+    const int c1 = reach(t1), c2 = reach(t2), c3 = reach(t3);
+    int c = c3;
+    if (c3 >= count) {
+      lo = t3;
+    } else if (c2 >= count) {
+      lo = t2;
+      hi = t3;
+      c = c2;
+    } else if (c1 >= count) {
+      lo = t1;
+      hi = t2;
+      c = c1;
+    } else {
+      hi = t1;
+    }
+    if (c >= count && c <= count + slack) break;
+  }
+  return lo;
+}
+// The `count` largest of K keys a lane, the first on ties (keys 64 r + lane), by one wave: their places, or what `of`
+// has there, in order.
+template <int K>
+__device__ __forceinline__ void sel_wave(const uint32_t* key, int n, int count, const uint32_t* of, int* out) {
+  const int lane = __lane_id();
+  uint32_t k[K];
+#pragma unroll
+  for (int r = 0; r < K; ++r) k[r] = 64 * r + lane < n ? key[64 * r + lane] : 0u;
+  const uint32_t t = sel_kth<K>(k, count, 0);
+  int above = 0, spare = count;  // of those equal to t
+#pragma unroll
+  for (int r = 0; r < K; ++r) spare -= __builtin_popcountll(__ballot(k[r] > t));
+  int equal = 0;
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int r = 0; r < K; ++r) {
+    const uint64_t ab = __ballot(k[r] > t), eb = __ballot(k[r] == t);
+    const int e = equal + __builtin_popcountll(eb & below), j = 64 * r + lane;
+    if ((ab >> lane & 1) || ((eb >> lane & 1) && e < spare))
+      out[above + __builtin_popcountll(ab & below) + min(e, spare)] = of != nullptr ? (int)of[j] : j;
+    above += __builtin_popcountll(ab);
+    equal += __builtin_popcountll(eb);
+  }
+}
+__device__ __forceinline__ void sel_wave(const uint32_t* key, int n, int count, const uint32_t* of, int* out) {
+  if (n <= 128) sel_wave<2>(key, n, count, of, out);
+  else if (n <= 256) sel_wave<4>(key, n, count, of, out);
+  else sel_wave<kSelWave / 64>(key, n, count, of, out);
+}
+
 // What the waves that work on one row of keys tell each other: one wave by itself, or all of a workgroup, each with a
 // part of the keys.
 struct SelAlone {
-  static constexpr int parts = 1, part = 0;
-  uint32_t* bins;  // [2][kSelBins]
+  static constexpr int parts = 1, part = 0, room = kSelBins;
+  uint32_t* bins;  // [2][kSelBins], or `room` keys and their places
+  __device__ __forceinline__ uint32_t kth(uint32_t v, int count) {
+    const uint32_t k[1] = {v};
+    return sel_kth<1>(k, count, max(min(count, room / 2 - count), 8));
+  }
   __device__ __forceinline__ void sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
   template <int N>
   __device__ __forceinline__ void all(uint32_t (&v)[N], const uint32_t (&none)[N]) {
@@ -92,10 +170,26 @@ struct SelAlone {
   }
 };
 struct SelTogether {
+  static constexpr int room = kSelWave;
   int parts, part;
-  uint32_t* bins;
-  uint32_t* box;  // [2][3][16]
+  uint32_t* bins;  // [2][kSelBins], or `room` keys and their places
+  uint32_t* box;   // [2][3][16]
   int turn = 0;
+  // of a value a lane
+  __device__ __forceinline__ uint32_t kth(uint32_t v, int count) {
+    const int lane = __lane_id();
+    bins[64 * part + lane] = v;
+    __syncthreads();
+    if (part == 0) {
+      uint32_t k[kSelWave / 64];
+#pragma unroll
+      for (int r = 0; r < kSelWave / 64; ++r) k[r] = r < parts ? bins[64 * r + lane] : 0u;
+      const uint32_t t = sel_kth(k, count, max(min(count, room / 2 - count), 8));
+      if (lane == 0) box[96] = t;
+    }
+    __syncthreads();
+    return (uint32_t)sread((int)box[96]);
+  }
   __device__ __forceinline__ void sync() { __syncthreads(); }
   // every wave's values, in lanes 0 .. parts - 1
   template <int N>
@@ -113,12 +207,21 @@ struct SelTogether {
   }
 };
 
-// The `count` largest of n > count keys, the first on ties, written in their order.  The range that holds the count-th
+// The `count` largest of n > count keys, the first on ties, written in their order, by parts of 64 lanes.
+//
+// Few keys are one wave's, in its registers.  Of more, each lane's largest is found first: as many of these as are wanted
+// lie at or past the `count`-th largest of them, and so do as many keys, so only keys from there on are candidates: little
+// more than `count` (64 of 8190 keys by 512 lanes: some 70), which one wave chooses from.
+// Where that leaves too many, or more are wanted than there are lanes, the range that holds the count-th
 // largest is narrowed by counting the keys in kSelBins equal parts of it; some two rounds leave as many keys as are
 // wanted, or keys that are all the same.
 template <typename W>
 __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, int* out, W w) {
   const int lane = __lane_id();
+  if (n <= kSelWave) {
+    if (w.part == 0) sel_wave(key, n, count, nullptr, out);
+    return;
+  }
   const int each = ((n + w.parts - 1) / w.parts + 63) & ~63;
   const int from = min(each * w.part, n), to = min(from + each, n);
   // f of all keys of this part, a lane's each, the loads of four in flight together
@@ -132,6 +235,34 @@ __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, 
       for (int e = 0; e < U; ++e) f(k[e], j0 + 64 * e + lane < to, j0 + 64 * e + lane);
     }
   };
+  if (count <= 64 * w.parts) {
+    uint32_t best = 0;
+    over([&](uint32_t k, bool there, int) __attribute__((always_inline)) { best = max(best, there ? k : 0u); });
+    const uint32_t from_on = w.kth(best, count);
+    int c = 0;
+    over([&](uint32_t k, bool there, int) __attribute__((always_inline)) { c += __builtin_popcountll(__ballot(there && k >= from_on)); });
+    uint32_t met[1] = {(uint32_t)c};
+    w.all(met, {0u});
+    const int upto = wave_scan((int)met[0]), all = __builtin_amdgcn_readlane(upto, 63);
+    if (all >= count && all <= w.room) {  // (lanes without keys may have been counted on)
+      int at = __builtin_amdgcn_readlane(upto, w.part) - c;
+      uint32_t *keys = w.bins, *places = w.bins + w.room;
+      const uint64_t below = (1ull << lane) - 1;
+      over([&](uint32_t k, bool there, int j) __attribute__((always_inline)) {
+        const uint64_t take = __ballot(there && k >= from_on);
+        if (take >> lane & 1) {
+          const int p = at + __builtin_popcountll(take & below);
+          keys[p] = k;
+          places[p] = (uint32_t)j;
+        }
+        at += __builtin_popcountll(take);
+      });
+      w.sync();
+      if (w.part == 0) sel_wave(keys, all, count, places, out);
+      return;
+    }
+    w.sync();  // (the counts start anew)
+  }
   uint32_t hi = 0, lo = ~0u;
   int first = 0;  // keys before all scores
   over([&](uint32_t k, bool there, int) __attribute__((always_inline)) {
@@ -218,15 +349,15 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
   constexpr int KS = 2 * HD / 64;  // matrix instructions of a tile
   constexpr int TOK = 16 / GP;     // tokens of a tile
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ uint32_t box[96];
+  __shared__ uint32_t box[97];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = sread(tid >> 6), waves = sread((int)(blockDim.x >> 6));
   const int c16 = lane & 15, q4 = lane >> 4;
   const int tiles = (g + 15) / 16;  // of a token's heads (GP 16)
   uint8_t* qc = smem;               // [rows][2 hd] codes of the queries
-  uint32_t* bins = (uint32_t*)(smem + 16 * tiles * 2 * HD);  // [waves or 1][2][kSelBins]
+  uint32_t* bins = (uint32_t*)(smem + 16 * tiles * 2 * HD);  // (a wave's each, or the workgroup's)
   const bool alone = tokens_a_group > 1;                     // (rows of keys are a wave's each)
-  uint32_t* keys = bins + (alone ? waves : 1) * 2 * kSelBins;
+  uint32_t* keys = bins + 2 * (alone ? waves * SelAlone::room : SelTogether::room);
   uint32_t* mine = sel.keys + (int64_t)blockIdx.x * tokens_a_group * sel.pitch;  // (split units only)
   const int kvh = blockIdx.x % kv.kv_heads, first = (blockIdx.x / kv.kv_heads) * tokens_a_group;
   const int past = min(first + tokens_a_group, kv.tokens);
@@ -249,12 +380,12 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
     if (seq >= kv.batch) return;  // behind the last sequence: left alone
     const int n = max(min(min(sq.q0 + sq.n, past) - t0, TOK), 1);  // tokens of this step (starts that are no batch's: one)
     const int i0 = sq.len - sq.n + (t0 - sq.q0);           // position of the first
-    const int most = min((i0 + n - 1 >> kv.page_shift) + 1, kv.table_width);  // pages that the last sees
+    const int most = min(((i0 + n - 1) >> kv.page_shift) + 1, kv.table_width);  // pages that the last sees
     int* to = blocks + ((int64_t)t0 * kv.kv_heads + kvh) * sel.count;
     const int64_t row = (int64_t)kv.kv_heads * sel.count;  // from a token's to the next one's
     if (most <= sel.count && blockIdx.y > 0) return;
     auto visible = [&](int t) __attribute__((always_inline)) {
-      return i0 + t < 0 ? 0 : min((i0 + t >> kv.page_shift) + 1, kv.table_width);
+      return i0 + t < 0 ? 0 : min(((i0 + t) >> kv.page_shift) + 1, kv.table_width);
     };
     if (most > sel.count) {
       const int* tab = kv.table + seq * kv.table_stride;
@@ -348,25 +479,23 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
         if (GP >= 16) m = max(m, (int)lane_xor_u<32>((uint32_t)m, lane));
         const int t = q4 * 4 / GP;  // the token of the lane's rows
         if (q4 % (GP / 4) == 0 && t < n && j < end) {
-          const int cur = i0 + t >> kv.page_shift;
-          uint32_t k = x.bad || x.scale == INFINITY ? kSelOdd : min(sel_key((float)m * x.scale), kSelOdd - 1);
+          const int cur = (i0 + t) >> kv.page_shift;
+          uint32_t k = x.bad || x.scale == INFINITY ? kSelOdd : min(max(sel_key((float)m * x.scale), 1u), kSelOdd - 1);
           if (j < sel.sink || j > min(cur, kv.table_width - 1) - sel.local) k = kSelForced;
           if (sel.chunks > 1) store_dev1(mine + t * sel.pitch + j, k);
           else keys[t * sel.pitch + j] = k;
         }
       };
+      // (behind the last pages the loads go on, at the last one: with a branch around them the bounds before them are waited
+      // for as if they were the newest)
       while (j0 < end) {
         score(ba, j0);
-        if (j0 + 2 * step < end) {
-          bounds_of(ba, pa);
-          pa = page_of(j0 + 4 * step);
-        }
+        bounds_of(ba, pa);
+        pa = page_of(j0 + 4 * step);
         if (j0 + step >= end) break;
         score(bb, j0 + step);
-        if (j0 + 3 * step < end) {
-          bounds_of(bb, pb);
-          pb = page_of(j0 + 5 * step);
-        }
+        bounds_of(bb, pb);
+        pb = page_of(j0 + 5 * step);
         j0 += 2 * step;
       }
       if (sel.chunks > 1) {  // (a unit of one step) the last to arrive chooses
@@ -391,7 +520,7 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
       for (int t = wave; t < n; t += waves) {
         const int v = visible(t);
         if (v > sel.count) {
-          sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{bins + wave * 2 * kSelBins});
+          sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{bins + wave * 2 * SelAlone::room});
         } else {
           for (int x = lane; x < sel.count; x += 64) to[t * row + x] = x < v ? x : -1;
         }
@@ -443,7 +572,7 @@ extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_
   // 34.6 with 1024; one user of 250 pages 9.0 with 256, 8.4 with 512, 9.7 with 1024)
   const int threads = tokens * kv->kv_heads >= 512 ? 256 : 512;
   // codes, counts and keys of a workgroup of `group` tokens
-  auto lds_of = [&](int group) { return rows * 2 * hd + 8 * kSelBins * (group > 1 ? threads / 64 : 1) + 4 * group * pitch; };
+  auto lds_of = [&](int group) { return rows * 2 * hd + 8 * (group > 1 ? threads / 64 * SelAlone::room : SelTogether::room) + 4 * group * pitch; };
   if (g > 256 || lds_of(1) > kSelLds)
     return fail(SPECTRA_ERR_UNSUPPORTED, "too many query heads a KV head, with a block table of this width");
   if (workspace != nullptr) {
