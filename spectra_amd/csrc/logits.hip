@@ -321,11 +321,11 @@ int logits_args(const spectra_logits_t* l, LogitsArgs* out, size_t* lds, int* th
   a.ldallowed = l->allowed_ld;
   a.states = l->states;
   a.state = l->state;
-  const bool large = logits_large(l->rows, l->vocab);
+  *wide = a.hist > (int)LgWord<uint32_t>::count || a.biases >= 65535;
+  const bool large = !*wide && logits_large(l->rows, l->vocab);  // (wide words of such a slice would not fit)
   const int slice = large ? 16384 : 2048;
   *threads = large ? 1024 : 256;
   *slices = (int)((l->vocab + slice - 1) / slice);
-  *wide = a.hist > (int)LgWord<uint32_t>::count || a.biases >= 65535;
   *lds = 0;
   if (counts || a.biases > 0)
     *lds = lg_zero(slice, *wide ? 8 : 4) + 2 * std::min<int64_t>(slice, (int64_t)a.hist + a.biases);
@@ -358,7 +358,7 @@ static const void* logits_of(int dtype) {
 }
 template <bool PICK>
 static const void* logits_of(int dtype, int threads, bool wide) {
-  if (wide) return threads == 256 ? logits_of<PICK, 256, 1, unsigned long long>(dtype) : logits_of<PICK, 1024, 2, unsigned long long>(dtype);
+  if (wide) return logits_of<PICK, 256, 1, unsigned long long>(dtype);
   return threads == 256 ? logits_of<PICK, 256, 1, uint32_t>(dtype) : logits_of<PICK, 1024, 2, uint32_t>(dtype);
 }
 

@@ -1156,3 +1156,102 @@ def test_registered_operators(hip):
     assert torch.equal(over, want)
     grad = K.paged_attend_blocks(b.q.clone().requires_grad_(), blocks, *where, b.k, b.v)
     assert grad.requires_grad and torch.equal(grad, K.paged_attend_blocks(b.q, blocks, *where, b.k, b.v))
+
+
+# -- the paths of larger and rarer shapes ----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 9])
+@pytest.mark.parametrize("levels", [1, 3, 300])
+def test_select_ties_of_many(hip, n, levels):
+    """More candidates than one wave holds, so many alike that no bound leaves few; more wanted than there are lanes."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [n], [16 * 1300 + 9], 4, 2, 64, 16, seed=48)
+    bounds = _random_bounds(b, 12, levels)
+    for count in (5, 70, 400, 700):
+        got = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, bounds, 16, count, workspace=K.paged_select_workspace())
+        _check_select(b, bounds, count, 1, 2, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 9])
+def test_select_infinite_bounds_of_many(hip, n):
+    """More pages come before all scores than are wanted."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [n], [16 * 900], 4, 2, 64, 16, seed=49)
+    codes, scales = _random_bounds(b, 13)
+    scales[::2] = math.inf
+    got = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, (codes, scales), 16, 30)
+    _check_select(b, (codes, scales), 30, 1, 2, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_sequences(hip, kind):
+    """More sequences than a wave has lanes, some without tokens, pages apart in a larger pool."""
+    from spectra_amd import kernels as K
+    g = torch.Generator().manual_seed(6)
+    lens = torch.randint(1, 400, (150,), generator=g).tolist()
+    n = [min(m, x) for m, x in zip(lens, torch.randint(0, 3, (150,), generator=g).tolist())]
+    b = Batch(kind, n, lens, 4, 2, 64, 16, seed=61, pages_apart=True)
+    before = K.paged_bounds(b.k)
+    bounds = K.paged_key_bounds(b.tokens, b.kv_lens, b.q_start, b.table, b.k, K.paged_bounds(b.k))
+    _check_bounds(b, bounds, before)
+    bounds = _random_bounds(b, 14)
+    blocks = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, bounds, 16, 5)
+    _check_select(b, bounds, 5, 1, 2, blocks)
+    want, tol = _blocks_reference(b, blocks)
+    _close(_attend(b, blocks), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_long_chunk(hip, kind):
+    """Many tokens of one sequence beside single ones; their tiles are shared out unevenly."""
+    from spectra_amd import kernels as K
+    b = Batch(kind, [1, 300, 1], [2000, 700, 5], 6, 1, 128, 32, seed=62)
+    bounds = _random_bounds(b, 15)
+    blocks = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, bounds, 32, 7, sink=2, local=1)
+    _check_select(b, bounds, 7, 2, 1, blocks)
+    want, tol = _blocks_reference(b, blocks)
+    _close(_attend(b, blocks), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_pages_gigabytes_apart(hip, kind):
+    """Pages further apart than 32 bits of bytes: the same as side by side."""
+    from spectra_amd import kernels as K
+    b = Batch(kind, [1, 3], [90, 40], 4, 2, 64, 16, seed=63)
+    pages = (b.k[0] if kind == "4bit" else b.k).shape[0]
+
+    def far(t):
+        step = (3 << 29) // t.element_size()
+        room = torch.zeros((pages - 1) * step + t[0].numel(), dtype=t.dtype, device="cuda")
+        x = room.as_strided(t.shape, (step, *t.stride()[1:]))
+        x.copy_(t)
+        return x
+
+    near = K.paged_key_bounds(4, b.kv_lens, b.q_start, b.table, b.k, K.paged_bounds(b.k))
+    blocks = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, near, 16, 4)
+    want = _attend(b, blocks)
+    k, v = [tuple(far(t) for t in c) if kind == "4bit" else far(c) for c in (b.k, b.v)]
+    bounds = far(near[0]).zero_(), far(near[1]).zero_()
+    K.paged_key_bounds(4, b.kv_lens, b.q_start, b.table, k, bounds)
+    assert torch.equal(bounds[0], near[0]) and torch.equal(bounds[1], near[1])
+    assert torch.equal(K.paged_bounds_values(bounds), K.paged_bounds_values(near))
+    assert torch.equal(K.paged_select(b.q, b.kv_lens, b.q_start, b.table, bounds, 16, 4), blocks)
+    assert torch.equal(K.paged_attend_blocks(b.q, blocks, b.kv_lens, b.q_start, b.table, k, v), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(2, 3001), (300, 700)])
+def test_logits_of_long_histories(hip, rows, vocab):
+    """Histories and lists of biases whose counts and places need more than 16 bits."""
+    x, kw = _case(rows, vocab, torch.float16, 65, history=40000 if rows == 2 else 33000)
+    kw["history"][:, : 32800] = 3  # one token, more often than 15 bits hold
+    kw["lens"].fill_(32900)
+    kw["prompt_lens"].fill_(5)
+    _check_logits(x, kw)
+    if rows == 2:
+        x, kw = _case(rows, vocab, torch.float32, 66, history=10, biases=70000)
+        _check_logits(x, kw)
