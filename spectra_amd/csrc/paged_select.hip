@@ -310,7 +310,7 @@ __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, 
         }
       above = before;
       lo += (uint32_t)part << shift;
-      hi = min(hi, lo + ((1u << shift) - 1));
+      hi = lo + min(hi - lo, (1u << shift) - 1);  // (a part of scores near the type's end may pass 32 bits)
       if (shift == 0 || above + of == count) break;
       // (the counts of the round before this one, which nobody reads any more)
       for (int i = w.part * 64 + lane; i < kSelBins; i += w.parts * 64) w.bins[(turn ^ 1) * kSelBins + i] = 0;

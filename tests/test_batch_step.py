@@ -263,13 +263,14 @@ def _selected(q, codes, scales, table, visible, count, sink, local):
     for j in range(visible):
         page = int(table[j])
         if j < sink or j >= visible - local:
-            keys.append(math.inf)
+            keys.append((2, 0.0))
         elif not 0 <= page < codes.shape[0] or scales[page] == np.inf:
-            keys.append(3.5e38)
+            keys.append((1, 0.0))
         else:
             hi, lo = codes[page].astype(np.int64)
-            keys.append(float(f(max((np.maximum(c, 0) * hi + np.minimum(c, 0) * lo).sum(1))) * scales[page]))
-    got = sorted(sorted(range(visible), key=lambda j: (-keys[j], j))[:count])
+            with np.errstate(over="ignore"):
+                keys.append((0, float(f(max((np.maximum(c, 0) * hi + np.minimum(c, 0) * lo).sum(1))) * scales[page])))
+    got = sorted(sorted(range(visible), key=lambda j: (-keys[j][0], -keys[j][1], j))[:count])
     return got + [-1] * (count - len(got))
 
 
@@ -1182,6 +1183,24 @@ def test_select_infinite_bounds_of_many(hip, n):
     scales[::2] = math.inf
     got = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, (codes, scales), 16, 30)
     _check_select(b, (codes, scales), 30, 1, 2, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 9])
+def test_select_scores_past_the_range(hip, n):
+    """More scores past fp32's range than are wanted, the others below zero: they tie, whatever range their keys are
+    counted in."""
+    from spectra_amd import kernels as K
+    b = Batch("bf16", [n], [16 * 1300], 2, 2, 64, 16, seed=50)
+    codes, scales = _random_bounds(b, 16)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    codes[:, :, :, 0] = -100  # (of queries with one positive dim the scores are its codes', times 127)
+    codes[::2, :, :, 0] = 127
+    scales[::2] = 3e38
+    for count in (5, 400, 600):
+        got = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, (codes, scales), 16, count)
+        _check_select(b, (codes, scales), count, 1, 2, got)
 
 
 @pytest.mark.gpu
