@@ -526,7 +526,7 @@ typedef struct spectra_logits {
 /* out [rows, vocab] of the logits' type, row stride ldo (out may be the logits themselves), rounded
  * once from fp32 (each operation rounded):
  *   x = logit;  seen in the history:  x > 0 ? x / repetition : x * repetition
- *   c times in it after the prompt:   x -= frequency c;  c > 0:  x -= presence
+ *   c > 0 times in it after the prompt:  x -= frequency c, then x -= presence
  *   biased:                           x += bias (of an id given twice, the last)
  *   not allowed:                      -inf
  * A history without penalties is not read; ids outside [0, vocab) count nothing. */

@@ -4,7 +4,7 @@
 // For row b and token v, all in fp32, each operation rounded as written:
 //   x = logits[b, v]
 //   v among the row's tokens so far (prompt or answer):   x = x > 0 ? x / repetition : x * repetition
-//   c times in the answer:                                x = x - frequency c,  x = x - presence (c > 0)
+//   c > 0 times in the answer:                            x = x - frequency c,  x = x - presence
 //   v among the row's biased tokens (the last wins):       x = x + bias
 //   the row's grammar state does not allow v:              x = -inf
 // and the choice is the largest x, the lowest v on ties, NaN before all (as torch.argmax); -1 when every x is -inf.
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* __
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int i = i0 + k * TH;
-        const uint64_t at = (uint64_t)(id[k] - begin);
+        const uint64_t at = (uint64_t)id[k] - (uint64_t)begin;
         if (i < len && at < (uint64_t)n) {
           const W was = i < prompt ? atomicOr(&words[at], Word::prompt) : atomicAdd(&words[at], W(1));
           if (was == 0) enlist((uint32_t)at);
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* __
       __syncthreads();  // (lower halves are what they will be)
       for (int i = tid; i < a.biases; i += TH) {
         if (i >= TH) bid = ids[i];
-        const uint64_t at = (uint64_t)(bid - begin);
+        const uint64_t at = (uint64_t)bid - (uint64_t)begin;
         if (at < (uint64_t)n) {
           if (atomicMax(&words[at], (W)(i + 1) << Word::half | (words[at] & Word::low)) == 0) enlist((uint32_t)at);
         }
@@ -190,8 +190,10 @@ __global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* __
       float v = LgType<DT>::get(x[at]);
       if ((s & Word::low) != 0) {
         v = v > 0.0f ? v / rep : v * rep;
-        v = v - freq * (float)c;
-        if (c != 0) v = v - pres;
+        if (c != 0) {  // (an infinite penalty forbids what the answer has, and says nothing of the prompt)
+          v = v - freq * (float)c;
+          v = v - pres;
+        }
       }
       const int place = (int)(s >> Word::half);
       if (place != 0) v = v + (place <= TH ? held[place - 1] : bias[place - 1]);

@@ -995,8 +995,8 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     their type (``out`` may be ``logits``).  In fp32, each operation rounded, the result once:
 
     * tokens in the row's ``history`` (int64 [B, L], the first ``lens[b]`` count, all by default): x / ``repetition`` where
-      x > 0, x * ``repetition`` otherwise; of the history's tokens behind the first ``prompt_lens[b]`` (0 by default), the answer, c
-      times there: x - ``frequency`` c, then x - ``presence``.  Each fp32 [B], or None; ids outside [0, V) count nothing;
+      x > 0, x * ``repetition`` otherwise; those among its tokens behind the first ``prompt_lens[b]`` (0 by default), the answer,
+      c times: x - ``frequency`` c, then x - ``presence``.  Each fp32 [B], or None; ids outside [0, V) count nothing;
     * x + ``bias`` (fp32 [B, n]) for the tokens ``bias_ids`` (int64 [B, n]; of an id given twice the last counts, ids
       outside [0, V), as -1, are filling);
     * -infinity where the row's mask has no bit: ``allowed`` int32 [M, ceil(V / 32)], token v's bit v % 32 of word v // 32;

@@ -617,7 +617,7 @@ def _adjusted(x, history=None, lens=None, prompt_lens=None, repetition=None, pre
                 r = f(1) if repetition is None else repetition[b]
                 x[b, seen] = np.where(x[b, seen] > 0, x[b, seen] / r, x[b, seen] * r)
                 if frequency is not None:
-                    x[b, seen] -= frequency[b] * count[seen]
+                    x[b, seen] = np.where(count[seen] > 0, x[b, seen] - frequency[b] * count[seen], x[b, seen])
                 if presence is not None:
                     x[b, seen] = np.where(count[seen] > 0, x[b, seen] - presence[b], x[b, seen])
             if bias is not None:
@@ -728,6 +728,19 @@ def test_logits_that_are_odd(hip, dtype):
     assert (K.next_tokens(x, allowed=none, allowed_rows=rows) == -1).all()
     assert int(K.next_tokens(x)[3]) == -1 and int(K.next_tokens(x)[5]) == 0
     assert int(K.greedy_next(x[0].half(), torch.zeros(1, dtype=torch.int64, device="cuda"))) == int(K.next_tokens(x)[0])
+
+
+@pytest.mark.gpu
+def test_logits_infinite_penalties(hip):
+    """They forbid the answer's tokens, not the prompt's; ids at the ends of their type count nothing."""
+    x = torch.randn(2, 3000, generator=_gen(67), device="cuda")
+    ends = [-2 ** 63, 2 ** 63 - 1, -1, 3000]
+    history = torch.tensor([[5, 2500, 7, 2600, 5] + ends] * 2, device="cuda")
+    kw = dict(history=history, prompt_lens=torch.tensor([2, 0], dtype=torch.int32, device="cuda"),
+              bias_ids=torch.tensor([ends] * 2, device="cuda"), bias=torch.ones(2, 4, device="cuda"))
+    for name in ("frequency", "presence"):
+        got = _check_logits(x, {**kw, name: torch.full((2,), math.inf, device="cuda")})
+        assert got[0, 2500] == x[0, 2500] and (got[0, [5, 7, 2600]] == -math.inf).all() and (got[1, [5, 7, 2500, 2600]] == -math.inf).all()
 
 
 @pytest.mark.gpu
