@@ -99,7 +99,7 @@ __device__ __forceinline__ PagedSeq paged_seq(int s0, int s1, int len, int token
 
 __device__ __forceinline__ int sread(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// A scalar load: p the same in every lane, its memory written by no kernel of this library.
+// A scalar load: p the same in every lane, its memory not written while the kernel runs.
 __device__ __forceinline__ int sload(const int* p) {
   return *(const __attribute__((address_space(4))) int*)p;
 }

@@ -467,6 +467,8 @@ extern "C" int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const v
   if (workspace == nullptr || workspace_bytes < spectra_paged_attend_workspace(hd))
     return fail(SPECTRA_ERR_WORKSPACE, "workspace missing or smaller than spectra_paged_attend_workspace bytes");
   SPECTRA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  const int64_t tiles = tokens * kv->kv_heads * ((g + 15) / 16);
+  SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
   const PagedPools pools = paged_pools(kv);
   if (int st = paged_apart({{"out", out, tokens * heads * hd * 2, 0, 1},
                             {"the workspace", workspace, (int64_t)spectra_paged_attend_workspace(hd), 0, 1}},
@@ -483,9 +485,7 @@ extern "C" int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const v
   SPECTRA_REQUIRE(sc.mul > 0.0f && sc.mul < 1e30f && sc.cap2 < 1e30f, "scale or cap out of range");
   const int mod = sc.cap2 > kPagedCap ? kModLargeCap : cap > 0.0f ? kMod : kModNone;
   // at most as many steps as the lists have
-  const int64_t tiles = tokens * kv->kv_heads * ((g + 15) / 16);
   const int64_t total = tiles * (((int64_t)count * kv->page_size + kBlkKeys - 1) / kBlkKeys);
-  SPECTRA_REQUIRE(tiles < (1LL << 28), "tokens out of range");
   const int64_t groups = std::min<int64_t>(total, 256 * kBlkResident);
   bool wide = total >= (1LL << 29);
   // (counters as far apart as there is room: atomics on one line wait for each other)

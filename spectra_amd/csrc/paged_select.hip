@@ -565,7 +565,8 @@ extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_
                   "q must be 16-byte aligned, blocks aligned");
   SPECTRA_REQUIRE(sink >= 0 && local >= 1 && count >= 1 && (int64_t)sink + local <= count,
                   "count must hold the first `sink` and the last `local` (at least one) blocks");
-  SPECTRA_REQUIRE(count <= kSelMost && tokens * kv->kv_heads * count < (1LL << 40), "count out of range");
+  SPECTRA_REQUIRE(count <= kSelMost, "count out of range");
+  SPECTRA_REQUIRE(tokens * kv->kv_heads < (1LL << 31), "tokens out of range");
   if (kv->table_width > kSelMost) return fail(SPECTRA_ERR_UNSUPPORTED, "block tables of more than 32768 pages");
   const int pitch = (kv->table_width + 63) & ~63, rows = 16 * ((g + 15) / 16);
   // (64 users of up to 250 pages: 12.6 us with 256 or 512 threads; a chunk of 300 on 30000 keys 21.5 with 256, 24.7 with 512,
@@ -598,7 +599,6 @@ extern "C" int spectra_paged_select(const spectra_paged_kv_t* kv, const spectra_
   int group = tokens < 32 / gp * seqs ? 1 : 16 / gp;
   while (lds_of(group) > kSelLds) group /= 2;
   const int64_t groups = (tokens + group - 1) / group * kv->kv_heads;
-  SPECTRA_REQUIRE(groups < (1LL << 31), "tokens out of range");
   const int lds = lds_of(group);
   // units of one step each, few of them, and pages enough for several workgroups
   if (workspace != nullptr && groups <= kSelSplit && kv->table_width >= 1024 && (group == 1 || kv->batch == 1)) {
