@@ -1287,3 +1287,40 @@ def test_logits_of_long_histories(hip, rows, vocab):
     if rows == 2:
         x, kw = _case(rows, vocab, torch.float32, 66, history=10, biases=70000)
         _check_logits(x, kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 300, 6000, 32767, 32768])
+def test_select_the_largest_tables(hip, count):
+    """32768 pages a sequence, as many as a selection takes; all of them, all but one, and few."""
+    from spectra_amd import kernels as K
+    n, pages = 32768, 500
+    g = _gen(68)
+    q = torch.randn(2, 4, 128, generator=g, device="cuda").half()
+    codes = torch.randint(-30, 128, (pages, 1, 2, 128), generator=g, device="cuda", dtype=torch.int8)
+    codes[:, :, 1] = -codes[:, :, 1]
+    scales = torch.rand(pages, 1, generator=g, device="cuda") + 0.1
+    table = torch.randint(0, pages, (1, n), generator=g, device="cuda", dtype=torch.int32)  # the pages again and again
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([16 * n], [0, 2]))
+    got = K.paged_select(q, lens, starts, table, (codes, scales), 16, count, sink=0, local=1)
+    c, s, t = codes.cpu().numpy(), scales.cpu().numpy(), table.cpu().numpy()
+    for i in range(2):
+        assert got[i, 0].tolist() == _selected(q[i], c[:, 0], s[:, 0], t[0], n, count, 0, 1)
+    assert torch.equal(got, K.paged_select(q, lens, starts, table, (codes, scales), 16, count, sink=0, local=1,
+                                           workspace=K.paged_select_workspace()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [256, 2048])
+def test_large_pages(hip, kind, page):
+    """Pages of more rows than a wave or a step takes at once."""
+    from spectra_amd import kernels as K
+    b = Batch(kind, [1, 3], [5 * page - 7, page + 130], 4, 2, 128, page, seed=69)
+    before = K.paged_bounds(b.k)
+    _check_bounds(b, K.paged_key_bounds(b.tokens, b.kv_lens, b.q_start, b.table, b.k, K.paged_bounds(b.k)), before)
+    bounds = _random_bounds(b, 17)
+    blocks = K.paged_select(b.q, b.kv_lens, b.q_start, b.table, bounds, page, 3)
+    _check_select(b, bounds, 3, 1, 2, blocks)
+    want, tol = _blocks_reference(b, blocks)
+    _close(_attend(b, blocks), want, tol)
