@@ -31,12 +31,21 @@ struct BlkTile {
   pu4_t k[2][HD / 32];
   uint32_t v[2][4][HD / 32];
 };
-// 32 keys of 4-bit K and V in LDS, a wave's own: codes, scales and zero points of both.
+// 32 keys of 4-bit K and V in LDS, a wave's own: codes (K's, then V's), scales, zero points.  A half's 16 keys are brought
+// by half of the lanes, so that a lane has one page: of 64 dims scales, and of both sizes zero points, lie as K's and V's of
+// the first 16 keys, then of the others.
 template <int HD>
 struct BlkCodes {
-  static constexpr int kCodes = 16 * HD, kScales = 2 * HD, kZeros = HD;  // bytes of 32 keys
-  static constexpr int kV = kCodes, kS = 2 * kCodes, kZ = kS + 2 * kScales, kBytes = kZ + 2 * kZeros;
+  static constexpr int kV = 16 * HD, kS = 2 * kV, kZ = kS + 4 * HD;
+  static constexpr int kBytes = kZ + (HD == 128 ? 256 : 192);
   static constexpr int kCopies = HD == 128 ? 7 : 4;  // instructions that bring them
+  // of a key of a half, and group of 32 dims
+  static __device__ __forceinline__ int scale(int v, int half, int key, int group) {
+    return kS + (HD == 128 ? 256 * v + 128 * half : 128 * half + 64 * v) + 2 * (key * (HD / 32) + group);
+  }
+  static __device__ __forceinline__ int zero(int v, int half, int key, int group) {
+    return kZ + 128 * half + (HD / 2) * v + key * (HD / 32) + group;
+  }
 };
 template <int HD, int KIND>
 constexpr int blk_lds() {
@@ -50,9 +59,17 @@ struct BlkHalf {
   bool bad;
 };
 
+// The larger of the values of lanes LB apart.
+template <int LB>
+__device__ __forceinline__ float lane_most(float v) {
+  const int iv = __builtin_bit_cast(int, v);
+  const auto r = LB == 16 ? __builtin_amdgcn_permlane16_swap(iv, iv, false, false) : __builtin_amdgcn_permlane32_swap(iv, iv, false, false);
+  return fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
+}
+
 template <int HD, int KIND, int MOD>
 __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
-    paged_blocks_kernel(const PagedKv kv, const PagedScore sc, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
+    paged_blocks_kernel(const PagedKv kv, float mul, float cap2, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                         const int* __restrict__ blocks, int count, bool wide, int apart,
                          uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
@@ -67,6 +84,7 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
   // neighbouring workgroups go to different XCDs: an eighth of the line each, so that the tokens of a sequence and KV head,
   // whose lists have pages in common, meet in one L2
   const int share = (gridDim.x & 7) != 0 ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const PagedScore sc = {mul, cap2, nullptr, nullptr, 0};
   PagedKv line = kv;  // (for the walk: rows are tokens, heads their tiles)
   line.kv_heads = kv.kv_heads * groups;
   PagedScore most{};
@@ -94,7 +112,6 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     }
 
     // the lane's row (column c): its queries, B operands
-    const float slope2 = 0.0f;
     pu4_t qf[KS];
     {
       const uint16_t* qr = q + (int64_t)tok * ldq + (int64_t)(h0 + min(c, nrows - 1)) * HD;
@@ -150,31 +167,37 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
         }
       }
     };
-    // 4 bits: to LDS at `to`, whose last reads are complete
+    // 4 bits: to LDS at `at`, whose last reads are complete.  Addresses are a lane's own: its half's page and 16 rows in
+    // units of 16 bytes, one product, and the arrays' bases (a wave's, they took half of the loop's scalar registers).
     typedef BlkCodes<HD> C;
+    const int hl = lane >> 5, group0 = kvh << (kv.page_shift - 4);
+    const bool zv = (lane & (HD / 8)) != 0;
+    const uint8_t* sbase = Q4 ? (HD == 128 || lane % 32 < 16 ? kv.ks : kv.vs) + 4 * (lane % (HD / 4)) : nullptr;
+    const uint8_t* zbase = Q4 ? (zv ? kv.vz : kv.kz) + 4 * (lane % (HD / 8)) : nullptr;
     auto fetch = [&](uint32_t at, int key0, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const int row0 = (kvh << kv.page_shift) + (key0 & pmask), row1 = (kvh << kv.page_shift) + ((key0 + 16) & pmask);
-      const int p0 = hf[0].page, p1 = hf[1].page;
-      const uint64_t a0 = paged_at(p0, kv.page_step) + row0 * ROWB, a1 = paged_at(p1, kv.page_step) + row1 * ROWB;
-      const uint64_t s0 = paged_at(p0, kv.scale_step) + row0 * (HD / 16), s1 = paged_at(p1, kv.scale_step) + row1 * (HD / 16);
-      const uint64_t z0 = paged_at(p0, kv.zero_step) + row0 * (HD / 32), z1 = paged_at(p1, kv.zero_step) + row1 * (HD / 32);
+      const uint32_t page = hl ? hf[1].page : hf[0].page, row = group0 + (((key0 >> 4) + hl) & (pmask >> 4));  // (16 rows each)
+      auto place = [&](uint32_t step, uint32_t each, uint32_t more) __attribute__((always_inline)) {
+        return ((uint64_t)page * step + (row * each + more)) << 4;
+      };
+      const uint64_t sc0 = place(kv.scale_step, HD / 16, 0), ze0 = place(kv.zero_step, HD / 32, 0);
       if constexpr (HD == 128) {
         const uint32_t off = 16 * lane;
+        const int row0 = (kvh << kv.page_shift) + (key0 & pmask), row1 = (kvh << kv.page_shift) + ((key0 + 16) & pmask);
+        const uint64_t a0 = paged_at(hf[0].page, kv.page_step) + row0 * ROWB, a1 = paged_at(hf[1].page, kv.page_step) + row1 * ROWB;
         copy_lds(kv.k + a0, off, at);
         copy_lds(kv.k + a1, off, at + 1024);
         copy_lds(kv.v + a0, off, at + C::kV);
         copy_lds(kv.v + a1, off, at + C::kV + 1024);
-        const uint64_t s = (lane < 32 ? s0 : s1) + 4 * (lane & 31);
-        copy_lds4(kv.ks + s, at + C::kS);
-        copy_lds4(kv.vs + s, at + C::kS + C::kScales);
-        copy_lds4((lane < 32 ? kv.kz : kv.vz) + ((lane & 16) == 0 ? z0 : z1) + 4 * (lane & 15), at + C::kZ);
+        copy_lds4(sbase + sc0, at + C::kS);
+        copy_lds4(sbase + (kv.vs - kv.ks) + sc0, at + C::kS + 256);
+        copy_lds4(zbase + ze0, at + C::kZ);
       } else {
-        const uint64_t a = (lane < 32 ? a0 : a1) + 16 * (lane & 31);
+        const uint64_t a = place(kv.page_step, HD / 2, lane & 31);
         copy_lds16(kv.k + a, at);
         copy_lds16(kv.v + a, at + C::kV);
-        copy_lds4((lane < 32 ? kv.ks : kv.vs) + ((lane & 16) == 0 ? s0 : s1) + 4 * (lane & 15), at + C::kS);
-        if (lane < 32) copy_lds4((lane < 16 ? kv.kz : kv.vz) + ((lane & 8) == 0 ? z0 : z1) + 4 * (lane & 7), at + C::kZ);
+        copy_lds4(sbase + sc0, at + C::kS);
+        if ((lane & 16) == 0) copy_lds4(zbase + ze0, at + C::kZ);
       }
     };
 
@@ -190,7 +213,7 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
         s[h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
         if constexpr (Q4) {
           const int key = 16 * h + c, kg = HD == 128 ? q4 : q4 >> 1;  // group of the lane's dims
-          const uint32_t zb = t[C::kZ + key * (HD / 32) + kg], sb = *(const uint16_t*)(t + C::kS + 2 * (key * (HD / 32) + kg));
+          const uint32_t zb = t[C::zero(0, h, c, kg)], sb = *(const uint16_t*)(t + C::scale(0, h, c, kg));
           const Kv4Zero z = kv4_zero(zb | zb << 16);
           const ph2_t sf = __builtin_bit_cast(ph2_t, sb | sb << 16);
           uint32_t w[KS];
@@ -211,22 +234,25 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
         }
       }
       const bool part = hf[0].seen < 16 || hf[1].seen < 16;  // keys that the row does not see: their values must not reach the product
-      // scores of the keys 16 (e / 4) + 4 q4 + e % 4
-      float y[8], mn = m, mul = sc.mul;
-      if constexpr (MOD != kModNone) mul = paged_scores<MOD, 2, 4>(s, sc, slope2, 0.0f, [](int n) { return n; });
+      // scores of the keys 16 (e / 4) + 4 q4 + e % 4, but for a positive factor
+      float y[8], by = sc.mul;
+      if constexpr (MOD != kModNone) by = paged_scores<MOD, 2, 4>(s, sc, 0.0f, 0.0f, [](int n) { return n; });
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3] * mul;
+      for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3];
       if (part || hf[0].bad || hf[1].bad) {
+        int seen[2] = {hf[0].seen, hf[1].seen};
+        asm volatile("" : "+v"(seen[0]), "+v"(seen[1]));  // (or the comparisons are made for every tile, ahead of the branch)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (hf[e >> 2].bad) y[e] = NAN;
-          if (4 * q4 + (e & 3) >= hf[e >> 2].seen) y[e] = -INFINITY;
+          if (4 * q4 + (e & 3) >= seen[e >> 2]) y[e] = -INFINITY;
         }
       }
+      float mn = y[0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mn = fmaxf(mn, y[e]);
-      mn = fmaxf(mn, lane_xor<16>(mn, lane));
-      mn = fmaxf(mn, lane_xor<32>(mn, lane));
+      for (int e = 1; e < 8; ++e) mn = fmaxf(mn, y[e]);
+      mn = lane_most<16>(mn);
+      mn = fmaxf(m, lane_most<32>(mn) * by);
       if (__ballot(mn > m + kPagedSlack) != 0) {
         const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
         l *= corr;
@@ -239,7 +265,7 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
       const float mu = m == -INFINITY ? 0.0f : m - kPagedRaise<BF>;
       pu4_t pf;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(y[e] - mu);
+      for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], by, -mu));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {  // (the total is of the weights as rounded, so that a mean of values lies among them)
         pf[e] = pack2<BF>(y[2 * e], y[2 * e + 1]);
@@ -263,9 +289,9 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const int key = 16 * (p >> 1) + 4 * q4 + 2 * (p & 1);  // and the next
-          const uint8_t* zp = t + C::kZ + C::kZeros + key * (HD / 32) + vg;
+          const uint8_t* zp = t + C::zero(1, p >> 1, 4 * q4 + 2 * (p & 1), vg);
           z2[p] = kv4_zero((uint32_t)zp[0] | (uint32_t)zp[HD / 32] << 16);
-          const uint8_t* sp = t + C::kS + C::kScales + 2 * (key * (HD / 32) + vg);
+          const uint8_t* sp = t + C::scale(1, p >> 1, 4 * q4 + 2 * (p & 1), vg);
           s2[p] = __builtin_bit_cast(ph2_t, ((uint32_t)*(const uint16_t*)sp | (uint32_t)*(const uint16_t*)(sp + HD / 16) << 16) & keep[p]);
           const uint8_t* vp = t + C::kV + key * ROWB + c * (ROWB / 16);
           if constexpr (HD == 128) {
@@ -495,7 +521,7 @@ extern "C" int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const v
   float* slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
   int gv = g, hv = heads, cv = count;
   const void* kern = hd == 64 ? blocks_of<64>(kv->kind, mod) : blocks_of<128>(kv->kind, mod);
-  void* args[] = {(void*)&p, (void*)&sc, (void*)&q, (void*)&ldq, (void*)&gv, (void*)&hv, (void*)&blocks, (void*)&cv,
+  void* args[] = {(void*)&p, (void*)&sc.mul, (void*)&sc.cap2, (void*)&q, (void*)&ldq, (void*)&gv, (void*)&hv, (void*)&blocks, (void*)&cv,
                   (void*)&wide, (void*)&apart, (void*)&counters, (void*)&slots, (void*)&out};
   SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)groups), dim3(kBlkThreads), args, 0, (hipStream_t)stream));
   SPECTRA_HIP_CHECK(hipGetLastError());
