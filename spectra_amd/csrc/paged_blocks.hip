@@ -47,9 +47,10 @@ struct BlkCodes {
     return kZ + 128 * half + (HD / 2) * v + key * (HD / 32) + group;
   }
 };
-template <int HD, int KIND>
+// GP: columns that a tile takes of 16 (its rows, at most as many).
+template <int HD, int KIND, int GP>
 constexpr int blk_lds() {
-  const int red = 4 * 16 * (HD + 4) * 4, ring = KIND == kKv4 ? 4 * 2 * BlkCodes<HD>::kBytes : 0;
+  const int red = 4 * 16 * (HD + 4) * 4, ring = KIND == kKv4 ? 4 * 2 * (16 / GP) * BlkCodes<HD>::kBytes : 0;
   return red > ring ? red : ring;
 }
 // Sixteen keys of one page: the position of the first, and how many of them the row sees; where they lie (page 0 for a
@@ -67,15 +68,15 @@ __device__ __forceinline__ float lane_most(float v) {
   return fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
 }
 
-template <int HD, int KIND, int MOD>
+template <int HD, int KIND, int MOD, int GP>
 __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     paged_blocks_kernel(const PagedKv kv, float mul, float cap2, const uint16_t* __restrict__ q, int64_t ldq, int g, int heads,
                         const int* __restrict__ blocks, int count, bool wide, int apart,
                          uint32_t* __restrict__ counters, float* __restrict__ slots, uint16_t* __restrict__ out) {
   constexpr bool Q4 = KIND == kKv4, BF = KIND == kKvBf16;
-  constexpr int ROWS = 16, KS = HD / 32, DPL = HD / 16, RS = HD + 4;
+  constexpr int ROWS = 16, KS = HD / 32, DPL = HD / 16, RS = HD + 4, PACK = 16 / GP;
   constexpr int ROWB = Q4 ? HD / 2 : 2 * HD;  // bytes of a row of a page
-  __shared__ __align__(16) uint8_t pool[blk_lds<HD, KIND>()];  // 4-bit keys on their way; at the end the waves' sums
+  __shared__ __align__(16) uint8_t pool[blk_lds<HD, KIND, GP>()];  // 4-bit keys on their way; at the end the waves' sums
   float* red = (float*)pool;
   __shared__ float wm[4][ROWS], wl[4][ROWS];
   __shared__ int flag;
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     // the lane's row (column c): its queries, B operands
     pu4_t qf[KS];
     {
-      const uint16_t* qr = q + (int64_t)tok * ldq + (int64_t)(h0 + min(c, nrows - 1)) * HD;
+      const uint16_t* qr = q + (int64_t)tok * ldq + (int64_t)(h0 + min(c % GP, nrows - 1)) * HD;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         pu4_t y = *(const pu4_t*)(qr + (Q4 ? (HD / 4) * q4 + 8 * s : 32 * s + 8 * q4));
@@ -124,6 +125,14 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
         qf[s] = y;
       }
     }
+
+    pu4_t qn[PACK][KS];  // 4 bits: the queries in tile n's columns
+#pragma unroll
+    for (int n = 0; n < PACK; ++n)
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qn[n][st][e] = c / GP == n ? qf[st][e] : 0u;
 
     // ---- loads: rows a tile ahead of their use, the pages' ids two, the list's entries three
     const int* tab = kv.table + un.b * kv.table_stride;
@@ -174,9 +183,8 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     const bool zv = (lane & (HD / 8)) != 0;
     const uint8_t* sbase = Q4 ? (HD == 128 || lane % 32 < 16 ? kv.ks : kv.vs) + 4 * (lane % (HD / 4)) : nullptr;
     const uint8_t* zbase = Q4 ? (zv ? kv.vz : kv.kz) + 4 * (lane % (HD / 8)) : nullptr;
-    auto fetch = [&](uint32_t at, int key0, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const uint32_t page = hl ? hf[1].page : hf[0].page, row = group0 + (((key0 >> 4) + hl) & (pmask >> 4));  // (16 rows each)
+    auto fetch = [&](uint32_t at, int key0, int p0, int p1) __attribute__((always_inline)) {
+      const uint32_t page = hl ? p1 : p0, row = group0 + (((key0 >> 4) + hl) & (pmask >> 4));  // (16 rows each)
       auto place = [&](uint32_t step, uint32_t each, uint32_t more) __attribute__((always_inline)) {
         return ((uint64_t)page * step + (row * each + more)) << 4;
       };
@@ -184,7 +192,7 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
       if constexpr (HD == 128) {
         const uint32_t off = 16 * lane;
         const int row0 = (kvh << kv.page_shift) + (key0 & pmask), row1 = (kvh << kv.page_shift) + ((key0 + 16) & pmask);
-        const uint64_t a0 = paged_at(hf[0].page, kv.page_step) + row0 * ROWB, a1 = paged_at(hf[1].page, kv.page_step) + row1 * ROWB;
+        const uint64_t a0 = paged_at(p0, kv.page_step) + row0 * ROWB, a1 = paged_at(p1, kv.page_step) + row1 * ROWB;
         copy_lds(kv.k + a0, off, at);
         copy_lds(kv.k + a1, off, at + 1024);
         copy_lds(kv.v + a0, off, at + C::kV);
@@ -205,49 +213,8 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     pf4_t o[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[j] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
-    // t: the tile's registers, or its place in LDS
-    auto compute = [&](const auto& t, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
-      pf4_t s[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (Q4) {
-          const int key = 16 * h + c, kg = HD == 128 ? q4 : q4 >> 1;  // group of the lane's dims
-          const uint32_t zb = t[C::zero(0, h, c, kg)], sb = *(const uint16_t*)(t + C::scale(0, h, c, kg));
-          const Kv4Zero z = kv4_zero(zb | zb << 16);
-          const ph2_t sf = __builtin_bit_cast(ph2_t, sb | sb << 16);
-          uint32_t w[KS];
-          if constexpr (HD == 128) {
-            const pu4_t y = *(const pu4_t*)(t + key * ROWB + 16 * q4);
-#pragma unroll
-            for (int st = 0; st < KS; ++st) w[st] = y[st];
-          } else {
-            const uint2 y = *(const uint2*)(t + key * ROWB + 8 * q4);
-            w[0] = y.x;
-            w[1] = y.y;
-          }
-#pragma unroll
-          for (int st = 0; st < KS; ++st) s[h] = mfma16<BF>(kv4_pairs(w[st], z, sf), qf[st], s[h]);
-        } else {
-#pragma unroll
-          for (int st = 0; st < KS; ++st) s[h] = mfma16<BF>(t.k[h][st], qf[st], s[h]);
-        }
-      }
-      const bool part = hf[0].seen < 16 || hf[1].seen < 16;  // keys that the row does not see: their values must not reach the product
-      // scores of the keys 16 (e / 4) + 4 q4 + e % 4, but for a positive factor
-      float y[8], by = sc.mul;
-      if constexpr (MOD != kModNone) by = paged_scores<MOD, 2, 4>(s, sc, 0.0f, 0.0f, [](int n) { return n; });
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3];
-      if (part || hf[0].bad || hf[1].bad) {
-        int seen[2] = {hf[0].seen, hf[1].seen};
-        asm volatile("" : "+v"(seen[0]), "+v"(seen[1]));  // (or the comparisons are made for every tile, ahead of the branch)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (hf[e >> 2].bad) y[e] = NAN;
-          if (4 * q4 + (e & 3) >= seen[e >> 2]) y[e] = -INFINITY;
-        }
-      }
+    // the weights of scores (but for a positive factor `by`), the running maximum and total
+    auto weights = [&](float (&y)[8], float by) __attribute__((always_inline)) {
       float mn = y[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mn = fmaxf(mn, y[e]);
@@ -271,29 +238,137 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
         pf[e] = pack2<BF>(y[2 * e], y[2 * e + 1]);
         l = add2<BF>(pf[e], l);
       }
-      // O^T += V^T P^T, dims DPL (l % 16) + j at step j: the 8 keys' values of a dim, in pairs of keys
-      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-      if (part) {
+      return pf;
+    };
+    // which of a pair's keys 16 (p / 2) + 4 q4 + 2 (p % 2) and the next the row sees, of two halves
+    auto kept = [&](uint32_t (&keep)[4], int s0, int s1) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int key = 4 * q4 + 2 * (p & 1), n = hf[p >> 1].seen;
-          keep[p] = (key < n ? 0xffffu : 0u) | (key + 1 < n ? 0xffff0000u : 0u);
+      for (int p = 0; p < 4; ++p) {
+        const int key = 4 * q4 + 2 * (p & 1), n = p < 2 ? s0 : s1;
+        keep[p] = (key < n ? 0xffffu : 0u) | (key + 1 < n ? 0xffff0000u : 0u);
+      }
+    };
+    // 16 bits: a tile in registers
+    auto compute = [&](const Tile& t, const BlkHalf (&hf)[2]) __attribute__((always_inline)) {
+      pf4_t s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < KS; ++st) s[h] = mfma16<BF>(t.k[h][st], qf[st], s[h]);
+      }
+      const bool part = hf[0].seen < 16 || hf[1].seen < 16;  // keys that the row does not see: their values must not reach the product
+      // scores of the keys 16 (e / 4) + 4 q4 + e % 4
+      float y[8], by = sc.mul;
+      if constexpr (MOD != kModNone) by = paged_scores<MOD, 2, 4>(s, sc, 0.0f, 0.0f, [](int n) { return n; });
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3];
+      if (part || hf[0].bad || hf[1].bad) {
+        int seen[2] = {hf[0].seen, hf[1].seen};
+        asm volatile("" : "+v"(seen[0]), "+v"(seen[1]));  // (or the comparisons are made for every tile, ahead of the branch)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (hf[e >> 2].bad) y[e] = NAN;
+          if (4 * q4 + (e & 3) >= seen[e >> 2]) y[e] = -INFINITY;
         }
       }
-      if constexpr (Q4) {
-        constexpr int HALF = HD / 64;  // codes of 4 dims each
-        const int vg = c * DPL / 32;   // group of the lane's dims
+      const pu4_t pf = weights(y, by);
+      // O^T += V^T P^T, dims DPL (l % 16) + j at step j: the 8 keys' values of a dim, in pairs of keys
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (part) kept(keep, hf[0].seen, hf[1].seen);
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) {
+        pu4_t a;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          a[p] = __builtin_amdgcn_perm(t.v[p >> 1][2 * (p & 1) + 1][j >> 1], t.v[p >> 1][2 * (p & 1)][j >> 1],
+                                       (j & 1) ? 0x07060302u : 0x05040100u);
+          if (part) a[p] &= keep[p];
+        }
+        o[j] = mfma16<BF>(a, pf, o[j]);
+      }
+    };
+    // 4 bits: up to PACK tiles, kBlkKeys keys apart, in LDS from `t` on, whose scores take columns of their own: tile n's
+    // products are those of queries that are zero in the other's columns, and its weights are zero there.  So a row's 8
+    // columns, not 16, are exponentiated for a tile.  (All columns are of one row's keys: a value or a key that is NaN or
+    // infinite, of one tile, makes the row so through either's columns.)  half(x): tile x / 2's half x % 2; odd: not all
+    // keys are seen, or a page is not there.
+    auto packed = [&](const uint8_t* t, int tiles, bool odd, auto half) __attribute__((always_inline)) {
+      const int mine = c / GP;  // the tile of the lane's column
+      pf4_t s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+      for (int n = 0; n < PACK; ++n) {
+        if (n >= tiles) break;
+        const uint8_t* tn = t + n * C::kBytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int kg = HD == 128 ? q4 : q4 >> 1;  // group of the lane's dims
+          const uint32_t zb = tn[C::zero(0, h, c, kg)];
+          uint32_t sb = *(const uint16_t*)(tn + C::scale(0, h, c, kg));
+          if (PACK > 1 && odd) sb = c < half(2 * n + h).seen ? sb : 0u;  // (NaN of no key would reach the other tile's columns)
+          const Kv4Zero z = kv4_zero(zb | zb << 16);
+          const ph2_t sf = __builtin_bit_cast(ph2_t, sb | sb << 16);
+          uint32_t w[KS];
+          if constexpr (HD == 128) {
+            const pu4_t y = *(const pu4_t*)(tn + (16 * h + c) * ROWB + 16 * q4);
+#pragma unroll
+            for (int st = 0; st < KS; ++st) w[st] = y[st];
+          } else {
+            const uint2 y = *(const uint2*)(tn + (16 * h + c) * ROWB + 8 * q4);
+            w[0] = y.x;
+            w[1] = y.y;
+          }
+#pragma unroll
+          for (int st = 0; st < KS; ++st) s[h] = mfma16<BF>(kv4_pairs(w[st], z, sf), qn[n][st], s[h]);
+        }
+      }
+      float y[8], by = sc.mul;
+      if constexpr (MOD != kModNone) by = paged_scores<MOD, 2, 4>(s, sc, 0.0f, 0.0f, [](int n) { return n; });
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3];
+      if (odd) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int seen = 0;
+          bool bad = false;
+#pragma unroll
+          for (int n = 0; n < PACK; ++n) {
+            seen = PACK == 1 || mine == n ? half(2 * n + h).seen : seen;
+            bad = PACK == 1 || mine == n ? half(2 * n + h).bad : bad;
+          }
+          asm volatile("" : "+v"(seen));  // (or the comparisons are made for every tile, ahead of the branch)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (bad) y[4 * h + e] = NAN;
+            if (4 * q4 + e >= seen) y[4 * h + e] = -INFINITY;
+          }
+        }
+      }
+      const pu4_t pf = weights(y, by);
+      constexpr int HALF = HD / 64;  // codes of 4 dims each
+      const int vg = c * DPL / 32;   // group of the lane's dims
+#pragma unroll
+      for (int n = 0; n < PACK; ++n) {
+        if (n >= tiles) break;
+        const uint8_t* tn = t + n * C::kBytes;
+        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+        if (odd) kept(keep, half(2 * n).seen, half(2 * n + 1).seen);
+        pu4_t pn = pf;
+        if constexpr (PACK > 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pn[e] = mine == n ? pf[e] : 0u;
+        }
         Kv4Zero z2[4];
         ph2_t s2[4];
         uint32_t v0[4], v1[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const int key = 16 * (p >> 1) + 4 * q4 + 2 * (p & 1);  // and the next
-          const uint8_t* zp = t + C::zero(1, p >> 1, 4 * q4 + 2 * (p & 1), vg);
+          const int key = 4 * q4 + 2 * (p & 1);  // of the half, and the next
+          const uint8_t* zp = tn + C::zero(1, p >> 1, key, vg);
           z2[p] = kv4_zero((uint32_t)zp[0] | (uint32_t)zp[HD / 32] << 16);
-          const uint8_t* sp = t + C::scale(1, p >> 1, 4 * q4 + 2 * (p & 1), vg);
+          const uint8_t* sp = tn + C::scale(1, p >> 1, key, vg);
           s2[p] = __builtin_bit_cast(ph2_t, ((uint32_t)*(const uint16_t*)sp | (uint32_t)*(const uint16_t*)(sp + HD / 16) << 16) & keep[p]);
-          const uint8_t* vp = t + C::kV + key * ROWB + c * (ROWB / 16);
+          const uint8_t* vp = tn + C::kV + (16 * (p >> 1) + key) * ROWB + c * (ROWB / 16);
           if constexpr (HD == 128) {
             v0[p] = *(const uint32_t*)vp;
             v1[p] = *(const uint32_t*)(vp + ROWB);
@@ -309,22 +384,10 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
           for (int p = 0; p < 4; ++p) {
             const pu4_t w = kv4_pairs(__builtin_amdgcn_perm(v1[p], v0[p], u ? 0x07060302u : 0x05040100u), z2[p], s2[p]);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) a[n][p] = w[n];
+            for (int i = 0; i < 4; ++i) a[i][p] = w[i];
           }
 #pragma unroll
-          for (int n = 0; n < 4; ++n) o[4 * u + n] = mfma16<BF>(a[n], pf, o[4 * u + n]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < DPL; ++j) {
-          pu4_t a;
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            a[p] = __builtin_amdgcn_perm(t.v[p >> 1][2 * (p & 1) + 1][j >> 1], t.v[p >> 1][2 * (p & 1)][j >> 1],
-                                         (j & 1) ? 0x07060302u : 0x05040100u);
-            if (part) a[p] &= keep[p];
-          }
-          o[j] = mfma16<BF>(a, pf, o[j]);
+          for (int i = 0; i < 4; ++i) o[4 * u + i] = mfma16<BF>(a[i], pn, o[4 * u + i]);
         }
       }
     };
@@ -333,8 +396,15 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     int key = sbeg * kBlkKeys + 32 * wave;
     if (key < kend) {
       // blocks and ids of the next tile's halves, blocks of the one after it
-      int b0 = listed(key), b1 = listed(key + 16), m0 = listed(key + kBlkKeys), m1 = listed(key + kBlkKeys + 16);
-      int id0 = page_of(b0), id1 = page_of(b1);
+      int b0 = 0, b1 = 0, m0 = 0, m1 = 0, id0 = 0, id1 = 0;
+      auto first = [&]() __attribute__((always_inline)) {
+        b0 = listed(key);
+        b1 = listed(key + 16);
+        m0 = listed(key + kBlkKeys);
+        m1 = listed(key + kBlkKeys + 16);
+        id0 = page_of(b0);
+        id1 = page_of(b1);
+      };
       auto next = [&](BlkHalf (&hf)[2], int k) __attribute__((always_inline)) {
         hf[0] = half_of(k, b0, id0);
         hf[1] = half_of(k + 16, b1, id1);
@@ -347,29 +417,82 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
         m0 = listed(k + kBlkKeys);
         m1 = listed(k + kBlkKeys + 16);
       };
-      BlkHalf ha[2], hb[2];
-      next(ha, key);
-      if constexpr (Q4) {
-        uint8_t* mine = pool + wave * 2 * C::kBytes;
-        const uint32_t at0 = (uint32_t)(uintptr_t)(lds_t)mine;
-        fetch(at0, key, ha);
+      uint8_t* mine = pool + wave * 2 * PACK * C::kBytes;  // (4 bits)
+      const uint32_t at0 = (uint32_t)(uintptr_t)(lds_t)mine;
+      if constexpr (Q4 && HD == 64) {
+        // PACK tiles at a time in LDS, and the next PACK on their way.  A lane looks up one of their halves (for the wave they
+        // would take more scalar registers than there are; of 128 dims a lane's lookups lost more than the packing gained, 64
+        // users 26 us, not 24), by loads that go before the tiles' copies, which are counted below.
+        constexpr int STEP = PACK * kBlkKeys;
+        const int tile = (lane % (2 * PACK)) >> 1, apart = tile * kBlkKeys + 16 * (lane & 1);
+        auto entry = [&](int k) __attribute__((always_inline)) { return list[max(min((k + apart) >> kv.page_shift, last), 0)]; };
+        auto id_of = [&](int b) __attribute__((always_inline)) { return tab[(uint32_t)b < (uint32_t)kv.table_width ? b : 0]; };
+        auto lane_of = [&](int k, int b, int id) __attribute__((always_inline)) {
+          BlkHalf h = half_of(k + apart, b, id);
+          if (k + tile * kBlkKeys >= kend) h.seen = 0;
+          return h;
+        };
+        auto bring = [&](int turn, int k, const BlkHalf& in) __attribute__((always_inline)) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+          for (int n = 0; n < PACK; ++n)
+            if (k + n * kBlkKeys < kend)
+              fetch(at0 + (turn * PACK + n) * C::kBytes, k + n * kBlkKeys, __builtin_amdgcn_readlane(in.page, 2 * n),
+                    __builtin_amdgcn_readlane(in.page, 2 * n + 1));
+        };
+        int b = entry(key), m = entry(key + STEP), id = id_of(b);
+        BlkHalf now = lane_of(key, b, id), then = now;
+        b = m;
+        id = id_of(b);
+        m = entry(key + 2 * STEP);
+        bring(0, key, now);
+        for (int turn = 0;; turn ^= 1) {
+          if (key + STEP < kend) {
+            then = lane_of(key + STEP, b, id);
+            b = m;
+            id = id_of(b);
+            m = entry(key + 3 * STEP);
+            bring(turn ^ 1, key + STEP, then);
+          }
+          const int left = (kend - key + kBlkKeys - 1) / kBlkKeys;  // tiles; the copies of those after PACK may be on their way
+          if (left >= 2 * PACK) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PACK * C::kCopies) : "memory");
+          else if (left > PACK) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::kCopies) : "memory");
+          else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          packed(mine + turn * PACK * C::kBytes, min(PACK, left), __ballot(now.seen < 16 || now.bad) != 0, [&](int x) __attribute__((always_inline)) {
+            return BlkHalf{0, __builtin_amdgcn_readlane(now.seen, x), __builtin_amdgcn_readlane((int)now.bad, x) != 0};
+          });
+          key += STEP;
+          if (key >= kend) break;
+          now = then;
+        }
+      } else if constexpr (Q4) {
+        BlkHalf ha[2], hb[2];
+        first();
+        next(ha, key);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fetch(at0, key, ha[0].page, ha[1].page);
         ahead(key + kBlkKeys);
         for (int turn = 0;; turn ^= 1) {
           if (key + kBlkKeys < kend) {
             next(hb, key + kBlkKeys);
-            fetch(at0 + (turn ^ 1) * C::kBytes, key + kBlkKeys, hb);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch(at0 + (turn ^ 1) * C::kBytes, key + kBlkKeys, hb[0].page, hb[1].page);
             ahead(key + 2 * kBlkKeys);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::kCopies) : "memory");  // all but the next tile's
           } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
           }
-          compute(mine + turn * C::kBytes, ha);
+          packed(mine + turn * C::kBytes, 1, ha[0].seen < 16 || ha[1].seen < 16 || ha[0].bad || ha[1].bad,
+                 [&](int x) __attribute__((always_inline)) { return ha[x]; });
           key += kBlkKeys;
           if (key >= kend) break;
           ha[0] = hb[0];
           ha[1] = hb[1];
         }
       } else {
+        BlkHalf ha[2], hb[2];
+        first();
+        next(ha, key);
         // (the next tile is asked for behind the last one, too, whose rows it then has again: a branch around the loads would
         // have the rows before them waited for as if they were the newest, 1.05 GB in 188 us, not 180)
         Tile ta, tb;
@@ -422,18 +545,26 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     __syncthreads();
     for (int it = tid; it < nrows * (HD / 4); it += kBlkThreads) {
       const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
-      float mm = -INFINITY, den = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      // (all reads ahead: one behind the other they took a microsecond)
+      float mm = -INFINITY, den = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ms[4 * PACK], ls[4 * PACK];
+      float4 y[4 * PACK];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, wm[w][row]);
+      for (int w = 0; w < 4 * PACK; ++w) {
+        const int col = row + GP * (w % PACK);
+        ms[w] = wm[w / PACK][col];
+        ls[w] = wl[w / PACK][col];
+        y[w] = *(const float4*)(red + (w / PACK * 16 + col) * RS + d);
+      }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = paged_weight(wm[w][row], wl[w][row], mm);
-        const float4 y = *(const float4*)(red + (w * 16 + row) * RS + d);
-        den += f * wl[w][row];
-        v[0] += f * y.x;
-        v[1] += f * y.y;
-        v[2] += f * y.z;
-        v[3] += f * y.w;
+      for (int w = 0; w < 4 * PACK; ++w) mm = fmaxf(mm, ms[w]);
+#pragma unroll
+      for (int w = 0; w < 4 * PACK; ++w) {
+        const float f = paged_weight(ms[w], ls[w], mm);
+        den += f * ls[w];
+        v[0] += f * y[w].x;
+        v[1] += f * y[w].y;
+        v[2] += f * y[w].z;
+        v[3] += f * y[w].w;
       }
       if (whole) {
         write(row, d, v, den);
@@ -461,15 +592,21 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
   }
 }
 
-template <int HD, int KIND>
+template <int HD, int KIND, int GP>
 static const void* blocks_of(int mod) {
-  return mod == kModNone ? (const void*)paged_blocks_kernel<HD, KIND, kModNone>
-         : mod == kMod   ? (const void*)paged_blocks_kernel<HD, KIND, kMod>
-                         : (const void*)paged_blocks_kernel<HD, KIND, kModLargeCap>;
+  return mod == kModNone ? (const void*)paged_blocks_kernel<HD, KIND, kModNone, GP>
+         : mod == kMod   ? (const void*)paged_blocks_kernel<HD, KIND, kMod, GP>
+                         : (const void*)paged_blocks_kernel<HD, KIND, kModLargeCap, GP>;
 }
+// pack: two tiles at a time.
 template <int HD>
-static const void* blocks_of(int kind, int mod) {
-  return kind == kKv4 ? blocks_of<HD, kKv4>(mod) : kind == kKvBf16 ? blocks_of<HD, kKvBf16>(mod) : blocks_of<HD, kKvF16>(mod);
+static const void* blocks_of(int kind, int mod, bool pack) {
+  if (kind == kKvBf16) return blocks_of<HD, kKvBf16, 16>(mod);
+  if (kind == kKvF16) return blocks_of<HD, kKvF16, 16>(mod);
+  if constexpr (HD == 64) {
+    if (pack) return blocks_of<HD, kKv4, 8>(mod);
+  }
+  return blocks_of<HD, kKv4, 16>(mod);
 }
 
 }  // namespace spectra
@@ -520,7 +657,9 @@ extern "C" int spectra_paged_attend_blocks(const spectra_paged_kv_t* kv, const v
   uint32_t* counters = (uint32_t*)workspace;
   float* slots = (float*)((uint8_t*)workspace + SPECTRA_PAGED_COUNTER_BYTES);
   int gv = g, hv = heads, cv = count;
-  const void* kern = hd == 64 ? blocks_of<64>(kv->kind, mod) : blocks_of<128>(kv->kind, mod);
+  // 4 bits, 64 dims, 8 heads a KV head at most: two tiles at a time where a workgroup has as many (60 tokens of 1536 keys 21.9
+  // us, not 25.0, of 256 keys 8.2 and 8.6; of 128 keys 7.1 and 6.3, one of 8192 14.6 and 14.1)
+  const void* kern = hd == 64 ? blocks_of<64>(kv->kind, mod, g <= 8 && total >= 2 * groups) : blocks_of<128>(kv->kind, mod, false);
   void* args[] = {(void*)&p, (void*)&sc.mul, (void*)&sc.cap2, (void*)&q, (void*)&ldq, (void*)&gv, (void*)&hv, (void*)&blocks, (void*)&cv,
                   (void*)&wide, (void*)&apart, (void*)&counters, (void*)&slots, (void*)&out};
   SPECTRA_HIP_CHECK(hipLaunchKernel(kern, dim3((unsigned)groups), dim3(kBlkThreads), args, 0, (hipStream_t)stream));

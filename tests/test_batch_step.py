@@ -1324,3 +1324,26 @@ def test_large_pages(hip, kind, page):
     _check_select(b, bounds, 3, 1, 2, blocks)
     want, tol = _blocks_reference(b, blocks)
     _close(_attend(b, blocks), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,page", [(6, 16), (16, 64), (2, 32), (18, 16)])
+@pytest.mark.parametrize("cap", [0.0, 20.0, 1e6])
+def test_blocks_of_4_bits_and_64_dims_in_numbers(hip, heads, page, cap):
+    """As many steps that workgroups have several each: two tiles' scores share the registers of one, up to 8 heads a KV
+    head.  Rows that no sequence has hold NaN; a page that is not there makes the rows that see it NaN, and no others."""
+    b = Batch("4bit", [5, 40, 3], [3900, 900, 3001], heads, 2, 64, page, seed=70)
+    blocks = _random_blocks(b, 2560 // page, 8)
+    blocks[7:11] = -1
+    blocks[8, :, 5] = 0  # a row with 17 keys of two tiles, one with 16, rows without
+    blocks[8, :, 9], blocks[9, :, 0] = 874 // page, 0
+    want, tol = _blocks_reference(b, blocks, cap=cap)
+    got = _attend(b, blocks, cap=cap)
+    _close(got, want, tol)
+    assert (got[7] == 0).all() and (got[10] == 0).all()
+    last = (blocks[45:] * page).clamp(min=0) + 15  # the third sequence loses a page
+    gone = int(blocks[46, 0][blocks[46, 0] > 3].min())
+    b.table[2, gone] = -5
+    sees = ((blocks[45:] == gone) & (last <= 3000)).any(-1).repeat_interleave(heads // 2, 1)
+    bad = _attend(b, blocks, cap=cap)
+    assert torch.isnan(bad[45:][sees]).all() and torch.equal(bad[45:][~sees], got[45:][~sees]) and torch.equal(bad[:45], got[:45])
