@@ -118,15 +118,20 @@ __device__ __forceinline__ int paged_find(const int* q_start, int batch, int t, 
   return sread(lo);
 }
 
-// The sequence of token t and its part of the call; up to 64 sequences' starts and lengths are asked for at once, where
-// paged_find and three scalar loads are one behind the other.
-__device__ __forceinline__ int paged_where(const PagedKv& kv, int t, int lane, PagedSeq& sq) {
+// The sequence of token t and its part of the call.  Up to 64 sequences' starts and lengths are a lane's each, asked for at
+// once and early, where paged_find and three scalar loads are one behind the other.
+struct PagedStarts {
+  int s0, s1, len;  // of sequence `lane`, or the last
+};
+__device__ __forceinline__ PagedStarts paged_starts_of(const PagedKv& kv, int lane) {
+  const int b = min(lane, kv.batch - 1);
+  return {kv.q_start[b], kv.q_start[b + 1], kv.lens[b]};
+}
+__device__ __forceinline__ int paged_where(const PagedKv& kv, const PagedStarts& st, int t, int lane, PagedSeq& sq) {
   if (kv.batch <= 64) {
-    const int b = min(lane, kv.batch - 1);
-    const int s0 = kv.q_start[b], s1 = kv.q_start[b + 1], len = kv.lens[b];
-    const int seq = __builtin_popcountll(__ballot(lane < kv.batch && s1 <= t));
+    const int seq = __builtin_popcountll(__ballot(lane < kv.batch && st.s1 <= t));
     const int at = min(seq, kv.batch - 1);
-    sq = paged_seq(__builtin_amdgcn_readlane(s0, at), __builtin_amdgcn_readlane(s1, at), __builtin_amdgcn_readlane(len, at), kv.tokens);
+    sq = paged_seq(__builtin_amdgcn_readlane(st.s0, at), __builtin_amdgcn_readlane(st.s1, at), __builtin_amdgcn_readlane(st.len, at), kv.tokens);
     return seq;
   }
   const int seq = paged_find(kv.q_start, kv.batch, t, lane), at = min(seq, kv.batch - 1);

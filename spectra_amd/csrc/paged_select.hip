@@ -15,6 +15,10 @@
 // A workgroup has one token (drafts and prompts: as many as fill the rows, whose pages are read once) and one KV head.
 // Few such units with long tables are split: workgroups score a run of pages each, and the last of a unit to arrive
 // chooses from the keys of all in the workspace.
+//
+// Bound by latencies, not by the bounds' bytes: starts and lengths, ids, bounds, then the choice, one behind the other (64
+// users of up to 250 pages, 18 MB: 10.7 us, of which the choice is 2.5; one of 8188 pages, 17 MB: 12.4 us, of which the
+// choice is 4).
 #include <algorithm>
 
 #include "paged_attend.h"
@@ -23,12 +27,13 @@ namespace spectra {
 
 typedef int pi4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kSelMost = 32768;            // pages of a table
+constexpr int kSelMost = 32768;                        // pages of a table
 constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;  // parts of a range that keys are counted in
 constexpr int kSelWave = 512;                          // keys that one wave chooses from in its registers
-constexpr int kSelLds = 160 * 1024 - 1024;  // codes, keys and counts of a workgroup
-constexpr int kSelSplit = 64;              // units whose pages are split among workgroups: at most as many
-constexpr int kSelApart = 256;             // bytes from one unit's counter to the next one's (atomics on one line wait for each other)
+constexpr int kSelRegs = 16;                           // keys that a lane holds where a workgroup chooses from more
+constexpr int kSelLds = 160 * 1024 - 1024;             // codes, keys and counts of a workgroup
+constexpr int kSelSplit = 64;                          // units whose pages are split among workgroups: at most as many
+constexpr int kSelApart = 256;                         // bytes from one unit's counter to the next one's (atomics on one line wait for each other)
 constexpr size_t kSelCounters = kSelApart * kSelSplit;
 constexpr uint32_t kSelForced = ~0u, kSelOdd = ~0u - 1;
 constexpr float kSelLeast = 7.8886091e-31f;  // 2^-100
@@ -175,20 +180,29 @@ struct SelTogether {
   uint32_t* bins;  // [2][kSelBins], or `room` keys and their places
   uint32_t* box;   // [2][3][16]
   int turn = 0;
-  // of a value a lane
+  // Of a value a lane; where twice as many groups of 2 or 4 lanes are left as are wanted, of their maxima, which are fewer.
   __device__ __forceinline__ uint32_t kth(uint32_t v, int count) {
     const int lane = __lane_id();
-    bins[64 * part + lane] = v;
+    const int few = 2 * count <= 16 * parts ? 2 : 2 * count <= 32 * parts ? 1 : 0;
+    if (few > 0) v = max(v, lane_xor_u<1>(v, lane));
+    if (few > 1) v = max(v, lane_xor_u<2>(v, lane));
+    if ((lane & ((1 << few) - 1)) == 0) bins[(64 * part + lane) >> few] = v;
     __syncthreads();
     if (part == 0) {
-      uint32_t k[kSelWave / 64];
-#pragma unroll
-      for (int r = 0; r < kSelWave / 64; ++r) k[r] = r < parts ? bins[64 * r + lane] : 0u;
-      const uint32_t t = sel_kth(k, count, max(min(count, room / 2 - count), 8));
+      const int n = 64 * parts >> few, slack = few > 0 ? 8 : max(min(count, room / 2 - count), 8);
+      const uint32_t t = n <= 128 ? of<2>(n, count, slack) : n <= 256 ? of<4>(n, count, slack) : of<kSelWave / 64>(n, count, slack);
       if (lane == 0) box[96] = t;
     }
     __syncthreads();
     return (uint32_t)sread((int)box[96]);
+  }
+  template <int K>
+  __device__ __forceinline__ uint32_t of(int n, int count, int slack) {
+    const int lane = __lane_id();
+    uint32_t k[K];
+#pragma unroll
+    for (int r = 0; r < K; ++r) k[r] = 64 * r + lane < n ? bins[64 * r + lane] : 0u;
+    return sel_kth(k, count, slack);
   }
   __device__ __forceinline__ void sync() { __syncthreads(); }
   // every wave's values, in lanes 0 .. parts - 1
@@ -211,7 +225,7 @@ struct SelTogether {
 //
 // Few keys are one wave's, in its registers.  Of more, each lane's largest is found first: as many of these as are wanted
 // lie at or past the `count`-th largest of them, and so do as many keys, so only keys from there on are candidates: little
-// more than `count` (64 of 8190 keys by 512 lanes: some 70), which one wave chooses from.
+// more than `count` (64 of 8190 keys by 512 lanes: some 70, by 128 groups of 4 lanes: some 90), which one wave chooses from.
 // Where that leaves too many, or more are wanted than there are lanes, the range that holds the count-th
 // largest is narrowed by counting the keys in kSelBins equal parts of it; some two rounds leave as many keys as are
 // wanted, or keys that are all the same.
@@ -341,6 +355,49 @@ __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, 
   });
 }
 
+// The same of up to 64 R keys a wave, which stay in registers (read from LDS three times: one of 8188 pages 15.2 us, not 12.4); key(j): the
+// j-th.  False: more candidates than fit, or more wanted than there are lanes, and nothing done.
+template <int R, typename F>
+__device__ __forceinline__ bool sel_pick_in_registers(F key, int n, int count, int* out, SelTogether w) {
+  if (count > 64 * w.parts) return false;
+  const int lane = __lane_id();
+  const int each = ((n + w.parts - 1) / w.parts + 63) & ~63;
+  const int from = min(each * w.part, n), to = min(from + each, n);
+  uint32_t k[R], best = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) k[r] = key(min(from + 64 * r + lane, n - 1));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    k[r] = from + 64 * r + lane < to ? k[r] : 0u;
+    best = max(best, k[r]);
+  }
+  const uint32_t from_on = max(w.kth(best, count), 1u);
+  int c = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) c += __builtin_popcountll(__ballot(k[r] >= from_on));
+  uint32_t met[1] = {(uint32_t)c};
+  w.all(met, {0u});
+  const int upto = wave_scan((int)met[0]), all = __builtin_amdgcn_readlane(upto, 63);
+  if (all < count || all > w.room) return false;
+  int at = __builtin_amdgcn_readlane(upto, w.part) - c;
+  uint32_t *keys = w.bins, *places = w.bins + w.room;
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint64_t take = __ballot(k[r] >= from_on);
+    if (take == 0) continue;
+    if (take >> lane & 1) {
+      const int p = at + __builtin_popcountll(take & below);
+      keys[p] = k[r];
+      places[p] = (uint32_t)(from + 64 * r + lane);
+    }
+    at += __builtin_popcountll(take);
+  }
+  w.sync();
+  if (w.part == 0) sel_wave(keys, all, count, places, out);
+  return true;
+}
+
 // GP: rows a token takes of a tile of 16 (its heads, rounded up to 4, 8, 16); more than 16 heads take several tiles.
 template <int HD, bool BF, int GP>
 __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, const PagedSelect sel,
@@ -373,10 +430,12 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
       u[k] = *(const uint4*)(qr + min(r, g - 1) * HD + d);
     }
   };
-  if (tokens_a_group == 1) ask(first);  // (on their way while the sequence is found)
+  // (on their way while the sequence is found)
+  const PagedStarts starts = paged_starts_of(kv, lane);
+  if (!alone) ask(first);
   for (int t0 = first; t0 < past;) {
     PagedSeq sq;
-    const int seq = paged_where(kv, t0, lane, sq);
+    const int seq = paged_where(kv, starts, t0, lane, sq);
     if (seq >= kv.batch) return;  // behind the last sequence: left alone
     const int n = max(min(min(sq.q0 + sq.n, past) - t0, TOK), 1);  // tokens of this step (starts that are no batch's: one)
     const int i0 = sq.len - sq.n + (t0 - sq.q0);           // position of the first
@@ -384,6 +443,7 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
     int* to = blocks + ((int64_t)t0 * kv.kv_heads + kvh) * sel.count;
     const int64_t row = (int64_t)kv.kv_heads * sel.count;  // from a token's to the next one's
     if (most <= sel.count && blockIdx.y > 0) return;
+    bool picked = false;
     auto visible = [&](int t) __attribute__((always_inline)) {
       return i0 + t < 0 ? 0 : min(((i0 + t) >> kv.page_shift) + 1, kv.table_width);
     };
@@ -417,8 +477,7 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
         pb = page_of(j0 + 3 * step);
       }
       // ---- the queries' codes: a wave a token
-      for (int t = wave; t < TOK; t += waves) {
-        if (tokens_a_group > 1) ask(t0 + min(t, n - 1));
+      auto encode = [&](int t) __attribute__((always_inline)) {
         const uint16_t* qr = q + (int64_t)(t0 + min(t, n - 1)) * ldq + (int64_t)kvh * g * HD;
         uint32_t big = 0;
         auto magnitude = [&](const uint4& x) __attribute__((always_inline)) {
@@ -455,6 +514,15 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
           if (lane + 64 * k < GP * HD / 8) codes(u[k], lane + 64 * k);
         for (int x = 16 * HD / 8 + lane; x < 16 * tiles * (HD / 8); x += 64)
           codes(*(const uint4*)(qr + min(x / (HD / 8), g - 1) * HD + 8 * (x % (HD / 8))), x);
+      };
+      // (apart: loads that only one of both asks for would have the bounds waited for, too)
+      if (!alone) {
+        if (wave == 0) encode(0);
+      } else {
+        for (int t = wave; t < TOK; t += waves) {
+          ask(t0 + min(t, n - 1));
+          encode(t);
+        }
       }
       __syncthreads();
       // ---- scores
@@ -500,22 +568,31 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
       }
       if (sel.chunks > 1) {  // (a unit of one step) the last to arrive chooses
         if (!paged_arrive(sel.counters + blockIdx.x * (kSelApart / 4), sel.chunks, &flag)) return;
+        if (!alone) {
+          auto met = [&](int j) __attribute__((always_inline)) { return load_dev1(mine + j); };
+          picked = most <= 64 * kSelRegs * waves && sel_pick_in_registers<kSelRegs>(met, most, sel.count, to, SelTogether{waves, wave, bins, box});
+        }
         constexpr int U = 8;  // loads in flight
-        for (int t = 0; t < n; ++t)
-          for (int j = tid; j < most; j += U * blockDim.x) {
-            uint32_t k[U];
+        if (!picked) {
+          for (int t = 0; t < n; ++t)
+            for (int j = tid; j < most; j += U * blockDim.x) {
+              uint32_t k[U];
 #pragma unroll
-            for (int e = 0; e < U; ++e) k[e] = load_dev1(mine + t * sel.pitch + min(j + e * (int)blockDim.x, most - 1));
+              for (int e = 0; e < U; ++e) k[e] = load_dev1(mine + t * sel.pitch + min(j + e * (int)blockDim.x, most - 1));
 #pragma unroll
-            for (int e = 0; e < U; ++e)
-              if (j + e * (int)blockDim.x < most) keys[t * sel.pitch + j + e * blockDim.x] = k[e];
-          }
+              for (int e = 0; e < U; ++e)
+                if (j + e * (int)blockDim.x < most) keys[t * sel.pitch + j + e * blockDim.x] = k[e];
+            }
+        }
       }
       __syncthreads();
     }
     // ---- the choice
     if (!alone && most > sel.count) {
-      sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, bins, box});
+      if (!picked && sel.chunks == 1 && most > kSelWave && most <= 64 * kSelRegs * waves)
+        picked = sel_pick_in_registers<kSelRegs>([&](int j) __attribute__((always_inline)) { return keys[j]; }, most, sel.count, to,
+                                                 SelTogether{waves, wave, bins, box});
+      if (!picked) sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, bins, box});
     } else {
       for (int t = wave; t < n; t += waves) {
         const int v = visible(t);
