@@ -278,10 +278,12 @@ __global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* __
   }
 }
 
-// Slices of 16384 logits by 1024 threads: a row's history is read by few workgroups, of which two fill a compute unit (64
-// rows of 128256 with 4096 tokens each: 14.9 us, in slices of 4096 by 256 or 512 threads 18.5 to 21.7, of 8192 by 1024 16.2); of 2048 by 256 while the batch has
-// too few of those for the card.
-bool logits_large(int64_t rows, int64_t vocab) { return rows * ((vocab + 16383) / 16384) >= 256; }
+// Slices of 16384 logits by 1024 threads, of which two fill a compute unit, or of 2048 by 256, which fill the card with few
+// rows and end sooner, but read a row's tokens eight times as often: where that is more than 2^20 tokens or so it costs more.
+// (Large and small, us, fp16 rows of 128256: 8 rows with 1000 tokens 7.5 and 6.3, 16 7.5 and 7.2, 24 7.8 and 8.3; 8 rows with
+// 4096 8.0 and 8.9, 64 13.2 and 21.0; 64 without 8.8 and 8.8, adjusted 10.0 and 9.6.  Slices of 4096 by 256 or 512 threads took
+// 18.5 to 21.7 where large ones took 14.9, of 8192 by 1024 16.2.)
+bool logits_large(int64_t rows, int64_t vocab, int64_t ids) { return rows * ((vocab + 2047) / 2048) * ids >= 5 << 18; }
 
 int logits_args(const spectra_logits_t* l, LogitsArgs* out, size_t* lds, int* threads, int* slices, bool* wide) {
   SPECTRA_REQUIRE(l != nullptr && l->logits, "NULL pointer");
@@ -328,7 +330,7 @@ int logits_args(const spectra_logits_t* l, LogitsArgs* out, size_t* lds, int* th
   a.states = l->states;
   a.state = l->state;
   *wide = a.hist > (int)LgWord<uint32_t>::count || a.biases >= 65535;
-  const bool large = !*wide && logits_large(l->rows, l->vocab);  // (wide words of such a slice would not fit)
+  const bool large = !*wide && logits_large(l->rows, l->vocab, (int64_t)a.hist + a.biases);  // (wide words of such a slice would not fit)
   const int slice = large ? 16384 : 2048;
   *threads = large ? 1024 : 256;
   *slices = (int)((l->vocab + slice - 1) / slice);

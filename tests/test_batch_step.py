@@ -695,6 +695,15 @@ def test_logits_of_a_large_batch(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(60, 16384), (60, 16385), (40, 40003), (9, 128256)])
+@pytest.mark.parametrize("kw", [dict(history=4000), dict(history=3001, biases=1100, masks=3), dict(biases=5000, masks=2)])
+def test_logits_in_large_slices(hip, dtype, rows, vocab, kw):
+    """So many tokens to adjust that a slice is 16384 logits, the last one of a row shorter."""
+    _check_logits(*_case(rows, vocab, dtype, 71, **kw))
+
+
+@pytest.mark.gpu
 def test_logits_masks_by_row(hip):
     x, kw = _case(3, 1000, torch.float32, 63, masks=3, row_masks=True)
     _check_logits(x, kw)
