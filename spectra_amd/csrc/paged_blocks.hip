@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     };
     // 4 bits: up to PACK tiles, kBlkKeys keys apart, in LDS from `t` on, whose scores take columns of their own: tile n's
     // products are those of queries that are zero in the other's columns, and its weights are zero there.  So a row's 8
-    // columns, not 16, are exponentiated for a tile.  (All columns are of one row's keys: a value or a key that is NaN or
-    // infinite, of one tile, makes the row so through either's columns.)  half(x): tile x / 2's half x % 2; odd: not all
+    // columns, not 16, are exponentiated for a tile.  (Zero times what is not finite is NaN: a page that the row sees whose
+    // scale is infinite makes the row NaN, through the other tile's columns, too, which are the same row's.)  half(x): tile x / 2's half x % 2; odd: not all
     // keys are seen, or a page is not there.
     auto packed = [&](const uint8_t* t, int tiles, bool odd, auto half) __attribute__((always_inline)) {
       const int mine = c / GP;  // the tile of the lane's column
