@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
         if (!paged_arrive(sel.counters + blockIdx.x * (kSelApart / 4), sel.chunks, &flag)) return;
         if (!alone) {
           auto met = [&](int j) __attribute__((always_inline)) { return load_dev1(mine + j); };
-          picked = most <= 64 * kSelRegs * waves && sel_pick_in_registers<kSelRegs>(met, most, sel.count, to, SelTogether{waves, wave, bins, box});
+          picked = most > kSelWave && most <= 64 * kSelRegs * waves && sel_pick_in_registers<kSelRegs>(met, most, sel.count, to, SelTogether{waves, wave, bins, box});
         }
         constexpr int U = 8;  // loads in flight
         if (!picked) {

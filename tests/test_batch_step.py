@@ -1071,6 +1071,17 @@ def test_blocks_refusals(change, status, text):
     _refused(st, lib.spectra_last_error(), status, text)
 
 
+def test_refusals_of_more_tokens_than_are_counted():
+    """Sizes are checked before they are multiplied: sums of bytes past 64 bits would pass for none."""
+    lib = L.load()
+    kv, b = _desc(k=0, v=0, page_stride=0, kv_heads=8), L.PagedBounds(0x40000, 8 * 128, 0x50000, 8)
+    st = lib.spectra_paged_select(ctypes.byref(kv), ctypes.byref(b), 0x90000, 8 * 64, L.F16, 1 << 29, 8, 32768, 1, 2, 0, 0, 1 << 60, None)
+    _refused(st, lib.spectra_last_error(), L.ERR_INVALID, "tokens")
+    kv = _desc(kv_heads=8, page_stride=8 * 16 * 64)
+    st = lib.spectra_paged_attend_blocks(ctypes.byref(kv), 0x90000, 8 * 64, 1 << 29, 8, 1 << 60, 1 << 25, 0.1, 0.0, 0x1000000, 1 << 30, 1 << 61, None)
+    _refused(st, lib.spectra_last_error(), L.ERR_INVALID, "tokens")
+
+
 @pytest.mark.parametrize("change,text", [
     (dict(logits=0), "NULL"), (dict(dtype=7), "dtype"), (dict(rows=0), "range"), (dict(vocab=0), "range"), (dict(ld=90), "stride"),
     (dict(repetition=0x20000), "history"), (dict(repetition=0x20000, history=0x30000, history_width=9, history_ld=5), "stride"),
@@ -1356,3 +1367,41 @@ def test_blocks_of_4_bits_and_64_dims_in_numbers(hip, heads, page, cap):
     sees = ((blocks[45:] == gone) & (last <= 3000)).any(-1).repeat_interleave(heads // 2, 1)
     bad = _attend(b, blocks, cap=cap)
     assert torch.isnan(bad[45:][sees]).all() and torch.equal(bad[45:][~sees], got[45:][~sees]) and torch.equal(bad[:45], got[:45])
+
+
+@pytest.mark.gpu
+def test_larger_calls_captured(hip):
+    """Many drafts on 4-bit pages of 64 dims, a long table split among workgroups, a batch's logits in large slices: each
+    replay of a captured graph, with eager calls of other shapes on the same workspaces between them, is the eager call's."""
+    from spectra_amd import kernels as K
+    b = Batch("4bit", [5, 40, 3], [3900, 900, 3001], 6, 2, 64, 16, seed=72)
+    blocks = _random_blocks(b, 160, 9)
+    long = Batch("bf16", [1], [16 * 8100 + 3], 8, 2, 64, 16, seed=73)
+    bounds = _random_bounds(long, 18)
+    x, kw = _case(40, 40003, torch.float16, 74, history=3001, biases=40, masks=3)
+    small, few = _case(3, 500, torch.float16, 75, history=20)
+    at, sel, nx = K.paged_attend_workspace(64), K.paged_select_workspace(), K.next_tokens_workspace()
+
+    def calls():
+        return (_attend(b, blocks, workspace=at, cap=9.0), K.paged_select(long.q, long.kv_lens, long.q_start, long.table, bounds, 16, 60, workspace=sel),
+                K.next_tokens(x, workspace=nx, **kw), K.adjust_logits(x, **kw))
+
+    want = calls()
+    _check_select(long, bounds, 60, 1, 2, want[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        calls()
+        with torch.cuda.graph(graph, stream=side):
+            got = calls()
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(4):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g.nan_to_num(), w.nan_to_num()) for g, w in zip(got, want))
+        _check_logits(small, few, nx)
+        K.paged_attend_blocks(b.q[:5], blocks[:5, :, :3].contiguous(), b.kv_lens[:1], b.q_start[:2], b.table[:1], b.k, b.v, workspace=at)
+        K.paged_select(long.q, torch.full_like(long.kv_lens, 16 * 1100), long.q_start, long.table, bounds, 16, 5, workspace=sel)
