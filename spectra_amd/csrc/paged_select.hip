@@ -221,7 +221,14 @@ struct SelTogether {
   }
 };
 
-// The `count` largest of n > count keys, the first on ties, written in their order, by parts of 64 lanes.
+// What is left for one wave to choose from: keys, and the places that they have (or their own); none: all is chosen.
+struct SelFew {
+  const uint32_t *key, *of;
+  int n;
+};
+
+// The `count` largest of n > count keys, the first on ties, written in their order, by parts of 64 lanes, or a few keys for
+// the first part's wave to choose from.
 //
 // Few keys are one wave's, in its registers.  Of more, each lane's largest is found first: as many of these as are wanted
 // lie at or past the `count`-th largest of them, and so do as many keys, so only keys from there on are candidates: little
@@ -230,12 +237,9 @@ struct SelTogether {
 // largest is narrowed by counting the keys in kSelBins equal parts of it; some two rounds leave as many keys as are
 // wanted, or keys that are all the same.
 template <typename W>
-__device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, int* out, W w) {
+__device__ __forceinline__ SelFew sel_pick(const uint32_t* key, int n, int count, int* out, W w) {
   const int lane = __lane_id();
-  if (n <= kSelWave) {
-    if (w.part == 0) sel_wave(key, n, count, nullptr, out);
-    return;
-  }
+  if (n <= kSelWave) return {key, nullptr, n};
   const int each = ((n + w.parts - 1) / w.parts + 63) & ~63;
   const int from = min(each * w.part, n), to = min(from + each, n);
   // f of all keys of this part, a lane's each, the loads of four in flight together
@@ -272,8 +276,7 @@ __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, 
         at += __builtin_popcountll(take);
       });
       w.sync();
-      if (w.part == 0) sel_wave(keys, all, count, places, out);
-      return;
+      return {keys, places, all};
     }
     w.sync();  // (the counts start anew)
   }
@@ -353,13 +356,14 @@ __device__ __forceinline__ void sel_pick(const uint32_t* key, int n, int count, 
     a += __builtin_popcountll(ab);
     e += __builtin_popcountll(eb);
   });
+  return {nullptr, nullptr, 0};
 }
 
 // The same of up to 64 R keys a wave, which stay in registers (read from LDS three times: one of 8188 pages 15.2 us, not 12.4); key(j): the
-// j-th.  False: more candidates than fit, or more wanted than there are lanes, and nothing done.
+// j-th.  None: more candidates than fit, or more wanted than there are lanes, and nothing done.
 template <int R, typename F>
-__device__ __forceinline__ bool sel_pick_in_registers(F key, int n, int count, int* out, SelTogether w) {
-  if (count > 64 * w.parts) return false;
+__device__ __forceinline__ SelFew sel_pick_in_registers(F key, int n, int count, SelTogether w) {
+  if (count > 64 * w.parts) return {nullptr, nullptr, 0};
   const int lane = __lane_id();
   const int each = ((n + w.parts - 1) / w.parts + 63) & ~63;
   const int from = min(each * w.part, n), to = min(from + each, n);
@@ -378,7 +382,7 @@ __device__ __forceinline__ bool sel_pick_in_registers(F key, int n, int count, i
   uint32_t met[1] = {(uint32_t)c};
   w.all(met, {0u});
   const int upto = wave_scan((int)met[0]), all = __builtin_amdgcn_readlane(upto, 63);
-  if (all < count || all > w.room) return false;
+  if (all < count || all > w.room) return {nullptr, nullptr, 0};
   int at = __builtin_amdgcn_readlane(upto, w.part) - c;
   uint32_t *keys = w.bins, *places = w.bins + w.room;
   const uint64_t below = (1ull << lane) - 1;
@@ -394,8 +398,7 @@ __device__ __forceinline__ bool sel_pick_in_registers(F key, int n, int count, i
     at += __builtin_popcountll(take);
   }
   w.sync();
-  if (w.part == 0) sel_wave(keys, all, count, places, out);
-  return true;
+  return {keys, places, all};
 }
 
 // GP: rows a token takes of a tile of 16 (its heads, rounded up to 4, 8, 16); more than 16 heads take several tiles.
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
     int* to = blocks + ((int64_t)t0 * kv.kv_heads + kvh) * sel.count;
     const int64_t row = (int64_t)kv.kv_heads * sel.count;  // from a token's to the next one's
     if (most <= sel.count && blockIdx.y > 0) return;
-    bool picked = false;
+    SelFew few = {nullptr, nullptr, 0};
     auto visible = [&](int t) __attribute__((always_inline)) {
       return i0 + t < 0 ? 0 : min(((i0 + t) >> kv.page_shift) + 1, kv.table_width);
     };
@@ -568,12 +571,11 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
       }
       if (sel.chunks > 1) {  // (a unit of one step) the last to arrive chooses
         if (!paged_arrive(sel.counters + blockIdx.x * (kSelApart / 4), sel.chunks, &flag)) return;
-        if (!alone) {
-          auto met = [&](int j) __attribute__((always_inline)) { return load_dev1(mine + j); };
-          picked = most > kSelWave && most <= 64 * kSelRegs * waves && sel_pick_in_registers<kSelRegs>(met, most, sel.count, to, SelTogether{waves, wave, bins, box});
-        }
+        if (!alone && most <= 64 * kSelRegs * waves)
+          few = sel_pick_in_registers<kSelRegs>([&](int j) __attribute__((always_inline)) { return load_dev1(mine + j); }, most,
+                                                sel.count, SelTogether{waves, wave, bins, box});
         constexpr int U = 8;  // loads in flight
-        if (!picked) {
+        if (few.n == 0) {
           for (int t = 0; t < n; ++t)
             for (int j = tid; j < most; j += U * blockDim.x) {
               uint32_t k[U];
@@ -589,15 +591,14 @@ __global__ void __launch_bounds__(512) paged_select_kernel(const PagedKv kv, con
     }
     // ---- the choice
     if (!alone && most > sel.count) {
-      if (!picked && sel.chunks == 1 && most > kSelWave && most <= 64 * kSelRegs * waves)
-        picked = sel_pick_in_registers<kSelRegs>([&](int j) __attribute__((always_inline)) { return keys[j]; }, most, sel.count, to,
-                                                 SelTogether{waves, wave, bins, box});
-      if (!picked) sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, bins, box});
+      if (few.n == 0) few = sel_pick(keys, most, sel.count, to, SelTogether{waves, wave, bins, box});
+      if (few.n > 0 && wave == 0) sel_wave(few.key, few.n, sel.count, few.of, to);
     } else {
       for (int t = wave; t < n; t += waves) {
         const int v = visible(t);
         if (v > sel.count) {
-          sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{bins + wave * 2 * SelAlone::room});
+          const SelFew left = sel_pick(keys + t * sel.pitch, v, sel.count, to + t * row, SelAlone{bins + wave * 2 * SelAlone::room});
+          if (left.n > 0) sel_wave(left.key, left.n, sel.count, left.of, to + t * row);
         } else {
           for (int x = lane; x < sel.count; x += 64) to[t * row + x] = x < v ? x : -1;
         }
