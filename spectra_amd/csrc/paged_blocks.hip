@@ -292,9 +292,9 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     };
     // 4 bits: up to PACK tiles, kBlkKeys keys apart, in LDS from `t` on, whose scores take columns of their own: tile n's
     // products are those of queries that are zero in the other's columns, and its weights are zero there.  So a row's 8
-    // columns, not 16, are exponentiated for a tile.  (Zero times what is not finite is NaN: a page that the row sees whose
-    // scale is infinite makes the row NaN, through the other tile's columns, too, which are the same row's.)  half(x): tile x / 2's half x % 2; odd: not all
-    // keys are seen, or a page is not there.
+    // columns, not 16, are exponentiated for a tile.  (Zero times what is not finite is NaN in the other tile's columns: sums
+    // that come out so are made again, a tile at a time.)  half(x): tile x / 2's half x % 2; odd: not all keys are seen, or
+    // a page is not there.
     auto packed = [&](const uint8_t* t, int tiles, bool odd, auto half) __attribute__((always_inline)) {
       const int mine = c / GP;  // the tile of the lane's column
       pf4_t s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -466,6 +466,37 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
           key += STEP;
           if (key >= kend) break;
           now = then;
+        }
+        if constexpr (PACK > 1) {
+          // Sums that are not finite, as a scale that is infinite leaves them: again, in the first tile's columns alone, so that
+          // they are what they are without another tile beside (values of some dims infinite, a score of -inf without weight).
+          float odd = l * 0.0f;
+#pragma unroll
+          for (int j = 0; j < DPL; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd = __builtin_fmaf(o[j][i], 0.0f, odd);
+          if (__ballot(odd != 0.0f) != 0) {
+            m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int j = 0; j < DPL; ++j) o[j] = (pf4_t){0.0f, 0.0f, 0.0f, 0.0f};
+            for (key = sbeg * kBlkKeys + 32 * wave; key < kend; key += kBlkKeys) {
+              BlkHalf ha[2];
+              b0 = listed(key);
+              b1 = listed(key + 16);
+              id0 = page_of(b0);
+              id1 = page_of(b1);
+              next(ha, key);
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+              fetch(at0, key, ha[0].page, ha[1].page);
+              asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+              packed(mine, 1, true, [&](int x) __attribute__((always_inline)) { return x < 2 ? ha[x] : BlkHalf{0, 0, false}; });
+            }
+#pragma unroll
+            for (int j = 0; j < DPL; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[j][i] = c < GP ? o[j][i] : 0.0f;
+          }
         }
       } else if constexpr (Q4) {
         BlkHalf ha[2], hb[2];

@@ -1405,3 +1405,62 @@ def test_larger_calls_captured(hip):
         _check_logits(small, few, nx)
         K.paged_attend_blocks(b.q[:5], blocks[:5, :, :3].contiguous(), b.kv_lens[:1], b.q_start[:2], b.table[:1], b.k, b.v, workspace=at)
         K.paged_select(long.q, torch.full_like(long.kv_lens, 16 * 1100), long.q_start, long.table, bounds, 16, 5, workspace=sel)
+
+
+def _one_token(b, s, t, row, blocks, cap):
+    """The output [heads, d] of token t of sequence s (row `row` of the call) and its tolerance, whose keys may score infinities."""
+    u, sub = torch.finfo(_DT[b.kind]).eps / 2, 2.0 ** -25 if b.kind != "bf16" else 0.0
+    k, v = b.rows(s)
+    out, tol = [], []
+    for h in range(b.heads):
+        kv = h * b.kv // b.heads
+        j = torch.cat([torch.arange(x * b.page, (x + 1) * b.page) for x in blocks[row, kv].tolist() if x >= 0]).cuda()
+        j = j[j <= b.lens[s] - b.n[s] + t]
+        kk, vv = k[kv, j], v[kv, j]
+        q = b.q[row, h].double()
+        x = (kk * q).sum(-1) / math.sqrt(b.d)
+        size = (kk * q).abs().sum(-1) / math.sqrt(b.d)
+        delta = b.d * 2.0 ** -24 * size[torch.isfinite(size)].max()
+        if cap:
+            x, delta = cap * torch.tanh(x / cap), delta + cap * 2.0 ** -20
+        e = torch.exp(x - x.max())
+        p = e / e.sum()
+        o, a = (p[:, None] * vv).sum(0), (p[:, None] * vv.abs()).sum(0)
+        out.append(o)
+        tol.append(u * o.abs() + (u + 2 * delta + 2.0 ** -20) * a + sub * (1 + vv.abs().sum(0) / e.sum()))
+    return torch.stack(out), torch.stack(tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,d", [(2, 2, 64), (12, 2, 64), (18, 1, 64), (6, 2, 128)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("what", ["values", "keys above", "keys below"])
+def test_blocks_of_4_bits_with_infinite_scales(hip, heads, kv, d, cap, what):
+    """A row that sees an infinite scale has what the formula gives, in a batch whose workgroups have many tiles and alone:
+    infinite values are infinite in their dims, a score of -inf weighs nothing, one of +inf is NaN (with a cap: the cap)."""
+    from spectra_amd import kernels as K
+    b = Batch("4bit", [5, 40, 3], [3900, 900, 3001], heads, kv, d, 16, seed=76)
+    blocks = _random_blocks(b, 160, 10, holes=False)
+    before = _attend(b, blocks, cap=cap)
+    page, row = 50, 7  # key 807 of the third sequence, which its second token lists in every KV head
+    blocks[46, :, 3] = torch.where((blocks[46] == page).any(-1), blocks[46, :, 3], page)
+    blocks[45], blocks[47] = torch.where(blocks[45] == page, -1, blocks[45]), torch.where(blocks[47] == page, -1, blocks[47])
+    at = b.table[2, page].long()
+    codes, scales, zeros = b.v if what == "values" else b.k
+    codes[at, :, row, :16] = 0x5A
+    zeros[at, :, row, 0] = 7 if what == "values" else 2
+    scales[at, :, row, 0] = math.inf
+    if what != "values":
+        b.q[46, :, :32] = b.q[46, :, :32].abs().clamp(min=0.01) * (1 if what == "keys above" else -1)
+    got = _attend(b, blocks, cap=cap)
+    want, tol = _one_token(b, 2, 1, 46, blocks, cap)
+    alone = K.paged_attend_blocks(b.q[46:47], blocks[46:47], torch.tensor([3000], dtype=torch.int32, device="cuda"), b.q_start.new_tensor([0, 1]),
+                                  b.table[2:], b.k, b.v, cap=cap)
+    finite = torch.isfinite(want)
+    assert finite.all(-1).all() == (what == "keys below" or (what == "keys above" and cap > 0))
+    for x in (got[46], alone[0]):
+        assert torch.equal(torch.isnan(x), torch.isnan(want))
+        assert torch.equal(torch.isposinf(x), torch.isposinf(want)) and torch.equal(torch.isneginf(x), torch.isneginf(want))
+        err = (x.double() - want).abs()
+        assert (err <= tol)[finite].all(), float((err - tol)[finite].max())
+    assert torch.equal(got[:45], before[:45])
