@@ -481,7 +481,8 @@ int spectra_paged_bounds_values(const spectra_paged_bounds_t* bounds, int64_t nu
  * others have the largest scores, the lowest block on ties:
  *   c_h = rint(q_h 127 / A), A = the largest magnitude of the KV head's query heads
  *   score_j = scale_j max_h sum_d (max(c_hd, 0) codes[j, 0, d] + min(c_hd, 0) codes[j, 1, d])
- * whole numbers, exact, and one product in fp32.  (A not finite or below 2^-100: c = 0.)  Blocks
+ * whole numbers, exact, and one product in fp32.  (A not finite or below 2^-100: c = 0.)  A score bounds
+ * the products of c with the block's keys, not those of q, of which it is an estimate.  Blocks
  * with a scale of +inf or of a page outside the pool come before all scores.  q [tokens, heads,
  * head_dim], act_dtype F16 or BF16, token stride ldq (a multiple of 8), 16-byte aligned.  Of kv
  * only the sizes, the table, the lengths and the starts are read (kv_lens count the call's tokens,

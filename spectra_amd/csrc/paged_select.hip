@@ -1,9 +1,11 @@
-// Selection of pages for sparse attention: for each token and KV head the pages whose bounds allow the largest products.
+// Selection of pages for sparse attention: for each token and KV head the pages whose bounds allow the largest products with
+// the queries as rounded to 8 bits.
 //
 // The token's g query heads of the KV head become whole numbers of one scale, A = max |q|, c = rint(q 127 / A) (both
 // operations fp32 as written), and page j scores
 //   s_j = scale_j max_h sum_d (max(c_hd, 0) M_jd + min(c_hd, 0) m_jd)
-// (M, m, scale: paged_bounds.hip): whole numbers below 2^23 summed exactly, one rounding by the product with the scale.
+// (M, m, scale: paged_bounds.hip): whole numbers below 2^23 summed exactly, one rounding by the product with the scale.  It
+// bounds the products of c, not of q: a dim below half a step of A counts nothing.
 // So a score is the same whatever order it is summed in, and the choice among near scores, too: the largest scores,
 // the lowest page on ties.  A scale of infinity, or a page that is not in the pool, is taken before all scores: the
 // attention then shows what is wrong.  The first `sink` and the last `local` pages of the visible are always taken.

@@ -935,11 +935,12 @@ def paged_select(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
     [T, kv, count], ascending, then -1.
 
     Of the blocks that the token at position i of its sequence sees (j <= i // page) the first ``sink`` and the last
-    ``local`` (at least one: its own) are always taken, then those with the largest scores, the lowest block on ties.  A
-    score bounds the largest product of any of the KV head's query heads with any key of the block: the heads of ``q``
-    [T, heads, d] (fp16 or bf16) rounded to 8 bits of one scale, times the ``bounds`` of ``paged_key_bounds`` in whole
-    numbers, exact, so the choice depends on nothing else.  Blocks whose bounds are infinite, and pages outside the pool, come
-    first.  Lengths, starts and the table are ``paged_attend``'s; rows behind q_start[-1] are left alone.  ``workspace``
+    ``local`` (at least one: its own) are always taken, then those with the largest scores, the lowest block on ties.  The
+    heads of ``q`` [T, heads, d] (fp16 or bf16) are rounded to 8 bits of one scale, the largest magnitude of a KV head's
+    query heads; a score is what the ``bounds`` of ``paged_key_bounds`` allow as the largest product of any of them, so
+    rounded, with any key of the block, in whole numbers, exact, so the choice depends on nothing else.  (Of the queries as they
+    are it is an estimate: a dim below 1 / 254 of the largest magnitude counts nothing, however large the keys are in it.)
+    Blocks whose bounds are infinite, and pages outside the pool, come first.  Lengths, starts and the table are ``paged_attend``'s; rows behind q_start[-1] are left alone.  ``workspace``
     (``paged_select_workspace``): shares one long sequence among more of the card; without one the result is the same."""
     if not q.is_cuda:
         raise ValueError("q must be on the GPU")

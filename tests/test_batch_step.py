@@ -1464,3 +1464,30 @@ def test_blocks_of_4_bits_with_infinite_scales(hip, heads, kv, d, cap, what):
         err = (x.double() - want).abs()
         assert (err <= tol)[finite].all(), float((err - tol)[finite].max())
     assert torch.equal(got[:45], before[:45])
+
+
+@pytest.mark.gpu
+def test_scores_bound_products_of_rounded_queries(hip):
+    """A block's score is at least the product of each rounded query with each of its keys; a dim below half a step of the
+    queries' scale counts nothing, however large the keys are in it."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [1], [400], 6, 2, 64, 16, seed=77)
+    codes, scales = K.paged_key_bounds(400, b.kv_lens, b.q_start.new_tensor([0, 400]), b.table, b.k, K.paged_bounds(b.k))
+    k, _ = b.rows(0)
+    for h in range(2):
+        q = b.q[0, 3 * h: 3 * h + 3].float()
+        c = torch.round(q * (127 / q.abs().max())).double()
+        for j in range(25):
+            page = b.table[0, j].long()
+            hi, lo = codes[page, h].double()
+            score = float(scales[page, h]) * float((c.clamp(min=0) @ hi + c.clamp(max=0) @ lo).max())
+            assert float((c @ k[h, 16 * j: 16 * j + 16].T).max()) <= score + 127 * 2.0 ** -22 * float(scales[page, h]) * float(c.abs().sum(-1).max())
+    one = Batch("fp16", [1], [80], 1, 1, 64, 16, seed=78)
+    one.q.zero_()
+    one.q[0, 0, 0], one.q[0, 0, 1] = 127.0, 0.4
+    one.k.zero_()
+    one.k[one.table[0, 1].long(), 0, 5, 1] = 100.0  # a product of 40, a score of 0
+    one.k[one.table[0, 2].long(), 0, 5, 0] = 0.01   # of 1.27, and a score as large
+    bounds = K.paged_key_bounds(80, one.kv_lens, one.q_start.new_tensor([0, 80]), one.table, one.k, K.paged_bounds(one.k))
+    got = K.paged_select(one.q, one.kv_lens, one.q_start, one.table, bounds, 16, 3, sink=1, local=1)
+    assert got[0, 0].tolist() == [0, 2, 4]
