@@ -1491,3 +1491,50 @@ def test_scores_bound_products_of_rounded_queries(hip):
     bounds = K.paged_key_bounds(80, one.kv_lens, one.q_start.new_tensor([0, 80]), one.table, one.k, K.paged_bounds(one.k))
     got = K.paged_select(one.q, one.kv_lens, one.q_start, one.table, bounds, 16, 3, sink=1, local=1)
     assert got[0, 0].tolist() == [0, 2, 4]
+
+
+@pytest.mark.gpu
+def test_calls_that_meet_in_workspaces_on_two_streams(hip):
+    """A selection split among workgroups, lists whose tiles are cut, choices over small and over large slices, on two streams
+    at once, each with workspaces of its own: what each gives alone."""
+    from spectra_amd import kernels as K
+    sides = []
+    for i in range(2):
+        long = Batch("bf16", [1, 1], [16 * 1100 + 3, 16 * 1300], 4, 2, 64, 16, seed=91 + i)
+        near = Batch("fp16", [1, 3], [1500, 1400], 8, 2, 64, 16, seed=93 + i)
+        sides.append(dict(long=long, bounds=_random_bounds(long, 95 + i), near=near, lists=_random_blocks(near, 80, 11 + i, holes=False),
+                          small=_case(3, 7001, torch.float16, 97 + i, history=50, masks=2),
+                          large=_case(40, 40003, torch.float32, 99 + i, history=3001, biases=20),
+                          select=K.paged_select_workspace(), attend=K.paged_attend_workspace(64), next=K.next_tokens_workspace(),
+                          busy=torch.randn(4096, 4096, device="cuda", dtype=torch.float16)))
+
+    def calls(s):
+        long, near = s["long"], s["near"]
+        return (K.paged_select(long.q, long.kv_lens, long.q_start, long.table, s["bounds"], 16, 70, workspace=s["select"]),
+                _attend(near, s["lists"], workspace=s["attend"]),
+                *[K.next_tokens(x, workspace=s["next"], **kw) for x, kw in (s["small"], s["large"])])
+
+    wants = [calls(s) for s in sides]
+    torch.cuda.synchronize()
+    for s, want in zip(sides, wants):
+        _check_select(s["long"], s["bounds"], 70, 1, 2, want[0])
+        _close(want[1], *_blocks_reference(s["near"], s["lists"]))
+        for (x, kw), t in zip((s["small"], s["large"]), want[2:]):
+            assert torch.equal(t.cpu(), _picked(_adjusted(x, **kw)))
+        assert s["select"][16384:].any() and s["attend"][16384:].any()  # (partial results have met there)
+    assert not any(torch.equal(x, y) for x, y in zip(*wants))
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], ([], [])
+    for st, s in zip(streams, sides):  # (work that the calls of both queue up behind)
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            for _ in range(4):
+                s["busy"] @ s["busy"]
+    for _ in range(25):
+        for st, s, out in zip(streams, sides, outs):
+            with torch.cuda.stream(st):
+                out.append(calls(s))
+    torch.cuda.synchronize()
+    for want, out in zip(wants, outs):
+        assert all(torch.equal(x, y) for one in out for x, y in zip(one, want))
+    for s in sides:
+        assert not s["select"][:16384].any() and not s["attend"][:16384].any() and not s["next"].any()
