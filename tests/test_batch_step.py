@@ -1538,3 +1538,33 @@ def test_calls_that_meet_in_workspaces_on_two_streams(hip):
         assert all(torch.equal(x, y) for one in out for x, y in zip(one, want))
     for s in sides:
         assert not s["select"][:16384].any() and not s["attend"][:16384].any() and not s["next"].any()
+
+
+@pytest.mark.gpu
+def test_clamped_starts_reach_only_what_they_name(hip):
+    """Starts that are no batch's are clamped to the call's tokens (a start below the one before it: no tokens).  Bounds are
+    worked out for the pages that they then name, and for no others; a selection leaves rows behind the last start alone."""
+    from spectra_amd import kernels as K
+    b = Batch("fp16", [40, 30], [40, 30], 2, 1, 64, 16, seed=79)
+    for starts, touched in (([0, 0, 0], ()), ([50, 20, 10], ()), ([70, 70, 70], ()), ([-5, 1000, 3], (0,)), ([0, 1, 1], (0,))):
+        # sequence 0 with all of the call's tokens, or one; its pages from the first of its tokens on
+        bad = b.q_start.new_tensor(starts)
+        codes, scales = K.paged_bounds(b.k)
+        codes.fill_(3)
+        scales.fill_(5.0)
+        want = codes.clone(), scales.clone()
+        K.paged_key_bounds(b.tokens, b.kv_lens, bad, b.table, b.k, (codes, scales))
+        for s in touched:
+            first = 0 if starts[1] > 1 else 39
+            for j in range(first // 16, 3):
+                page = int(b.table[s, j])
+                c, a = _bounds_of(b.k[page, 0, : min(16, 40 - 16 * j)])
+                want[0][page, 0], want[1][page, 0] = torch.from_numpy(c).cuda(), float(a)
+        assert torch.equal(codes, want[0]) and torch.equal(scales, want[1]), starts
+    b = Batch("fp16", [2, 1], [400, 90], 4, 2, 64, 16, seed=80)
+    bounds = _random_bounds(b, 19)
+    for starts in ([0, 0, 0], [2, 1, 1], [0, 1, 1], [-5, 1, 2], [0, 2, 2]):
+        out = torch.full((3, 2, 4), 77, dtype=torch.int32, device="cuda")
+        K.paged_select(b.q, b.kv_lens, b.q_start.new_tensor(starts), b.table, bounds, 16, 4, out=out)
+        last = max(starts[-1], 0)
+        assert (out[last:] == 77).all() and not (out[:last] == 77).any(), starts
