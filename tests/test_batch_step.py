@@ -1568,3 +1568,28 @@ def test_clamped_starts_reach_only_what_they_name(hip):
         K.paged_select(b.q, b.kv_lens, b.q_start.new_tensor(starts), b.table, bounds, 16, 4, out=out)
         last = max(starts[-1], 0)
         assert (out[last:] == 77).all() and not (out[:last] == 77).any(), starts
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [3, 6])
+@pytest.mark.parametrize("width", [9000, 10000, 32768])
+def test_select_chunks_on_wide_tables(hip, g, width):
+    """Tokens beside each other on tables so wide that their keys do not fit: groups of fewer tokens than a tile holds, or one,
+    with their pages split among workgroups or not."""
+    from spectra_amd import kernels as K
+    n, pages, d = 9, 700, 64
+    gen = _gen(82)
+    q = torch.randn(n, g, d, generator=gen, device="cuda").half()
+    codes = torch.randint(-30, 128, (pages, 1, 2, d), generator=gen, device="cuda", dtype=torch.int8)
+    codes[:, :, 1] = -codes[:, :, 1]
+    scales = torch.rand(pages, 1, generator=gen, device="cuda") + 0.1
+    table = torch.randint(0, pages, (1, width), generator=gen, device="cuda", dtype=torch.int32)  # the pages again and again
+    last = 16 * (width - 1) + 4  # (the tokens' own page changes after the fifth)
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([last], [0, n]))
+    c, s, t = codes.cpu().numpy(), scales.cpu().numpy(), table.cpu().numpy()
+    for count in (40, 300):
+        got = K.paged_select(q, lens, starts, table, (codes, scales), 16, count)
+        assert torch.equal(got, K.paged_select(q, lens, starts, table, (codes, scales), 16, count, workspace=K.paged_select_workspace()))
+        for i in range(n) if width < 32768 else (0, 4, 5, 8):
+            want = _selected(q[i], c[:, 0], s[:, 0], t[0], (last - n + i) // 16 + 1, count, 1, 2)
+            assert got[i, 0].tolist() == want, (count, i)
