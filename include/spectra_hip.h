@@ -487,7 +487,8 @@ int spectra_paged_bounds_values(const spectra_paged_bounds_t* bounds, int64_t nu
  * head_dim], act_dtype F16 or BF16, token stride ldq (a multiple of 8), 16-byte aligned.  Of kv
  * only the sizes, the table, the lengths and the starts are read (kv_lens count the call's tokens,
  * whose bounds are there: spectra_paged_key_bounds).  Rows behind the last sequence are left alone.  Tables of
- * up to 32768 pages (SPECTRA_ERR_UNSUPPORTED otherwise).  workspace: NULL, or
+ * up to 32768 pages and up to 256 query heads a KV head, of which the widest tables leave 96 of 128 dims or
+ * 208 of 64 (SPECTRA_ERR_UNSUPPORTED otherwise).  workspace: NULL, or
  * spectra_paged_select_workspace() bytes, 16-byte aligned, by which few tokens with long tables are shared
  * among workgroups.  ZERO it before its first use; every complete call leaves its counters at zero; calls
  * sharing one must not overlap. */

@@ -940,8 +940,10 @@ def paged_select(q: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, 
     query heads; a score is what the ``bounds`` of ``paged_key_bounds`` allow as the largest product of any of them, so
     rounded, with any key of the block, in whole numbers, exact, so the choice depends on nothing else.  (Of the queries as they
     are it is an estimate: a dim below 1 / 254 of the largest magnitude counts nothing, however large the keys are in it.)
-    Blocks whose bounds are infinite, and pages outside the pool, come first.  Lengths, starts and the table are ``paged_attend``'s; rows behind q_start[-1] are left alone.  ``workspace``
-    (``paged_select_workspace``): shares one long sequence among more of the card; without one the result is the same."""
+    Blocks whose bounds are infinite, and pages outside the pool, come first.  Lengths, starts and the table are
+    ``paged_attend``'s; rows behind q_start[-1] are left alone.  Tables have up to 32768 pages, KV heads up to 256 query heads
+    (96 of 128 dims, 208 of 64, beside the widest tables).  ``workspace`` (``paged_select_workspace``): shares one long
+    sequence among more of the card; without one the result is the same."""
     if not q.is_cuda:
         raise ValueError("q must be on the GPU")
     codes, scales = bounds

@@ -1593,3 +1593,29 @@ def test_select_chunks_on_wide_tables(hip, g, width):
         for i in range(n) if width < 32768 else (0, 4, 5, 8):
             want = _selected(q[i], c[:, 0], s[:, 0], t[0], (last - n + i) // 16 + 1, count, 1, 2)
             assert got[i, 0].tolist() == want, (count, i)
+
+
+@pytest.mark.parametrize("heads,d,width", [(97, 128, 32768), (209, 64, 32768), (257, 128, 16), (257, 64, 1)])
+def test_select_refuses_more_heads_than_fit(heads, d, width):
+    """Query heads a KV head: 256, and 96 of 128 dims or 208 of 64 beside a table of 32768 pages."""
+    lib = L.load()
+    kv = _desc(k=0, v=0, page_stride=0, kv_heads=1, head_dim=d, table_width=width, table_stride=width)
+    b = L.PagedBounds(0x40000, 2 * d, 0x50000, 1)
+    st = lib.spectra_paged_select(ctypes.byref(kv), ctypes.byref(b), 0x100000, heads * d, L.F16, 3, heads, 4, 1, 2, 0, 0, 0x200000, None)
+    _refused(st, lib.spectra_last_error(), L.ERR_UNSUPPORTED, "heads")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,d,width", [(96, 128, 32768), (208, 64, 32768), (256, 128, 100), (256, 64, 100)])
+def test_select_with_the_most_heads(hip, heads, d, width):
+    from spectra_amd import kernels as K
+    gen = _gen(83)
+    q = torch.randn(1, heads, d, generator=gen, device="cuda").half()
+    codes = torch.randint(-30, 128, (300, 1, 2, d), generator=gen, device="cuda", dtype=torch.int8)
+    codes[:, :, 1] = -codes[:, :, 1]
+    scales = torch.rand(300, 1, generator=gen, device="cuda") + 0.1
+    table = torch.randint(0, 300, (1, width), generator=gen, device="cuda", dtype=torch.int32)
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([16 * width], [0, 1]))
+    want = _selected(q[0], codes[:, 0].cpu().numpy(), scales[:, 0].cpu().numpy(), table[0].cpu().numpy(), width, 20, 1, 2)
+    for ws in (None, K.paged_select_workspace()):
+        assert K.paged_select(q, lens, starts, table, (codes, scales), 16, 20, workspace=ws)[0, 0].tolist() == want
