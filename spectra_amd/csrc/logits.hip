@@ -97,9 +97,11 @@ struct LgWord {
 constexpr size_t lg_zero(int slice, size_t word) { return slice / 8 + slice * word; }
 
 // TH: threads of a workgroup; C: chunks of 8 logits a lane; W: the words' type.
+// (out may be the logits themselves: a workgroup reads its slice before it writes it, and no others', and nothing tells the
+// compiler that the two lie apart)
 template <int DT, bool PICK, int TH, int C, typename W>
-__global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* __restrict__ out, int64_t ldo,
-                                                    int64_t* __restrict__ tokens, int slices, uint8_t* __restrict__ meeting) {
+__global__ void __launch_bounds__(TH) logits_kernel(const LogitsArgs a, void* out, int64_t ldo, int64_t* __restrict__ tokens,
+                                                    int slices, uint8_t* __restrict__ meeting) {
   typedef typename LgType<DT>::T T;
   typedef LgWord<W> Word;
   constexpr int S = 8 * TH * C, U = 2048 / TH > 4 ? 8 : 4;

@@ -1619,3 +1619,16 @@ def test_select_with_the_most_heads(hip, heads, d, width):
     want = _selected(q[0], codes[:, 0].cpu().numpy(), scales[:, 0].cpu().numpy(), table[0].cpu().numpy(), width, 20, 1, 2)
     for ws in (None, K.paged_select_workspace()):
         assert K.paged_select(q, lens, starts, table, (codes, scales), 16, 20, workspace=ws)[0, 0].tolist() == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(40, 40003), (3, 40003)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_logits_in_place_of_large_and_small_slices(hip, dtype, rows, vocab):
+    """Logits that are their own output, adjusted tokens spread over all slices."""
+    from spectra_amd import kernels as K
+    x, kw = _case(rows, vocab, dtype, 84, history=3001, biases=1100, masks=3)
+    want = K.adjust_logits(x, **kw)
+    for _ in range(3):
+        mine = x.clone()
+        assert K.adjust_logits(mine, **kw, out=mine) is mine and torch.equal(_bits(mine), _bits(want))
