@@ -15,9 +15,11 @@
 // without.  So nothing is kept between steps, and the history may change in any way.  The choice meets over a row's slices
 // in 64-bit maxima of (value, token) in the workspace, whose last arrival writes the token.
 //
-// Bound by memory and the launch where nothing is adjusted (64 rows of 128256 fp16 logits read and written: 10.3 us; chosen
-// from: 8.9), with long histories by their reading and counting a slice before the logits are looked at (4096 tokens a row,
-// 40 biases and masks: 14.9 and 13.9).
+// Bound by memory and the launch where nothing is adjusted and logits are written (64 rows of 128256 in fp16 9.7 us, 33 MB).
+// Choices take as long for fp16 as for fp32 (9.0 us for either; one slice a row 2.8), so not by their bytes but by 4032 small
+// workgroups with a read, a reduction and a meeting each.  With long histories by a chain of dependent steps in every slice:
+// the tokens, the counts between barriers, each listed token's logit once more, then the rest (4096 tokens a row, 40 biases
+// and masks: 14.8, chosen from 13.8).
 #include <algorithm>
 
 #include "paged.h"

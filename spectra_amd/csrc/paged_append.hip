@@ -15,7 +15,8 @@
 // scalar loads behind a search of the starts that the row's loads overlap.  Bound by that chain
 // of dependent loads for a few tokens (one: 3.5 to 4.5 us, most of it the launch), by memory for prompts: 8.1
 // thousand bf16 tokens (32 heads of 128 on 8) read and write 199 MB in 34 us, 5.8 TB/s.  With axes, a token of each of 48
-// users 3.8 us, 126 MB of bf16 prompts 27.8 us, 4.5 TB/s (40.1 where every lane gathered its pairs' angles).
+// users 3.1 us in a graph, 126 MB of bf16 prompts 27.8 us, 4.5 TB/s (40.1 where every lane gathered its pairs' angles); on
+// 4-bit pages 3.9 us, and the prompts' 112 MB 28.2 us, 4.0 TB/s (the plain append 25.6).
 // Roundings: the rotated values to their 16 bits, once, from fp32 products and sums; 4-bit rows as the
 // quantizer rounds.
 #include <algorithm>

@@ -12,10 +12,11 @@
 // to arrive joins them in the order of their keys.  (Shares by `count` alone: 64 users of 100 to 2000 keys with room for
 // 4096 took 105 us, not 73.)
 //
-// Bound by reading the listed pages for a served batch: 64 users of 4096 keys, 1.05 GB, 181 us, 5.8 TB/s.  On 4 bits by the
-// vector instructions of the expansion: the same 82 us, 3.8 TB/s; 60 drafted tokens of 1536 keys of 64 dims with a cap 21.9
-// us.  A single token is a chain of the launch, starts, list, ids, rows and the join: 2048 keys 9.7 us.  Roundings: the weights to the activations' 16 bits for the product with V, 4-bit
-// values to fp16, the output.
+// Bound by reading the listed pages for a served batch: 64 users of 4096 keys, 1.05 GB, 180 to 188 us, 5.8 to 5.6 TB/s; 4-bit
+// pages 81 us, 3.8 TB/s.  60 drafted tokens of 1536 keys of 64 dims on 4-bit pages with a cap take 22.0 us: the vector unit issues
+// 57 % of the cycles (the expansion, anew for each token, and the cap), by two waves a SIMD that wait 38 % of theirs.  A
+// single token is a chain of the launch, starts, list, ids, rows and the join: 2048 keys in 64 pages 9.4 us.  Roundings: the
+// weights to the activations' 16 bits for the product with V, 4-bit values to fp16, the output.
 #include "paged_attend.h"
 
 namespace spectra {
@@ -100,7 +101,8 @@ __global__ void __launch_bounds__(kBlkThreads, kBlkResident)
     const int pos = un.seq.len - un.seq.n + un.tile;  // the row's position: it sees the keys up to that
     const bool past = pos >= kv.table_width << kv.page_shift;
     const bool whole = un.from == 0 && un.to == un.steps;
-    // the list up to its last entry, and this part of it
+    // the list up to its last entry, and this part of it (a round trip for each 64 entries, in every workgroup that has a
+    // part: lists of 32 pages of 16 rows 8.0 us, of 128 9.9, of 1024 28.6, of 8192 158)
     const int* list = blocks + ((int64_t)tok * kv.kv_heads + kvh) * count;
     int extent = 0;
     for (int s0 = 0; s0 < count; s0 += 64) {

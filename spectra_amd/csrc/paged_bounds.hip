@@ -15,8 +15,9 @@
 // order (five instructions for two; as fp32 values, eighteen), in which infinities and NaN end up at the ends, so that
 // the maxima show them.  No LDS, no workspace.
 // Bound by its chain of dependent loads (starts and lengths, the id, the rows) for a served batch's tokens: 64 users 4.0 us
-// in a graph; by memory for prompts: 64 MB of bf16 keys 13.2 us, 4.8 TB/s; on 4 bits by the expansion: 9.4 MB of rows of 64
-// dims 9.1 us (15.3 with the values compared as fp32).  More than one head a wave was slower for tokens (4.2 us with one,
+// in a graph; by memory for prompts: 55 MB of bf16 keys 12.2 us, 4.6 TB/s; on 4 bits by vector instructions, the expansion's and
+// the comparisons', some 520 a wave, which take 71 % of the cycles: 8.9 MB of rows of 64 dims 8.9 us (15.3 with the
+// values compared as fp32).  More than one head a wave was slower for tokens (4.2 us with one,
 // 5.7, 8.9 and 15.4 with 2, 4 and 8).
 #include <algorithm>
 #include <type_traits>

@@ -19,8 +19,10 @@
 // chooses from the keys of all in the workspace.
 //
 // Bound by latencies, not by the bounds' bytes: starts and lengths, ids, bounds, then the choice, one behind the other (64
-// users of up to 250 pages, 18 MB: 10.7 us, of which the choice is 2.5; one of 8188 pages, 17 MB: 12.4 us, of which the
-// choice is 4).
+// users of up to 250 pages, 18 MB: 10.6 us, of which the choice is 2.5; one of 8188 pages, 17 MB: 12.4 us, of which the
+// choice is 4; vector unit busy 15 % of the cycles).  A unit that is not split is one workgroup's, however long: 16 users
+// of 2000 pages 24 us, 67 MB; one of 8000 pages among 64 users 75 us.  Keys take a word of LDS a column of the table,
+// whatever the lengths: 64 short users on a table of 260 or 8001 columns 9.9 us, of 32768 14.7.
 #include <algorithm>
 
 #include "paged_attend.h"
@@ -361,8 +363,11 @@ __device__ __forceinline__ SelFew sel_pick(const uint32_t* key, int n, int count
   return {nullptr, nullptr, 0};
 }
 
-// The same of up to 64 R keys a wave, which stay in registers (read from LDS three times: one of 8188 pages 15.2 us, not 12.4); key(j): the
-// j-th.  None: more candidates than fit, or more wanted than there are lanes, and nothing done.
+// The same of up to 64 R keys a wave, which stay in registers; key(j): the j-th.  None: more candidates than fit, or more
+// wanted than there are lanes, and nothing done.  For keys that have met in the workspace: brought to LDS first and read there
+// three times, one of 8188 pages took 15.2 us, not 12.4.  Keys that are in LDS already are read from there (sel_pick): 16
+// users of 600 pages 12.6 us (by registers 12.8), of 2000 24.3 (24.6), 64 of 600 21.4 (21.7), of 1000 35.9 (36.2); only
+// the longest gain by registers, 16 of 8000 103.7 (102.3).
 template <int R, typename F>
 __device__ __forceinline__ SelFew sel_pick_in_registers(F key, int n, int count, SelTogether w) {
   if (count > 64 * w.parts) return {nullptr, nullptr, 0};
