@@ -61,3 +61,11 @@ def test_traffic_hash_covers_the_kernel_sources():
     assert found <= hashed, found - hashed
     assert {"gemv_rows.h", "gemv_stream.h", "gemv_kernel.h", "common.h"} <= hashed
     assert bench.kernel_source_hash() == bench.kernel_source_hash()
+
+
+def test_traffic_was_measured_on_these_sources():
+    """The committed summary is of the sources in the tree, the public header among them: a change to any of them takes the
+    benchmark's traffic figure away until it is measured again (profiles/gemv_cfg2_down_traffic.md says how)."""
+    import bench
+    value, why = bench.measured_traffic()
+    assert value is not None, why
